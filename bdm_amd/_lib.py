@@ -42,6 +42,9 @@ EXPORTED_SYMBOLS = (
     'bdm_output_backward_partials',
     'bdm_output_backward',
     'bdm_router_backward',
+    'bdm_beam_select_workspace_size',
+    'bdm_beam_select',
+    'bdm_reorder_states',
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -195,6 +198,17 @@ class AdamwArgs(ctypes.Structure):
     ]
 
 
+class BeamArgs(ctypes.Structure):
+    """Mirror of ``bdm_beam_args``."""
+    _fields_ = [
+        ('logits', _vp), ('scores', _vp), ('finished', _vp), ('lengths', _vp),
+        ('out_scores', _vp), ('out_tokens', _vp), ('out_parents', _vp), ('out_finished', _vp), ('out_lengths', _vp),
+        ('batch', _i64), ('batch_stride', _i64), ('beam_stride', _i64), ('eos', _i64),
+        ('length_penalty', ctypes.c_double),
+        ('beams', _i32), ('vocab', _i32), ('width', _i32), ('dtype', _i32),
+    ]
+
+
 class BDMError(RuntimeError):
     """A call into libbdm_hip returned a non-zero status."""
 
@@ -275,6 +289,12 @@ def library() -> ctypes.CDLL:
     lib.bdm_output_backward.restype = _i32
     lib.bdm_router_backward.argtypes = [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]
     lib.bdm_router_backward.restype = _i32
+    lib.bdm_beam_select_workspace_size.argtypes = [ctypes.POINTER(BeamArgs)]
+    lib.bdm_beam_select_workspace_size.restype = _size_t
+    lib.bdm_beam_select.argtypes = [ctypes.POINTER(BeamArgs), _vp, _size_t, _vp]
+    lib.bdm_beam_select.restype = _i32
+    lib.bdm_reorder_states.argtypes = [ctypes.POINTER(_vp), ctypes.POINTER(_i64), _i32, _vp, _i64, _i32, _vp]
+    lib.bdm_reorder_states.restype = _i32
     return lib
 
 

@@ -1,0 +1,751 @@
+// Beam search: the selection over beams and vocabulary, and the dense caches
+// of several layers put in the order of the chosen parents.
+//
+// Selection.  With x the logits of beam k of a prompt, l = log sum exp x and
+// s the beam's score, the candidate (k, t) has the total s + x_t - l; an ended
+// beam offers one candidate, (eos, s).  The W best totals (divided by
+// length^a where lengths are normalized) are wanted, ties to the lower
+// k * V + t.  Within a beam the order of the totals is that of the logits, so
+// one pass over the logits is enough: it keeps, for each part of a row, the
+// maximum, the sum of exponentials and the W best logits (scan), and the
+// parts of a prompt's rows are then joined (join).
+//
+// The scan holds its part in registers.  A lower bound of the W-th best value
+// is the W-th best of the lanes' own maxima, found by bisection over the top
+// 16 bits of the ordered bit pattern with one ballot a bit; the few values at
+// or above the bound go to LDS and are ranked there by counting.  Where ties
+// or an unlucky layout put more there than it holds, the exact W-th value and
+// index are found by bisection over all their bits instead.
+//
+// The exponentials and their sums are FP32 (each exponent relative to its
+// part's maximum), everything behind them is FP64: candidates of different
+// beams are compared by totals, which lie near each other.
+#include "bdm_common.h"
+
+namespace bdm {
+namespace {
+
+constexpr int kBeamMax = 64;       // beams in, and candidates out, per prompt
+constexpr int kReorderTensors = 32;  // tensors of one reordering launch
+
+// ------------------------------------------------------------------ ordered bit patterns
+// Unsigned integers in the order of the floating values; -0 counts as +0.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ uint64_t ordered(double x) {
+    const uint64_t u = uint64_t(__double_as_longlong(x + 0.0));
+    return u ^ (uint64_t(int64_t(u) >> 63) | 0x8000000000000000ull);
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int d = kWave / 2; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int d = kWave / 2; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+__device__ __forceinline__ int popcount(uint64_t m) { return __popcll(m); }
+
+// The W-th largest of the lanes' BITS-bit values by bisection (0 where fewer
+// than W lanes hold one above 0).
+template <int BITS>
+__device__ __forceinline__ uint32_t nth_of_lanes(uint32_t value, int nth) {
+    uint32_t bound = 0;
+#pragma unroll 4
+    for (int bit = BITS - 1; bit >= 0; --bit) {
+        const uint32_t next = bound | (1u << bit);
+        if (popcount(__ballot(value >= next)) >= nth) bound = next;
+    }
+    return bound;
+}
+
+// ------------------------------------------------------------------ a team's part of a row
+// A team of WAVES waves holds E values a lane: its shared memory.
+template <int WAVES>
+struct TeamShared {
+    static constexpr int kRoom = 256 * WAVES;
+    uint64_t list[kRoom];  // ordered value, then ~index: descending order is value, then lowest index
+    float high[WAVES], sum[WAVES];
+    uint32_t bound[WAVES];
+    int count;
+};
+
+template <int WAVES>
+__device__ __forceinline__ void team_sync() {
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+    } else {
+        // one wave: its LDS accesses are in order, the compiler has to keep them so
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// How many of the team's values satisfy `test`, in every lane.
+template <int WAVES, int E, typename F>
+__device__ int team_count(TeamShared<WAVES> &sh, int lane, F test) {
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine += popcount(__ballot(test(e)));
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        if (lane == 0) atomicAdd(&sh.count, mine);
+        __syncthreads();
+        mine = sh.count;
+        __syncthreads();
+    }
+    return mine;
+}
+
+// Maximum, sum of exponentials and the `width` best of the team's values
+// (index(e) is value e's index): sets high and sum in every lane, leaves the
+// candidates in sh.list and returns how many there are.  Values of -inf are no candidates.
+template <int WAVES, int E, typename Index>
+__device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index, int width, int wave, int lane,
+                         float &high, float &sum) {
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
+    const uint32_t mine = top > -INFINITY ? ordered(top) >> 16 : 0u;
+    uint32_t bound = nth_of_lanes<16>(mine, width);
+    high = wave_max(top);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) {
+            sh.high[wave] = high;
+            sh.bound[wave] = bound;
+        }
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            high = fmaxf(high, sh.high[i]);
+            bound = max(bound, sh.bound[i]);
+        }
+    } else {
+        if (lane == 0) sh.count = 0;
+        team_sync<WAVES>();
+    }
+    // the sum relative to the part's maximum; a part without a finite value has the sum 0, one with a NaN
+    // or +inf (inf - inf) a NaN
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += x[e] == -INFINITY ? 0.f : __expf(x[e] - high);
+    sum = wave_sum(sum);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) sh.sum[wave] = sum;
+    }
+    if (mine >= bound && mine) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t key = ordered(x[e]);
+            if (x[e] > -INFINITY && key >> 16 >= bound) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < TeamShared<WAVES>::kRoom) sh.list[at] = uint64_t(key) << 32 | uint32_t(~index(e));
+            }
+        }
+    }
+    team_sync<WAVES>();
+    int count = sh.count;
+    if constexpr (WAVES > 1) {
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) sum += sh.sum[i];
+    }
+    if (count <= TeamShared<WAVES>::kRoom) return count;
+    // too many at or above the bound: the exact width-th value, then the lowest indices of those equal to it
+    team_sync<WAVES>();
+    uint32_t value = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t next = value | (1u << bit);
+        if (team_count<WAVES, E>(sh, lane, [&](int e) { return x[e] > -INFINITY && ordered(x[e]) >= next; }) >= width)
+            value = next;
+    }
+    const int above =
+        team_count<WAVES, E>(sh, lane, [&](int e) { return x[e] > -INFINITY && ordered(x[e]) > value; });
+    uint32_t last = 0;  // the largest bound with fewer than width - above of the equal ones below it
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t next = last | (1u << bit);
+        if (team_count<WAVES, E>(sh, lane, [&](int e) { return x[e] > -INFINITY && ordered(x[e]) == value && index(e) < next; }) <
+            width - above)
+            last = next;
+    }
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x == 0) sh.count = 0;
+    } else {
+        if (lane == 0) sh.count = 0;
+    }
+    team_sync<WAVES>();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint32_t key = ordered(x[e]);
+        if (x[e] > -INFINITY && (key > value || (key == value && index(e) <= last)))
+            sh.list[atomicAdd(&sh.count, 1)] = uint64_t(key) << 32 | uint32_t(~index(e));
+    }
+    team_sync<WAVES>();
+    return sh.count;
+}
+
+template <typename T> struct Vec;
+template <> struct Vec<bf16_t> {
+    static constexpr int kSize = 8;
+    static __device__ __forceinline__ void load(const bf16_t *p, float *out) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            out[2 * i] = __uint_as_float(w[i] << 16);
+            out[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+template <> struct Vec<float> {
+    static constexpr int kSize = 4;
+    static __device__ __forceinline__ void load(const float *p, float *out) {
+        const float4 u = *reinterpret_cast<const float4 *>(p);
+        out[0] = u.x, out[1] = u.y, out[2] = u.z, out[3] = u.w;
+    }
+};
+
+struct BeamParams {
+    const void *logits;
+    const float *scores;
+    const uint8_t *finished;
+    const int32_t *lengths;
+    float *out_scores;
+    int64_t *out_tokens, *out_parents;
+    uint8_t *out_finished;
+    int32_t *out_lengths;
+    float2 *parts;    // [rows, splits] maximum and sum
+    uint64_t *lists;  // [rows, splits, width] ordered logit, ~token; 0 behind the last
+    int64_t batch_stride, beam_stride, eos;
+    double penalty;
+    int beams, vocab, width, splits;
+};
+
+// Whether a beam's logits count: it has not ended and its score is finite.
+__device__ __forceinline__ bool beam_live(const BeamParams &p, int64_t row) {
+    return !(p.finished && p.finished[row]) && isfinite(p.scores[row]);
+}
+
+// One part of one row.  The row starts anywhere: the values before its first
+// 16-byte boundary and those behind its last whole vector are a tail that the
+// first part takes one by one.
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
+    constexpr int VE = Vec<T>::kSize, E = NV * VE + 1;
+    __shared__ TeamShared<4> sh;
+    const int64_t row = blockIdx.x / p.splits;
+    const int split = blockIdx.x % p.splits;
+    if (!beam_live(p, row)) return;
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    const T *x = static_cast<const T *>(p.logits) + row / p.beams * p.batch_stride + row % p.beams * p.beam_stride;
+    const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
+    const int vectors = (p.vocab - head) / VE;
+    float v[E];
+    int first[NV];  // first index of each vector
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (split * NV + i) * 256 + int(threadIdx.x);
+        first[i] = head + at * VE;
+        if (at < vectors) {
+            Vec<T>::load(x + first[i], v + i * VE);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[i * VE + j] = -INFINITY;
+        }
+    }
+    // the row's odd ends: fewer than 2 * VE values
+    const int odd = int(threadIdx.x) < head ? int(threadIdx.x) : vectors * VE + int(threadIdx.x);
+    v[E - 1] = split == 0 && odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
+    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : first[e / VE] + e % VE); };
+    float high, sum;
+    const int count = team_scan<4, E>(sh, v, index, p.width, wave, lane, high, sum);
+    const int64_t part = row * p.splits + split;
+    if (threadIdx.x == 0) p.parts[part] = make_float2(high, sum);
+    uint64_t *out = p.lists + part * p.width;
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const uint64_t mine = sh.list[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += sh.list[j] > mine;
+        if (rank < p.width) out[rank] = mine;
+    }
+    for (int i = count + int(threadIdx.x); i < p.width; i += 256) out[i] = 0;
+}
+
+// ------------------------------------------------------------------ joining a prompt's beams
+template <int THREADS>
+struct JoinShared {
+    static constexpr int kRoom = 1024;
+    double log_sum[kBeamMax], norm[kBeamMax], score[kBeamMax];
+    uint64_t key[kRoom];    // ordered compared value
+    uint64_t place[kRoom];  // beam * vocab + token
+    double total[kRoom];
+    uint64_t chosen[kBeamMax];
+    double chosen_total[kBeamMax];
+    uint32_t bound[THREADS / kWave];
+    int count;
+};
+
+// A beam's score and the divisor of its candidates.
+template <int THREADS>
+__device__ __forceinline__ void join_beam(const BeamParams &p, JoinShared<THREADS> &sh, int64_t row, int beam) {
+    sh.score[beam] = double(p.scores[row]);
+    const bool ended = p.finished && p.finished[row];
+    sh.norm[beam] = p.penalty != 0.0 ? pow(double(p.lengths[row] + (ended ? 0 : 1)), p.penalty) : 1.0;
+}
+
+// The `width` best of a prompt's candidates: entries [0, entries) of its
+// beams' lists, entry(i, beam) being entry i's list value (0: none; a beam
+// without totals has the log_sum NaN), then the ended beams' own.  Called by the whole workgroup, behind a barrier that made
+// log_sum, norm and score of every beam visible.
+template <int THREADS, typename Entry>
+__device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t prompt, int entries, Entry entry) {
+    constexpr int kRoom = JoinShared<THREADS>::kRoom;
+    const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
+    const int all = entries + (p.finished ? p.beams : 0);
+    // candidate i's ordered compared value (0: it has none), its place and total
+    auto candidate = [&](int i, uint64_t &place, double &total) -> uint64_t {
+        int beam;
+        if (i < entries) {
+            const uint64_t item = entry(i, beam);
+            if (!item) return 0;
+            place = uint64_t(beam) * uint32_t(p.vocab) + uint32_t(~uint32_t(item));
+            total = sh.score[beam] + (double(unordered(uint32_t(item >> 32))) - sh.log_sum[beam]);
+        } else {
+            beam = i - entries;
+            if (!p.finished[prompt * p.beams + beam]) return 0;
+            place = uint64_t(beam) * uint32_t(p.vocab) + uint64_t(p.eos);
+            total = sh.score[beam];
+        }
+        const double compared = total / sh.norm[beam];
+        return isfinite(compared) ? ordered(compared) : 0;
+    };
+    uint64_t place = 0;
+    double total = 0;
+    uint32_t mine = 0;
+    for (int i = thread; i < all; i += THREADS) mine = max(mine, uint32_t(candidate(i, place, total) >> 32));
+    const uint32_t part = nth_of_lanes<32>(mine, p.width);
+    if (lane == 0) sh.bound[wave] = part;
+    if (thread == 0) sh.count = 0;
+    __syncthreads();
+    uint32_t bound = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / kWave; ++w) bound = max(bound, sh.bound[w]);
+    auto take = [&](uint64_t key) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kRoom) {
+            sh.key[at] = key;
+            sh.place[at] = place;
+            sh.total[at] = total;
+        }
+    };
+    for (int i = thread; i < all; i += THREADS) {
+        const uint64_t key = candidate(i, place, total);
+        if (key && uint32_t(key >> 32) >= bound) take(key);
+    }
+    __syncthreads();
+    if (sh.count > kRoom) {
+        // more than LDS holds: the exact width-th value, then the lowest places of those equal to it
+        auto counted = [&](auto test) {
+            __syncthreads();
+            if (thread == 0) sh.count = 0;
+            __syncthreads();
+            int found = 0;
+            for (int i = thread; i < all; i += THREADS) {
+                const uint64_t key = candidate(i, place, total);
+                if (key && test(key, place)) ++found;
+            }
+            if (found) atomicAdd(&sh.count, found);
+            __syncthreads();
+            return sh.count;
+        };
+        uint64_t value = 0, last = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t next = value | (1ull << bit);
+            if (counted([&](uint64_t key, uint64_t) { return key >= next; }) >= p.width) value = next;
+        }
+        const int above = counted([&](uint64_t key, uint64_t) { return key > value; });
+        for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t next = last | (1ull << bit);
+            if (counted([&](uint64_t key, uint64_t at) { return key == value && at < next; }) < p.width - above)
+                last = next;
+        }
+        __syncthreads();
+        if (thread == 0) sh.count = 0;
+        __syncthreads();
+        for (int i = thread; i < all; i += THREADS) {
+            const uint64_t key = candidate(i, place, total);
+            if (key && (key > value || (key == value && place <= last))) take(key);
+        }
+        __syncthreads();
+    }
+    const int count = sh.count;
+    for (int i = thread; i < count; i += THREADS) {
+        const uint64_t key = sh.key[i], at = sh.place[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += sh.key[j] > key || (sh.key[j] == key && sh.place[j] < at);
+        if (rank < p.width) {
+            sh.chosen[rank] = at;
+            sh.chosen_total[rank] = sh.total[i];
+        }
+    }
+    __syncthreads();
+    if (thread == 0 && count < p.width) {
+        // fewer candidates than places: the lowest places that are none of them, with the score -inf
+        uint64_t next = 0;
+        for (int i = count; i < p.width; ++next) {
+            bool taken = false;
+            for (int j = 0; j < count; ++j) taken |= sh.chosen[j] == next;
+            if (!taken) {
+                sh.chosen_total[i] = -INFINITY;
+                sh.chosen[i++] = next;
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = thread; i < p.width; i += THREADS) {
+        const uint64_t at = sh.chosen[i];
+        const int64_t beam = int64_t(at / uint32_t(p.vocab)), token = int64_t(at % uint32_t(p.vocab));
+        const int64_t row = prompt * p.beams + beam, out = prompt * p.width + i;
+        const bool ended = p.finished && p.finished[row];
+        p.out_scores[out] = float(sh.chosen_total[i]);
+        p.out_tokens[out] = token;
+        p.out_parents[out] = row;
+        if (p.out_finished) p.out_finished[out] = ended || token == p.eos;
+        if (p.out_lengths) p.out_lengths[out] = p.lengths[row] + (ended ? 0 : 1);
+    }
+}
+
+// One workgroup a prompt: the parts of its rows joined.
+__global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
+    __shared__ JoinShared<256> sh;
+    const int64_t prompt = blockIdx.x;
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    for (int beam = wave; beam < p.beams; beam += 4) {
+        const int64_t row = prompt * p.beams + beam;
+        if (!beam_live(p, row)) {  // no totals: its lists were not written
+            if (lane == 0) sh.log_sum[beam] = NAN;
+            continue;
+        }
+        const float2 *parts = p.parts + row * p.splits;
+        float high = -INFINITY;
+        for (int i = lane; i < p.splits; i += kWave) high = fmaxf(high, parts[i].x);
+        high = wave_max(high);
+        double sum = 0;
+        for (int i = lane; i < p.splits; i += kWave) {
+            const float2 part = parts[i];
+            if (part.y != 0.f) sum += double(part.y) * exp(double(part.x) - double(high));
+        }
+#pragma unroll
+        for (int d = kWave / 2; d; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) sh.log_sum[beam] = double(high) + log(sum);
+    }
+    if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
+    __syncthreads();
+    const int per_beam = p.splits * p.width;
+    const uint64_t *lists = p.lists + prompt * p.beams * per_beam;
+    join_beams<256>(p, sh, prompt, p.beams * per_beam, [&](int i, int &beam) {
+        beam = i / per_beam;
+        return lists[i];
+    });
+}
+
+// Small vocabularies, one launch: one workgroup a prompt, a wave a row.
+constexpr int kRowWaves = 8;
+constexpr int kRowLists = 1024;  // beams * width
+
+template <typename T, int NV>
+__global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams p) {
+    constexpr int VE = Vec<T>::kSize, E = NV * VE + 1;
+    __shared__ TeamShared<1> teams[kRowWaves];
+    __shared__ JoinShared<kRowWaves * kWave> sh;
+    __shared__ uint64_t lists[kRowLists];
+    const int64_t prompt = blockIdx.x;
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    TeamShared<1> &team = teams[wave];
+    for (int beam = wave; beam < p.beams; beam += kRowWaves) {
+        const int64_t row = prompt * p.beams + beam;
+        if (!beam_live(p, row)) {  // no totals: its list is not written
+            if (lane == 0) sh.log_sum[beam] = NAN;
+            continue;
+        }
+        const T *x = static_cast<const T *>(p.logits) + prompt * p.batch_stride + beam * p.beam_stride;
+        const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
+        const int vectors = (p.vocab - head) / VE;
+        float v[E];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int at = i * kWave + lane;
+            if (at < vectors) {
+                Vec<T>::load(x + head + at * VE, v + i * VE);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) v[i * VE + j] = -INFINITY;
+            }
+        }
+        const int odd = lane < head ? lane : vectors * VE + lane;
+        v[E - 1] = odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
+        auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
+        float high, sum;
+        const int count = team_scan<1, E>(team, v, index, p.width, 0, lane, high, sum);
+        uint64_t *out = lists + beam * p.width;
+        for (int i = lane; i < count; i += kWave) {
+            const uint64_t mine = team.list[i];
+            int rank = 0;
+            for (int j = 0; j < count; ++j) rank += team.list[j] > mine;
+            if (rank < p.width) out[rank] = mine;
+        }
+        for (int i = count + lane; i < p.width; i += kWave) out[i] = 0;
+        if (lane == 0) sh.log_sum[beam] = double(high) + log(double(sum));
+        team_sync<1>();
+    }
+    if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
+    __syncthreads();
+    join_beams<kRowWaves * kWave>(p, sh, prompt, p.beams * p.width, [&](int i, int &beam) {
+        beam = i / p.width;
+        return lists[i];
+    });
+}
+
+// How a call is cut: whole rows by a wave each (splits 0), or parts of `vectors` 16-byte vectors a thread.
+struct BeamPlan {
+    int vectors, splits;
+};
+
+BeamPlan beam_plan(const bdm_beam_args &a) {
+    const int ve = a.dtype == BDM_BF16 ? Vec<bf16_t>::kSize : Vec<float>::kSize;
+    if (a.vocab <= 2048 && a.beams <= 2 * kRowWaves && a.beams * a.width <= kRowLists)
+        return {a.vocab <= 512 ? 512 / (kWave * ve) : 2048 / (kWave * ve), 0};
+    int vectors = 32 / ve;
+    const int64_t rows = a.batch * a.beams;
+    while (vectors > 8 / ve && rows * ((a.vocab + vectors * 256 * ve - 1) / (vectors * 256 * ve)) < 512)
+        vectors /= 2;
+    const int part = vectors * 256 * ve;
+    return {vectors, (a.vocab + part - 1) / part};
+}
+
+// ------------------------------------------------------------------ reordering
+struct ReorderTensor {
+    char *data;
+    int64_t row_bytes;
+    unsigned first_block;  // of the tensor's workgroups of one prompt
+};
+
+struct ReorderParams {
+    ReorderTensor tensors[kReorderTensors];
+    const int64_t *parents;
+    int count, beams;
+    unsigned blocks;  // workgroups of one prompt
+};
+
+// data[i] <- data[parents[i]] within a prompt's beams, in place: a thread owns
+// one vector column of all the prompt's rows, so it has every row that it
+// moves in registers before it stores the first, and no other thread touches
+// the column.  Rows that stay are neither read nor written.  Two beams of one
+// parent read the same lines at the same time, from the caches.
+template <typename V, int K>
+__global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
+    const int64_t prompt = blockIdx.x / p.blocks;
+    const unsigned block = blockIdx.x % p.blocks;
+    int which = 0;
+    while (which + 1 < p.count && p.tensors[which + 1].first_block <= block) ++which;
+    const ReorderTensor t = p.tensors[which];
+    const int64_t column = (int64_t(block - t.first_block) * 256 + threadIdx.x) * int64_t(sizeof(V));
+    if (column >= t.row_bytes) return;
+    const int64_t first = prompt * p.beams;
+    char *base = t.data + first * t.row_bytes + column;
+    V held[K];
+    int from[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        from[k] = k;
+        if (k < p.beams) {
+            const int64_t parent = p.parents[first + k] - first;
+            from[k] = int(parent < 0 ? 0 : parent >= p.beams ? p.beams - 1 : parent);
+            if (from[k] != k) held[k] = *reinterpret_cast<const V *>(base + from[k] * t.row_bytes);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k < p.beams && from[k] != k) *reinterpret_cast<V *>(base + k * t.row_bytes) = held[k];
+}
+
+template <typename V>
+int launch_reorder(ReorderParams &p, int64_t batch, hipStream_t stream) {
+    unsigned blocks = 0;
+    for (int i = 0; i < p.count; ++i) {
+        p.tensors[i].first_block = blocks;
+        const int64_t need = (p.tensors[i].row_bytes / int64_t(sizeof(V)) + 255) / 256;
+        if (need + blocks > int64_t(UINT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: rows too long");
+        blocks += unsigned(need);
+    }
+    if (blocks == 0) return BDM_OK;
+    if (batch * int64_t(blocks) > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: grid too large");
+    p.blocks = blocks;
+    const unsigned grid = unsigned(batch * blocks);
+    if (p.beams <= 4)
+        reorder_kernel<V, 4><<<grid, 256, 0, stream>>>(p);
+    else if (p.beams <= 8)
+        reorder_kernel<V, 8><<<grid, 256, 0, stream>>>(p);
+    else if (p.beams <= 16)
+        reorder_kernel<V, 16><<<grid, 256, 0, stream>>>(p);
+    else if (p.beams <= 32)
+        reorder_kernel<V, 32><<<grid, 256, 0, stream>>>(p);
+    else
+        reorder_kernel<V, 64><<<grid, 256, 0, stream>>>(p);
+    return check_launch("reorder_kernel");
+}
+
+template <typename T, int NV>
+void launch_scan(const BeamParams &p, int64_t batch, hipStream_t stream) {
+    beam_scan_kernel<T, NV><<<unsigned(batch * p.beams * p.splits), 256, 0, stream>>>(p);
+}
+
+int check_beam(const bdm_beam_args *a) {
+    if (!a) return fail(BDM_ERR_INVALID, "beam_select: null args");
+    if (a->batch < 0 || a->beams <= 0 || a->vocab <= 0 || a->width <= 0)
+        return fail(BDM_ERR_INVALID, "beam_select: bad geometry");
+    if (a->dtype != BDM_BF16 && a->dtype != BDM_F32) return fail(BDM_ERR_INVALID, "beam_select: logits dtype");
+    if (a->beams > kBeamMax || a->width > kBeamMax)
+        return fail(BDM_ERR_UNSUPPORTED, "beam_select: more than %d beams", kBeamMax);
+    if (int64_t(a->width) > int64_t(a->beams) * a->vocab)
+        return fail(BDM_ERR_INVALID, "beam_select: width %d exceeds the candidates", a->width);
+    return BDM_OK;
+}
+
+}  // namespace
+}  // namespace bdm
+
+extern "C" size_t bdm_beam_select_workspace_size(const bdm_beam_args *a) {
+    using namespace bdm;
+    if (check_beam(a) != BDM_OK) return 0;
+    const size_t parts = size_t(a->batch) * a->beams * beam_plan(*a).splits;
+    return parts * (sizeof(float2) + size_t(a->width) * sizeof(uint64_t));
+}
+
+extern "C" int bdm_beam_select(const bdm_beam_args *a, void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace bdm;
+    const int rc = check_beam(a);
+    if (rc != BDM_OK) return rc;
+    if (a->batch == 0) return BDM_OK;
+    if (!a->logits || !a->scores || !a->out_scores || !a->out_tokens || !a->out_parents)
+        return fail(BDM_ERR_INVALID, "beam_select: null pointer");
+    if (a->finished && (a->eos < 0 || a->eos >= a->vocab))
+        return fail(BDM_ERR_INVALID, "beam_select: ended beams need an eos token of the vocabulary");
+    if ((a->length_penalty != 0.0 || a->out_lengths) && !a->lengths)
+        return fail(BDM_ERR_INVALID, "beam_select: length normalization needs lengths");
+    if (!(a->length_penalty - a->length_penalty == 0.0))
+        return fail(BDM_ERR_INVALID, "beam_select: length_penalty must be finite");
+    const size_t es = a->dtype == BDM_BF16 ? 2 : 4;
+    if (!aligned(a->logits, es)) return fail(BDM_ERR_INVALID, "beam_select: logits not aligned to their type");
+    const size_t need = bdm_beam_select_workspace_size(a);
+    if (need && (!workspace || workspace_bytes < need)) return fail(BDM_ERR_WORKSPACE, "beam_select: workspace of %zu bytes", need);
+    if (need && !aligned(workspace, 8)) return fail(BDM_ERR_INVALID, "beam_select: workspace must be 8-byte aligned");
+    const BeamPlan plan = beam_plan(*a);
+    if (a->batch * a->beams * (plan.splits ? plan.splits : 1) > int64_t(INT32_MAX))
+        return fail(BDM_ERR_UNSUPPORTED, "beam_select: grid too large");
+    BeamParams p{};
+    p.logits = a->logits;
+    p.scores = a->scores;
+    p.finished = a->finished;
+    p.lengths = a->lengths;
+    p.out_scores = a->out_scores;
+    p.out_tokens = a->out_tokens;
+    p.out_parents = a->out_parents;
+    p.out_finished = a->out_finished;
+    p.out_lengths = a->out_lengths;
+    p.lists = static_cast<uint64_t *>(workspace);
+    p.parts = reinterpret_cast<float2 *>(p.lists + size_t(a->batch) * a->beams * plan.splits * a->width);
+    p.batch_stride = a->batch_stride;
+    p.beam_stride = a->beam_stride;
+    p.eos = a->eos;
+    p.penalty = a->length_penalty;
+    p.beams = a->beams;
+    p.vocab = a->vocab;
+    p.width = a->width;
+    p.splits = plan.splits;
+    hipStream_t s = as_stream(stream);
+    const unsigned prompts = unsigned(a->batch);
+    if (plan.splits == 0) {
+        constexpr int threads = kRowWaves * kWave;
+        if (a->dtype == BDM_BF16) {
+            if (plan.vectors == 1)
+                beam_rows_kernel<bf16_t, 1><<<prompts, threads, 0, s>>>(p);
+            else
+                beam_rows_kernel<bf16_t, 4><<<prompts, threads, 0, s>>>(p);
+        } else {
+            if (plan.vectors == 2)
+                beam_rows_kernel<float, 2><<<prompts, threads, 0, s>>>(p);
+            else
+                beam_rows_kernel<float, 8><<<prompts, threads, 0, s>>>(p);
+        }
+        return check_launch("beam_rows_kernel");
+    }
+    if (a->dtype == BDM_BF16) {
+        if (plan.vectors == 4)
+            launch_scan<bf16_t, 4>(p, a->batch, s);
+        else if (plan.vectors == 2)
+            launch_scan<bf16_t, 2>(p, a->batch, s);
+        else
+            launch_scan<bf16_t, 1>(p, a->batch, s);
+    } else {
+        if (plan.vectors == 8)
+            launch_scan<float, 8>(p, a->batch, s);
+        else if (plan.vectors == 4)
+            launch_scan<float, 4>(p, a->batch, s);
+        else
+            launch_scan<float, 2>(p, a->batch, s);
+    }
+    const int scanned = check_launch("beam_scan_kernel");
+    if (scanned != BDM_OK) return scanned;
+    beam_join_kernel<<<prompts, 256, 0, s>>>(p);
+    return check_launch("beam_join_kernel");
+}
+
+extern "C" int bdm_reorder_states(void *const *states, const int64_t *row_bytes, int32_t count, const int64_t *parents,
+                                  int64_t batch, int32_t beams, void *stream) {
+    using namespace bdm;
+    if (count < 0 || batch < 0 || beams <= 0) return fail(BDM_ERR_INVALID, "reorder_states: bad geometry");
+    if (beams > kBeamMax) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: more than %d beams", kBeamMax);
+    if (count == 0 || batch == 0) return BDM_OK;
+    if (!states || !row_bytes || !parents) return fail(BDM_ERR_INVALID, "reorder_states: null pointer");
+    for (int i = 0; i < count; ++i) {
+        if (row_bytes[i] < 0) return fail(BDM_ERR_INVALID, "reorder_states: bad geometry");
+        if (row_bytes[i] && !states[i]) return fail(BDM_ERR_INVALID, "reorder_states: null pointer");
+    }
+    for (int done = 0; done < count; done += kReorderTensors) {
+        ReorderParams p{};
+        p.parents = parents;
+        p.beams = beams;
+        p.count = count - done < kReorderTensors ? count - done : kReorderTensors;
+        uintptr_t bits = 0;  // what every base and row length is a multiple of
+        for (int i = 0; i < p.count; ++i) {
+            p.tensors[i].data = static_cast<char *>(states[done + i]);
+            p.tensors[i].row_bytes = row_bytes[done + i];
+            bits |= reinterpret_cast<uintptr_t>(states[done + i]) | uintptr_t(row_bytes[done + i]);
+        }
+        int rc;
+        // 64 rows of 16 bytes would be 256 registers: 8 bytes a row beyond 32 beams
+        if (bits % 16 == 0 && beams <= 32)
+            rc = launch_reorder<uint4>(p, batch, as_stream(stream));
+        else if (bits % 8 == 0)
+            rc = launch_reorder<uint2>(p, batch, as_stream(stream));
+        else if (bits % 4 == 0)
+            rc = launch_reorder<uint32_t>(p, batch, as_stream(stream));
+        else if (bits % 2 == 0)
+            rc = launch_reorder<uint16_t>(p, batch, as_stream(stream));
+        else
+            rc = launch_reorder<uint8_t>(p, batch, as_stream(stream));
+        if (rc != BDM_OK) return rc;
+    }
+    return BDM_OK;
+}

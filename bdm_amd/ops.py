@@ -8,9 +8,11 @@ current stream without synchronising.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -52,6 +54,16 @@ def _require_gpu(*tensors: Tensor) -> torch.device:
         elif t.device != device:
             raise ValueError('all tensors must be on the same device')
     return device
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device made current for a launch, where another one is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_SWITCH
+    return torch.cuda.device(device)
 
 
 def _aligned(t: Tensor) -> Tensor:
@@ -986,3 +998,116 @@ def written_bank_curve(first_write: Tensor, prefixes) -> Tensor:
         _addr(first), batch, banks, _addr(ends), ends.numel(), _addr(written), _stream(device)),
         'bdm_written_bank_curve')
     return written
+
+
+# ---------------------------------------------------------------------------
+# beam search: the selection and the order of the dense caches
+
+BEAM_MAX = 64  # beams in, and continuations out, per prompt
+
+
+class BeamSelection(NamedTuple):
+    """The chosen continuations of each prompt, best first, all [B, width]."""
+    scores: Tensor            # FP32 summed log-probabilities
+    tokens: Tensor            # int64
+    parents: Tensor           # int64 rows of the flattened [B * K]
+    finished: Tensor | None   # bool, where an eos token was given
+    lengths: Tensor | None    # int32, where lengths were given
+
+
+def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, finished: Tensor | None = None,
+                eos: int | None = None, lengths: Tensor | None = None,
+                length_penalty: float = 0.0) -> BeamSelection:
+    """One selection of beam search: the ``width`` (default K) best
+    continuations of each prompt's K beams by one token.
+
+    logits [B, K, V] BF16 or FP32; scores [B, K] FP32, the beams' summed
+    log-probabilities.  A continuation's score is its beam's plus the log-softmax
+    of its logit.  A beam marked in ``finished`` [B, K] (bool) has one
+    continuation, token ``eos`` with its score unchanged.  With
+    ``length_penalty`` a, continuations compare by score / length**a, where
+    ``lengths`` [B, K] int32 are the beams' lengths and a continuation of an
+    unfinished beam is one longer.  Ties go to the lower beam, then the lower
+    token.  A logit of -inf is no candidate, nor is any of a beam whose score is
+    not finite or whose logits hold a NaN, +inf or nothing finite; where fewer
+    than ``width`` remain, the rest of the prompt's rows has the score -inf."""
+    if logits.ndim != 3 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError('logits must be BF16 or FP32 [batch, beams, vocab]')
+    batch, beams, vocab = logits.shape
+    width = beams if width is None else int(width)
+    if beams == 0 or vocab == 0 or not 1 <= width <= beams * vocab:
+        raise ValueError('beam_select needs beams, a vocabulary and a width of 1 to beams * vocab')
+    if beams > BEAM_MAX or width > BEAM_MAX:
+        raise NotImplementedError(f'beam_select takes at most {BEAM_MAX} beams')
+    if scores.shape != (batch, beams) or scores.dtype != torch.float32:
+        raise ValueError('scores must be FP32 [batch, beams]')
+    if finished is not None and (finished.shape != (batch, beams) or finished.dtype != torch.bool or eos is None):
+        raise ValueError('finished must be bool [batch, beams] and needs eos')
+    if eos is not None and not 0 <= eos < vocab:
+        raise ValueError('eos must be a token of the vocabulary')
+    if lengths is not None and (lengths.shape != (batch, beams) or lengths.dtype != torch.int32):
+        raise ValueError('lengths must be int32 [batch, beams]')
+    if length_penalty and lengths is None:
+        raise ValueError('length_penalty needs lengths')
+    device = _require_gpu(logits, scores, finished, lengths)
+    if logits.stride(-1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    finished = finished.contiguous() if finished is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    shape = (batch, width)
+    out = BeamSelection(torch.empty(shape, device=device), torch.empty(shape, device=device, dtype=torch.int64),
+                        torch.empty(shape, device=device, dtype=torch.int64),
+                        torch.empty(shape, device=device, dtype=torch.bool) if eos is not None else None,
+                        torch.empty(shape, device=device, dtype=torch.int32) if lengths is not None else None)
+    args = _lib.BeamArgs()
+    args.logits, args.scores = logits.data_ptr(), scores.data_ptr()
+    args.finished, args.lengths = _addr(finished), _addr(lengths)
+    args.out_scores, args.out_tokens, args.out_parents = (t.data_ptr() for t in out[:3])
+    args.out_finished, args.out_lengths = _addr(out.finished), _addr(out.lengths)
+    args.batch, args.batch_stride, args.beam_stride = batch, logits.stride(0), logits.stride(1)
+    args.eos = -1 if eos is None else int(eos)
+    args.length_penalty = float(length_penalty)
+    args.beams, args.vocab, args.width, args.dtype = beams, vocab, width, _dtype_code(logits.dtype)
+    lib = _lib.library()
+    nbytes = lib.bdm_beam_select_workspace_size(ctypes.byref(args))
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    with _on(device):
+        _lib.check(lib.bdm_beam_select(ctypes.byref(args), _addr(workspace), nbytes, _stream(device)),
+                   'bdm_beam_select')
+    return out
+
+
+def reorder_states(states, parents: Tensor, *, beams: int) -> None:
+    """Puts the caches of beams in the order of their parents, in place:
+    ``state[i] = state[parents[i]]`` for each tensor of ``states``.
+
+    states: contiguous tensors [N, ...] of any dtype, N = prompts * beams (the
+    per-layer caches of a model, for instance); parents: int64, N rows (or
+    [prompts, beams], as ``beam_select`` returns them), each a row of the same
+    prompt's group of ``beams``.  Rows that keep their place are not touched; no
+    second copy of a cache is made."""
+    states = list(states)
+    if not states:
+        return
+    rows = parents.numel()
+    if parents.dtype != torch.int64 or beams < 1 or rows % beams:
+        raise ValueError('parents must be int64, one for each row of whole groups of beams')
+    if beams > BEAM_MAX:
+        raise NotImplementedError(f'reorder_states takes at most {BEAM_MAX} beams')
+    device = _require_gpu(parents, *states)
+    for t in states:
+        if t.ndim < 1 or t.shape[0] != rows or not t.is_contiguous():
+            raise ValueError('states must be contiguous tensors with one row for each parent')
+    spans = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in states)
+    if any(a + size > b for (a, size), (b, _) in zip(spans, spans[1:])):
+        raise ValueError('states must not share memory')
+    if rows == 0:
+        return
+    parents = parents.contiguous()
+    count = len(states)
+    pointers = (ctypes.c_void_p * count)(*(t.data_ptr() for t in states))
+    sizes = (ctypes.c_int64 * count)(*(t.numel() * t.element_size() // rows for t in states))
+    with _on(device):
+        _lib.check(_lib.library().bdm_reorder_states(pointers, sizes, count, parents.data_ptr(), rows // beams, beams,
+                                                     _stream(device)), 'bdm_reorder_states')

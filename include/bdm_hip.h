@@ -602,6 +602,52 @@ typedef struct bdm_adamw_args {
 
 int bdm_adamw_step(const bdm_adamw_args *args, void *stream);
 
+/*
+ * Beam search's selection over beams and vocabulary.  No counterpart in the
+ * reference, which decodes single continuations.
+ *
+ * With x the logits of beam k of a prompt and s its score, candidate (k, t)
+ * has the total s + x_t - log sum exp x; a beam marked in `finished` offers
+ * (eos, s) alone.  The `width` best totals of each prompt are chosen, compared
+ * as total / length^length_penalty (length: the beam's, plus one unless it is
+ * finished), ties to the lower k * vocab + t.  Totals and compared values are
+ * formed in FP64 from FP32 sums of exponentials; within a beam the order is
+ * that of the logits.  A logit of -inf is no candidate; a beam whose
+ * score or sum is not finite (a NaN or +inf logit, no finite logit) has none.
+ * Where a prompt has fewer than `width` candidates the lowest places without
+ * one fill the rest, each with the score -inf.
+ *
+ * logits [batch, beams, vocab] of dtype, the last dimension contiguous,
+ * strides in elements; out_parents are rows of the flattened [batch * beams].
+ * At most 64 beams and a width of at most 64.
+ */
+typedef struct bdm_beam_args {
+    const void *logits;
+    const float *scores;       /* [batch, beams] */
+    const uint8_t *finished;   /* optional: [batch, beams], nonzero: ended */
+    const int32_t *lengths;    /* optional: [batch, beams], needed by length_penalty and out_lengths */
+    float *out_scores;         /* [batch, width] */
+    int64_t *out_tokens, *out_parents;
+    uint8_t *out_finished;     /* optional: the parent's flag, or a token equal to eos */
+    int32_t *out_lengths;      /* optional */
+    int64_t batch, batch_stride, beam_stride, eos; /* eos < 0: none */
+    double length_penalty;
+    int32_t beams, vocab, width, dtype;
+} bdm_beam_args;
+
+size_t bdm_beam_select_workspace_size(const bdm_beam_args *args);
+int bdm_beam_select(const bdm_beam_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * states[i][r] <- states[i][parents[r]] for the batch * beams rows of each of
+ * `count` tensors, in place.  A row of tensor i has row_bytes[i] bytes, rows
+ * follow each other; parents [batch * beams] are rows of the same prompt's
+ * group of `beams` (others are clamped into it).  `states` and `row_bytes` are
+ * host arrays, read before the call returns.  At most 64 beams.
+ */
+int bdm_reorder_states(void *const *states, const int64_t *row_bytes, int32_t count, const int64_t *parents,
+                       int64_t batch, int32_t beams, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
