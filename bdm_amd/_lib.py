@@ -45,6 +45,14 @@ EXPORTED_SYMBOLS = (
     'bdm_beam_select_workspace_size',
     'bdm_beam_select',
     'bdm_reorder_states',
+    'bdm_pages_fork',
+    'bdm_pages_load_workspace_size',
+    'bdm_pages_load',
+    'bdm_pages_dense',
+    'bdm_pages_compact_workspace_size',
+    'bdm_pages_compact',
+    'bdm_pages_decode_workspace_size',
+    'bdm_pages_decode',
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -209,6 +217,15 @@ class BeamArgs(ctypes.Structure):
     ]
 
 
+class Pages(ctypes.Structure):
+    """Mirror of ``bdm_pages``."""
+    _fields_ = [
+        ('pool', _vp), ('table', _vp), ('references', _vp), ('free_bits', _vp), ('status', _vp),
+        ('pages', _i64), ('layers', _i32), ('sequences', _i32), ('banks', _i32),
+        ('heads', _i32), ('bank_size', _i32), ('head_width', _i32), ('dtype', _i32),
+    ]
+
+
 class BDMError(RuntimeError):
     """A call into libbdm_hip returned a non-zero status."""
 
@@ -295,6 +312,23 @@ def library() -> ctypes.CDLL:
     lib.bdm_beam_select.restype = _i32
     lib.bdm_reorder_states.argtypes = [ctypes.POINTER(_vp), ctypes.POINTER(_i64), _i32, _vp, _i64, _i32, _vp]
     lib.bdm_reorder_states.restype = _i32
+    pages, sequences = ctypes.POINTER(Pages), ctypes.POINTER(_i32)
+    lib.bdm_pages_fork.argtypes = [pages, _vp, sequences, _i32, _vp]
+    lib.bdm_pages_fork.restype = _i32
+    lib.bdm_pages_load_workspace_size.argtypes = [pages, _i32]
+    lib.bdm_pages_load_workspace_size.restype = _size_t
+    lib.bdm_pages_load.argtypes = [pages, _i32, sequences, _i32, _i32, _vp, _vp, _size_t, _vp]
+    lib.bdm_pages_load.restype = _i32
+    lib.bdm_pages_dense.argtypes = [pages, _i32, sequences, _i32, _vp, _vp]
+    lib.bdm_pages_dense.restype = _i32
+    lib.bdm_pages_compact_workspace_size.argtypes = [pages]
+    lib.bdm_pages_compact_workspace_size.restype = _size_t
+    lib.bdm_pages_compact.argtypes = [pages, _vp, _size_t, _vp]
+    lib.bdm_pages_compact.restype = _i32
+    lib.bdm_pages_decode_workspace_size.argtypes = [pages, _i32, _i32]
+    lib.bdm_pages_decode_workspace_size.restype = _size_t
+    lib.bdm_pages_decode.argtypes = [pages, _i32, ctypes.POINTER(DecodeArgs), _vp, _size_t, _vp]
+    lib.bdm_pages_decode.restype = _i32
     return lib
 
 

@@ -20,6 +20,7 @@
 
 #include "bdm_common.h"
 #include "epilogue_ops.h"
+#include "pages.h"
 #include "recurrence_ops.h"
 #include "router_ops.h"
 
@@ -66,6 +67,8 @@ struct DecodeParams {
     const T *f_weight;
     T *f_out;
     int f_col, f_width;
+    // paged step (bdm_pages_decode): the state is a pool of pages
+    const int32_t *source, *target, *read_pages;
 };
 
 // SE: the state element type (bf16_t or float, the state_dtype argument);
@@ -76,8 +79,15 @@ struct DecodeParams {
 // rows and every lane its own v, w columns (the controller epilogue's
 // helpers of epilogue_ops.h), so the inputs equal those the separate kernels
 // would have stored, bit for bit.
-template <typename T, typename SE, int S, int CPL, bool VEC, int KMAX, bool KFIX, bool FUSED = false>
+// PAGED: the states are pages of a pool, and a written bank that is shared is
+// read from one page and stored to another (copy on write without a copy).
+// The products with the route weights and the sum of the reads stay in FP32
+// there and y is rounded once; with FP32 controllers that is the dense step
+// bit for bit.
+template <typename T, typename SE, int S, int CPL, bool VEC, int KMAX, bool KFIX, bool FUSED = false,
+          bool PAGED = false>
 __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
+    using R = std::conditional_t<PAGED, float, T>;  // what intermediate values are rounded to
     extern __shared__ float smem[];
     // smem layout: written states [kw][S][span], read values [kr][span]
     float *written = smem;
@@ -254,6 +264,15 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
         }
     }
     if (!has_write) pw = 0.f;
+    int from_page = 0, to_page = -1, read_page = 0;
+    if constexpr (PAGED) {
+        if (p.kw > 0) {
+            const int at = int(seq) * p.kw + (has_write ? slot : 0);
+            from_page = p.source[at];
+            to_page = p.target[at];
+        }
+        if (p.kr > 0) read_page = p.read_pages[int(seq) * p.kr + (has_read ? slot : 0)];
+    }
     // a read of a bank written by the same token is served from the stored
     // post-write value in LDS
     int read_from_write = -1;
@@ -275,9 +294,12 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
     // write loads bank 0, a read served from a same-step write re-reads the
     // write bank's lines, already requested by the write load.
     const bool load_read = has_read && read_from_write < 0;
+    const int64_t page_base = int64_t(head) * p.s_real * p.width + col0;
     {
-        const int64_t wbase = seq_base + my_w * bank_stride;
-        const int64_t rbase = load_read ? seq_base + my_r * bank_stride : wbase;
+        const int64_t wbase = PAGED ? page_base + max(from_page, 0) * bank_stride : seq_base + my_w * bank_stride;
+        const int64_t rbase = !load_read ? wbase
+                              : PAGED    ? page_base + max(read_page, 0) * bank_stride
+                                         : seq_base + my_r * bank_stride;
         const SE *st = static_cast<const SE *>(p.state);
 #pragma unroll
         for (int r = 0; r < S; ++r) {
@@ -286,6 +308,13 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
                 load_row<CPL>(st + rbase + int64_t(r) * p.width, hr[r]);
             }
         }
+    }
+    if constexpr (PAGED) {  // a sequence without pages reads zeros
+#pragma unroll
+        for (int r = 0; r < S; ++r)
+#pragma unroll
+            for (int c = 0; c < CPL; ++c)
+                if (read_page < 0) hr[r][c] = 0.f;
     }
     // thread t < KR ranks read slot t by (bank id, slot)
     if (int(threadIdx.x) < p.kr) {
@@ -304,12 +333,19 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
     // ---- writes (inference.py:21-34 with the write rule of role_bank_kernel.py:40-43)
     if (has_write) {
         WriteRows<S> rows;
-        prepare_write_rows<T, S>(kk, gg, bb, pw, p.routed_decay, rows);
+        prepare_write_rows<R, S>(kk, gg, bb, pw, p.routed_decay, rows);
         float ew[CPL];
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) ew[c] = round_to<T>(wv[c] * pw);
+        for (int c = 0; c < CPL; ++c) ew[c] = round_to<R>(wv[c] * pw);
         apply_write<S, CPL>(hw, rows, ew, vv);
-        const int64_t base = seq_base + my_w * bank_stride;
+        if constexpr (PAGED) {  // and it is not written
+#pragma unroll
+            for (int r = 0; r < S; ++r)
+#pragma unroll
+                for (int c = 0; c < CPL; ++c)
+                    if (from_page < 0) hw[r][c] = 0.f;
+        }
+        const int64_t base = PAGED ? page_base + to_page * bank_stride : seq_base + my_w * bank_stride;
 #pragma unroll
         for (int r = 0; r < S; ++r) {
             if (!VEC && r >= p.s_real) continue;
@@ -317,7 +353,7 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
 #pragma unroll
                 for (int c = 0; c < CPL; ++c) hw[r][c] = round_bf16(hw[r][c]);
             }
-            store_row<CPL>(static_cast<SE *>(p.state) + base + int64_t(r) * p.width, hw[r]);
+            if (!PAGED || to_page >= 0) store_row<CPL>(static_cast<SE *>(p.state) + base + int64_t(r) * p.width, hw[r]);
 #pragma unroll
             for (int c = 0; c < CPL; ++c) written[(slot * S + r) * p.span + lc + c] = hw[r][c];
         }
@@ -335,13 +371,13 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
         }
         float qr[S];
 #pragma unroll
-        for (int r = 0; r < S; ++r) qr[r] = round_to<T>(qq[r] * pr);
+        for (int r = 0; r < S; ++r) qr[r] = round_to<R>(qq[r] * pr);
 #pragma unroll
         for (int c = 0; c < CPL; ++c) {
             float acc = 0.f;
 #pragma unroll
             for (int r = 0; r < S; ++r) acc = fmaf(qr[r], hr[r][c], acc);
-            reads[slot * p.span + lc + c] = round_to<T>(acc * p.scale);
+            reads[slot * p.span + lc + c] = round_to<R>(acc * p.scale);
         }
     }
     __syncthreads();
@@ -355,14 +391,19 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
         float total = 0.f;
 #pragma unroll
         for (int j = 0; j < kMaxSlots; ++j)
-            if (j < p.kr) total = round_to<T>(total + v[j]);
+            if (j < p.kr) total = round_to<R>(total + v[j]);
         out[c] = from_f32<T>(total);
     }
 }
 
-template <typename T, int S, int CPL>
-int launch_decode(const bdm_decode_args &a, hipStream_t stream) {
+template <typename T, int S, int CPL, bool PAGED>
+int launch_decode(const bdm_decode_args &a, const PageTables *tables, hipStream_t stream) {
     DecodeParams<T> p{};
+    if constexpr (PAGED) {
+        p.source = tables->source;
+        p.target = tables->target;
+        p.read_pages = tables->read;
+    }
     p.q = static_cast<const T *>(a.q);
     p.k = static_cast<const T *>(a.k);
     p.b = static_cast<const T *>(a.b);
@@ -413,14 +454,14 @@ int launch_decode(const bdm_decode_args &a, hipStream_t stream) {
                       aligned(a.read_weights, 16) && aligned(a.write_indices, 16) && aligned(a.read_indices, 16);
     if (a.state_dtype == BDM_BF16) {
         if (fast)
-            decode_kernel<T, bf16_t, S, CPL, true, 8, true><<<grid, threads, lds, stream>>>(p);
+            decode_kernel<T, bf16_t, S, CPL, true, 8, true, false, PAGED><<<grid, threads, lds, stream>>>(p);
         else
-            decode_kernel<T, bf16_t, S, CPL, false, kMaxSlots, false><<<grid, threads, lds, stream>>>(p);
+            decode_kernel<T, bf16_t, S, CPL, false, kMaxSlots, false, false, PAGED><<<grid, threads, lds, stream>>>(p);
     } else {
         if (fast)
-            decode_kernel<T, float, S, CPL, true, 8, true><<<grid, threads, lds, stream>>>(p);
+            decode_kernel<T, float, S, CPL, true, 8, true, false, PAGED><<<grid, threads, lds, stream>>>(p);
         else
-            decode_kernel<T, float, S, CPL, false, kMaxSlots, false><<<grid, threads, lds, stream>>>(p);
+            decode_kernel<T, float, S, CPL, false, kMaxSlots, false, false, PAGED><<<grid, threads, lds, stream>>>(p);
     }
     return check_launch("decode_kernel");
 }
@@ -472,30 +513,31 @@ int launch_decode_fused(const bdm_decode_fused_args &a, hipStream_t stream) {
     return check_launch("decode_kernel (fused step)");
 }
 
-template <typename T>
-int dispatch_decode(const bdm_decode_args &a, hipStream_t stream) {
+template <typename T, bool PAGED = false>
+int dispatch_decode(const bdm_decode_args &a, hipStream_t stream, const PageTables *tables = nullptr) {
     if (a.bank_size <= 8) {
         // two columns per lane: 64 lanes per slot, more loads in flight per
         // step (wide heads run as spans of 128 columns)
         if (a.head_width % 2 == 0 && (a.head_width / 2 <= 64 || a.head_width % 128 == 0))
-            return launch_decode<T, 8, 2>(a, stream);
-        if (a.head_width % 4 == 0 && a.head_width / 4 <= 64) return launch_decode<T, 8, 4>(a, stream);
-        if (a.head_width % 8 == 0) return launch_decode<T, 8, 8>(a, stream);
-        return launch_decode<T, 8, 1>(a, stream);
+            return launch_decode<T, 8, 2, PAGED>(a, tables, stream);
+        if (a.head_width % 4 == 0 && a.head_width / 4 <= 64) return launch_decode<T, 8, 4, PAGED>(a, tables, stream);
+        if (a.head_width % 8 == 0) return launch_decode<T, 8, 8, PAGED>(a, tables, stream);
+        return launch_decode<T, 8, 1, PAGED>(a, tables, stream);
     }
     if (a.bank_size <= 16) {
-        if (a.head_width % 4 == 0) return launch_decode<T, 16, 4>(a, stream);
-        return launch_decode<T, 16, 1>(a, stream);
+        if (a.head_width % 4 == 0) return launch_decode<T, 16, 4, PAGED>(a, tables, stream);
+        return launch_decode<T, 16, 1, PAGED>(a, tables, stream);
     }
-    if (a.head_width % 2 == 0) return launch_decode<T, 32, 2>(a, stream);
-    return launch_decode<T, 32, 1>(a, stream);
+    if (a.head_width % 2 == 0) return launch_decode<T, 32, 2, PAGED>(a, tables, stream);
+    return launch_decode<T, 32, 1, PAGED>(a, tables, stream);
 }
 
 }  // namespace
 }  // namespace bdm
 
-extern "C" int bdm_decode(const bdm_decode_args *a, void *stream) {
-    using namespace bdm;
+namespace bdm {
+
+int check_decode(const bdm_decode_args *a) {
     if (!a) return fail(BDM_ERR_INVALID, "decode: null args");
     if (a->batch <= 0 || a->heads <= 0 || a->bank_size <= 0 || a->head_width <= 0 || a->bank_count <= 0 ||
         a->write_banks < 0 || a->read_banks < 0 || a->write_banks + a->read_banks == 0)
@@ -513,6 +555,20 @@ extern "C" int bdm_decode(const bdm_decode_args *a, void *stream) {
     const void *ptrs[] = {a->v, a->w, a->state, a->output};
     for (const void *ptr : ptrs)
         if (!aligned(ptr, 16)) return fail(BDM_ERR_INVALID, "decode: tensors must be 16-byte aligned");
+    return BDM_OK;
+}
+
+int launch_decode_pages(const bdm_decode_args &a, const PageTables &tables, hipStream_t stream) {
+    if (a.ctrl_dtype == BDM_BF16) return dispatch_decode<bf16_t, true>(a, stream, &tables);
+    return dispatch_decode<float, true>(a, stream, &tables);
+}
+
+}  // namespace bdm
+
+extern "C" int bdm_decode(const bdm_decode_args *a, void *stream) {
+    using namespace bdm;
+    const int rc = check_decode(a);
+    if (rc != BDM_OK) return rc;
     hipStream_t s = as_stream(stream);
     if (a->ctrl_dtype == BDM_BF16) return dispatch_decode<bf16_t>(*a, s);
     return dispatch_decode<float>(*a, s);

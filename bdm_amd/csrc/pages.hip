@@ -1,0 +1,639 @@
+// A paged bank cache: the banks of all sequences and layers in pages of one
+// pool, shared between sequences until one of them writes.
+//
+// table[layer][sequence][bank] is the page of a bank (-1: the sequence holds
+// none), references[page] counts its table entries and free_bits has a bit for
+// each page with none.  A page is only ever an entry of one layer and bank.
+// New pages are the lowest-numbered free ones, taken in the order of the
+// requests, and reference counts are integers, so every result is the same
+// from run to run whatever the order of the atomics.
+//
+//   resolve  before a decode step: the pages of the banks that the step reads,
+//            and a page of its own for each bank that it writes and shares
+//   fork     the table rows in the order of the parents
+//   load     dense states into pages, equal banks shared with a base sequence
+//   dense    pages into dense states
+//   compact  the used pages moved to the front of the pool
+#include "bdm_common.h"
+#include "pages.h"
+
+namespace bdm {
+namespace {
+
+constexpr int kMaxSequences = 512;
+constexpr int kMaxSlots = 16;
+constexpr int kBlock = 1024;  // the single workgroup of resolve, assign and compact's plan
+constexpr int kBlockWaves = kBlock / kWave;
+
+struct Pages {
+    char *pool;
+    int32_t *table, *references;
+    unsigned long long *free_bits;
+    int32_t *status;
+    int64_t pages, page_bytes;
+    int layers, sequences, banks;
+};
+
+// A table entry as a page of the pool, or -1.
+__device__ __forceinline__ int checked(const Pages &p, int page) { return uint32_t(page) < uint64_t(p.pages) ? page : -1; }
+
+// One reference less; the last one frees the page.
+__device__ __forceinline__ void drop_reference(const Pages &p, int page) {
+    if (atomicSub(p.references + page, 1) == 1) atomicOr(p.free_bits + page / 64, 1ull << (page % 64));
+}
+
+// Sum of the values of the lower lanes.
+__device__ __forceinline__ int wave_before(int value, int lane) {
+    int sum = value;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int other = __shfl_up(sum, d);
+        if (lane >= d) sum += other;
+    }
+    return sum - value;
+}
+
+// Sum of the values of the lower threads of the workgroup; `all`: of all of them.
+__device__ __forceinline__ int block_before(int value, int *waves, int &all) {
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    const int before = wave_before(value, lane);
+    if (lane == kWave - 1) waves[wave] = before + value;
+    __syncthreads();
+    int lower = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kBlockWaves; ++w) {
+        if (w < wave) lower += waves[w];
+        all += waves[w];
+    }
+    __syncthreads();
+    return lower + before;
+}
+
+// The lowest `need` free pages, ascending, into list, and their bits cleared:
+// returns how many there were.  Called by the whole workgroup, which sees the
+// list behind its next barrier.
+__device__ int take_free(const Pages &p, int need, int32_t *list, int *waves) {
+    const int64_t words = (p.pages + 63) / 64;
+    int found = 0;
+    for (int64_t base = 0; base < words && found < need; base += kBlock) {
+        const int64_t at = base + threadIdx.x;
+        unsigned long long word = at < words ? p.free_bits[at] : 0;
+        const int count = __popcll(word);
+        int all;
+        const int before = found + block_before(count, waves, all);
+        const int take = min(count, need - before);
+        for (int i = 0; i < take; ++i) {
+            list[before + i] = int32_t(at * 64 + __ffsll(word) - 1);
+            word &= word - 1;
+        }
+        if (take > 0) p.free_bits[at] = word;
+        found += all;
+    }
+    return min(found, need);
+}
+
+// ------------------------------------------------------------------ resolve
+// One workgroup for a step's N * KW written and N * KR read banks: a written
+// bank whose page other sequences hold gets a page of its own.  All of the
+// sharers that write take new pages, so the page that they read from is stored
+// to by none of them in this step; where none is left it is free for the next.
+// A chain of dependent loads (bank, table, references, free bits), so it is
+// latency that bounds it.
+constexpr int kTiles = kMaxSequences * kMaxSlots / kBlock;
+
+__global__ __launch_bounds__(kBlock) void resolve_kernel(Pages p, int layer, const int64_t *write, const int64_t *read,
+                                                         int kw, int kr, int32_t *source, int32_t *target,
+                                                         int32_t *read_pages, int32_t *list) {
+    __shared__ int waves[kBlockWaves];
+    __shared__ int counts[kTiles][kBlockWaves];
+    const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
+    int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
+    auto bank_of = [&](const int64_t *index, int at) {
+        const int64_t bank = index[at];
+        return int(bank < 0 ? 0 : bank >= p.banks ? p.banks - 1 : bank);
+    };
+    const int writes = p.sequences * kw, reads = p.sequences * kr;
+    for (int r = thread; r < reads; r += kBlock)
+        read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + bank_of(read, r)]);
+    int page[kTiles], before[kTiles], bank[kTiles], first[kTiles];
+    bool shared[kTiles];
+    int need = 0;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        if (t * kBlock >= writes) break;
+        const int r = t * kBlock + thread;
+        shared[t] = false;
+        page[t] = -1;
+        first[t] = 0;
+        bank[t] = 0;
+        if (r < writes) {
+            const int row = r / kw * kw;
+            bank[t] = bank_of(write, r);
+            first[t] = r;  // the first slot of the token with this bank
+            for (int other = r - 1; other >= row; --other)
+                if (bank_of(write, other) == bank[t]) first[t] = other;
+            page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
+            shared[t] = page[t] >= 0 && first[t] == r && p.references[page[t]] > 1;
+            source[r] = page[t];
+        }
+        const uint64_t mask = __ballot(shared[t]);
+        before[t] = __popcll(mask & ((1ull << lane) - 1));
+        if (lane == 0) counts[t][wave] = __popcll(mask);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        if (t * kBlock >= writes) break;
+#pragma unroll
+        for (int w = 0; w < kBlockWaves; ++w) {
+            if (w == wave) before[t] += need;
+            need += counts[t][w];
+        }
+    }
+    int found = 0;
+    if (need) {
+        found = take_free(p, need, list, waves);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        if (t * kBlock >= writes) break;
+        const int r = t * kBlock + thread;
+        if (r >= writes) continue;
+        int to = page[t];
+        if (shared[t]) {
+            to = -1;
+            if (before[t] < found) {
+                to = list[before[t]];
+                table[int64_t(r / kw) * p.banks + bank[t]] = to;
+                p.references[to] = 1;
+                drop_reference(p, page[t]);
+            } else {
+                atomicOr(p.status, 1);
+            }
+        }
+        if (first[t] == r) target[r] = to;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        if (t * kBlock >= writes) break;
+        const int r = t * kBlock + thread;
+        if (r < writes && first[t] != r) target[r] = target[first[t]];
+    }
+}
+
+// ------------------------------------------------------------------ fork
+struct ReleaseMask {
+    uint64_t bits[kMaxSequences / 64];
+};
+
+// table[:, i] <- table[:, parents[i]].  A workgroup owns `span` banks of a
+// layer and holds their column of all sequences in LDS.  The references of a
+// page change by what each of its rows gains or loses, (children of the row)
+// - 1: no partial sum of these reaches the page's zero before the last, so
+// whoever sees zero frees the page.
+constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
+
+__global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *parents, ReleaseMask released, int span) {
+    __shared__ int tile[kForkInts];
+    __shared__ int parent[kMaxSequences], children[kMaxSequences];
+    const int tiles = (p.banks + span - 1) / span;
+    const int layer = blockIdx.x / tiles;
+    const int bank = blockIdx.x % tiles * span + int(threadIdx.x) % span;
+    for (int i = threadIdx.x; i < p.sequences; i += 256) {
+        int64_t from = parents ? parents[i] : (released.bits[i / 64] >> (i % 64) & 1 ? -1 : i);
+        parent[i] = int(from < 0 ? -1 : from >= p.sequences ? p.sequences - 1 : from);
+        children[i] = 0;
+    }
+    __syncthreads();
+    int moved = 0;
+    for (int i = threadIdx.x; i < p.sequences; i += 256) {
+        moved |= parent[i] != i;
+        if (parent[i] >= 0) atomicAdd(&children[parent[i]], 1);
+    }
+    if (!__syncthreads_or(moved)) return;
+    int32_t *column = p.table + int64_t(layer) * p.sequences * p.banks + bank;
+    const int step = 256 / span;
+    if (bank < p.banks) {
+        for (int i = threadIdx.x / span; i < p.sequences; i += step) {
+            const int page = checked(p, column[int64_t(i) * p.banks]);
+            tile[i * span + int(threadIdx.x) % span] = page;
+            const int change = children[i] - 1;
+            if (page < 0 || change == 0) continue;
+            if (change > 0)
+                atomicAdd(p.references + page, change);
+            else
+                drop_reference(p, page);
+        }
+    }
+    __syncthreads();
+    if (bank >= p.banks) return;
+    for (int i = threadIdx.x / span; i < p.sequences; i += step)
+        if (parent[i] != i)
+            column[int64_t(i) * p.banks] = parent[i] < 0 ? -1 : tile[parent[i] * span + int(threadIdx.x) % span];
+}
+
+// ------------------------------------------------------------------ load and dense
+struct Rows {
+    int16_t at[kMaxSequences];  // sequence of each dense row
+};
+
+__device__ __forceinline__ bool bits_differ(uint4 a, uint4 b) {
+    return ((a.x ^ b.x) | (a.y ^ b.y) | (a.z ^ b.z) | (a.w ^ b.w)) != 0;
+}
+__device__ __forceinline__ bool bits_differ(uint2 a, uint2 b) { return ((a.x ^ b.x) | (a.y ^ b.y)) != 0; }
+__device__ __forceinline__ bool bits_differ(uint32_t a, uint32_t b) { return a != b; }
+
+// Whether a dense bank differs from the base sequence's page of it; the old
+// page is dropped, an equal base page taken.  One workgroup a bank.
+template <typename V>
+__global__ __launch_bounds__(256) void compare_kernel(Pages p, int layer, Rows rows, int base, const char *states,
+                                                      uint8_t *differs) {
+    const int64_t at = blockIdx.x;
+    const int row = int(at / p.banks), bank = int(at % p.banks);
+    int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
+    const int shared = base < 0 ? -1 : checked(p, table[int64_t(base) * p.banks + bank]);
+    const int count = int(p.page_bytes / int64_t(sizeof(V)));
+    int other = shared < 0;
+    if (!other) {
+        const V *x = reinterpret_cast<const V *>(states + at * p.page_bytes);
+        const V *y = reinterpret_cast<const V *>(p.pool + shared * p.page_bytes);
+        auto unequal = [&](int i) { return bits_differ(x[i], y[i]); };
+        // a written bank shows it in its first vectors
+        const int ahead = min(count, int(blockDim.x));
+        other = __syncthreads_or(int(threadIdx.x) < ahead && unequal(threadIdx.x));
+        if (!other && count > ahead) {
+            int found = 0;
+            for (int i = ahead + int(threadIdx.x); i < count; i += blockDim.x) found |= unequal(i);
+            other = __syncthreads_or(found);
+        }
+    }
+    if (threadIdx.x == 0) {
+        int32_t *entry = table + int64_t(rows.at[row]) * p.banks + bank;
+        const int old = checked(p, *entry);
+        if (!other) atomicAdd(p.references + shared, 1);
+        if (old >= 0) drop_reference(p, old);
+        *entry = other ? -1 : shared;
+        differs[at] = uint8_t(other != 0);
+    }
+}
+
+// Pages for the banks that differ, in their order: target[i], or -1.
+__global__ __launch_bounds__(kBlock) void assign_kernel(Pages p, int layer, Rows rows, int64_t banks,
+                                                        const uint8_t *differs, int32_t *target, int32_t *list) {
+    __shared__ int waves[kBlockWaves];
+    constexpr int kEach = 8;
+    auto flags = [&](int64_t first) {
+        uint64_t f = 0;
+        for (int i = 0; i < kEach; ++i)
+            if (first + i < banks && differs[first + i]) f |= 1ull << i;
+        return f;
+    };
+    int need = 0;
+    for (int64_t base = 0; base < banks; base += kBlock * kEach) need += __popcll(flags(base + threadIdx.x * kEach));
+    int all;
+    block_before(need, waves, all);
+    const int found = all ? take_free(p, all, list, waves) : 0;
+    __syncthreads();
+    int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
+    int done = 0;
+    for (int64_t base = 0; base < banks; base += kBlock * kEach) {
+        const int64_t first = base + threadIdx.x * kEach;
+        const uint64_t f = flags(first);
+        int tile;
+        int rank = done + block_before(__popcll(f), waves, tile);
+        done += tile;
+        for (int i = 0; i < kEach && first + i < banks; ++i) {
+            int page = -1;
+            if (f >> i & 1) {
+                if (rank < found) {
+                    page = list[rank];
+                    p.references[page] = 1;
+                    table[int64_t(rows.at[(first + i) / p.banks]) * p.banks + (first + i) % p.banks] = page;
+                } else {
+                    atomicOr(p.status, 1);
+                }
+                ++rank;
+            }
+            target[first + i] = page;
+        }
+    }
+}
+
+template <typename V>
+__device__ __forceinline__ void copy_page(const char *from, char *to, int64_t bytes) {
+    const int count = int(bytes / int64_t(sizeof(V)));
+    const V *x = reinterpret_cast<const V *>(from);
+    V *y = reinterpret_cast<V *>(to);
+    for (int i = threadIdx.x; i < count; i += blockDim.x) y[i] = x[i];
+}
+
+template <typename V>
+__global__ __launch_bounds__(256) void store_kernel(Pages p, const char *states, const int32_t *target) {
+    const int64_t at = blockIdx.x;
+    const int page = target[at];
+    if (page < 0) return;
+    copy_page<V>(states + at * p.page_bytes, p.pool + page * p.page_bytes, p.page_bytes);
+}
+
+template <typename V>
+__global__ __launch_bounds__(256) void dense_kernel(Pages p, int layer, Rows rows, char *states) {
+    const int64_t at = blockIdx.x;
+    const int row = int(at / p.banks), bank = int(at % p.banks);
+    const int page = checked(p, p.table[(int64_t(layer) * p.sequences + rows.at[row]) * p.banks + bank]);
+    char *out = states + at * p.page_bytes;
+    if (page >= 0) {
+        copy_page<V>(p.pool + page * p.page_bytes, out, p.page_bytes);
+    } else {
+        const int count = int(p.page_bytes / int64_t(sizeof(V)));
+        for (int i = threadIdx.x; i < count; i += blockDim.x) reinterpret_cast<V *>(out)[i] = V{};
+    }
+}
+
+// ------------------------------------------------------------------ compact
+struct CompactPlan {
+    int32_t used, moves;
+};
+
+// With U pages in use, the k-th used page at or above U goes to the k-th free
+// page below it: the lists of both, ascending, and where each moved page went.
+__global__ __launch_bounds__(kBlock) void compact_plan_kernel(Pages p, CompactPlan *plan, int32_t *from, int32_t *to,
+                                                              int32_t *moved) {
+    __shared__ int waves[kBlockWaves];
+    const int64_t words = (p.pages + 63) / 64;
+    auto valid = [&](int64_t word) {
+        const int64_t left = p.pages - word * 64;
+        return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+    };
+    auto below = [&](int64_t word, int64_t border) {
+        const int64_t left = border - word * 64;
+        return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+    };
+    int mine = 0;
+    for (int64_t at = threadIdx.x; at < words; at += kBlock) mine += __popcll(~p.free_bits[at] & valid(at));
+    int used;
+    block_before(mine, waves, used);
+    int holes = 0, movers = 0;
+    for (int64_t base = 0; base < words; base += kBlock) {
+        const int64_t at = base + threadIdx.x;
+        const unsigned long long bits = at < words ? p.free_bits[at] : 0;
+        const unsigned long long low = below(at, used);
+        unsigned long long hole = bits & low, mover = ~bits & valid(at) & ~low;
+        int all;
+        int rank = holes + block_before(__popcll(hole), waves, all);
+        holes += all;
+        for (; hole; hole &= hole - 1) to[rank++] = int32_t(at * 64 + __ffsll(hole) - 1);
+        rank = movers + block_before(__popcll(mover), waves, all);
+        movers += all;
+        for (; mover; mover &= mover - 1) from[rank++] = int32_t(at * 64 + __ffsll(mover) - 1);
+        if (at < words) p.free_bits[at] = valid(at) & ~low;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < movers; i += kBlock) moved[from[i]] = to[i];
+    if (threadIdx.x == 0) {
+        plan->used = used;
+        plan->moves = movers;
+    }
+}
+
+template <typename V>
+__global__ __launch_bounds__(256) void compact_kernel(Pages p, const CompactPlan *plan, const int32_t *from,
+                                                      const int32_t *to, const int32_t *moved) {
+    const int moves = plan->moves, used = plan->used;
+    if (!moves) return;
+    for (int i = blockIdx.x; i < moves; i += gridDim.x) {
+        const int a = from[i], b = to[i];
+        copy_page<V>(p.pool + a * p.page_bytes, p.pool + b * p.page_bytes, p.page_bytes);
+        if (threadIdx.x == 0) {
+            p.references[b] = p.references[a];
+            p.references[a] = 0;
+        }
+    }
+    const int64_t entries = int64_t(p.layers) * p.sequences * p.banks;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < entries; i += int64_t(gridDim.x) * 256) {
+        const int page = p.table[i];
+        if (page >= used && page < p.pages) p.table[i] = moved[page];
+    }
+}
+
+// ------------------------------------------------------------------ host side
+int check_pages(const bdm_pages *p, Pages &out) {
+    if (!p) return fail(BDM_ERR_INVALID, "pages: null args");
+    if (p->pages <= 0 || p->layers <= 0 || p->sequences <= 0 || p->banks <= 0 || p->heads <= 0 || p->bank_size <= 0 ||
+        p->head_width <= 0)
+        return fail(BDM_ERR_INVALID, "pages: bad geometry");
+    if (p->dtype != BDM_BF16 && p->dtype != BDM_F32) return fail(BDM_ERR_INVALID, "pages: dtype");
+    if (p->sequences > kMaxSequences)
+        return fail(BDM_ERR_UNSUPPORTED, "pages: more than %d sequences", kMaxSequences);
+    if (p->pages > int64_t(INT32_MAX) - 64) return fail(BDM_ERR_UNSUPPORTED, "pages: more than 2^31 pages");
+    const int64_t elements = int64_t(p->heads) * p->bank_size * p->head_width;
+    if (elements > int64_t(INT32_MAX) / 4) return fail(BDM_ERR_UNSUPPORTED, "pages: page too large");
+    if (int64_t(p->sequences) * p->banks > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "pages: table too large");
+    if (!p->pool || !p->table || !p->references || !p->free_bits || !p->status)
+        return fail(BDM_ERR_INVALID, "pages: null pointer");
+    if (!aligned(p->pool, 16) || !aligned(p->free_bits, 8))
+        return fail(BDM_ERR_INVALID, "pages: the pool must be 16-byte aligned");
+    out.pool = static_cast<char *>(p->pool);
+    out.table = p->table;
+    out.references = p->references;
+    out.free_bits = reinterpret_cast<unsigned long long *>(p->free_bits);
+    out.status = p->status;
+    out.pages = p->pages;
+    out.page_bytes = elements * (p->dtype == BDM_BF16 ? 2 : 4);
+    out.layers = p->layers;
+    out.sequences = p->sequences;
+    out.banks = p->banks;
+    return BDM_OK;
+}
+
+int check_rows(const bdm_pages *p, int layer, const int32_t *sequences, int count, Rows &rows) {
+    if (layer < 0 || layer >= p->layers) return fail(BDM_ERR_INVALID, "pages: layer %d", layer);
+    if (count < 0 || count > p->sequences || (count && !sequences))
+        return fail(BDM_ERR_INVALID, "pages: bad sequence list");
+    bool seen[kMaxSequences] = {};
+    for (int i = 0; i < count; ++i) {
+        if (sequences[i] < 0 || sequences[i] >= p->sequences || seen[sequences[i]])
+            return fail(BDM_ERR_INVALID, "pages: sequence %d out of range or twice in one call", sequences[i]);
+        seen[sequences[i]] = true;
+        rows.at[i] = int16_t(sequences[i]);
+    }
+    return BDM_OK;
+}
+
+// The widest vector that every page of the pool and of `dense` starts on a multiple of.
+template <typename F>
+int with_vector(int64_t page_bytes, const void *dense, F run) {
+    const uintptr_t bits = uintptr_t(page_bytes) | reinterpret_cast<uintptr_t>(dense);
+    if (bits % 16 == 0) return run(uint4{});
+    if (bits % 8 == 0) return run(uint2{});
+    if (bits % 4 == 0) return run(uint32_t{});
+    return run(uint16_t{});
+}
+
+// Threads that a page of `count` vectors keeps busy.
+int page_threads(int64_t count) {
+    const int64_t waves = (count + kWave - 1) / kWave;
+    return int(waves >= 4 ? 256 : waves * kWave);
+}
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace bdm
+
+extern "C" int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, const int32_t *released, int32_t count,
+                              void *stream) {
+    using namespace bdm;
+    Pages p;
+    Rows rows;
+    int rc = check_pages(pages, p);
+    if (rc == BDM_OK) rc = check_rows(pages, 0, released, count, rows);
+    if (rc != BDM_OK) return rc;
+    if (parents && count) return fail(BDM_ERR_INVALID, "pages_fork: parents or a list of released sequences");
+    if (!parents && !count) return BDM_OK;
+    ReleaseMask mask{};
+    for (int i = 0; i < count; ++i) mask.bits[rows.at[i] / 64] |= 1ull << (rows.at[i] % 64);
+    int span = 64;
+    while (span * p.sequences > kForkInts) span /= 2;
+    const int64_t grid = int64_t(p.layers) * ((p.banks + span - 1) / span);
+    if (grid > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "pages_fork: grid too large");
+    fork_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(p, parents, mask, span);
+    return check_launch("fork_kernel");
+}
+
+extern "C" size_t bdm_pages_load_workspace_size(const bdm_pages *pages, int32_t count) {
+    using namespace bdm;
+    if (!pages || count <= 0 || pages->banks <= 0) return 0;
+    const size_t banks = size_t(count) * pages->banks;
+    return round16(banks) + 2 * round16(banks * sizeof(int32_t));
+}
+
+extern "C" int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32_t *sequences, int32_t count,
+                              int32_t base, const void *states, void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace bdm;
+    Pages p;
+    Rows rows;
+    int rc = check_pages(pages, p);
+    if (rc == BDM_OK) rc = check_rows(pages, layer, sequences, count, rows);
+    if (rc != BDM_OK) return rc;
+    if (base >= p.sequences) return fail(BDM_ERR_INVALID, "pages_load: base %d", base);
+    for (int i = 0; i < count; ++i)
+        if (sequences[i] == base) return fail(BDM_ERR_INVALID, "pages_load: the base is loaded itself");
+    if (count == 0) return BDM_OK;
+    const int64_t banks = int64_t(count) * p.banks;
+    if (!states) return fail(BDM_ERR_INVALID, "pages_load: null pointer");
+    if (!aligned(states, pages->dtype == BDM_BF16 ? 2 : 4))
+        return fail(BDM_ERR_INVALID, "pages_load: states not aligned to their type");
+    if (!workspace || workspace_bytes < bdm_pages_load_workspace_size(pages, count))
+        return fail(BDM_ERR_WORKSPACE, "pages_load: workspace of %zu bytes", bdm_pages_load_workspace_size(pages, count));
+    if (!aligned(workspace, 16)) return fail(BDM_ERR_INVALID, "pages_load: workspace must be 16-byte aligned");
+    uint8_t *differs = static_cast<uint8_t *>(workspace);
+    int32_t *target = reinterpret_cast<int32_t *>(differs + round16(banks));
+    int32_t *list = target + round16(banks * sizeof(int32_t)) / sizeof(int32_t);
+    const char *data = static_cast<const char *>(states);
+    hipStream_t s = as_stream(stream);
+    return with_vector(p.page_bytes, states, [&](auto vector) {
+        using V = decltype(vector);
+        const int threads = page_threads(p.page_bytes / int64_t(sizeof(V)));
+        compare_kernel<V><<<unsigned(banks), threads, 0, s>>>(p, layer, rows, base, data, differs);
+        int code = check_launch("compare_kernel");
+        if (code != BDM_OK) return code;
+        assign_kernel<<<1, kBlock, 0, s>>>(p, layer, rows, banks, differs, target, list);
+        code = check_launch("assign_kernel");
+        if (code != BDM_OK) return code;
+        store_kernel<V><<<unsigned(banks), threads, 0, s>>>(p, data, target);
+        return check_launch("store_kernel");
+    });
+}
+
+extern "C" int bdm_pages_dense(const bdm_pages *pages, int32_t layer, const int32_t *sequences, int32_t count,
+                               void *states, void *stream) {
+    using namespace bdm;
+    Pages p;
+    Rows rows;
+    int rc = check_pages(pages, p);
+    if (rc == BDM_OK) rc = check_rows(pages, layer, sequences, count, rows);
+    if (rc != BDM_OK) return rc;
+    if (count == 0) return BDM_OK;
+    if (!states) return fail(BDM_ERR_INVALID, "pages_dense: null pointer");
+    if (!aligned(states, pages->dtype == BDM_BF16 ? 2 : 4))
+        return fail(BDM_ERR_INVALID, "pages_dense: states not aligned to their type");
+    const int64_t banks = int64_t(count) * p.banks;
+    hipStream_t s = as_stream(stream);
+    return with_vector(p.page_bytes, states, [&](auto vector) {
+        using V = decltype(vector);
+        dense_kernel<V><<<unsigned(banks), page_threads(p.page_bytes / int64_t(sizeof(V))), 0, s>>>(
+            p, layer, rows, static_cast<char *>(states));
+        return check_launch("dense_kernel");
+    });
+}
+
+extern "C" size_t bdm_pages_compact_workspace_size(const bdm_pages *pages) {
+    using namespace bdm;
+    if (!pages || pages->pages <= 0) return 0;
+    return 16 + 3 * round16(size_t(pages->pages) * sizeof(int32_t));
+}
+
+extern "C" int bdm_pages_compact(const bdm_pages *pages, void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace bdm;
+    Pages p;
+    const int rc = check_pages(pages, p);
+    if (rc != BDM_OK) return rc;
+    if (!workspace || workspace_bytes < bdm_pages_compact_workspace_size(pages))
+        return fail(BDM_ERR_WORKSPACE, "pages_compact: workspace of %zu bytes", bdm_pages_compact_workspace_size(pages));
+    if (!aligned(workspace, 16)) return fail(BDM_ERR_INVALID, "pages_compact: workspace must be 16-byte aligned");
+    CompactPlan *plan = static_cast<CompactPlan *>(workspace);
+    const size_t each = round16(size_t(p.pages) * sizeof(int32_t)) / sizeof(int32_t);
+    int32_t *from = static_cast<int32_t *>(workspace) + 4, *to = from + each, *moved = to + each;
+    hipStream_t s = as_stream(stream);
+    compact_plan_kernel<<<1, kBlock, 0, s>>>(p, plan, from, to, moved);
+    const int code = check_launch("compact_plan_kernel");
+    if (code != BDM_OK) return code;
+    return with_vector(p.page_bytes, nullptr, [&](auto vector) {
+        using V = decltype(vector);
+        compact_kernel<V><<<2048, 256, 0, s>>>(p, plan, from, to, moved);
+        return check_launch("compact_kernel");
+    });
+}
+
+extern "C" size_t bdm_pages_decode_workspace_size(const bdm_pages *pages, int32_t write_banks, int32_t read_banks) {
+    if (!pages || pages->sequences <= 0 || write_banks < 0 || read_banks < 0) return 0;
+    return size_t(pages->sequences) * (3 * size_t(write_banks) + read_banks) * sizeof(int32_t);
+}
+
+extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm_decode_args *a, void *workspace,
+                                size_t workspace_bytes, void *stream) {
+    using namespace bdm;
+    Pages p;
+    const int rc = check_pages(pages, p);
+    if (rc != BDM_OK) return rc;
+    if (!a) return fail(BDM_ERR_INVALID, "pages_decode: null args");
+    if (layer < 0 || layer >= p.layers) return fail(BDM_ERR_INVALID, "pages_decode: layer %d", layer);
+    if (a->batch != p.sequences || a->bank_count != p.banks || a->heads != pages->heads ||
+        a->bank_size != pages->bank_size || a->head_width != pages->head_width || a->state_dtype != pages->dtype)
+        return fail(BDM_ERR_INVALID, "pages_decode: the step's geometry is not the pages'");
+    if (a->write_banks < 0 || a->read_banks < 0 || a->write_banks + a->read_banks == 0)
+        return fail(BDM_ERR_INVALID, "pages_decode: bad geometry");
+    if (a->write_banks > kMaxSlots || a->read_banks > kMaxSlots)
+        return fail(BDM_ERR_UNSUPPORTED, "pages_decode: more than %d selected banks", kMaxSlots);
+    if ((a->write_banks && !a->write_indices) || (a->read_banks && !a->read_indices))
+        return fail(BDM_ERR_INVALID, "pages_decode: null pointer");
+    const size_t need = bdm_pages_decode_workspace_size(pages, a->write_banks, a->read_banks);
+    if (!workspace || workspace_bytes < need) return fail(BDM_ERR_WORKSPACE, "pages_decode: workspace of %zu bytes", need);
+    if (!aligned(workspace, 16)) return fail(BDM_ERR_INVALID, "pages_decode: workspace must be 16-byte aligned");
+    bdm_decode_args args = *a;
+    args.state = p.pool;
+    const int checked_args = check_decode(&args);
+    if (checked_args != BDM_OK) return checked_args;
+    const int writes = p.sequences * a->write_banks;
+    int32_t *source = static_cast<int32_t *>(workspace), *target = source + writes, *list = target + writes,
+            *read = list + writes;
+    hipStream_t s = as_stream(stream);
+    resolve_kernel<<<1, kBlock, 0, s>>>(p, layer, a->write_indices, a->read_indices, a->write_banks, a->read_banks,
+                                        source, target, read, list);
+    const int code = check_launch("resolve_kernel");
+    if (code != BDM_OK) return code;
+    return launch_decode_pages(args, PageTables{p.pool, source, target, read}, s);
+}

@@ -648,6 +648,58 @@ int bdm_beam_select(const bdm_beam_args *args, void *workspace, size_t workspace
 int bdm_reorder_states(void *const *states, const int64_t *row_bytes, int32_t count, const int64_t *parents,
                        int64_t batch, int32_t beams, void *stream);
 
+/*
+ * A paged bank cache: the banks of every layer and sequence are pages of one
+ * pool, which sequences share until one of them writes.  No counterpart in
+ * the reference, which counts what such a cache would hold (APPENDIX.md:511-584).
+ *
+ * table[layer][sequence][bank] is a bank's page, or -1 (a sequence holds a page
+ * for every bank or none); references[page] counts a page's table entries; bit
+ * page % 64 of free_bits[page / 64] is set where it has none (bits behind the
+ * last page are 0).  A page belongs to one layer and bank.  New pages are the
+ * lowest-numbered free ones in the order of the requests.  Bit 0 of *status is
+ * set where none was left: a bank then keeps no page (load) or its old content
+ * (decode), and nothing else is written.  Entries outside the pool count as -1.
+ * At most 512 sequences.  Calls on one cache must be ordered by the caller.
+ */
+typedef struct bdm_pages {
+    void *pool;                /* [pages, H, S, v] of dtype */
+    int32_t *table;            /* [layers, sequences, banks] */
+    int32_t *references;       /* [pages] */
+    uint64_t *free_bits;       /* [ceil(pages / 64)] */
+    int32_t *status;           /* [1] */
+    int64_t pages;
+    int32_t layers, sequences, banks, heads, bank_size, head_width, dtype;
+} bdm_pages;
+
+/* table[:, i] <- table[:, parents[i]] in every layer, i < sequences; a negative
+ * parent releases sequence i, one behind the last counts as the last.  With
+ * parents NULL the `count` sequences of the host array `released` are released
+ * and the others stay. */
+int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, const int32_t *released, int32_t count,
+                   void *stream);
+/* Dense states [count, banks, H, S, v] become the banks of the sequences of the
+ * host array `sequences` (distinct), in place of what they held.  A bank that
+ * equals sequence `base`'s bit for bit shares its page (base < 0: none). */
+size_t bdm_pages_load_workspace_size(const bdm_pages *pages, int32_t count);
+int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32_t *sequences, int32_t count, int32_t base,
+                   const void *states, void *workspace, size_t workspace_bytes, void *stream);
+/* The banks of the sequences as dense states [count, banks, H, S, v]; zeros where there is no page. */
+int bdm_pages_dense(const bdm_pages *pages, int32_t layer, const int32_t *sequences, int32_t count, void *states,
+                    void *stream);
+/* With U pages in use, the k-th used page at or above U moves to the k-th free
+ * page below it.  Pages from U on keep their content. */
+size_t bdm_pages_compact_workspace_size(const bdm_pages *pages);
+int bdm_pages_compact(const bdm_pages *pages, void *workspace, size_t workspace_bytes, void *stream);
+/* One token for each sequence over its pages: the step of bdm_decode (whose
+ * args.state is not read; batch = sequences, state_dtype = dtype) with every
+ * written bank that other sequences hold too stored to a new page.  The
+ * products with the route weights and the sum of the reads stay in FP32 and y
+ * is rounded once.  A sequence without pages has the output 0. */
+size_t bdm_pages_decode_workspace_size(const bdm_pages *pages, int32_t write_banks, int32_t read_banks);
+int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm_decode_args *args, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,4 +1,4 @@
-"""What beam search's entry points refuse, in Python and at the C ABI, before
+"""What the entry points of beam search and the paged cache refuse, in Python and at the C ABI, before
 anything is launched.  Runs without a GPU."""
 
 import ctypes
@@ -71,12 +71,63 @@ def test_c_entry_points_refuse():
     assert lib.bdm_reorder_states(pointer, size, 1, 4096, 1, 4, None) == -1
 
 
+def test_pages_refuse():
+    from bdm_amd import BankPages
+    sizes = dict(banks=8, heads=1, bank_size=8, head_width=16)
+    for args, options in (((0, 4), sizes), ((4, 0), sizes), ((4, 4), {**sizes, 'layers': 0}), ((4, 4.0), sizes),
+                          ((4, 4), {**sizes, 'dtype': torch.float16}), ((4, 4), {**sizes, 'device': 'cpu'})):
+        with pytest.raises(ValueError):
+            BankPages(*args, **options)
+    pool, table = torch.zeros(4, 1, 8, 16), torch.zeros(1, 2, 8, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        BankPages.over(pool, table, torch.zeros(4, dtype=torch.int32))  # CPU tensors
+
+
+def test_c_pages_refuse():
+    from bdm_amd import _lib
+    lib = _lib.library()
+    pages, ref = _lib.Pages(), None
+    ref = ctypes.byref(pages)
+    assert lib.bdm_pages_fork(None, None, None, 0, None) == -1
+    assert lib.bdm_pages_fork(ref, 4096, None, 0, None) == -1
+    pages.pages, pages.layers, pages.sequences, pages.banks = 64, 2, 4, 8
+    pages.heads, pages.bank_size, pages.head_width, pages.dtype = 1, 8, 16, _lib.BDM_BF16
+    assert lib.bdm_pages_fork(ref, 4096, None, 0, None) == -1 and b'null' in lib.bdm_last_error_string()
+    for name in ('pool', 'table', 'references', 'free_bits', 'status'):
+        setattr(pages, name, 4096)
+    rows = (ctypes.c_int32 * 2)(1, 1)
+    assert lib.bdm_pages_fork(ref, None, rows, 2, None) == -1          # a sequence twice
+    assert lib.bdm_pages_fork(ref, 4096, rows, 1, None) == -1          # parents and a list
+    assert lib.bdm_pages_fork(ref, None, None, 0, None) == 0
+    assert lib.bdm_pages_load(ref, 2, rows, 1, -1, 4096, 4096, 1 << 20, None) == -1   # layer
+    assert lib.bdm_pages_load(ref, 0, rows, 2, -1, 4096, 4096, 1 << 20, None) == -1
+    assert lib.bdm_pages_load(ref, 0, rows, 1, 1, 4096, 4096, 1 << 20, None) == -1    # the base itself
+    assert lib.bdm_pages_load(ref, 0, rows, 1, 4, 4096, 4096, 1 << 20, None) == -1
+    assert lib.bdm_pages_load(ref, 0, rows, 1, 0, None, 4096, 1 << 20, None) == -1
+    assert lib.bdm_pages_load(ref, 0, rows, 1, 0, 4096, 4096, 8, None) == -3
+    assert lib.bdm_pages_load(ref, 0, rows, 0, 0, None, None, 0, None) == 0
+    assert lib.bdm_pages_dense(ref, 0, rows, 2, 4096, None) == -1
+    assert lib.bdm_pages_dense(ref, 0, rows, 1, None, None) == -1
+    assert lib.bdm_pages_compact(ref, None, 0, None) == -3
+    step = _lib.DecodeArgs()
+    assert lib.bdm_pages_decode(ref, 0, None, None, 0, None) == -1
+    assert lib.bdm_pages_decode(ref, 0, ctypes.byref(step), 4096, 1 << 20, None) == -1
+    step.batch, step.heads, step.bank_size, step.head_width, step.bank_count = 4, 1, 8, 16, 8
+    step.write_banks = step.read_banks = 2
+    step.ctrl_dtype = step.state_dtype = _lib.BDM_BF16
+    assert lib.bdm_pages_decode(ref, 0, ctypes.byref(step), 4096, 1 << 20, None) == -1   # null operands
+    step.write_banks = 17
+    assert lib.bdm_pages_decode(ref, 0, ctypes.byref(step), 4096, 1 << 20, None) == -2
+    pages.sequences = 513
+    assert lib.bdm_pages_fork(ref, 4096, None, 0, None) == -2
+
+
 def test_struct_mirrors(tmp_path):
     import os
     import subprocess
     from bdm_amd import _lib
     from conftest import ROOT
-    mirrors = {'bdm_beam_args': _lib.BeamArgs}
+    mirrors = {'bdm_beam_args': _lib.BeamArgs, 'bdm_pages': _lib.Pages}
     lines = [f'printf("%zu\\n", sizeof({s}));' + ''.join(f'printf("%zu\\n", offsetof({s}, {f}));' for f, _ in m._fields_)
              for s, m in mirrors.items()]
     source = tmp_path / 'm.c'
