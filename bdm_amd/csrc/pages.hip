@@ -103,7 +103,7 @@ __device__ int take_free(const Pages &p, int need, int32_t *list, int *waves) {
 constexpr int kTiles = kMaxSequences * kMaxSlots / kBlock;
 
 __global__ __launch_bounds__(kBlock) void resolve_kernel(Pages p, int layer, const int64_t *write, const int64_t *read,
-                                                         int kw, int kr, int32_t *source, int32_t *target,
+                                                         int rows, int kw, int kr, int32_t *source, int32_t *target,
                                                          int32_t *read_pages, int32_t *list) {
     __shared__ int waves[kBlockWaves];
     __shared__ int counts[kTiles][kBlockWaves];
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kBlock) void resolve_kernel(Pages p, int layer, con
         const int64_t bank = index[at];
         return int(bank < 0 ? 0 : bank >= p.banks ? p.banks - 1 : bank);
     };
-    const int writes = p.sequences * kw, reads = p.sequences * kr;
+    const int writes = rows * kw, reads = rows * kr;
     for (int r = thread; r < reads; r += kBlock)
         read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + bank_of(read, r)]);
     int page[kTiles], before[kTiles], bank[kTiles], first[kTiles];
@@ -196,14 +196,16 @@ struct ReleaseMask {
 // whoever sees zero frees the page.
 constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
 
-__global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *parents, ReleaseMask released, int span) {
+__global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *parents, int count, ReleaseMask released,
+                                                   int span) {
     __shared__ int tile[kForkInts];
     __shared__ int parent[kMaxSequences], children[kMaxSequences];
     const int tiles = (p.banks + span - 1) / span;
     const int layer = blockIdx.x / tiles;
     const int bank = blockIdx.x % tiles * span + int(threadIdx.x) % span;
     for (int i = threadIdx.x; i < p.sequences; i += 256) {
-        int64_t from = parents ? parents[i] : (released.bits[i / 64] >> (i % 64) & 1 ? -1 : i);
+        int64_t from = released.bits[i / 64] >> (i % 64) & 1 ? -1 : i;
+        if (parents && i < count) from = parents[i];
         parent[i] = int(from < 0 ? -1 : from >= p.sequences ? p.sequences - 1 : from);
         children[i] = 0;
     }
@@ -489,17 +491,19 @@ extern "C" int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, co
     Pages p;
     Rows rows;
     int rc = check_pages(pages, p);
-    if (rc == BDM_OK) rc = check_rows(pages, 0, released, count, rows);
     if (rc != BDM_OK) return rc;
-    if (parents && count) return fail(BDM_ERR_INVALID, "pages_fork: parents or a list of released sequences");
-    if (!parents && !count) return BDM_OK;
+    if (parents && released) return fail(BDM_ERR_INVALID, "pages_fork: parents or a list of released sequences");
+    if (count < 0 || count > p.sequences) return fail(BDM_ERR_INVALID, "pages_fork: %d of %d sequences", count, p.sequences);
+    if (count == 0) return BDM_OK;
+    if (!parents) rc = check_rows(pages, 0, released, count, rows);
+    if (rc != BDM_OK) return rc;
     ReleaseMask mask{};
-    for (int i = 0; i < count; ++i) mask.bits[rows.at[i] / 64] |= 1ull << (rows.at[i] % 64);
+    for (int i = 0; !parents && i < count; ++i) mask.bits[rows.at[i] / 64] |= 1ull << (rows.at[i] % 64);
     int span = 64;
     while (span * p.sequences > kForkInts) span /= 2;
     const int64_t grid = int64_t(p.layers) * ((p.banks + span - 1) / span);
     if (grid > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "pages_fork: grid too large");
-    fork_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(p, parents, mask, span);
+    fork_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(p, parents, count, mask, span);
     return check_launch("fork_kernel");
 }
 
@@ -611,7 +615,7 @@ extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm
     if (rc != BDM_OK) return rc;
     if (!a) return fail(BDM_ERR_INVALID, "pages_decode: null args");
     if (layer < 0 || layer >= p.layers) return fail(BDM_ERR_INVALID, "pages_decode: layer %d", layer);
-    if (a->batch != p.sequences || a->bank_count != p.banks || a->heads != pages->heads ||
+    if (a->batch < 0 || a->batch > p.sequences || a->bank_count != p.banks || a->heads != pages->heads ||
         a->bank_size != pages->bank_size || a->head_width != pages->head_width || a->state_dtype != pages->dtype)
         return fail(BDM_ERR_INVALID, "pages_decode: the step's geometry is not the pages'");
     if (a->write_banks < 0 || a->read_banks < 0 || a->write_banks + a->read_banks == 0)
@@ -620,6 +624,7 @@ extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm
         return fail(BDM_ERR_UNSUPPORTED, "pages_decode: more than %d selected banks", kMaxSlots);
     if ((a->write_banks && !a->write_indices) || (a->read_banks && !a->read_indices))
         return fail(BDM_ERR_INVALID, "pages_decode: null pointer");
+    if (a->batch == 0) return BDM_OK;
     const size_t need = bdm_pages_decode_workspace_size(pages, a->write_banks, a->read_banks);
     if (!workspace || workspace_bytes < need) return fail(BDM_ERR_WORKSPACE, "pages_decode: workspace of %zu bytes", need);
     if (!aligned(workspace, 16)) return fail(BDM_ERR_INVALID, "pages_decode: workspace must be 16-byte aligned");
@@ -627,12 +632,12 @@ extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm
     args.state = p.pool;
     const int checked_args = check_decode(&args);
     if (checked_args != BDM_OK) return checked_args;
-    const int writes = p.sequences * a->write_banks;
+    const int rows = int(a->batch), writes = rows * a->write_banks;
     int32_t *source = static_cast<int32_t *>(workspace), *target = source + writes, *list = target + writes,
             *read = list + writes;
     hipStream_t s = as_stream(stream);
-    resolve_kernel<<<1, kBlock, 0, s>>>(p, layer, a->write_indices, a->read_indices, a->write_banks, a->read_banks,
-                                        source, target, read, list);
+    resolve_kernel<<<1, kBlock, 0, s>>>(p, layer, a->write_indices, a->read_indices, rows, a->write_banks,
+                                        a->read_banks, source, target, read, list);
     const int code = check_launch("resolve_kernel");
     if (code != BDM_OK) return code;
     return launch_decode_pages(args, PageTables{p.pool, source, target, read}, s);

@@ -29,6 +29,7 @@ from torch import nn
 from . import ops
 from .config import BDMConfig
 from .model import BankedDeltaMemory
+from .pages import BankPages
 
 Tensor = torch.Tensor
 
@@ -272,6 +273,49 @@ class BDMLanguageModel(nn.Module):
             raise ValueError('step needs the caches returned by prefill')
         return self._run(tokens, list(caches), decode=True)
 
+    # -- the paged cache ---------------------------------------------------------------
+    def create_pages(self, sequences: int, pages: int, *, dtype=torch.bfloat16) -> BankPages:
+        """A paged cache (``BankPages``) of the model's layers."""
+        memory = self.config.memory
+        return BankPages(sequences, pages, layers=len(self.layers), banks=memory.bank_count, heads=memory.num_heads,
+                         bank_size=memory.bank_size, head_width=memory.head_value_width, dtype=dtype,
+                         device=self.output.weight.device)
+
+    def load_initial(self, pages: BankPages, sequence: int) -> None:
+        """``sequence`` takes the layers' initial states: the base with which
+        ``prefill_pages`` shares the banks that its prompts do not write."""
+        with torch.no_grad():
+            for i, block in enumerate(self.layers):
+                pages.load(i, [sequence], block.attention.create_state(1, dtype=pages.dtype))
+
+    def prefill_pages(self, tokens: Tensor, pages: BankPages, sequences, *, base: int | None = None) -> Tensor:
+        """``prefill`` of new prompts [B, T] into the pages of ``sequences``: the
+        logits of the last position [B, 1, vocab].  Banks that equal the
+        ``base`` sequence's share its pages.  One layer's dense cache exists at a
+        time."""
+        if torch.is_grad_enabled():
+            raise RuntimeError('Stateful inference requires no_grad or inference_mode')
+        sequences = list(sequences)
+        if len(sequences) != tokens.shape[0]:
+            raise ValueError('one sequence per prompt is required')
+
+        def run(i, normed):
+            out, state = self.layers[i].attention.prefill(normed, state_dtype=pages.dtype)
+            pages.load(i, sequences, state, base=base)
+            return out
+
+        return self._run_blocks(self.tok_embeddings(tokens), run)
+
+    def step_pages(self, tokens: Tensor, pages: BankPages) -> Tensor:
+        """``step`` over a paged cache: [N, 1] tokens of its first N sequences,
+        whose pages advance in place; returns the logits [N, 1, vocab]."""
+        if torch.is_grad_enabled():
+            raise RuntimeError('Stateful inference requires no_grad or inference_mode')
+        if tokens.ndim != 2 or tokens.shape[1] != 1:
+            raise ValueError('step takes [batch, 1] tokens')
+        return self._run_blocks(self.tok_embeddings(tokens),
+                                lambda i, normed: self.layers[i].attention.step_pages(normed, pages, i))
+
     def _fused_decode_supported(self, hidden: Tensor) -> bool:
         ffn = self.layers[0].feed_forward
         return (hidden.shape[0] <= ops.GEMV_MAX_ROWS and ffn.hidden_dim % 8 == 0 and self.dim % 8 == 0
@@ -308,14 +352,24 @@ class BDMLanguageModel(nn.Module):
         hidden = self.tok_embeddings(tokens)
         if decode and self._fused_decode_supported(hidden):
             return self._decode_fused(hidden, caches)
+
+        def run(i, normed):
+            attention = self.layers[i].attention
+            out, caches[i] = (attention.step if decode else attention.prefill)(normed, caches[i])
+            return out
+
+        return self._run_blocks(hidden, run), caches
+
+    def _run_blocks(self, hidden: Tensor, run) -> Tensor:
+        """Every block without autograd, ``run(i, normed)`` being layer i's memory
+        sublayer: the logits of the last position."""
         normed = self.layers[0].attention_norm(hidden)
         for i, block in enumerate(self.layers):
-            run = block.attention.step if decode else block.attention.prefill
-            out, caches[i] = run(normed, caches[i])
+            out = run(i, normed)
             hidden, normed = block.ffn_norm.add_norm(out, hidden)
             after = self.layers[i + 1].attention_norm if i + 1 < len(self.layers) else self.norm
             hidden, normed = after.add_norm(block.feed_forward(normed), hidden)
-        return ops.linear(normed[:, -1:], self.output.weight), caches
+        return ops.linear(normed[:, -1:], self.output.weight)
 
 
 BSDMLanguageModel = BDMLanguageModel

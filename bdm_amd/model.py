@@ -610,6 +610,23 @@ class BankedDeltaMemory(nn.Module):
         raw = self._decode_banks((q, k, v, g, b, w), (read_routes, write_routes), hidden.shape[0], state)
         return self._inference_output(hidden, gate, raw.unsqueeze(1)), state
 
+    def step_pages(self, hidden: Tensor, pages, layer: int) -> Tensor:
+        """``step`` over a paged cache (``BankPages``): one token [N, 1, dim] for
+        each of the first N sequences, whose pages of ``layer`` advance in place.
+        Returns the output alone."""
+        self._validate_stateful(hidden, None)
+        if torch.is_grad_enabled() or hidden.shape[1] != 1:
+            raise ValueError('step requires one token under no_grad/inference_mode')
+        if (pages.banks, pages.heads, pages.bank_size, pages.head_width) != (
+                self.bank_count, self.num_heads, self.bank_size, self.head_value_width):
+            raise ValueError("the pages' geometry is not the layer's")
+        controllers, (read_routes, write_routes), gate = self._inference_inputs(hidden)
+        (ww, wi), (rw, ri) = self._route_both(write_routes, read_routes)
+        q, k, v, g, b, w = (t[:, 0] for t in controllers)
+        raw = pages.decode(layer, q, k, v, g, b, w, wi[:, 0], ww[:, 0], ri[:, 0], rw[:, 0],
+                           scale=self.bank_size ** -0.5, routed_decay=self.config.routed_decay)
+        return self._inference_output(hidden, gate, raw.unsqueeze(1))
+
     def _decode_fused(self, proj: Tensor, state: Tensor) -> Tensor | None:
         """The step's controller epilogue, routes and decode kernel in one
         launch from the fused projection ``proj`` [B, P]: the bank reads [B, V],

@@ -155,14 +155,15 @@ class BankPages:
 
     def fork(self, parents: Tensor) -> None:
         """Sequence i continues sequence ``parents[i]``, in every layer: int64,
-        one entry for each sequence.  A negative entry releases the sequence's
-        pages.  Tables and reference counts change, no page is copied."""
-        if parents.dtype != torch.int64 or parents.numel() != self.sequences:
-            raise ValueError(f'parents must be int64, one for each of {self.sequences} sequences')
+        entries for the first sequences (the others stay).  A negative entry
+        releases the sequence's pages.  Tables and reference counts change, no
+        page is copied."""
+        if parents.dtype != torch.int64 or not 1 <= parents.numel() <= self.sequences:
+            raise ValueError(f'parents must be int64, for 1 to {self.sequences} sequences')
         if ops._require_gpu(parents) != self.device:
             raise ValueError('all tensors must be on the same device')
         parents = parents.contiguous()
-        self._call('bdm_pages_fork', parents.data_ptr(), None, 0)
+        self._call('bdm_pages_fork', parents.data_ptr(), None, parents.numel())
 
     def release(self, sequences) -> None:
         """Drops the pages of ``sequences`` (Python ints) in every layer."""
@@ -178,16 +179,17 @@ class BankPages:
 
     # -- the decode step ----------------------------------------------------------------
     def decode(self, layer: int, q, k, v, g, b, w, wi, ww, ri, rw, *, scale: float, routed_decay: bool) -> Tensor:
-        """One token for every sequence over its pages of ``layer``: the step of
-        ``ops.decode_step``, q, k, g, b [N, H, S], v, w [N, H, v], wi, ww [N, KW],
-        ri, rw [N, KR] for all N sequences of the cache.  Returns y [N, H*v].  A
-        bank that is written while other sequences hold its page too moves to a
+        """One token for each of the first N sequences over its pages of ``layer``:
+        the step of ``ops.decode_step``, q, k, g, b [N, H, S], v, w [N, H, v], wi,
+        ww [N, KW], ri, rw [N, KR].  Returns y [N, H*v].  A bank that is written while other sequences hold its page too moves to a
         new page.  Products with the route weights and the sum over the read
         banks are FP32 here and y is rounded once: with FP32 controllers the
         result is ``decode_step``'s bit for bit, with BF16 ones it is nearer to
         the exact one.  Sequences without pages give 0 and stay without."""
         layer = self._layer(layer)
-        n, heads, s, width = self.sequences, self.heads, self.bank_size, self.head_width
+        n, heads, s, width = q.shape[0] if q.ndim else 0, self.heads, self.bank_size, self.head_width
+        if not 1 <= n <= self.sequences:
+            raise ValueError(f'decode takes 1 to {self.sequences} sequences')
         if any(tuple(t.shape) != (n, heads, s) for t in (q, k, g, b)) or any(
                 tuple(t.shape) != (n, heads, width) for t in (v, w)):
             raise ValueError(f'q, k, g, b must be {(n, heads, s)} and v, w {(n, heads, width)}')

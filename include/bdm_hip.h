@@ -672,10 +672,10 @@ typedef struct bdm_pages {
     int32_t layers, sequences, banks, heads, bank_size, head_width, dtype;
 } bdm_pages;
 
-/* table[:, i] <- table[:, parents[i]] in every layer, i < sequences; a negative
- * parent releases sequence i, one behind the last counts as the last.  With
- * parents NULL the `count` sequences of the host array `released` are released
- * and the others stay. */
+/* table[:, i] <- table[:, parents[i]] in every layer, i < count <= sequences,
+ * parents on the device; a negative parent releases sequence i, one behind the
+ * last sequence counts as the last.  With parents NULL the `count` sequences of
+ * the host array `released` are released.  The other sequences stay. */
 int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, const int32_t *released, int32_t count,
                    void *stream);
 /* Dense states [count, banks, H, S, v] become the banks of the sequences of the
@@ -691,8 +691,8 @@ int bdm_pages_dense(const bdm_pages *pages, int32_t layer, const int32_t *sequen
  * page below it.  Pages from U on keep their content. */
 size_t bdm_pages_compact_workspace_size(const bdm_pages *pages);
 int bdm_pages_compact(const bdm_pages *pages, void *workspace, size_t workspace_bytes, void *stream);
-/* One token for each sequence over its pages: the step of bdm_decode (whose
- * args.state is not read; batch = sequences, state_dtype = dtype) with every
+/* One token for each of the first args.batch sequences over its pages: the step
+ * of bdm_decode (args.state is not read, state_dtype = dtype) with every
  * written bank that other sequences hold too stored to a new page.  The
  * products with the route weights and the sum of the reads stay in FP32 and y
  * is rounded once.  A sequence without pages has the output 0. */

@@ -92,12 +92,13 @@ def test_c_pages_refuse():
     assert lib.bdm_pages_fork(ref, 4096, None, 0, None) == -1
     pages.pages, pages.layers, pages.sequences, pages.banks = 64, 2, 4, 8
     pages.heads, pages.bank_size, pages.head_width, pages.dtype = 1, 8, 16, _lib.BDM_BF16
-    assert lib.bdm_pages_fork(ref, 4096, None, 0, None) == -1 and b'null' in lib.bdm_last_error_string()
+    assert lib.bdm_pages_fork(ref, 4096, None, 4, None) == -1 and b'null' in lib.bdm_last_error_string()
     for name in ('pool', 'table', 'references', 'free_bits', 'status'):
         setattr(pages, name, 4096)
     rows = (ctypes.c_int32 * 2)(1, 1)
     assert lib.bdm_pages_fork(ref, None, rows, 2, None) == -1          # a sequence twice
     assert lib.bdm_pages_fork(ref, 4096, rows, 1, None) == -1          # parents and a list
+    assert lib.bdm_pages_fork(ref, 4096, None, 5, None) == -1          # more than the sequences
     assert lib.bdm_pages_fork(ref, None, None, 0, None) == 0
     assert lib.bdm_pages_load(ref, 2, rows, 1, -1, 4096, 4096, 1 << 20, None) == -1   # layer
     assert lib.bdm_pages_load(ref, 0, rows, 2, -1, 4096, 4096, 1 << 20, None) == -1

@@ -1,0 +1,174 @@
+"""Beam search over the language model: the step, the selection, the dense and
+the paged caches together, against a search that keeps its books on the CPU."""
+
+import pytest
+import torch
+
+from test_gpu_beam import reference
+
+pytestmark = pytest.mark.gpu
+
+
+def build(device, dtype, *, heads=2, banks=64, vocab=61, layers=2, dim=64, defaults='bsdm'):
+    from bdm_amd import BDMConfig, BSDMConfig
+    from bdm_amd.lm import BDMLanguageModel, LanguageModelConfig
+    memory = (BSDMConfig if defaults == 'bsdm' else BDMConfig)(
+        dim=dim, bank_count=banks, bank_size=8, selected_banks=4, value_width=dim, num_heads=heads)
+    model = BDMLanguageModel(LanguageModelConfig(memory=memory, vocab_size=vocab, layers=layers, ffn_multiple_of=32,
+                                                 seed=3)).to(device=device, dtype=dtype)
+    with torch.no_grad():
+        model.output.weight.mul_(4)  # logits spread enough that the search has something to choose
+    return model
+
+
+def plain_search(model, prompt, beams, length, eos, penalty):
+    """The same search with whole sequences, index copies of the caches and a
+    selection in 64 bits on the CPU."""
+    batch = prompt.shape[0]
+    with torch.no_grad():
+        logits, caches = model.prefill(prompt)
+        scores = torch.zeros(batch, 1, device=prompt.device)
+        finished = torch.zeros(batch, 1, dtype=torch.bool, device=prompt.device)
+        lengths = torch.zeros(batch, 1, dtype=torch.int32, device=prompt.device)
+        history = [[[] for _ in range(1)] for _ in range(batch)]
+        for t in range(length):
+            vocab = logits.shape[-1]
+            x = logits.view(batch, -1, vocab)
+            flags = finished if eos is not None else None
+            total, compared = reference(x, scores, beams, flags, eos, lengths, penalty)
+            place = compared.sort(dim=-1, descending=True, stable=True).indices[:, :beams]
+            parent, token = place // vocab, place % vocab
+            scores = total.gather(1, place).float().to(prompt.device)
+            history = [[history[b][p] + [k] for p, k in zip(parent[b].tolist(), token[b].tolist())] for b in range(batch)]
+            ended = finished.cpu().gather(1, parent)
+            lengths = (lengths.cpu().gather(1, parent) + (~ended).int()).to(prompt.device)
+            finished = (ended | (token == eos)).to(prompt.device) if eos is not None else ended.to(prompt.device)
+            rows = (torch.arange(batch)[:, None] * x.shape[1] + parent).flatten().to(prompt.device)
+            caches = [c.index_select(0, rows) for c in caches]
+            logits, caches = model.step(token.view(-1, 1).to(prompt.device), caches)
+    return torch.tensor(history), scores, lengths
+
+
+@pytest.mark.parametrize('heads,defaults', [(1, 'bsdm'), (2, 'bdm')])
+@pytest.mark.parametrize('penalty', [0.0, 0.8])
+def test_search(device, heads, defaults, penalty):
+    from bdm_amd import beam_search
+    print('CASE beam search', heads, defaults, penalty, flush=True)
+    model = build(device, torch.float32, heads=heads, defaults=defaults)
+    gen = torch.Generator().manual_seed(heads)
+    prompt = torch.randint(0, 61, (2, 9), generator=gen).to(device)
+    beams, length = 5, 21
+    tokens, scores, lengths = plain_search(model, prompt, beams, length, None, penalty)
+    got = beam_search(model, prompt, beams=beams, length=length, length_penalty=penalty)
+    assert torch.equal(got.tokens.cpu(), tokens)
+    # each score is a sum of `length` FP32 steps of at most the magnitude of the last
+    assert ((got.scores - scores).abs() <= length * 2.0 ** -20 * scores.abs()).all()
+    assert (got.lengths == length).all()
+    eos = int(tokens[0, 0, length // 2])      # a token that the search takes
+    tokens, scores, lengths = plain_search(model, prompt, beams, length, eos, penalty)
+    want = beam_search(model, prompt, beams=beams, length=length, eos=eos, length_penalty=penalty)
+    assert torch.equal(want.tokens.cpu(), tokens)
+    assert torch.equal(want.lengths, lengths) and (lengths < length).any()
+    for options in (dict(paged=True), dict(graph=True), dict(paged=True, graph=True)):
+        print('CASE', options, flush=True)
+        other = beam_search(model, prompt, beams=beams, length=length, eos=eos, length_penalty=penalty, **options)
+        torch.cuda.synchronize()
+        for a, b in zip(want, other):
+            assert torch.equal(a, b), options
+
+
+def test_search_ends_early_and_takes_one_token(device):
+    from bdm_amd import beam_search
+    model = build(device, torch.float32)
+    prompt = torch.randint(0, 61, (1, 5), generator=torch.Generator().manual_seed(4)).to(device)
+    one = beam_search(model, prompt, beams=61, length=1)
+    with torch.no_grad():
+        logits = model.prefill(prompt)[0].view(-1).double()
+    want = torch.log_softmax(logits, 0).sort(descending=True)
+    assert torch.equal(one.tokens.flatten(), want.indices)
+    eos = int(want.indices[0])
+    got = beam_search(model, prompt, beams=1, length=40, eos=eos)   # ended by its first token
+    assert (got.tokens == eos).all() and got.lengths.item() == 1
+
+
+def test_pages_of_a_search_suffice(device):
+    from bdm_amd import beam
+    model = build(device, torch.bfloat16, banks=16)
+    prompt = torch.randint(0, 61, (2, 3), generator=torch.Generator().manual_seed(5)).to(device)
+    with torch.no_grad():
+        search = beam._Search(model, prompt, 6, None, 0.0, True, 30)
+        used = int(search.pages.used())
+        # the initial state, and what three tokens a prompt write, shared by the beams
+        assert used <= 2 * (16 + 2 * 12)
+        for _ in range(29):
+            search.step()
+        search.pages.check()
+    table = search.pages.table.cpu()
+    count = torch.bincount(table.flatten(), minlength=search.pages.pages)
+    assert torch.equal(count.int(), search.pages.references.cpu())
+    assert torch.isfinite(search.scores).all() and (search.scores.diff(dim=1) <= 0).all()
+
+
+@pytest.mark.parametrize('graph', [False, True])
+def test_search_bf16(device, graph):
+    """BF16, eight heads of the serving geometry: both caches run, and each
+    continuation's score is what the model gives it."""
+    from bdm_amd import beam_search
+    model = build(device, torch.bfloat16, heads=2, banks=256, vocab=192, dim=256)
+    prompt = torch.randint(0, 192, (2, 17), generator=torch.Generator().manual_seed(6)).to(device)
+    for paged in (False, True):
+        got = beam_search(model, prompt, beams=4, length=12, paged=paged, graph=graph)
+        assert got.tokens.shape == (2, 4, 12) and torch.isfinite(got.scores).all()
+        assert (got.scores.diff(dim=1) <= 0).all()
+        assert len({tuple(x) for x in got.tokens[0].tolist()}) == 4
+
+
+def test_model_steps_over_pages(device):
+    """Prompts into pages and steps over them against the dense caches, FP32."""
+    model = build(device, torch.float32)
+    prompt = torch.randint(0, 61, (6, 7), generator=torch.Generator().manual_seed(7)).to(device)
+    with torch.no_grad():
+        pages = model.create_pages(7, 2 * 7 * 64 + 14, dtype=torch.float32)
+        model.load_initial(pages, 6)
+        logits = model.prefill_pages(prompt, pages, range(6), base=6)
+        dense = []
+        for i, block in enumerate(model.layers):
+            dense.append(pages.dense(i, range(6)))
+        # the dense caches of a prefill hold the same states
+        hidden = model.tok_embeddings(prompt)
+        normed = model.layers[0].attention_norm(hidden)
+        _, state = model.layers[0].attention.prefill(normed, state_dtype=torch.float32)
+        assert torch.equal(state.view_as(dense[0]), dense[0])
+        assert int(pages.used()) < 2 * 7 * 64
+        assert torch.equal(logits, model.prefill(prompt)[0])
+        for t in range(3):
+            tokens = logits.argmax(-1)
+            logits = model.step_pages(tokens, pages)
+            want, dense = model.step(tokens, dense)
+            assert torch.equal(want, logits)
+            for i, d in enumerate(dense):
+                assert torch.equal(d, pages.dense(i, range(6)))
+        pages.check()
+        assert torch.equal(pages.dense(0, [6]), model.layers[0].attention.create_state(1, dtype=torch.float32))
+
+
+def test_search_refuses(device):
+    from bdm_amd import beam_search
+    model = build(device, torch.float32)
+    prompt = torch.zeros(1, 4, dtype=torch.int64, device=device)
+    for tokens, options in ((prompt[0], {}), (prompt.int(), {}), (prompt[:, :0], {}), (prompt.cpu(), {}),
+                            (prompt, dict(beams=0)), (prompt, dict(beams=62)), (prompt, dict(length=0)),
+                            (prompt, dict(eos=61))):
+        with pytest.raises(ValueError):
+            beam_search(model, tokens, **{'beams': 2, 'length': 3, **options})
+    pages = model.create_pages(2, 64)
+    with pytest.raises(RuntimeError):
+        model.step_pages(prompt[:, :1], pages)
+    with torch.no_grad():
+        with pytest.raises(ValueError):
+            model.step_pages(prompt, pages)
+        with pytest.raises(ValueError):
+            model.prefill_pages(prompt, pages, [0, 1])
+        other = build(device, torch.float32, banks=16)
+        with pytest.raises(ValueError):
+            other.step_pages(prompt[:, :1], pages)

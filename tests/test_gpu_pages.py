@@ -484,6 +484,25 @@ def test_graph_of_fork_and_decode(device):
                 cache.load(0, [4], states[:1])
 
 
+def test_the_first_sequences_alone(device):
+    """A step and a fork of fewer sequences leave the others as they were."""
+    pages, book, gen = make(device, n=6, banks=16, layers=1, s=8, width=16, dtype=torch.float32)
+    states = torch.randn(6, 16, 1, 8, 16, generator=gen)
+    pages.load(0, range(6), states.to(device))
+    book.load(0, range(6), states)
+    parents = torch.tensor([5, 0, 2, -1])
+    pages.fork(parents.to(device))
+    book.fork([5, 0, 2, -1, 4, 5])
+    agree(pages, book)
+    before = torch.stack([book.dense(0, i) for i in range(6)])
+    step = token(3, 1, 8, 16, 16, 4, 4, torch.float32, gen, device)
+    y = pages.decode(0, *step, scale=1.0, routed_decay=True)
+    book.write(0, step[6].tolist())
+    agree(pages, book, contents=False)
+    check_step(pages, 0, step, 1.0, True, y, before[:3])
+    assert torch.equal(pages.dense(0, [3, 4, 5]).cpu(), before[3:])
+
+
 def test_on_a_side_stream(device):
     pages, book, gen = make(device, n=4, banks=8, layers=1, s=8, width=16, dtype=torch.float32)
     side = torch.cuda.Stream()
@@ -533,7 +552,8 @@ def test_calls_refuse(device):
     refused(pages.dense, 0, [-1])
     refused(pages.release, [5])
     refused(pages.fork, torch.zeros(3, dtype=torch.int32, device=device))
-    refused(pages.fork, torch.zeros(2, dtype=torch.int64, device=device))
+    refused(pages.fork, torch.zeros(4, dtype=torch.int64, device=device))
+    refused(pages.fork, torch.zeros(0, dtype=torch.int64, device=device))
     refused(pages.fork, torch.zeros(3, dtype=torch.int64))
 
     def changed(i, t):
