@@ -243,11 +243,12 @@ template <typename T, int NV>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     constexpr int VE = Vec<T>::kSize, E = NV * VE + 1;
     __shared__ TeamShared<4> sh;
-    const int64_t row = blockIdx.x / p.splits;
-    const int split = blockIdx.x % p.splits;
+    const uint32_t row = blockIdx.x / uint32_t(p.splits);
+    const int split = int(blockIdx.x % uint32_t(p.splits));
     if (!beam_live(p, row)) return;
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
-    const T *x = static_cast<const T *>(p.logits) + row / p.beams * p.batch_stride + row % p.beams * p.beam_stride;
+    const T *x = static_cast<const T *>(p.logits) + int64_t(row / uint32_t(p.beams)) * p.batch_stride +
+                 int64_t(row % uint32_t(p.beams)) * p.beam_stride;
     const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
     const int vectors = (p.vocab - head) / VE;
     float v[E];
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : first[e / VE] + e % VE); };
     float high, sum;
     const int count = team_scan<4, E>(sh, v, index, p.width, wave, lane, high, sum);
-    const int64_t part = row * p.splits + split;
+    const int64_t part = int64_t(row) * p.splits + split;
     if (threadIdx.x == 0) p.parts[part] = make_float2(high, sum);
     uint64_t *out = p.lists + part * p.width;
     for (int i = threadIdx.x; i < count; i += 256) {
@@ -329,11 +330,19 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
         const double compared = total / sh.norm[beam];
         return isfinite(compared) ? ordered(compared) : 0;
     };
-    uint64_t place = 0;
-    double total = 0;
+    // a thread's first candidates stay in registers between the bound and the list
+    constexpr int kKept = 2;
+    uint64_t kept[kKept], kept_place[kKept], place = 0;
+    double kept_total[kKept], total = 0;
     uint32_t mine = 0;
-    for (int i = thread; i < all; i += THREADS) mine = max(mine, uint32_t(candidate(i, place, total) >> 32));
-    const uint32_t part = nth_of_lanes<32>(mine, p.width);
+#pragma unroll
+    for (int n = 0; n < kKept; ++n) {
+        kept[n] = 0;
+        if (thread + n * THREADS < all) kept[n] = candidate(thread + n * THREADS, kept_place[n], kept_total[n]);
+        mine = max(mine, uint32_t(kept[n] >> 32));
+    }
+    for (int i = thread + kKept * THREADS; i < all; i += THREADS) mine = max(mine, uint32_t(candidate(i, place, total) >> 32));
+    const uint32_t part = nth_of_lanes<24>(mine >> 8, p.width) << 8;
     if (lane == 0) sh.bound[wave] = part;
     if (thread == 0) sh.count = 0;
     __syncthreads();
@@ -348,7 +357,15 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
             sh.total[at] = total;
         }
     };
-    for (int i = thread; i < all; i += THREADS) {
+#pragma unroll
+    for (int n = 0; n < kKept; ++n) {
+        if (kept[n] && uint32_t(kept[n] >> 32) >= bound) {
+            place = kept_place[n];
+            total = kept_total[n];
+            take(kept[n]);
+        }
+    }
+    for (int i = thread + kKept * THREADS; i < all; i += THREADS) {
         const uint64_t key = candidate(i, place, total);
         if (key && uint32_t(key >> 32) >= bound) take(key);
     }
@@ -426,11 +443,15 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
 }
 
 // One workgroup a prompt: the parts of its rows joined.
-__global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
-    __shared__ JoinShared<256> sh;
+constexpr int kJoinThreads = 1024;
+
+__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamParams p) {
+    __shared__ JoinShared<kJoinThreads> sh;
     const int64_t prompt = blockIdx.x;
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
-    for (int beam = wave; beam < p.beams; beam += 4) {
+    const int last = int(threadIdx.x) - (kJoinThreads - kWave);  // the last wave: it has the fewest rows
+    if (last >= 0 && last < p.beams) join_beam(p, sh, prompt * p.beams + last, last);
+    for (int beam = wave; beam < p.beams; beam += kJoinThreads / kWave) {
         const int64_t row = prompt * p.beams + beam;
         if (!beam_live(p, row)) {  // no totals: its lists were not written
             if (lane == 0) sh.log_sum[beam] = NAN;
@@ -449,11 +470,10 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
         for (int d = kWave / 2; d; d >>= 1) sum += __shfl_xor(sum, d);
         if (lane == 0) sh.log_sum[beam] = double(high) + log(sum);
     }
-    if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
     __syncthreads();
     const int per_beam = p.splits * p.width;
     const uint64_t *lists = p.lists + prompt * p.beams * per_beam;
-    join_beams<256>(p, sh, prompt, p.beams * per_beam, [&](int i, int &beam) {
+    join_beams<kJoinThreads>(p, sh, prompt, p.beams * per_beam, [&](int i, int &beam) {
         beam = i / per_beam;
         return lists[i];
     });
@@ -707,7 +727,7 @@ extern "C" int bdm_beam_select(const bdm_beam_args *a, void *workspace, size_t w
     }
     const int scanned = check_launch("beam_scan_kernel");
     if (scanned != BDM_OK) return scanned;
-    beam_join_kernel<<<prompts, 256, 0, s>>>(p);
+    beam_join_kernel<<<prompts, kJoinThreads, 0, s>>>(p);
     return check_launch("beam_join_kernel");
 }
 

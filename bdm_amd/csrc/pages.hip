@@ -43,54 +43,100 @@ __device__ __forceinline__ void drop_reference(const Pages &p, int page) {
 }
 
 // Sum of the values of the lower lanes.
-__device__ __forceinline__ int wave_before(int value, int lane) {
-    int sum = value;
+template <typename N>
+__device__ __forceinline__ N wave_before(N value, int lane) {
+    N sum = value;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
-        const int other = __shfl_up(sum, d);
+        const N other = __shfl_up(sum, d);
         if (lane >= d) sum += other;
     }
     return sum - value;
 }
 
 // Sum of the values of the lower threads of the workgroup; `all`: of all of them.
-__device__ __forceinline__ int block_before(int value, int *waves, int &all) {
+template <int THREADS, typename N>
+__device__ __forceinline__ N block_before(N value, N *waves, N &all) {
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
-    const int before = wave_before(value, lane);
+    const N before = wave_before(value, lane);
     if (lane == kWave - 1) waves[wave] = before + value;
     __syncthreads();
-    int lower = 0;
+    N lower = 0;
     all = 0;
 #pragma unroll
-    for (int w = 0; w < kBlockWaves; ++w) {
-        if (w < wave) lower += waves[w];
-        all += waves[w];
+    for (int w = 0; w < THREADS / kWave; ++w) {
+        const N sum = waves[w];
+        if (w < wave) lower += sum;
+        all += sum;
     }
     __syncthreads();
     return lower + before;
 }
 
+// The pages of the wave's lanes with `free` set, free from now on.  Pages that
+// were taken together are released together, so neighbouring lanes share words
+// of the bits: each run of them is one atomic (64 on one word took 5 us).
+// Called by all lanes of the wave.
+__device__ __forceinline__ void free_pages(const Pages &p, bool free, int page) {
+    if (!__ballot(free)) return;
+    const int lane = int(threadIdx.x) % kWave;
+    const int word = free ? page / 64 : -1 - lane;
+    unsigned long long bits = free ? 1ull << (page % 64) : 0;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int other = __shfl_up(word, d);
+        const unsigned long long more = __shfl_up(bits, d);
+        if (lane >= d && other == word) bits |= more;
+    }
+    const int next = __shfl_down(word, 1);
+    if (free && (lane == kWave - 1 || next != word)) atomicOr(p.free_bits + word, bits);
+}
+
+// store(rank, lane, bit) for every set bit of the wave's words, in order: the
+// wave takes a word at a time, a lane a bit.  `before`: bits of the words ahead.
+template <typename F>
+__device__ __forceinline__ void each_bit(unsigned long long word, int before, F store) {
+    const int lane = int(threadIdx.x) % kWave;
+    for (uint64_t left = __ballot(word != 0); left; left &= left - 1) {
+        const int from = __ffsll(static_cast<unsigned long long>(left)) - 1;
+        const uint64_t low = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(word)), from));
+        const uint64_t bits = low | uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(word >> 32)), from))) << 32;
+        const int first = __builtin_amdgcn_readlane(before, from);
+        if (bits >> lane & 1) store(first + __popcll(bits & ((1ull << lane) - 1)), from, lane);
+    }
+}
+
 // The lowest `need` free pages, ascending, into list, and their bits cleared:
-// returns how many there were.  Called by the whole workgroup, which sees the
-// list behind its next barrier.
-__device__ int take_free(const Pages &p, int need, int32_t *list, int *waves) {
+// returns how many there were.  `word`: this thread's word of the bits, read
+// ahead.  Called by the whole workgroup, which sees the list behind its next
+// barrier.
+template <int THREADS>
+__device__ int take_free(const Pages &p, int need, int32_t *list, int *waves, unsigned long long word) {
     const int64_t words = (p.pages + 63) / 64;
     int found = 0;
-    for (int64_t base = 0; base < words && found < need; base += kBlock) {
+    for (int64_t base = 0; base < words && found < need; base += THREADS) {
         const int64_t at = base + threadIdx.x;
-        unsigned long long word = at < words ? p.free_bits[at] : 0;
-        const int count = __popcll(word);
+        if (base) word = at < words ? p.free_bits[at] : 0;
         int all;
-        const int before = found + block_before(count, waves, all);
-        const int take = min(count, need - before);
-        for (int i = 0; i < take; ++i) {
-            list[before + i] = int32_t(at * 64 + __ffsll(word) - 1);
-            word &= word - 1;
+        const int before = found + block_before<THREADS>(int(__popcll(word)), waves, all);
+        unsigned long long rest = word;
+        if (before < need) {
+            if (before + __popcll(word) <= need) {
+                rest = 0;
+            } else {
+                for (int i = before; i < need; ++i) rest &= rest - 1;
+            }
         }
-        if (take > 0) p.free_bits[at] = word;
+        if (rest != word) p.free_bits[at] = rest;
+        const int64_t first = base + threadIdx.x / kWave * kWave;
+        each_bit(word & ~rest, before, [&](int rank, int from, int bit) { list[rank] = int32_t((first + from) * 64 + bit); });
         found += all;
     }
     return min(found, need);
+}
+
+__device__ __forceinline__ unsigned long long first_free_word(const Pages &p) {
+    return int64_t(threadIdx.x) < (p.pages + 63) / 64 ? p.free_bits[threadIdx.x] : 0;
 }
 
 // ------------------------------------------------------------------ resolve
@@ -100,13 +146,14 @@ __device__ int take_free(const Pages &p, int need, int32_t *list, int *waves) {
 // to by none of them in this step; where none is left it is free for the next.
 // A chain of dependent loads (bank, table, references, free bits), so it is
 // latency that bounds it.
-constexpr int kTiles = kMaxSequences * kMaxSlots / kBlock;
-
-__global__ __launch_bounds__(kBlock) void resolve_kernel(Pages p, int layer, const int64_t *write, const int64_t *read,
-                                                         int rows, int kw, int kr, int32_t *source, int32_t *target,
-                                                         int32_t *read_pages, int32_t *list) {
-    __shared__ int waves[kBlockWaves];
-    __shared__ int counts[kTiles][kBlockWaves];
+template <int THREADS, int TILES>
+__global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, const int64_t *write, const int64_t *read,
+                                                          int rows, int kw, int kr, int32_t *source, int32_t *target,
+                                                          int32_t *read_pages) {
+    constexpr int kWaves = THREADS / kWave;
+    __shared__ int waves[kWaves];
+    __shared__ int counts[TILES][kWaves];
+    __shared__ int32_t list[TILES * THREADS];  // the new pages; then every request's target
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
     auto bank_of = [&](const int64_t *index, int at) {
@@ -114,26 +161,24 @@ __global__ __launch_bounds__(kBlock) void resolve_kernel(Pages p, int layer, con
         return int(bank < 0 ? 0 : bank >= p.banks ? p.banks - 1 : bank);
     };
     const int writes = rows * kw, reads = rows * kr;
-    for (int r = thread; r < reads; r += kBlock)
-        read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + bank_of(read, r)]);
-    int page[kTiles], before[kTiles], bank[kTiles], first[kTiles];
-    bool shared[kTiles];
-    int need = 0;
+    const unsigned long long word = first_free_word(p);  // in flight beside the chain below
+    int page[TILES], before[TILES], bank[TILES], first[TILES];
+    bool shared[TILES];
+    int repeated = 0;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        if (t * kBlock >= writes) break;
-        const int r = t * kBlock + thread;
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread;
         shared[t] = false;
         page[t] = -1;
-        first[t] = 0;
+        first[t] = r;  // the first slot of the token with this bank
         bank[t] = 0;
         if (r < writes) {
             const int row = r / kw * kw;
             bank[t] = bank_of(write, r);
-            first[t] = r;  // the first slot of the token with this bank
+            page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
             for (int other = r - 1; other >= row; --other)
                 if (bank_of(write, other) == bank[t]) first[t] = other;
-            page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
+            repeated |= first[t] != r;
             shared[t] = page[t] >= 0 && first[t] == r && p.references[page[t]] > 1;
             source[r] = page[t];
         }
@@ -141,46 +186,50 @@ __global__ __launch_bounds__(kBlock) void resolve_kernel(Pages p, int layer, con
         before[t] = __popcll(mask & ((1ull << lane) - 1));
         if (lane == 0) counts[t][wave] = __popcll(mask);
     }
-    __syncthreads();
+    for (int r = thread; r < reads; r += THREADS)
+        read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + bank_of(read, r)]);
+    repeated = __syncthreads_or(repeated);
+    int need = 0;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        if (t * kBlock >= writes) break;
+    for (int t = 0; t < TILES; ++t) {
 #pragma unroll
-        for (int w = 0; w < kBlockWaves; ++w) {
+        for (int w = 0; w < kWaves; ++w) {
             if (w == wave) before[t] += need;
             need += counts[t][w];
         }
     }
     int found = 0;
     if (need) {
-        found = take_free(p, need, list, waves);
+        found = take_free<THREADS>(p, need, list, waves, word);
         __syncthreads();
     }
+    int to[TILES];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        if (t * kBlock >= writes) break;
-        const int r = t * kBlock + thread;
-        if (r >= writes) continue;
-        int to = page[t];
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread;
+        to[t] = page[t];
         if (shared[t]) {
-            to = -1;
-            if (before[t] < found) {
-                to = list[before[t]];
-                table[int64_t(r / kw) * p.banks + bank[t]] = to;
-                p.references[to] = 1;
+            to[t] = before[t] < found ? list[before[t]] : -1;
+            if (to[t] >= 0) {
+                table[int64_t(r / kw) * p.banks + bank[t]] = to[t];
+                p.references[to[t]] = 1;
                 drop_reference(p, page[t]);
             } else {
                 atomicOr(p.status, 1);
             }
         }
-        if (first[t] == r) target[r] = to;
+        if (r < writes && first[t] == r) target[r] = to[t];
     }
+    if (!repeated) return;
+    // slots that repeat a bank store where its first slot does
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        if (t * kBlock >= writes) break;
-        const int r = t * kBlock + thread;
-        if (r < writes && first[t] != r) target[r] = target[first[t]];
+    for (int t = 0; t < TILES; ++t) list[t * THREADS + thread] = to[t];
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread;
+        if (r < writes && first[t] != r) target[r] = list[first[t]];
     }
 }
 
@@ -190,51 +239,75 @@ struct ReleaseMask {
 };
 
 // table[:, i] <- table[:, parents[i]].  A workgroup owns `span` banks of a
-// layer and holds their column of all sequences in LDS.  The references of a
-// page change by what each of its rows gains or loses, (children of the row)
-// - 1: no partial sum of these reaches the page's zero before the last, so
-// whoever sees zero frees the page.
+// layer and holds their column of every row that moves, is continued elsewhere
+// or ends in LDS.  The references of a page change by what each of its rows
+// gains or loses, (children of the row) - 1, at least -1: the count is zero
+// behind the page's last row only, so whoever leaves zero frees the page.  A
+// thread has kForkRows loads, then atomics, in flight: one at a time, each a
+// trip to the L2, 64 rows took 13 us.
 constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
+constexpr int kForkRows = 8;
 
 __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *parents, int count, ReleaseMask released,
                                                    int span) {
     __shared__ int tile[kForkInts];
     __shared__ int parent[kMaxSequences], children[kMaxSequences];
+    __shared__ int rows[kMaxSequences], place[kMaxSequences], changed;
     const int tiles = (p.banks + span - 1) / span;
     const int layer = blockIdx.x / tiles;
-    const int bank = blockIdx.x % tiles * span + int(threadIdx.x) % span;
+    const int mine = int(threadIdx.x) % span, bank = blockIdx.x % tiles * span + mine;
     for (int i = threadIdx.x; i < p.sequences; i += 256) {
         int64_t from = released.bits[i / 64] >> (i % 64) & 1 ? -1 : i;
         if (parents && i < count) from = parents[i];
         parent[i] = int(from < 0 ? -1 : from >= p.sequences ? p.sequences - 1 : from);
         children[i] = 0;
     }
+    if (threadIdx.x == 0) changed = 0;
     __syncthreads();
-    int moved = 0;
-    for (int i = threadIdx.x; i < p.sequences; i += 256) {
-        moved |= parent[i] != i;
+    for (int i = threadIdx.x; i < p.sequences; i += 256)
         if (parent[i] >= 0) atomicAdd(&children[parent[i]], 1);
-    }
-    if (!__syncthreads_or(moved)) return;
-    int32_t *column = p.table + int64_t(layer) * p.sequences * p.banks + bank;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.sequences; i += 256)
+        if (children[i] != 1 || parent[i] != i) rows[place[i] = atomicAdd(&changed, 1)] = i;
+    __syncthreads();
+    if (!changed) return;
+    int32_t *column = p.table + int64_t(layer) * p.sequences * p.banks + min(bank, p.banks - 1);
     const int step = 256 / span;
-    if (bank < p.banks) {
-        for (int i = threadIdx.x / span; i < p.sequences; i += step) {
-            const int page = checked(p, column[int64_t(i) * p.banks]);
-            tile[i * span + int(threadIdx.x) % span] = page;
-            const int change = children[i] - 1;
-            if (page < 0 || change == 0) continue;
-            if (change > 0)
-                atomicAdd(p.references + page, change);
-            else
-                drop_reference(p, page);
+    // every lane takes every turn: the lanes of a wave read each other's below
+    for (int turn = 0; turn < changed; turn += step * kForkRows) {
+        const int base = turn + int(threadIdx.x) / span;
+        int page[kForkRows], change[kForkRows], old[kForkRows];
+#pragma unroll
+        for (int u = 0; u < kForkRows; ++u) {
+            const int at = min(base + u * step, changed - 1);
+            page[u] = checked(p, column[int64_t(rows[at]) * p.banks]);
+            change[u] = base + u * step < changed && bank < p.banks ? children[rows[at]] - 1 : 0;
+            tile[at * span + mine] = page[u];
         }
+        // one change for the rows of a thread that hold one page
+#pragma unroll
+        for (int u = 1; u < kForkRows; ++u)
+#pragma unroll
+            for (int w = 0; w < u; ++w)
+                if (page[w] == page[u]) {
+                    change[w] += change[u];
+                    change[u] = 0;
+                }
+#pragma unroll
+        for (int u = 0; u < kForkRows; ++u) {
+            old[u] = 0;
+            if (page[u] >= 0 && change[u] < 0) old[u] = atomicAdd(p.references + page[u], change[u]);
+            if (page[u] >= 0 && change[u] > 0) atomicAdd(p.references + page[u], change[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kForkRows; ++u) free_pages(p, old[u] + change[u] == 0 && change[u] < 0, page[u]);
     }
     __syncthreads();
     if (bank >= p.banks) return;
-    for (int i = threadIdx.x / span; i < p.sequences; i += step)
-        if (parent[i] != i)
-            column[int64_t(i) * p.banks] = parent[i] < 0 ? -1 : tile[parent[i] * span + int(threadIdx.x) % span];
+    for (int at = int(threadIdx.x) / span; at < changed; at += step) {
+        const int i = rows[at], from = parent[i];
+        if (from != i) column[int64_t(i) * p.banks] = from < 0 ? -1 : tile[place[from] * span + mine];
+    }
 }
 
 // ------------------------------------------------------------------ load and dense
@@ -254,9 +327,11 @@ template <typename V>
 __global__ __launch_bounds__(256) void compare_kernel(Pages p, int layer, Rows rows, int base, const char *states,
                                                       uint8_t *differs) {
     const int64_t at = blockIdx.x;
-    const int row = int(at / p.banks), bank = int(at % p.banks);
+    const int row = int(blockIdx.x / uint32_t(p.banks)), bank = int(blockIdx.x % uint32_t(p.banks));
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
+    int32_t *entry = table + int64_t(rows.at[row]) * p.banks + bank;
     const int shared = base < 0 ? -1 : checked(p, table[int64_t(base) * p.banks + bank]);
+    const int old = checked(p, *entry);
     const int count = int(p.page_bytes / int64_t(sizeof(V)));
     int other = shared < 0;
     if (!other) {
@@ -273,8 +348,6 @@ __global__ __launch_bounds__(256) void compare_kernel(Pages p, int layer, Rows r
         }
     }
     if (threadIdx.x == 0) {
-        int32_t *entry = table + int64_t(rows.at[row]) * p.banks + bank;
-        const int old = checked(p, *entry);
         if (!other) atomicAdd(p.references + shared, 1);
         if (old >= 0) drop_reference(p, old);
         *entry = other ? -1 : shared;
@@ -283,37 +356,47 @@ __global__ __launch_bounds__(256) void compare_kernel(Pages p, int layer, Rows r
 }
 
 // Pages for the banks that differ, in their order: target[i], or -1.
+constexpr int kAssignList = 8192;  // new pages kept in LDS, more go to the workspace
+
 __global__ __launch_bounds__(kBlock) void assign_kernel(Pages p, int layer, Rows rows, int64_t banks,
-                                                        const uint8_t *differs, int32_t *target, int32_t *list) {
+                                                        const uint8_t *differs, int32_t *target, int32_t *spill) {
     __shared__ int waves[kBlockWaves];
+    __shared__ int32_t local[kAssignList];
     constexpr int kEach = 8;
-    auto flags = [&](int64_t first) {
-        uint64_t f = 0;
-        for (int i = 0; i < kEach; ++i)
-            if (first + i < banks && differs[first + i]) f |= 1ull << i;
-        return f;
+    const unsigned long long word = first_free_word(p);  // in flight beside the count
+    // the flags, 0 or 1, of 8 banks (the workspace has room behind the last)
+    auto flags = [&](int64_t first) -> uint64_t {
+        if (first >= banks) return 0;
+        const uint64_t f = *reinterpret_cast<const uint64_t *>(differs + first);
+        return first + kEach <= banks ? f : f & ((1ull << 8 * (banks - first)) - 1);
     };
-    int need = 0;
-    for (int64_t base = 0; base < banks; base += kBlock * kEach) need += __popcll(flags(base + threadIdx.x * kEach));
-    int all;
-    block_before(need, waves, all);
-    const int found = all ? take_free(p, all, list, waves) : 0;
+    const uint64_t mine = flags(int64_t(threadIdx.x) * kEach);
+    int count = __popcll(mine);
+    for (int64_t base = kBlock * kEach; base < banks; base += kBlock * kEach)
+        count += __popcll(flags(base + threadIdx.x * kEach));
+    int need;
+    block_before<kBlock>(count, waves, need);
+    int32_t *list = need <= kAssignList ? local : spill;
+    const int found = need ? take_free<kBlock>(p, need, list, waves, word) : 0;
     __syncthreads();
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
     int done = 0;
     for (int64_t base = 0; base < banks; base += kBlock * kEach) {
         const int64_t first = base + threadIdx.x * kEach;
-        const uint64_t f = flags(first);
-        int tile;
-        int rank = done + block_before(__popcll(f), waves, tile);
-        done += tile;
-        for (int i = 0; i < kEach && first + i < banks; ++i) {
+        const uint64_t f = base ? flags(first) : mine;
+        int all;
+        int rank = done + block_before<kBlock>(int(__popcll(f)), waves, all);
+        done += all;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (first + i >= banks) break;
             int page = -1;
-            if (f >> i & 1) {
+            if (f >> 8 * i & 1) {
                 if (rank < found) {
                     page = list[rank];
                     p.references[page] = 1;
-                    table[int64_t(rows.at[(first + i) / p.banks]) * p.banks + (first + i) % p.banks] = page;
+                    const uint32_t row = uint32_t(first + i) / uint32_t(p.banks);
+                    table[int64_t(rows.at[row]) * p.banks + uint32_t(first + i) % uint32_t(p.banks)] = page;
                 } else {
                     atomicOr(p.status, 1);
                 }
@@ -343,7 +426,7 @@ __global__ __launch_bounds__(256) void store_kernel(Pages p, const char *states,
 template <typename V>
 __global__ __launch_bounds__(256) void dense_kernel(Pages p, int layer, Rows rows, char *states) {
     const int64_t at = blockIdx.x;
-    const int row = int(at / p.banks), bank = int(at % p.banks);
+    const int row = int(blockIdx.x / uint32_t(p.banks)), bank = int(blockIdx.x % uint32_t(p.banks));
     const int page = checked(p, p.table[(int64_t(layer) * p.sequences + rows.at[row]) * p.banks + bank]);
     char *out = states + at * p.page_bytes;
     if (page >= 0) {
@@ -363,40 +446,39 @@ struct CompactPlan {
 // page below it: the lists of both, ascending, and where each moved page went.
 __global__ __launch_bounds__(kBlock) void compact_plan_kernel(Pages p, CompactPlan *plan, int32_t *from, int32_t *to,
                                                               int32_t *moved) {
-    __shared__ int waves[kBlockWaves];
+    __shared__ int counts[kBlockWaves];
+    __shared__ uint64_t waves[kBlockWaves];
     const int64_t words = (p.pages + 63) / 64;
-    auto valid = [&](int64_t word) {
-        const int64_t left = p.pages - word * 64;
-        return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
-    };
-    auto below = [&](int64_t word, int64_t border) {
+    // the pages of a word that lie below a border
+    auto below = [](int64_t word, int64_t border) {
         const int64_t left = border - word * 64;
         return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
     };
+    const unsigned long long word = first_free_word(p);
     int mine = 0;
-    for (int64_t at = threadIdx.x; at < words; at += kBlock) mine += __popcll(~p.free_bits[at] & valid(at));
+    for (int64_t at = threadIdx.x; at < words; at += kBlock)
+        mine += __popcll(~(at < kBlock ? word : p.free_bits[at]) & below(at, p.pages));
     int used;
-    block_before(mine, waves, used);
-    int holes = 0, movers = 0;
+    block_before<kBlock>(mine, counts, used);
+    uint64_t done = 0;  // movers in the upper half, holes in the lower
     for (int64_t base = 0; base < words; base += kBlock) {
-        const int64_t at = base + threadIdx.x;
-        const unsigned long long bits = at < words ? p.free_bits[at] : 0;
-        const unsigned long long low = below(at, used);
-        unsigned long long hole = bits & low, mover = ~bits & valid(at) & ~low;
-        int all;
-        int rank = holes + block_before(__popcll(hole), waves, all);
-        holes += all;
-        for (; hole; hole &= hole - 1) to[rank++] = int32_t(at * 64 + __ffsll(hole) - 1);
-        rank = movers + block_before(__popcll(mover), waves, all);
-        movers += all;
-        for (; mover; mover &= mover - 1) from[rank++] = int32_t(at * 64 + __ffsll(mover) - 1);
-        if (at < words) p.free_bits[at] = valid(at) & ~low;
+        const int64_t at = base + threadIdx.x, first = base + threadIdx.x / kWave * kWave;
+        const unsigned long long bits = base == 0 ? word : at < words ? p.free_bits[at] : 0;
+        const unsigned long long low = below(at, used), hole = bits & low, mover = ~bits & below(at, p.pages) & ~low;
+        uint64_t all;
+        const uint64_t rank = done + block_before<kBlock>(uint64_t(__popcll(mover)) << 32 | uint32_t(__popcll(hole)), waves, all);
+        done += all;
+        each_bit(hole, int(uint32_t(rank)), [&](int k, int lane, int bit) { to[k] = int32_t((first + lane) * 64 + bit); });
+        each_bit(mover, int(rank >> 32), [&](int k, int lane, int bit) { from[k] = int32_t((first + lane) * 64 + bit); });
+        const unsigned long long left = below(at, p.pages) & ~low;
+        if (at < words && left != bits) p.free_bits[at] = left;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < movers; i += kBlock) moved[from[i]] = to[i];
+    const int moves = int(done >> 32);
+    for (int i = threadIdx.x; i < moves; i += kBlock) moved[from[i]] = to[i];
     if (threadIdx.x == 0) {
         plan->used = used;
-        plan->moves = movers;
+        plan->moves = moves;
     }
 }
 
@@ -499,8 +581,9 @@ extern "C" int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, co
     if (rc != BDM_OK) return rc;
     ReleaseMask mask{};
     for (int i = 0; !parents && i < count; ++i) mask.bits[rows.at[i] / 64] |= 1ull << (rows.at[i] % 64);
+    // whole lines of a table row where that leaves a few hundred workgroups and a column in one go
     int span = 64;
-    while (span * p.sequences > kForkInts) span /= 2;
+    while (span > 16 && (span * p.sequences > 256 * kForkRows || int64_t(p.layers) * p.banks < 256 * span)) span /= 2;
     const int64_t grid = int64_t(p.layers) * ((p.banks + span - 1) / span);
     if (grid > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "pages_fork: grid too large");
     fork_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(p, parents, count, mask, span);
@@ -604,7 +687,7 @@ extern "C" int bdm_pages_compact(const bdm_pages *pages, void *workspace, size_t
 
 extern "C" size_t bdm_pages_decode_workspace_size(const bdm_pages *pages, int32_t write_banks, int32_t read_banks) {
     if (!pages || pages->sequences <= 0 || write_banks < 0 || read_banks < 0) return 0;
-    return size_t(pages->sequences) * (3 * size_t(write_banks) + read_banks) * sizeof(int32_t);
+    return size_t(pages->sequences) * (2 * size_t(write_banks) + read_banks) * sizeof(int32_t);
 }
 
 extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm_decode_args *a, void *workspace,
@@ -633,11 +716,18 @@ extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm
     const int checked_args = check_decode(&args);
     if (checked_args != BDM_OK) return checked_args;
     const int rows = int(a->batch), writes = rows * a->write_banks;
-    int32_t *source = static_cast<int32_t *>(workspace), *target = source + writes, *list = target + writes,
-            *read = list + writes;
+    int32_t *source = static_cast<int32_t *>(workspace), *target = source + writes, *read = target + writes;
     hipStream_t s = as_stream(stream);
-    resolve_kernel<<<1, kBlock, 0, s>>>(p, layer, a->write_indices, a->read_indices, rows, a->write_banks,
-                                        a->read_banks, source, target, read, list);
+    auto resolve = [&](auto kernel, int threads) {
+        kernel<<<1, threads, 0, s>>>(p, layer, a->write_indices, a->read_indices, rows, a->write_banks, a->read_banks,
+                                     source, target, read);
+    };
+    if (writes <= 256)
+        resolve(resolve_kernel<256, 1>, 256);
+    else if (writes <= kBlock)
+        resolve(resolve_kernel<kBlock, 1>, kBlock);
+    else
+        resolve(resolve_kernel<kBlock, kMaxSequences * kMaxSlots / kBlock>, kBlock);
     const int code = check_launch("resolve_kernel");
     if (code != BDM_OK) return code;
     return launch_decode_pages(args, PageTables{p.pool, source, target, read}, s);

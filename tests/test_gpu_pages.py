@@ -307,6 +307,23 @@ def test_pool_of_many_words(device):
     assert int(cache.table.max()) == int(cache.used()) - 1
 
 
+def test_many_new_pages_at_once(device):
+    pages, book, gen = make(device, n=4, banks=3001, layers=1, s=1, width=4, dtype=torch.float32)
+    first = torch.randn(1, 3001, 1, 1, 4, generator=gen)
+    pages.load(0, [1], first.to(device))
+    states = torch.where(torch.rand(3, 3001, 1, 1, 1, generator=gen) < 0.97, first + 1, first)
+    pages.load(0, [3, 0, 2], states.to(device), base=1)
+    book.load(0, [1], first)
+    book.load(0, [3, 0, 2], states, base=1)
+    agree(pages, book)
+    pages.release([0, 1])
+    book.drop(0, 0)
+    book.drop(0, 1)
+    pages.compact()
+    book.compact()
+    agree(pages, book)
+
+
 def test_offsets_beyond_32_bits(device):
     """Pages behind the first 4 GiB of the pool, and behind 2^31 elements."""
     from bdm_amd import BankPages
