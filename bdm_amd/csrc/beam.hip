@@ -194,6 +194,20 @@ __device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index
     return sh.count;
 }
 
+// The team's candidates in descending order, the first `width` of them to out, 0 behind the last.
+template <int WAVES>
+__device__ __forceinline__ void team_rank(const TeamShared<WAVES> &sh, int count, int width, int wave, int lane,
+                                          uint64_t *out) {
+    for (int i = wave * kWave + lane; i < count; i += WAVES * kWave) {
+        const uint64_t mine = sh.list[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < count; ++j) rank += sh.list[j] > mine;
+        if (rank < width) out[rank] = mine;
+    }
+    for (int i = count + wave * kWave + lane; i < width; i += WAVES * kWave) out[i] = 0;
+}
+
 template <typename T> struct Vec;
 template <> struct Vec<bf16_t> {
     static constexpr int kSize = 8;
@@ -273,13 +287,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     const int64_t part = int64_t(row) * p.splits + split;
     if (threadIdx.x == 0) p.parts[part] = make_float2(high, sum);
     uint64_t *out = p.lists + part * p.width;
-    for (int i = threadIdx.x; i < count; i += 256) {
-        const uint64_t mine = sh.list[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += sh.list[j] > mine;
-        if (rank < p.width) out[rank] = mine;
-    }
-    for (int i = count + int(threadIdx.x); i < p.width; i += 256) out[i] = 0;
+    team_rank<4>(sh, count, p.width, wave, lane, out);
 }
 
 // ------------------------------------------------------------------ joining a prompt's beams
@@ -406,11 +414,16 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
         __syncthreads();
     }
     const int count = sh.count;
-    for (int i = thread; i < count; i += THREADS) {
+    // candidate i's rank, 64 others at a time (one at a time, 56 of them took 5.5 us)
+    for (int i = wave; i < count; i += THREADS / kWave) {
         const uint64_t key = sh.key[i], at = sh.place[i];
         int rank = 0;
-        for (int j = 0; j < count; ++j) rank += sh.key[j] > key || (sh.key[j] == key && sh.place[j] < at);
-        if (rank < p.width) {
+        for (int j = 0; j < count; j += kWave) {
+            const int other = min(j + lane, count - 1);
+            const uint64_t k = sh.key[other], place_of = sh.place[other];
+            rank += popcount(__ballot(j + lane < count && (k > key || (k == key && place_of < at))));
+        }
+        if (lane == 0 && rank < p.width) {
             sh.chosen[rank] = at;
             sh.chosen_total[rank] = sh.total[i];
         }
@@ -473,9 +486,11 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamParams p) {
     __syncthreads();
     const int per_beam = p.splits * p.width;
     const uint64_t *lists = p.lists + prompt * p.beams * per_beam;
+    const uint32_t rows = uint32_t(p.beams * p.splits);  // the lists' best first, so that one wave holds many of the best
     join_beams<kJoinThreads>(p, sh, prompt, p.beams * per_beam, [&](int i, int &beam) {
-        beam = i / per_beam;
-        return lists[i];
+        const uint32_t rank = uint32_t(i) / rows, list = uint32_t(i) % rows;
+        beam = int(list / uint32_t(p.splits));
+        return lists[list * uint32_t(p.width) + rank];
     });
 }
 
@@ -518,21 +533,16 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
         float high, sum;
         const int count = team_scan<1, E>(team, v, index, p.width, 0, lane, high, sum);
         uint64_t *out = lists + beam * p.width;
-        for (int i = lane; i < count; i += kWave) {
-            const uint64_t mine = team.list[i];
-            int rank = 0;
-            for (int j = 0; j < count; ++j) rank += team.list[j] > mine;
-            if (rank < p.width) out[rank] = mine;
-        }
-        for (int i = count + lane; i < p.width; i += kWave) out[i] = 0;
+        team_rank<1>(team, count, p.width, 0, lane, out);
         if (lane == 0) sh.log_sum[beam] = double(high) + log(double(sum));
         team_sync<1>();
     }
     if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
     __syncthreads();
     join_beams<kRowWaves * kWave>(p, sh, prompt, p.beams * p.width, [&](int i, int &beam) {
-        beam = i / p.width;
-        return lists[i];
+        const uint32_t rank = uint32_t(i) / uint32_t(p.beams);
+        beam = int(uint32_t(i) % uint32_t(p.beams));
+        return lists[uint32_t(beam) * uint32_t(p.width) + rank];
     });
 }
 

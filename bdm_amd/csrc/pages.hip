@@ -73,23 +73,32 @@ __device__ __forceinline__ N block_before(N value, N *waves, N &all) {
     return lower + before;
 }
 
-// The pages of the wave's lanes with `free` set, free from now on.  Pages that
-// were taken together are released together, so neighbouring lanes share words
-// of the bits: each run of them is one atomic (64 on one word took 5 us).
-// Called by all lanes of the wave.
+// x of the lane N below in the row of 16 (N < 0: above), `none` where there is no such lane.
+template <int N>
+__device__ __forceinline__ int in_row(int x, int none) {
+    return __builtin_amdgcn_update_dpp(none, x, N > 0 ? 0x110 + N : 0x100 - N, 0xf, 0xf, false);
+}
+
+// The pages of the lanes with `free` set, free from now on.  Pages that were
+// taken together are released together, so neighbouring lanes share words of
+// the bits: a run of them within 16 lanes is one atomic (64 lanes on one word
+// took 5 us).  Called by all lanes of the wave.
 __device__ __forceinline__ void free_pages(const Pages &p, bool free, int page) {
     if (!__ballot(free)) return;
-    const int lane = int(threadIdx.x) % kWave;
-    const int word = free ? page / 64 : -1 - lane;
-    unsigned long long bits = free ? 1ull << (page % 64) : 0;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int other = __shfl_up(word, d);
-        const unsigned long long more = __shfl_up(bits, d);
-        if (lane >= d && other == word) bits |= more;
-    }
-    const int next = __shfl_down(word, 1);
-    if (free && (lane == kWave - 1 || next != word)) atomicOr(p.free_bits + word, bits);
+    const int word = free ? page / 64 : -1;
+    uint32_t low = free && !(page & 32) ? 1u << (page & 31) : 0, high = free && page & 32 ? 1u << (page & 31) : 0;
+    auto join = [&](int other, int more_low, int more_high) {
+        if (other == word) {
+            low |= uint32_t(more_low);
+            high |= uint32_t(more_high);
+        }
+    };
+    // a lane's bits reach every lane above it in its row that has its word
+    join(in_row<1>(word, -2), in_row<1>(int(low), 0), in_row<1>(int(high), 0));
+    join(in_row<2>(word, -2), in_row<2>(int(low), 0), in_row<2>(int(high), 0));
+    join(in_row<4>(word, -2), in_row<4>(int(low), 0), in_row<4>(int(high), 0));
+    join(in_row<8>(word, -2), in_row<8>(int(low), 0), in_row<8>(int(high), 0));
+    if (free && in_row<-1>(word, -2) != word) atomicOr(p.free_bits + word, uint64_t(high) << 32 | low);
 }
 
 // store(rank, lane, bit) for every set bit of the wave's words, in order: the
@@ -176,8 +185,9 @@ __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, co
             const int row = r / kw * kw;
             bank[t] = bank_of(write, r);
             page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
-            for (int other = r - 1; other >= row; --other)
-                if (bank_of(write, other) == bank[t]) first[t] = other;
+#pragma unroll
+            for (int d = 1; d < kMaxSlots; ++d)  // a loop would wait for each
+                if (d < kw && r - d >= row && bank_of(write, max(r - d, 0)) == bank[t]) first[t] = r - d;
             repeated |= first[t] != r;
             shared[t] = page[t] >= 0 && first[t] == r && p.references[page[t]] > 1;
             source[r] = page[t];
@@ -245,14 +255,17 @@ struct ReleaseMask {
 // behind the page's last row only, so whoever leaves zero frees the page.  A
 // thread has kForkRows loads, then atomics, in flight: one at a time, each a
 // trip to the L2, 64 rows took 13 us.
-constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
+// The rows of a thread are neighbours, as beams of one prompt are, and where they
+// share a page their changes are one (none for a prompt whose beams all share it).
 constexpr int kForkRows = 8;
+constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
 
 __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *parents, int count, ReleaseMask released,
                                                    int span) {
+    constexpr int kParts = kMaxSequences / 256;
     __shared__ int tile[kForkInts];
     __shared__ int parent[kMaxSequences], children[kMaxSequences];
-    __shared__ int rows[kMaxSequences], place[kMaxSequences], changed;
+    __shared__ int rows[kMaxSequences], place[kMaxSequences], counts[kParts][4];
     const int tiles = (p.banks + span - 1) / span;
     const int layer = blockIdx.x / tiles;
     const int mine = int(threadIdx.x) % span, bank = blockIdx.x % tiles * span + mine;
@@ -262,49 +275,73 @@ __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *paren
         parent[i] = int(from < 0 ? -1 : from >= p.sequences ? p.sequences - 1 : from);
         children[i] = 0;
     }
-    if (threadIdx.x == 0) changed = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < p.sequences; i += 256)
         if (parent[i] >= 0) atomicAdd(&children[parent[i]], 1);
     __syncthreads();
-    for (int i = threadIdx.x; i < p.sequences; i += 256)
-        if (children[i] != 1 || parent[i] != i) rows[place[i] = atomicAdd(&changed, 1)] = i;
+    // the rows that move, are continued elsewhere or end, in order
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    uint64_t changes[kParts];
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) {
+        const int i = c * 256 + int(threadIdx.x);
+        changes[c] = __ballot(i < p.sequences && (children[i] != 1 || parent[i] != i));
+        if (lane == 0) counts[c][wave] = __popcll(changes[c]);
+    }
     __syncthreads();
+    int changed = 0;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int i = c * 256 + int(threadIdx.x);
+            if (w == wave && changes[c] >> lane & 1) {
+                place[i] = changed + __popcll(changes[c] & ((1ull << lane) - 1));
+                rows[place[i]] = i;
+            }
+            changed += counts[c][w];
+        }
+    }
     if (!changed) return;
+    __syncthreads();
     int32_t *column = p.table + int64_t(layer) * p.sequences * p.banks + min(bank, p.banks - 1);
-    const int step = 256 / span;
     // every lane takes every turn: the lanes of a wave read each other's below
-    for (int turn = 0; turn < changed; turn += step * kForkRows) {
-        const int base = turn + int(threadIdx.x) / span;
+    const int threads = 256 / span, each = min((changed + threads - 1) / threads, kForkRows);
+    for (int turn = 0; turn < changed; turn += threads * each) {
+        const int base = turn + int(threadIdx.x) / span * each;
         int page[kForkRows], change[kForkRows], old[kForkRows];
 #pragma unroll
         for (int u = 0; u < kForkRows; ++u) {
-            const int at = min(base + u * step, changed - 1);
+            page[u] = -1;
+            change[u] = 0;
+            if (u >= each) continue;
+            const int at = min(base + u, changed - 1);
             page[u] = checked(p, column[int64_t(rows[at]) * p.banks]);
-            change[u] = base + u * step < changed && bank < p.banks ? children[rows[at]] - 1 : 0;
+            if (base + u < changed && bank < p.banks) change[u] = children[rows[at]] - 1;
             tile[at * span + mine] = page[u];
         }
-        // one change for the rows of a thread that hold one page
 #pragma unroll
         for (int u = 1; u < kForkRows; ++u)
 #pragma unroll
             for (int w = 0; w < u; ++w)
-                if (page[w] == page[u]) {
+                if (u < each && page[w] == page[u]) {
                     change[w] += change[u];
                     change[u] = 0;
                 }
 #pragma unroll
         for (int u = 0; u < kForkRows; ++u) {
             old[u] = 0;
+            if (u >= each) continue;
             if (page[u] >= 0 && change[u] < 0) old[u] = atomicAdd(p.references + page[u], change[u]);
             if (page[u] >= 0 && change[u] > 0) atomicAdd(p.references + page[u], change[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kForkRows; ++u) free_pages(p, old[u] + change[u] == 0 && change[u] < 0, page[u]);
+        for (int u = 0; u < kForkRows; ++u)
+            if (u < each) free_pages(p, old[u] + change[u] == 0 && change[u] < 0, page[u]);
     }
     __syncthreads();
     if (bank >= p.banks) return;
-    for (int at = int(threadIdx.x) / span; at < changed; at += step) {
+    for (int at = int(threadIdx.x) / span; at < changed; at += threads) {
         const int i = rows[at], from = parent[i];
         if (from != i) column[int64_t(i) * p.banks] = from < 0 ? -1 : tile[place[from] * span + mine];
     }
@@ -322,37 +359,61 @@ __device__ __forceinline__ bool bits_differ(uint2 a, uint2 b) { return ((a.x ^ b
 __device__ __forceinline__ bool bits_differ(uint32_t a, uint32_t b) { return a != b; }
 
 // Whether a dense bank differs from the base sequence's page of it; the old
-// page is dropped, an equal base page taken.  One workgroup a bank.
+// page is dropped, an equal base page taken.  A wave a bank; the books of a
+// workgroup's banks are kept together, whose old pages mostly share a word of
+// the free bits (one bank a workgroup, the atomics on these took 4 of 12 us).
+constexpr int kCompareWaves = 8;
+
 template <typename V>
-__global__ __launch_bounds__(256) void compare_kernel(Pages p, int layer, Rows rows, int base, const char *states,
-                                                      uint8_t *differs) {
-    const int64_t at = blockIdx.x;
-    const int row = int(blockIdx.x / uint32_t(p.banks)), bank = int(blockIdx.x % uint32_t(p.banks));
+__global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, int layer, Rows rows, int base,
+                                                                       uint32_t banks, const char *states,
+                                                                       uint8_t *differs) {
+    __shared__ int unequal[kCompareWaves];
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
-    int32_t *entry = table + int64_t(rows.at[row]) * p.banks + bank;
-    const int shared = base < 0 ? -1 : checked(p, table[int64_t(base) * p.banks + bank]);
-    const int old = checked(p, *entry);
     const int count = int(p.page_bytes / int64_t(sizeof(V)));
-    int other = shared < 0;
-    if (!other) {
-        const V *x = reinterpret_cast<const V *>(states + at * p.page_bytes);
-        const V *y = reinterpret_cast<const V *>(p.pool + shared * p.page_bytes);
-        auto unequal = [&](int i) { return bits_differ(x[i], y[i]); };
-        // a written bank shows it in its first vectors
-        const int ahead = min(count, int(blockDim.x));
-        other = __syncthreads_or(int(threadIdx.x) < ahead && unequal(threadIdx.x));
-        if (!other && count > ahead) {
-            int found = 0;
-            for (int i = ahead + int(threadIdx.x); i < count; i += blockDim.x) found |= unequal(i);
-            other = __syncthreads_or(found);
+    const uint32_t mine = blockIdx.x * kCompareWaves + wave;
+    if (mine < banks) {
+        const int shared = base < 0 ? -1 : checked(p, table[int64_t(base) * p.banks + mine % uint32_t(p.banks)]);
+        const V *x = reinterpret_cast<const V *>(states + mine * p.page_bytes);
+        const V *y = reinterpret_cast<const V *>(p.pool + max(shared, 0) * p.page_bytes);
+        bool other = shared < 0;
+        // a written bank shows it in its first vectors; the others of an equal one are loaded 8 at a time
+        if (!other) other = __any(lane < count && bits_differ(x[lane], y[lane]));
+        for (int i = kWave + lane; i - lane < count && !other; i += 8 * kWave) {
+            V a[8], b[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int at = min(i + u * kWave, count - 1);
+                a[u] = x[at];
+                b[u] = y[at];
+            }
+            bool found = false;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) found |= bits_differ(a[u], b[u]);
+            other = __any(found);
         }
+        if (lane == 0) unequal[wave] = other;
     }
-    if (threadIdx.x == 0) {
-        if (!other) atomicAdd(p.references + shared, 1);
-        if (old >= 0) drop_reference(p, old);
-        *entry = other ? -1 : shared;
-        differs[at] = uint8_t(other != 0);
+    __syncthreads();
+    if (wave) return;
+    const uint32_t at = blockIdx.x * kCompareWaves + lane;
+    bool free = false;
+    int old = -1;
+    if (lane < kCompareWaves && at < banks) {
+        const uint32_t bank = at % uint32_t(p.banks);
+        int32_t *entry = table + int64_t(rows.at[at / uint32_t(p.banks)]) * p.banks + bank;
+        const bool other = unequal[lane];
+        const int taken = other ? -1 : checked(p, table[int64_t(base) * p.banks + bank]);
+        old = checked(p, *entry);
+        if (old != taken) {
+            if (taken >= 0) atomicAdd(p.references + taken, 1);
+            if (old >= 0) free = atomicSub(p.references + old, 1) == 1;
+            *entry = taken;
+        }
+        differs[at] = uint8_t(other);
     }
+    free_pages(p, free, old);
 }
 
 // Pages for the banks that differ, in their order: target[i], or -1.
@@ -581,9 +642,10 @@ extern "C" int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, co
     if (rc != BDM_OK) return rc;
     ReleaseMask mask{};
     for (int i = 0; !parents && i < count; ++i) mask.bits[rows.at[i] / 64] |= 1ull << (rows.at[i] % 64);
-    // whole lines of a table row where that leaves a few hundred workgroups and a column in one go
-    int span = 64;
-    while (span > 16 && (span * p.sequences > 256 * kForkRows || int64_t(p.layers) * p.banks < 256 * span)) span /= 2;
+    // 128 bytes of a table row where that fills the card (16 layers, 64 rows, 1,024 banks: 10.8 us, 16.6 with 64
+    // bytes), else 64 with more rows in flight at once (one layer, 256 banks: 8.3 us, 11.2 with 128)
+    const bool wide = p.sequences * 32 <= kForkInts && int64_t(p.layers) * p.banks >= 256 * 32;
+    const int span = wide ? 32 : kForkInts / kMaxSequences;
     const int64_t grid = int64_t(p.layers) * ((p.banks + span - 1) / span);
     if (grid > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "pages_fork: grid too large");
     fork_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(p, parents, count, mask, span);
@@ -624,7 +686,8 @@ extern "C" int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32
     return with_vector(p.page_bytes, states, [&](auto vector) {
         using V = decltype(vector);
         const int threads = page_threads(p.page_bytes / int64_t(sizeof(V)));
-        compare_kernel<V><<<unsigned(banks), threads, 0, s>>>(p, layer, rows, base, data, differs);
+        compare_kernel<V><<<unsigned((banks + kCompareWaves - 1) / kCompareWaves), kCompareWaves * kWave, 0, s>>>(
+            p, layer, rows, base, uint32_t(banks), data, differs);
         int code = check_launch("compare_kernel");
         if (code != BDM_OK) return code;
         assign_kernel<<<1, kBlock, 0, s>>>(p, layer, rows, banks, differs, target, list);
