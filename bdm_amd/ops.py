@@ -1050,31 +1050,31 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, fin
     if length_penalty and lengths is None:
         raise ValueError('length_penalty needs lengths')
     device = _require_gpu(logits, scores, finished, lengths)
-    if logits.stride(-1) != 1 and vocab > 1:
+    batch_stride, beam_stride, token_stride = logits.stride()
+    if token_stride != 1 and vocab > 1:
         logits = logits.contiguous()
+        batch_stride, beam_stride = beams * vocab, vocab
     scores = scores.contiguous()
     finished = finished.contiguous() if finished is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    shape = (batch, width)
-    out = BeamSelection(torch.empty(shape, device=device), torch.empty(shape, device=device, dtype=torch.int64),
-                        torch.empty(shape, device=device, dtype=torch.int64),
-                        torch.empty(shape, device=device, dtype=torch.bool) if eos is not None else None,
-                        torch.empty(shape, device=device, dtype=torch.int32) if lengths is not None else None)
-    args = _lib.BeamArgs()
-    args.logits, args.scores = logits.data_ptr(), scores.data_ptr()
-    args.finished, args.lengths = _addr(finished), _addr(lengths)
-    args.out_scores, args.out_tokens, args.out_parents = (t.data_ptr() for t in out[:3])
-    args.out_finished, args.out_lengths = _addr(out.finished), _addr(out.lengths)
-    args.batch, args.batch_stride, args.beam_stride = batch, logits.stride(0), logits.stride(1)
-    args.eos = -1 if eos is None else int(eos)
-    args.length_penalty = float(length_penalty)
-    args.beams, args.vocab, args.width, args.dtype = beams, vocab, width, _dtype_code(logits.dtype)
-    lib = _lib.library()
-    nbytes = lib.bdm_beam_select_workspace_size(ctypes.byref(args))
+    shape, empty = (batch, width), torch.empty
+    out = BeamSelection(empty(shape, device=device, dtype=torch.float32),
+                        empty(shape, device=device, dtype=torch.int64), empty(shape, device=device, dtype=torch.int64),
+                        empty(shape, device=device, dtype=torch.bool) if eos is not None else None,
+                        empty(shape, device=device, dtype=torch.int32) if lengths is not None else None)
+    args = _lib.BeamArgs(logits.data_ptr(), scores.data_ptr(), _addr(finished), _addr(lengths), out.scores.data_ptr(),
+                         out.tokens.data_ptr(), out.parents.data_ptr(), _addr(out.finished), _addr(out.lengths), batch,
+                         batch_stride, beam_stride, -1 if eos is None else eos, length_penalty, beams, vocab, width,
+                         _dtype_code(logits.dtype))
+    lib, ref = _lib.library(), ctypes.byref(args)
+    nbytes = lib.bdm_beam_select_workspace_size(ref)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    with _on(device):
-        _lib.check(lib.bdm_beam_select(ctypes.byref(args), _addr(workspace), nbytes, _stream(device)),
-                   'bdm_beam_select')
+    if device.index == torch.cuda.current_device():
+        status = lib.bdm_beam_select(ref, _addr(workspace), nbytes, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = lib.bdm_beam_select(ref, _addr(workspace), nbytes, _stream(device))
+    _lib.check(status, 'bdm_beam_select')
     return out
 
 
@@ -1095,19 +1095,24 @@ def reorder_states(states, parents: Tensor, *, beams: int) -> None:
         raise ValueError('parents must be int64, one for each row of whole groups of beams')
     if beams > BEAM_MAX:
         raise NotImplementedError(f'reorder_states takes at most {BEAM_MAX} beams')
-    device = _require_gpu(parents, *states)
+    device, spans, sizes = _require_gpu(parents), [], []
     for t in states:
+        if t.device != device:
+            raise ValueError('all tensors must be on the same device')
         if t.ndim < 1 or t.shape[0] != rows or not t.is_contiguous():
             raise ValueError('states must be contiguous tensors with one row for each parent')
-    spans = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in states)
-    if any(a + size > b for (a, size), (b, _) in zip(spans, spans[1:])):
-        raise ValueError('states must not share memory')
+        spans.append(t.data_ptr())
+        sizes.append(t.nbytes)
     if rows == 0:
         return
+    end = 0
+    for start, size in sorted(zip(spans, sizes)):
+        if start < end:
+            raise ValueError('states must not share memory')
+        end = max(end, start + size)
     parents = parents.contiguous()
     count = len(states)
-    pointers = (ctypes.c_void_p * count)(*(t.data_ptr() for t in states))
-    sizes = (ctypes.c_int64 * count)(*(t.numel() * t.element_size() // rows for t in states))
+    pointers, lengths = (ctypes.c_void_p * count)(*spans), (ctypes.c_int64 * count)(*[n // rows for n in sizes])
     with _on(device):
-        _lib.check(_lib.library().bdm_reorder_states(pointers, sizes, count, parents.data_ptr(), rows // beams, beams,
+        _lib.check(_lib.library().bdm_reorder_states(pointers, lengths, count, parents.data_ptr(), rows // beams, beams,
                                                      _stream(device)), 'bdm_reorder_states')

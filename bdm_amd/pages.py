@@ -95,6 +95,12 @@ class BankPages:
         args.heads, args.bank_size, args.head_width = self.heads, self.bank_size, self.head_width
         args.dtype = ops._dtype_code(pool.dtype)
         self._ref = ctypes.byref(args)
+        step = self._step = _lib.DecodeArgs()  # the fields that every step shares
+        step.heads, step.bank_size, step.head_width, step.bank_count = (self.heads, self.bank_size, self.head_width,
+                                                                        self.banks)
+        step.state_dtype = args.dtype
+        self._step_ref = ctypes.byref(step)
+        self._library = _lib.library()
 
     # -- bookkeeping ------------------------------------------------------------------
     def used(self) -> Tensor:
@@ -108,7 +114,7 @@ class BankPages:
 
     def _rows(self, sequences) -> list[int]:
         rows = [sequences] if isinstance(sequences, int) else [int(i) for i in sequences]
-        if any(not 0 <= i < self.sequences for i in rows) or len(set(rows)) != len(rows):
+        if rows and (min(rows) < 0 or max(rows) >= self.sequences or len(set(rows)) != len(rows)):
             raise ValueError(f'sequences must be distinct and below {self.sequences}')
         return rows
 
@@ -118,8 +124,14 @@ class BankPages:
         return int(layer)
 
     def _call(self, name: str, *arguments) -> None:
-        with ops._on(self.device):
-            _lib.check(getattr(_lib.library(), name)(self._ref, *arguments, ops._stream(self.device)), name)
+        device = self.device
+        if device.index == torch.cuda.current_device():
+            status = getattr(self._library, name)(self._ref, *arguments, ops._stream(device))
+        else:
+            with torch.cuda.device(device):
+                status = getattr(self._library, name)(self._ref, *arguments, ops._stream(device))
+        if status:
+            _lib.check(status, name)
 
     # -- copying, forking, compacting and freeing -------------------------------------
     def load(self, layer: int, sequences, states: Tensor, base: int | None = None) -> None:
@@ -136,8 +148,8 @@ class BankPages:
             raise ValueError(f'states must be {self.dtype} {shape}')
         if base is not None and (not 0 <= base < self.sequences or base in rows):
             raise ValueError('base must be another sequence')
-        if ops._require_gpu(states) != self.device:
-            raise ValueError('all tensors must be on the same device')
+        if states.device != self.device:
+            raise ValueError('all tensors must be on the device of the pages')
         states = states.contiguous()
         nbytes = _lib.library().bdm_pages_load_workspace_size(self._ref, len(rows))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -160,8 +172,8 @@ class BankPages:
         page is copied."""
         if parents.dtype != torch.int64 or not 1 <= parents.numel() <= self.sequences:
             raise ValueError(f'parents must be int64, for 1 to {self.sequences} sequences')
-        if ops._require_gpu(parents) != self.device:
-            raise ValueError('all tensors must be on the same device')
+        if parents.device != self.device:
+            raise ValueError('all tensors must be on the device of the pages')
         parents = parents.contiguous()
         self._call('bdm_pages_fork', parents.data_ptr(), None, parents.numel())
 
@@ -186,33 +198,43 @@ class BankPages:
         banks are FP32 here and y is rounded once: with FP32 controllers the
         result is ``decode_step``'s bit for bit, with BF16 ones it is nearer to
         the exact one.  Sequences without pages give 0 and stay without."""
-        layer = self._layer(layer)
+        layer, device, dtype = self._layer(layer), self.device, q.dtype
         n, heads, s, width = q.shape[0] if q.ndim else 0, self.heads, self.bank_size, self.head_width
         if not 1 <= n <= self.sequences:
             raise ValueError(f'decode takes 1 to {self.sequences} sequences')
-        if any(tuple(t.shape) != (n, heads, s) for t in (q, k, g, b)) or any(
-                tuple(t.shape) != (n, heads, width) for t in (v, w)):
-            raise ValueError(f'q, k, g, b must be {(n, heads, s)} and v, w {(n, heads, width)}')
-        if any(t.ndim != 2 or t.shape[0] != n for t in (wi, ri)) or wi.shape != ww.shape or ri.shape != rw.shape:
+        rows, columns = (n, heads, s), (n, heads, width)
+        if (q.shape != rows or k.shape != rows or g.shape != rows or b.shape != rows or v.shape != columns
+                or w.shape != columns):
+            raise ValueError(f'q, k, g, b must be {rows} and v, w {columns}')
+        if wi.ndim != 2 or ri.ndim != 2 or wi.shape[0] != n or ri.shape[0] != n or wi.shape != ww.shape or (
+                ri.shape != rw.shape):
             raise ValueError('routes must be [sequences, selected banks]')
-        if wi.dtype != torch.int64 or ri.dtype != torch.int64:
+        if wi.dtype is not torch.int64 or ri.dtype is not torch.int64:
             raise ValueError('bank indices must be int64')
-        if any(t.dtype != q.dtype for t in (k, v, b, w, ww, rw)):
-            raise ValueError('controllers and route weights must share a dtype')
-        if ops._require_gpu(q, k, v, g, b, w, wi, ww, ri, rw) != self.device:
-            raise ValueError('all tensors must be on the same device')
-        held = [ops._aligned(t) for t in (q, k, b, g.float(), v, w, ww, rw, wi, ri)]
-        output = torch.empty((n, heads * width), device=self.device, dtype=q.dtype)
-        args = _lib.DecodeArgs()
+        held, pointers = [], []
+        for t in (q, k, b, g, v, w, ww, rw, wi, ri):
+            if t.device != device:
+                raise ValueError('all tensors must be on the device of the pages')
+            if t is g and g.dtype is not torch.float32:
+                t = g.float()
+            elif t.dtype is not dtype and t is not g and t is not wi and t is not ri:
+                raise ValueError('controllers and route weights must share a dtype')
+            if not t.is_contiguous():
+                t = t.contiguous()
+            pointer = t.data_ptr()
+            if pointer % 16:
+                t = t.clone()
+                pointer = t.data_ptr()
+            held.append(t)  # copies live until the launch is enqueued
+            pointers.append(pointer)
+        kw, kr = wi.shape[1], ri.shape[1]
+        output = torch.empty((n, heads * width), device=device, dtype=dtype)
+        args = self._step
         (args.q, args.k, args.b, args.g, args.v, args.w, args.write_weights, args.read_weights, args.write_indices,
-         args.read_indices) = (t.data_ptr() for t in held)
-        args.output = output.data_ptr()
-        args.batch = n
-        args.heads, args.bank_size, args.head_width, args.bank_count = heads, s, width, self.banks
-        args.write_banks, args.read_banks = wi.shape[1], ri.shape[1]
-        args.ctrl_dtype, args.state_dtype = ops._dtype_code(q.dtype), self._args.dtype
-        args.routed_decay, args.scale = int(bool(routed_decay)), float(scale)
-        nbytes = _lib.library().bdm_pages_decode_workspace_size(self._ref, wi.shape[1], ri.shape[1])
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        self._call('bdm_pages_decode', layer, ctypes.byref(args), workspace.data_ptr(), nbytes)
+         args.read_indices) = pointers
+        args.output, args.batch, args.write_banks, args.read_banks = output.data_ptr(), n, kw, kr
+        args.ctrl_dtype, args.routed_decay, args.scale = ops._dtype_code(dtype), bool(routed_decay), scale
+        nbytes = self._library.bdm_pages_decode_workspace_size(self._ref, kw, kr)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self._call('bdm_pages_decode', layer, self._step_ref, workspace.data_ptr(), nbytes)
         return output
