@@ -564,6 +564,9 @@ BeamPlan beam_plan(const bdm_beam_args &a) {
 }
 
 // ------------------------------------------------------------------ reordering
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 struct ReorderTensor {
     char *data;
     int64_t row_bytes;
@@ -582,18 +585,23 @@ struct ReorderParams {
 // moves in registers before it stores the first, and no other thread touches
 // the column.  Rows that stay are neither read nor written.  Two beams of one
 // parent read the same lines at the same time, from the caches.
+// HBM's rate bounds it, and that wants long runs: a workgroup takes 512 vectors
+// of each row (4 KiB of a row at a time reached 3.3 TB/s on 64 rows of 4 MiB,
+// 8 KiB 5.2, past the caches, as the rows stream, 5.4; a large copy 4.8).
+constexpr int kReorderRun = 512;  // vectors of a row
+
 template <typename V, int K>
 __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
+    constexpr int U = kReorderRun / 256;
     const int64_t prompt = blockIdx.x / p.blocks;
     const unsigned block = blockIdx.x % p.blocks;
     int which = 0;
     while (which + 1 < p.count && p.tensors[which + 1].first_block <= block) ++which;
     const ReorderTensor t = p.tensors[which];
-    const int64_t column = (int64_t(block - t.first_block) * 256 + threadIdx.x) * int64_t(sizeof(V));
-    if (column >= t.row_bytes) return;
+    const int64_t column = int64_t(block - t.first_block) * kReorderRun + threadIdx.x, columns = t.row_bytes / int64_t(sizeof(V));
     const int64_t first = prompt * p.beams;
-    char *base = t.data + first * t.row_bytes + column;
-    V held[K];
+    V *base = reinterpret_cast<V *>(t.data + first * t.row_bytes);
+    V held[K][U];
     int from[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -601,12 +609,23 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
         if (k < p.beams) {
             const int64_t parent = p.parents[first + k] - first;
             from[k] = int(parent < 0 ? 0 : parent >= p.beams ? p.beams - 1 : parent);
-            if (from[k] != k) held[k] = *reinterpret_cast<const V *>(base + from[k] * t.row_bytes);
+            if (from[k] != k) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (column + u * 256 < columns)
+                        held[k][u] = __builtin_nontemporal_load(base + from[k] * columns + column + u * 256);
+            }
         }
     }
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-        if (k < p.beams && from[k] != k) *reinterpret_cast<V *>(base + k * t.row_bytes) = held[k];
+    for (int k = 0; k < K; ++k) {
+        if (k < p.beams && from[k] != k) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (column + u * 256 < columns)
+                    __builtin_nontemporal_store(held[k][u], base + k * columns + column + u * 256);
+        }
+    }
 }
 
 template <typename V>
@@ -614,7 +633,7 @@ int launch_reorder(ReorderParams &p, int64_t batch, hipStream_t stream) {
     unsigned blocks = 0;
     for (int i = 0; i < p.count; ++i) {
         p.tensors[i].first_block = blocks;
-        const int64_t need = (p.tensors[i].row_bytes / int64_t(sizeof(V)) + 255) / 256;
+        const int64_t need = (p.tensors[i].row_bytes / int64_t(sizeof(V)) + kReorderRun - 1) / kReorderRun;
         if (need + blocks > int64_t(UINT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: rows too long");
         blocks += unsigned(need);
     }
@@ -622,6 +641,7 @@ int launch_reorder(ReorderParams &p, int64_t batch, hipStream_t stream) {
     if (batch * int64_t(blocks) > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: grid too large");
     p.blocks = blocks;
     const unsigned grid = unsigned(batch * blocks);
+    constexpr int kMost = sizeof(V) == 16 ? 16 : sizeof(V) == 8 ? 32 : kBeamMax;  // rows that registers hold
     if (p.beams <= 4)
         reorder_kernel<V, 4><<<grid, 256, 0, stream>>>(p);
     else if (p.beams <= 8)
@@ -629,9 +649,9 @@ int launch_reorder(ReorderParams &p, int64_t batch, hipStream_t stream) {
     else if (p.beams <= 16)
         reorder_kernel<V, 16><<<grid, 256, 0, stream>>>(p);
     else if (p.beams <= 32)
-        reorder_kernel<V, 32><<<grid, 256, 0, stream>>>(p);
+        reorder_kernel<V, kMost < 32 ? kMost : 32><<<grid, 256, 0, stream>>>(p);
     else
-        reorder_kernel<V, 64><<<grid, 256, 0, stream>>>(p);
+        reorder_kernel<V, kMost><<<grid, 256, 0, stream>>>(p);
     return check_launch("reorder_kernel");
 }
 
@@ -764,11 +784,12 @@ extern "C" int bdm_reorder_states(void *const *states, const int64_t *row_bytes,
             bits |= reinterpret_cast<uintptr_t>(states[done + i]) | uintptr_t(row_bytes[done + i]);
         }
         int rc;
-        // 64 rows of 16 bytes would be 256 registers: 8 bytes a row beyond 32 beams
-        if (bits % 16 == 0 && beams <= 32)
-            rc = launch_reorder<uint4>(p, batch, as_stream(stream));
-        else if (bits % 8 == 0)
-            rc = launch_reorder<uint2>(p, batch, as_stream(stream));
+        // a thread holds two vectors of each row in registers: 16 bytes of 16 rows are 128 of them, and beyond
+        // that the vectors are shorter
+        if (bits % 16 == 0 && beams <= 16)
+            rc = launch_reorder<u32x4>(p, batch, as_stream(stream));
+        else if (bits % 8 == 0 && beams <= 32)
+            rc = launch_reorder<u32x2>(p, batch, as_stream(stream));
         else if (bits % 4 == 0)
             rc = launch_reorder<uint32_t>(p, batch, as_stream(stream));
         else if (bits % 2 == 0)
