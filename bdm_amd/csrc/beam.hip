@@ -89,12 +89,16 @@ __device__ __forceinline__ void team_sync() {
     }
 }
 
-// How many of the team's values satisfy `test`, in every lane.
-template <int WAVES, int E, typename F>
-__device__ int team_count(TeamShared<WAVES> &sh, int lane, F test) {
+// How many of the team's values satisfy test(value, index), in every lane; read(e, index) loads value e again.
+template <int WAVES, int E, typename Read, typename F>
+__device__ int team_count(TeamShared<WAVES> &sh, int lane, Read read, F test) {
     int mine = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) mine += popcount(__ballot(test(e)));
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+        uint32_t index;
+        const float x = read(e, index);
+        mine += popcount(__ballot(x > -INFINITY && test(ordered(x), index)));
+    }
     if constexpr (WAVES > 1) {
         if (threadIdx.x == 0) sh.count = 0;
         __syncthreads();
@@ -108,10 +112,13 @@ __device__ int team_count(TeamShared<WAVES> &sh, int lane, F test) {
 
 // Maximum, sum of exponentials and the `width` best of the team's values
 // (index(e) is value e's index): sets high and sum in every lane, leaves the
-// candidates in sh.list and returns how many there are.  Values of -inf are no candidates.
-template <int WAVES, int E, typename Index>
-__device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index, int width, int wave, int lane,
-                         float &high, float &sum) {
+// candidates in sh.list and returns how many there are.  Values of -inf are no
+// candidates.  read(e, index) loads a value and its index once more, for the
+// few parts with too many ties: kept alive for those, the values and their
+// patterns took 108 registers of a lane with 33, and half the waves.
+template <int WAVES, int E, typename Index, typename Read>
+__device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index, Read read, int width, int wave,
+                         int lane, float &high, float &sum) {
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
@@ -137,8 +144,9 @@ __device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index
     // the sum relative to the part's maximum; a part without a finite value has the sum 0, one with a NaN
     // or +inf (inf - inf) a NaN
     sum = 0.f;
+    const float from = high > -INFINITY ? high : 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += x[e] == -INFINITY ? 0.f : __expf(x[e] - high);
+    for (int e = 0; e < E; ++e) sum += __expf(x[e] - from);
     sum = wave_sum(sum);
     if constexpr (WAVES > 1) {
         if (lane == 0) sh.sum[wave] = sum;
@@ -166,29 +174,25 @@ __device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index
     uint32_t value = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t next = value | (1u << bit);
-        if (team_count<WAVES, E>(sh, lane, [&](int e) { return x[e] > -INFINITY && ordered(x[e]) >= next; }) >= width)
-            value = next;
+        if (team_count<WAVES, E>(sh, lane, read, [&](uint32_t key, uint32_t) { return key >= next; }) >= width) value = next;
     }
-    const int above =
-        team_count<WAVES, E>(sh, lane, [&](int e) { return x[e] > -INFINITY && ordered(x[e]) > value; });
+    const int above = team_count<WAVES, E>(sh, lane, read, [&](uint32_t key, uint32_t) { return key > value; });
     uint32_t last = 0;  // the largest bound with fewer than width - above of the equal ones below it
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t next = last | (1u << bit);
-        if (team_count<WAVES, E>(sh, lane, [&](int e) { return x[e] > -INFINITY && ordered(x[e]) == value && index(e) < next; }) <
+        if (team_count<WAVES, E>(sh, lane, read, [&](uint32_t key, uint32_t at) { return key == value && at < next; }) <
             width - above)
             last = next;
     }
-    if constexpr (WAVES > 1) {
-        if (threadIdx.x == 0) sh.count = 0;
-    } else {
-        if (lane == 0) sh.count = 0;
-    }
+    if (WAVES > 1 ? threadIdx.x == 0 : lane == 0) sh.count = 0;
     team_sync<WAVES>();
-#pragma unroll
+#pragma unroll 1
     for (int e = 0; e < E; ++e) {
-        const uint32_t key = ordered(x[e]);
-        if (x[e] > -INFINITY && (key > value || (key == value && index(e) <= last)))
-            sh.list[atomicAdd(&sh.count, 1)] = uint64_t(key) << 32 | uint32_t(~index(e));
+        uint32_t at;
+        const float v = read(e, at);
+        const uint32_t key = ordered(v);
+        if (v > -INFINITY && (key > value || (key == value && at <= last)))
+            sh.list[atomicAdd(&sh.count, 1)] = uint64_t(key) << 32 | uint32_t(~at);
     }
     team_sync<WAVES>();
     return sh.count;
@@ -266,13 +270,12 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
     const int vectors = (p.vocab - head) / VE;
     float v[E];
-    int first[NV];  // first index of each vector
+    const int begin = split * NV * 256 + int(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = (split * NV + i) * 256 + int(threadIdx.x);
-        first[i] = head + at * VE;
+        const int at = begin + i * 256;
         if (at < vectors) {
-            Vec<T>::load(x + first[i], v + i * VE);
+            Vec<T>::load(x + head + at * VE, v + i * VE);
         } else {
 #pragma unroll
             for (int j = 0; j < VE; ++j) v[i * VE + j] = -INFINITY;
@@ -281,9 +284,14 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     // the row's odd ends: fewer than 2 * VE values
     const int odd = int(threadIdx.x) < head ? int(threadIdx.x) : vectors * VE + int(threadIdx.x);
     v[E - 1] = split == 0 && odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
-    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : first[e / VE] + e % VE); };
+    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (begin + e / VE * 256) * VE + e % VE); };
+    auto read = [&](int e, uint32_t &at) {
+        at = index(e);
+        const bool held = e == E - 1 ? split == 0 && odd < p.vocab : begin + e / VE * 256 < vectors;
+        return held ? to_f32(x[at]) : -INFINITY;
+    };
     float high, sum;
-    const int count = team_scan<4, E>(sh, v, index, p.width, wave, lane, high, sum);
+    const int count = team_scan<4, E>(sh, v, index, read, p.width, wave, lane, high, sum);
     const int64_t part = int64_t(row) * p.splits + split;
     if (threadIdx.x == 0) p.parts[part] = make_float2(high, sum);
     uint64_t *out = p.lists + part * p.width;
@@ -530,8 +538,13 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
         const int odd = lane < head ? lane : vectors * VE + lane;
         v[E - 1] = odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
         auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
+        auto read = [&](int e, uint32_t &at) {
+            at = index(e);
+            const bool held = e == E - 1 ? odd < p.vocab : e / VE * kWave + lane < vectors;
+            return held ? to_f32(x[at]) : -INFINITY;
+        };
         float high, sum;
-        const int count = team_scan<1, E>(team, v, index, p.width, 0, lane, high, sum);
+        const int count = team_scan<1, E>(team, v, index, read, p.width, 0, lane, high, sum);
         uint64_t *out = lists + beam * p.width;
         team_rank<1>(team, count, p.width, 0, lane, out);
         if (lane == 0) sh.log_sum[beam] = double(high) + log(double(sum));
