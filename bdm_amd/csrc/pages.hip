@@ -101,11 +101,16 @@ __device__ __forceinline__ void free_pages(const Pages &p, bool free, int page) 
     if (free && in_row<-1>(word, -2) != word) atomicOr(p.free_bits + word, uint64_t(high) << 32 | low);
 }
 
-// store(rank, lane, bit) for every set bit of the wave's words, in order: the
-// wave takes a word at a time, a lane a bit.  `before`: bits of the words ahead.
+// store(rank, lane, bit) for every set bit of the wave's words, in order;
+// `before`: bits of the words ahead.  Few bits a word: each lane goes through its
+// own; else the wave takes a word at a time, a lane a bit.
 template <typename F>
 __device__ __forceinline__ void each_bit(unsigned long long word, int before, F store) {
     const int lane = int(threadIdx.x) % kWave;
+    if (!__any(__popcll(word) > 8)) {
+        for (; word; word &= word - 1) store(before++, lane, __ffsll(word) - 1);
+        return;
+    }
     for (uint64_t left = __ballot(word != 0); left; left &= left - 1) {
         const int from = __ffsll(static_cast<unsigned long long>(left)) - 1;
         const uint64_t low = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(word)), from));
@@ -115,37 +120,57 @@ __device__ __forceinline__ void each_bit(unsigned long long word, int before, F 
     }
 }
 
-// The lowest `need` free pages, ascending, into list, and their bits cleared:
-// returns how many there were.  `word`: this thread's word of the bits, read
-// ahead.  Called by the whole workgroup, which sees the list behind its next
-// barrier.
-template <int THREADS>
-__device__ int take_free(const Pages &p, int need, int32_t *list, int *waves, unsigned long long word) {
-    const int64_t words = (p.pages + 63) / 64;
-    int found = 0;
-    for (int64_t base = 0; base < words && found < need; base += THREADS) {
-        const int64_t at = base + threadIdx.x;
-        if (base) word = at < words ? p.free_bits[at] : 0;
-        int all;
-        const int before = found + block_before<THREADS>(int(__popcll(word)), waves, all);
-        unsigned long long rest = word;
-        if (before < need) {
-            if (before + __popcll(word) <= need) {
-                rest = 0;
-            } else {
-                for (int i = before; i < need; ++i) rest &= rest - 1;
-            }
-        }
-        if (rest != word) p.free_bits[at] = rest;
-        const int64_t first = base + threadIdx.x / kWave * kWave;
-        each_bit(word & ~rest, before, [&](int rank, int from, int bit) { list[rank] = int32_t((first + from) * 64 + bit); });
-        found += all;
-    }
-    return min(found, need);
+// `word` without its n lowest set bits (n of them at least).
+__device__ __forceinline__ unsigned long long without_lowest(unsigned long long word, int n) {
+    int low = 0;  // the largest number of low places with n set bits at most
+#pragma unroll
+    for (int step = 32; step; step >>= 1)
+        if (__popcll(word & ((1ull << (low + step)) - 1)) <= n) low += step;
+    // with 63 places taken the last one is left to look at
+    if (low == 63 && __popcll(word) <= n) return 0;
+    return word >> low << low;
 }
 
-__device__ __forceinline__ unsigned long long first_free_word(const Pages &p) {
-    return int64_t(threadIdx.x) < (p.pages + 63) / 64 ? p.free_bits[threadIdx.x] : 0;
+// The free pages of THREADS words, found by their rank: a list of them, written
+// a bit at a time, took 2 to 3 us of the kernels that take a few hundred.
+template <int THREADS>
+struct FreeTile {
+    int waves[THREADS / kWave];
+    int ahead[THREADS];  // free pages of the words below each
+    unsigned long long words[THREADS];
+};
+
+// Fills the tile with the words from `base` on (`word` is the thread's), behind
+// `below` free pages; those of the lowest `need` are free no more.  Returns how
+// many there are.  Called by the whole workgroup, which has left the tile.
+template <int THREADS>
+__device__ __forceinline__ int fill_tile(const Pages &p, FreeTile<THREADS> &tile, int64_t base, unsigned long long word,
+                                         int below, int need) {
+    int all;
+    const int ahead = below + block_before<THREADS>(int(__popcll(word)), tile.waves, all);
+    tile.ahead[threadIdx.x] = ahead;
+    tile.words[threadIdx.x] = word;
+    if (word && ahead < need) {
+        const int take = need - ahead;
+        p.free_bits[base + threadIdx.x] = __popcll(word) <= take ? 0 : without_lowest(word, take);
+    }
+    __syncthreads();
+    return all;
+}
+
+// The free page of a rank that the tile holds.
+template <int THREADS>
+__device__ __forceinline__ int free_page(const FreeTile<THREADS> &tile, int64_t base, int rank) {
+    int low = 0;  // the last word with no more than `rank` pages below it
+#pragma unroll
+    for (int step = THREADS / 2; step; step >>= 1)
+        if (tile.ahead[low + step] <= rank) low += step;
+    const unsigned long long rest = without_lowest(tile.words[low], rank - tile.ahead[low]);
+    return int((base + low) * 64 + __ffsll(rest) - 1);
+}
+
+__device__ __forceinline__ unsigned long long free_word(const Pages &p, int64_t at) {
+    return at < (p.pages + 63) / 64 ? p.free_bits[at] : 0;
 }
 
 // ------------------------------------------------------------------ resolve
@@ -160,9 +185,8 @@ __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, co
                                                           int rows, int kw, int kr, int32_t *source, int32_t *target,
                                                           int32_t *read_pages) {
     constexpr int kWaves = THREADS / kWave;
-    __shared__ int waves[kWaves];
+    __shared__ FreeTile<THREADS> tile;
     __shared__ int counts[TILES][kWaves];
-    __shared__ int32_t list[TILES * THREADS];  // the new pages; then every request's target
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
     auto bank_of = [&](const int64_t *index, int at) {
@@ -170,33 +194,51 @@ __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, co
         return int(bank < 0 ? 0 : bank >= p.banks ? p.banks - 1 : bank);
     };
     const int writes = rows * kw, reads = rows * kr;
-    const unsigned long long word = first_free_word(p);  // in flight beside the chain below
-    int page[TILES], before[TILES], bank[TILES], first[TILES];
+    unsigned long long word = free_word(p, threadIdx.x);  // in flight beside the chain below
+    // each link of the chain for all requests at once
+    int page[TILES], before[TILES], bank[TILES], first[TILES], to[TILES];
     bool shared[TILES];
-    int repeated = 0;
+    int read_bank = 0, read_page = 0, repeated = 0;
+    if (thread < reads) read_bank = bank_of(read, thread);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread, at = min(r, max(writes - 1, 0)), row = at / max(kw, 1) * kw;
+        bank[t] = 0;
+        first[t] = r;  // the first slot of the token with this bank
+        if (writes == 0) continue;
+        bank[t] = bank_of(write, at);
+        int others[kMaxSlots];
+#pragma unroll
+        for (int d = 1; d < kMaxSlots; ++d) others[d] = bank_of(write, max(at - d, row));
+#pragma unroll
+        for (int d = 1; d < kMaxSlots; ++d)
+            if (at - d >= row && others[d] == bank[t]) first[t] = r - d;
+        repeated |= r < writes && first[t] != r;
+    }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
         const int r = t * THREADS + thread;
-        shared[t] = false;
         page[t] = -1;
-        first[t] = r;  // the first slot of the token with this bank
-        bank[t] = 0;
-        if (r < writes) {
-            const int row = r / kw * kw;
-            bank[t] = bank_of(write, r);
-            page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
+        if (r < writes) page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
+    }
+    if (thread < reads) read_page = checked(p, table[int64_t(thread / kr) * p.banks + read_bank]);
 #pragma unroll
-            for (int d = 1; d < kMaxSlots; ++d)  // a loop would wait for each
-                if (d < kw && r - d >= row && bank_of(write, max(r - d, 0)) == bank[t]) first[t] = r - d;
-            repeated |= first[t] != r;
-            shared[t] = page[t] >= 0 && first[t] == r && p.references[page[t]] > 1;
-            source[r] = page[t];
-        }
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread;
+        shared[t] = page[t] >= 0 && first[t] == r;
+        if (shared[t]) shared[t] = p.references[page[t]] > 1;
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread;
         const uint64_t mask = __ballot(shared[t]);
         before[t] = __popcll(mask & ((1ull << lane) - 1));
         if (lane == 0) counts[t][wave] = __popcll(mask);
+        to[t] = shared[t] ? -1 : page[t];
+        if (r < writes) source[r] = page[t];
     }
-    for (int r = thread; r < reads; r += THREADS)
+    if (thread < reads) read_pages[thread] = read_page;
+    for (int r = thread + THREADS; r < reads; r += THREADS)
         read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + bank_of(read, r)]);
     repeated = __syncthreads_or(repeated);
     int need = 0;
@@ -208,18 +250,23 @@ __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, co
             need += counts[t][w];
         }
     }
+    // the before[t]-th lowest free page for each
     int found = 0;
-    if (need) {
-        found = take_free<THREADS>(p, need, list, waves, word);
-        __syncthreads();
+    for (int64_t base = 0; base * 64 < p.pages && found < need; base += THREADS) {
+        if (base) {
+            __syncthreads();
+            word = free_word(p, base + thread);
+        }
+        const int all = fill_tile(p, tile, base, word, found, need);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+            if (shared[t] && before[t] >= found && before[t] < found + all) to[t] = free_page(tile, base, before[t]);
+        found += all;
     }
-    int to[TILES];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
         const int r = t * THREADS + thread;
-        to[t] = page[t];
         if (shared[t]) {
-            to[t] = before[t] < found ? list[before[t]] : -1;
             if (to[t] >= 0) {
                 table[int64_t(r / kw) * p.banks + bank[t]] = to[t];
                 p.references[to[t]] = 1;
@@ -232,14 +279,12 @@ __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, co
     }
     if (!repeated) return;
     // slots that repeat a bank store where its first slot does
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) list[t * THREADS + thread] = to[t];
+    __threadfence_block();
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
         const int r = t * THREADS + thread;
-        if (r < writes && first[t] != r) target[r] = list[first[t]];
+        if (r < writes && first[t] != r) target[r] = target[first[t]];
     }
 }
 
@@ -417,53 +462,62 @@ __global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, 
 }
 
 // Pages for the banks that differ, in their order: target[i], or -1.
-constexpr int kAssignList = 8192;  // new pages kept in LDS, more go to the workspace
+constexpr int kEach = 2;  // banks of a thread: 8 took 3 us more for 2,048
 
 __global__ __launch_bounds__(kBlock) void assign_kernel(Pages p, int layer, Rows rows, int64_t banks,
-                                                        const uint8_t *differs, int32_t *target, int32_t *spill) {
+                                                        const uint8_t *differs, int32_t *target) {
+    __shared__ FreeTile<kBlock> tile;
     __shared__ int waves[kBlockWaves];
-    __shared__ int32_t local[kAssignList];
-    constexpr int kEach = 8;
-    const unsigned long long word = first_free_word(p);  // in flight beside the count
-    // the flags, 0 or 1, of 8 banks (the workspace has room behind the last)
-    auto flags = [&](int64_t first) -> uint64_t {
+    __shared__ int16_t row_at[kMaxSequences];
+    auto flags = [&](int64_t first) {
         if (first >= banks) return 0;
-        const uint64_t f = *reinterpret_cast<const uint64_t *>(differs + first);
-        return first + kEach <= banks ? f : f & ((1ull << 8 * (banks - first)) - 1);
+        return int(differs[first] != 0) | int(first + 1 < banks && differs[first + 1] != 0) << 1;
     };
-    const uint64_t mine = flags(int64_t(threadIdx.x) * kEach);
-    int count = __popcll(mine);
-    for (int64_t base = kBlock * kEach; base < banks; base += kBlock * kEach)
-        count += __popcll(flags(base + threadIdx.x * kEach));
+    unsigned long long word = free_word(p, threadIdx.x);  // in flight beside the count
+    const int mine = flags(int64_t(threadIdx.x) * kEach);
+    int count = __popc(mine);
+    for (int64_t base = kBlock * kEach; base < banks; base += kBlock * kEach) count += __popc(flags(base + threadIdx.x * kEach));
+    if (threadIdx.x < kMaxSequences) row_at[threadIdx.x] = rows.at[threadIdx.x];
     int need;
     block_before<kBlock>(count, waves, need);
-    int32_t *list = need <= kAssignList ? local : spill;
-    const int found = need ? take_free<kBlock>(p, need, list, waves, word) : 0;
-    __syncthreads();
+    if (!need) {
+        for (int64_t i = threadIdx.x; i < banks; i += kBlock) target[i] = -1;
+        return;
+    }
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
-    int done = 0;
+    // requests and free pages both ascend: a tile of one beside a tile of the other
+    int64_t words = 0;
+    int below = 0, held = fill_tile(p, tile, words, word, 0, need), done = 0;
     for (int64_t base = 0; base < banks; base += kBlock * kEach) {
         const int64_t first = base + threadIdx.x * kEach;
-        const uint64_t f = base ? flags(first) : mine;
+        const int f = base ? flags(first) : mine;
         int all;
-        int rank = done + block_before<kBlock>(int(__popcll(f)), waves, all);
+        const int rank = done + block_before<kBlock>(int(__popc(f)), waves, all);
+        int page[kEach] = {-1, -1};
+        while (true) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int at = rank + (i ? f & 1 : 0);
+                if (f >> i & 1 && at >= below && at < below + held) page[i] = free_page(tile, words, at);
+            }
+            if (done + all <= below + held || (words + kBlock) * 64 >= p.pages) break;
+            below += held;
+            words += kBlock;
+            __syncthreads();
+            held = fill_tile(p, tile, words, free_word(p, words + threadIdx.x), below, need);
+        }
         done += all;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (first + i >= banks) break;
-            int page = -1;
-            if (f >> 8 * i & 1) {
-                if (rank < found) {
-                    page = list[rank];
-                    p.references[page] = 1;
-                    const uint32_t row = uint32_t(first + i) / uint32_t(p.banks);
-                    table[int64_t(rows.at[row]) * p.banks + uint32_t(first + i) % uint32_t(p.banks)] = page;
-                } else {
-                    atomicOr(p.status, 1);
-                }
-                ++rank;
+            if (page[i] >= 0) {
+                const uint32_t at = uint32_t(first + i), row = at / uint32_t(p.banks);
+                p.references[page[i]] = 1;
+                table[int64_t(row_at[row]) * p.banks + (at - row * uint32_t(p.banks))] = page[i];
+            } else if (f >> i & 1) {
+                atomicOr(p.status, 1);
             }
-            target[first + i] = page;
+            target[first + i] = page[i];
         }
     }
 }
@@ -515,7 +569,7 @@ __global__ __launch_bounds__(kBlock) void compact_plan_kernel(Pages p, CompactPl
         const int64_t left = border - word * 64;
         return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
     };
-    const unsigned long long word = first_free_word(p);
+    const unsigned long long word = free_word(p, threadIdx.x);
     int mine = 0;
     for (int64_t at = threadIdx.x; at < words; at += kBlock)
         mine += __popcll(~(at < kBlock ? word : p.free_bits[at]) & below(at, p.pages));
@@ -656,7 +710,7 @@ extern "C" size_t bdm_pages_load_workspace_size(const bdm_pages *pages, int32_t 
     using namespace bdm;
     if (!pages || count <= 0 || pages->banks <= 0) return 0;
     const size_t banks = size_t(count) * pages->banks;
-    return round16(banks) + 2 * round16(banks * sizeof(int32_t));
+    return round16(banks) + round16(banks * sizeof(int32_t));
 }
 
 extern "C" int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32_t *sequences, int32_t count,
@@ -680,7 +734,6 @@ extern "C" int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32
     if (!aligned(workspace, 16)) return fail(BDM_ERR_INVALID, "pages_load: workspace must be 16-byte aligned");
     uint8_t *differs = static_cast<uint8_t *>(workspace);
     int32_t *target = reinterpret_cast<int32_t *>(differs + round16(banks));
-    int32_t *list = target + round16(banks * sizeof(int32_t)) / sizeof(int32_t);
     const char *data = static_cast<const char *>(states);
     hipStream_t s = as_stream(stream);
     return with_vector(p.page_bytes, states, [&](auto vector) {
@@ -690,7 +743,7 @@ extern "C" int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32
             p, layer, rows, base, uint32_t(banks), data, differs);
         int code = check_launch("compare_kernel");
         if (code != BDM_OK) return code;
-        assign_kernel<<<1, kBlock, 0, s>>>(p, layer, rows, banks, differs, target, list);
+        assign_kernel<<<1, kBlock, 0, s>>>(p, layer, rows, banks, differs, target);
         code = check_launch("assign_kernel");
         if (code != BDM_OK) return code;
         store_kernel<V><<<unsigned(banks), threads, 0, s>>>(p, data, target);
@@ -787,6 +840,8 @@ extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm
     };
     if (writes <= 256)
         resolve(resolve_kernel<256, 1>, 256);
+    else if (writes <= 512)
+        resolve(resolve_kernel<512, 1>, 512);
     else if (writes <= kBlock)
         resolve(resolve_kernel<kBlock, 1>, kBlock);
     else
