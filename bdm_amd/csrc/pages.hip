@@ -79,27 +79,41 @@ __device__ __forceinline__ int in_row(int x, int none) {
     return __builtin_amdgcn_update_dpp(none, x, N > 0 ? 0x110 + N : 0x100 - N, 0xf, 0xf, false);
 }
 
-// The pages of the lanes with `free` set, free from now on.  Pages that were
-// taken together are released together, so neighbouring lanes share words of
-// the bits: a run of them within 16 lanes is one atomic (64 lanes on one word
-// took 5 us).  Called by all lanes of the wave.
-__device__ __forceinline__ void free_pages(const Pages &p, bool free, int page) {
-    if (!__ballot(free)) return;
-    const int word = free ? page / 64 : -1;
-    uint32_t low = free && !(page & 32) ? 1u << (page & 31) : 0, high = free && page & 32 ? 1u << (page & 31) : 0;
-    auto join = [&](int other, int more_low, int more_high) {
+// The free bits of the lanes' pages.  Pages that were taken together are
+// released together, so neighbouring lanes share words of the bits: a run of
+// them within 16 lanes is one atomic, by its last lane (64 lanes on one word
+// took 5 us).  Made by all lanes of a wave together.
+struct FreeRun {
+    int word;
+    uint32_t low, high;
+    bool last;
+
+    FreeRun() = default;
+    __device__ __forceinline__ FreeRun(bool free, int page) {
+        word = free ? page / 64 : -1;
+        low = free && !(page & 32) ? 1u << (page & 31) : 0;
+        high = free && page & 32 ? 1u << (page & 31) : 0;
+        // a lane's bits reach every lane above it in its row that has its word
+        join<1>();
+        join<2>();
+        join<4>();
+        join<8>();
+        last = free && in_row<-1>(word, -2) != word;
+    }
+
+    template <int N>
+    __device__ __forceinline__ void join() {
+        const int other = in_row<N>(word, -2), more_low = in_row<N>(int(low), 0), more_high = in_row<N>(int(high), 0);
         if (other == word) {
             low |= uint32_t(more_low);
             high |= uint32_t(more_high);
         }
-    };
-    // a lane's bits reach every lane above it in its row that has its word
-    join(in_row<1>(word, -2), in_row<1>(int(low), 0), in_row<1>(int(high), 0));
-    join(in_row<2>(word, -2), in_row<2>(int(low), 0), in_row<2>(int(high), 0));
-    join(in_row<4>(word, -2), in_row<4>(int(low), 0), in_row<4>(int(high), 0));
-    join(in_row<8>(word, -2), in_row<8>(int(low), 0), in_row<8>(int(high), 0));
-    if (free && in_row<-1>(word, -2) != word) atomicOr(p.free_bits + word, uint64_t(high) << 32 | low);
-}
+    }
+
+    __device__ __forceinline__ void store(const Pages &p) const {
+        if (last) atomicOr(p.free_bits + word, uint64_t(high) << 32 | low);
+    }
+};
 
 // store(rank, lane, bit) for every set bit of the wave's words, in order;
 // `before`: bits of the words ahead.  Few bits a word: each lane goes through its
@@ -189,57 +203,57 @@ __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, co
     __shared__ int counts[TILES][kWaves];
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
-    auto bank_of = [&](const int64_t *index, int at) {
-        const int64_t bank = index[at];
-        return int(bank < 0 ? 0 : bank >= p.banks ? p.banks - 1 : bank);
-    };
+    auto clamped = [&](int64_t index) { return int(index < 0 ? 0 : index >= p.banks ? p.banks - 1 : index); };
     const int writes = rows * kw, reads = rows * kr;
     unsigned long long word = free_word(p, threadIdx.x);  // in flight beside the chain below
-    // each link of the chain for all requests at once
+    // each link of the chain (bank, page, references) for all requests at once and without a branch, behind which
+    // the compiler would wait for it alone; a thread without a request repeats the last
     int page[TILES], before[TILES], bank[TILES], first[TILES], to[TILES];
     bool shared[TILES];
-    int read_bank = 0, read_page = 0, repeated = 0;
-    if (thread < reads) read_bank = bank_of(read, thread);
+    int64_t asked[TILES][kMaxSlots], read_asked = 0;
+    int read_page = -1, repeated = 0;
+    // (a step without written, or read, banks looks at the other ones)
+    const int64_t *writing = writes ? write : read, *reading = reads ? read : write;
+    const int every = writes ? kw : kr, most = max(writes ? writes : reads, 1) - 1;
+    const int read_every = reads ? kr : kw, read_at = min(thread, (reads ? reads : writes) - 1);
+    read_asked = reading[read_at];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-        const int r = t * THREADS + thread, at = min(r, max(writes - 1, 0)), row = at / max(kw, 1) * kw;
-        bank[t] = 0;
-        first[t] = r;  // the first slot of the token with this bank
-        if (writes == 0) continue;
-        bank[t] = bank_of(write, at);
-        int others[kMaxSlots];
+        const int at = min(t * THREADS + thread, most), row = at / every * every;
 #pragma unroll
-        for (int d = 1; d < kMaxSlots; ++d) others[d] = bank_of(write, max(at - d, row));
+        for (int d = 0; d < kMaxSlots; ++d) asked[t][d] = writing[max(at - d, row)];
+    }
+    read_page = table[int64_t(read_at / read_every) * p.banks + clamped(read_asked)];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread, at = min(r, most);
+        bank[t] = clamped(asked[t][0]);
+        page[t] = table[int64_t(at / every) * p.banks + bank[t]];
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread, slot = min(r, most) % every;
+        first[t] = r;  // the first slot of the token with this bank
 #pragma unroll
         for (int d = 1; d < kMaxSlots; ++d)
-            if (at - d >= row && others[d] == bank[t]) first[t] = r - d;
+            if (d <= slot && clamped(asked[t][d]) == bank[t]) first[t] = r - d;
+        page[t] = checked(p, page[t]);
+        to[t] = p.references[max(page[t], 0)];
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int r = t * THREADS + thread;
+        shared[t] = r < writes && page[t] >= 0 && first[t] == r && to[t] > 1;
         repeated |= r < writes && first[t] != r;
-    }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const int r = t * THREADS + thread;
-        page[t] = -1;
-        if (r < writes) page[t] = checked(p, table[int64_t(r / kw) * p.banks + bank[t]]);
-    }
-    if (thread < reads) read_page = checked(p, table[int64_t(thread / kr) * p.banks + read_bank]);
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const int r = t * THREADS + thread;
-        shared[t] = page[t] >= 0 && first[t] == r;
-        if (shared[t]) shared[t] = p.references[page[t]] > 1;
-    }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const int r = t * THREADS + thread;
         const uint64_t mask = __ballot(shared[t]);
         before[t] = __popcll(mask & ((1ull << lane) - 1));
         if (lane == 0) counts[t][wave] = __popcll(mask);
         to[t] = shared[t] ? -1 : page[t];
         if (r < writes) source[r] = page[t];
     }
-    if (thread < reads) read_pages[thread] = read_page;
+    if (thread < reads) read_pages[thread] = checked(p, read_page);
     for (int r = thread + THREADS; r < reads; r += THREADS)
-        read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + bank_of(read, r)]);
+        read_pages[r] = checked(p, table[int64_t(r / kr) * p.banks + clamped(read[r])]);
     repeated = __syncthreads_or(repeated);
     int need = 0;
 #pragma unroll
@@ -305,6 +319,53 @@ struct ReleaseMask {
 constexpr int kForkRows = 8;
 constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
 
+// Rows [base, end) of the changed ones in one column, R of them at most: into the tile, and what they change of the
+// references.  Each step for all rows at once: a load or atomic that the next row waited for was a trip of its own.
+template <int R>
+__device__ __forceinline__ void fork_rows(const Pages &p, const int32_t *column, const int *rows, const int *children,
+                                          int *tile, int base, int end, int span, int mine, bool held) {
+    int page[R], change[R], old[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) page[u] = column[int64_t(rows[max(min(base + u, end - 1), 0)]) * p.banks];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        page[u] = checked(p, page[u]);
+        change[u] = 0;
+        if (base + u < end) {
+            if (held && page[u] >= 0) change[u] = children[rows[base + u]] - 1;
+            tile[(base + u) * span + mine] = page[u];
+        }
+    }
+#pragma unroll
+    for (int u = 1; u < R; ++u)
+#pragma unroll
+        for (int w = 0; w < u; ++w)
+            if (page[w] == page[u]) {
+                change[w] += change[u];
+                change[u] = 0;
+            }
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        old[u] = 0;
+        if (change[u] < 0) old[u] = atomicAdd(p.references + page[u], change[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (change[u] > 0) atomicAdd(p.references + page[u], change[u]);
+    bool free[R], any = false;
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        free[u] = change[u] < 0 && old[u] + change[u] == 0;
+        any |= free[u];
+    }
+    if (!__any(any)) return;
+    FreeRun runs[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) runs[u] = FreeRun(free[u], page[u]);
+#pragma unroll
+    for (int u = 0; u < R; ++u) runs[u].store(p);
+}
+
 __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *parents, int count, ReleaseMask released,
                                                    int span) {
     constexpr int kParts = kMaxSequences / 256;
@@ -354,35 +415,14 @@ __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int64_t *paren
     const int threads = 256 / span, each = min((changed + threads - 1) / threads, kForkRows);
     for (int turn = 0; turn < changed; turn += threads * each) {
         const int base = turn + int(threadIdx.x) / span * each;
-        int page[kForkRows], change[kForkRows], old[kForkRows];
-#pragma unroll
-        for (int u = 0; u < kForkRows; ++u) {
-            page[u] = -1;
-            change[u] = 0;
-            if (u >= each) continue;
-            const int at = min(base + u, changed - 1);
-            page[u] = checked(p, column[int64_t(rows[at]) * p.banks]);
-            if (base + u < changed && bank < p.banks) change[u] = children[rows[at]] - 1;
-            tile[at * span + mine] = page[u];
-        }
-#pragma unroll
-        for (int u = 1; u < kForkRows; ++u)
-#pragma unroll
-            for (int w = 0; w < u; ++w)
-                if (u < each && page[w] == page[u]) {
-                    change[w] += change[u];
-                    change[u] = 0;
-                }
-#pragma unroll
-        for (int u = 0; u < kForkRows; ++u) {
-            old[u] = 0;
-            if (u >= each) continue;
-            if (page[u] >= 0 && change[u] < 0) old[u] = atomicAdd(p.references + page[u], change[u]);
-            if (page[u] >= 0 && change[u] > 0) atomicAdd(p.references + page[u], change[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kForkRows; ++u)
-            if (u < each) free_pages(p, old[u] + change[u] == 0 && change[u] < 0, page[u]);
+        if (each == 1)
+            fork_rows<1>(p, column, rows, children, tile, base, changed, span, mine, bank < p.banks);
+        else if (each == 2)
+            fork_rows<2>(p, column, rows, children, tile, base, min(changed, base + each), span, mine, bank < p.banks);
+        else if (each <= 4)
+            fork_rows<4>(p, column, rows, children, tile, base, min(changed, base + each), span, mine, bank < p.banks);
+        else
+            fork_rows<kForkRows>(p, column, rows, children, tile, base, min(changed, base + each), span, mine, bank < p.banks);
     }
     __syncthreads();
     if (bank >= p.banks) return;
@@ -417,6 +457,16 @@ __global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, 
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     int32_t *table = p.table + int64_t(layer) * p.sequences * p.banks;
     const int count = int(p.page_bytes / int64_t(sizeof(V)));
+    // what the books need of the workgroup's banks, in flight beside the comparison: lane i's is bank i's
+    const uint32_t at = blockIdx.x * kCompareWaves + min(lane, kCompareWaves - 1);
+    int32_t *entry = table;
+    int old = -1, taken = -1;
+    if (wave == 0) {
+        const uint32_t kept = min(at, banks - 1), row = kept / uint32_t(p.banks), bank = kept - row * uint32_t(p.banks);
+        entry = table + int64_t(rows.at[row]) * p.banks + bank;
+        old = *entry;
+        taken = table[int64_t(max(base, 0)) * p.banks + bank];
+    }
     const uint32_t mine = blockIdx.x * kCompareWaves + wave;
     if (mine < banks) {
         const int shared = base < 0 ? -1 : checked(p, table[int64_t(base) * p.banks + mine % uint32_t(p.banks)]);
@@ -424,14 +474,14 @@ __global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, 
         const V *y = reinterpret_cast<const V *>(p.pool + max(shared, 0) * p.page_bytes);
         bool other = shared < 0;
         // a written bank shows it in its first vectors; the others of an equal one are loaded 8 at a time
-        if (!other) other = __any(lane < count && bits_differ(x[lane], y[lane]));
+        if (!other) other = __any(lane < count && bits_differ(x[min(lane, count - 1)], y[min(lane, count - 1)]));
         for (int i = kWave + lane; i - lane < count && !other; i += 8 * kWave) {
             V a[8], b[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const int at = min(i + u * kWave, count - 1);
-                a[u] = x[at];
-                b[u] = y[at];
+                const int v = min(i + u * kWave, count - 1);
+                a[u] = x[v];
+                b[u] = y[v];
             }
             bool found = false;
 #pragma unroll
@@ -442,15 +492,11 @@ __global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, 
     }
     __syncthreads();
     if (wave) return;
-    const uint32_t at = blockIdx.x * kCompareWaves + lane;
     bool free = false;
-    int old = -1;
+    old = checked(p, old);
     if (lane < kCompareWaves && at < banks) {
-        const uint32_t bank = at % uint32_t(p.banks);
-        int32_t *entry = table + int64_t(rows.at[at / uint32_t(p.banks)]) * p.banks + bank;
         const bool other = unequal[lane];
-        const int taken = other ? -1 : checked(p, table[int64_t(base) * p.banks + bank]);
-        old = checked(p, *entry);
+        taken = other ? -1 : checked(p, taken);
         if (old != taken) {
             if (taken >= 0) atomicAdd(p.references + taken, 1);
             if (old >= 0) free = atomicSub(p.references + old, 1) == 1;
@@ -458,7 +504,7 @@ __global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, 
         }
         differs[at] = uint8_t(other);
     }
-    free_pages(p, free, old);
+    if (__any(free)) FreeRun(free, old).store(p);
 }
 
 // Pages for the banks that differ, in their order: target[i], or -1.
@@ -471,13 +517,15 @@ __global__ __launch_bounds__(kBlock) void assign_kernel(Pages p, int layer, Rows
     __shared__ int16_t row_at[kMaxSequences];
     auto flags = [&](int64_t first) {
         if (first >= banks) return 0;
-        return int(differs[first] != 0) | int(first + 1 < banks && differs[first + 1] != 0) << 1;
+        const int two = *reinterpret_cast<const uint16_t *>(differs + first);  // the workspace has room behind the last
+        return (two & 0xff ? 1 : 0) | (first + 1 < banks && two >> 8 ? 2 : 0);
     };
     unsigned long long word = free_word(p, threadIdx.x);  // in flight beside the count
+    const int16_t row_of = rows.at[threadIdx.x % kMaxSequences];
     const int mine = flags(int64_t(threadIdx.x) * kEach);
     int count = __popc(mine);
     for (int64_t base = kBlock * kEach; base < banks; base += kBlock * kEach) count += __popc(flags(base + threadIdx.x * kEach));
-    if (threadIdx.x < kMaxSequences) row_at[threadIdx.x] = rows.at[threadIdx.x];
+    row_at[threadIdx.x % kMaxSequences] = row_of;
     int need;
     block_before<kBlock>(count, waves, need);
     if (!need) {

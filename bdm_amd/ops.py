@@ -1057,11 +1057,10 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, fin
     scores = scores.contiguous()
     finished = finished.contiguous() if finished is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    shape, empty = (batch, width), torch.empty
-    out = BeamSelection(empty(shape, device=device, dtype=torch.float32),
-                        empty(shape, device=device, dtype=torch.int64), empty(shape, device=device, dtype=torch.int64),
-                        empty(shape, device=device, dtype=torch.bool) if eos is not None else None,
-                        empty(shape, device=device, dtype=torch.int32) if lengths is not None else None)
+    tokens, like = torch.empty((batch, width), device=device, dtype=torch.int64), torch.empty_like
+    out = BeamSelection(like(tokens, dtype=torch.float32), tokens, like(tokens),
+                        like(tokens, dtype=torch.bool) if eos is not None else None,
+                        like(tokens, dtype=torch.int32) if lengths is not None else None)
     args = _lib.BeamArgs(logits.data_ptr(), scores.data_ptr(), _addr(finished), _addr(lengths), out.scores.data_ptr(),
                          out.tokens.data_ptr(), out.parents.data_ptr(), _addr(out.finished), _addr(out.lengths), batch,
                          batch_stride, beam_stride, -1 if eos is None else eos, length_penalty, beams, vocab, width,

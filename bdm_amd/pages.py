@@ -27,6 +27,7 @@ from torch import Tensor
 from . import _lib, ops
 
 MAX_SEQUENCES = 512
+MAX_SELECTED = 16  # written, and read, banks of a token
 
 
 class BankPages:
@@ -100,6 +101,9 @@ class BankPages:
                                                                         self.banks)
         step.state_dtype = args.dtype
         self._step_ref = ctypes.byref(step)
+        # the tables of one step, the handle's own: calls on one cache are ordered, so nothing else uses them meanwhile
+        nbytes = _lib.library().bdm_pages_decode_workspace_size(self._ref, MAX_SELECTED, MAX_SELECTED)
+        self._tables = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._library = _lib.library()
 
     # -- bookkeeping ------------------------------------------------------------------
@@ -234,7 +238,5 @@ class BankPages:
          args.read_indices) = pointers
         args.output, args.batch, args.write_banks, args.read_banks = output.data_ptr(), n, kw, kr
         args.ctrl_dtype, args.routed_decay, args.scale = ops._dtype_code(dtype), bool(routed_decay), scale
-        nbytes = self._library.bdm_pages_decode_workspace_size(self._ref, kw, kr)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        self._call('bdm_pages_decode', layer, self._step_ref, workspace.data_ptr(), nbytes)
+        self._call('bdm_pages_decode', layer, self._step_ref, self._tables.data_ptr(), self._tables.nbytes)
         return output
