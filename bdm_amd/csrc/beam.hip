@@ -678,6 +678,7 @@ int check_beam(const bdm_beam_args *a) {
     if (a->batch < 0 || a->beams <= 0 || a->vocab <= 0 || a->width <= 0)
         return fail(BDM_ERR_INVALID, "beam_select: bad geometry");
     if (a->dtype != BDM_BF16 && a->dtype != BDM_F32) return fail(BDM_ERR_INVALID, "beam_select: logits dtype");
+    if (a->vocab > 1 << 30) return fail(BDM_ERR_UNSUPPORTED, "beam_select: vocabulary of %d", a->vocab);
     if (a->beams > kBeamMax || a->width > kBeamMax)
         return fail(BDM_ERR_UNSUPPORTED, "beam_select: more than %d beams", kBeamMax);
     if (int64_t(a->width) > int64_t(a->beams) * a->vocab)

@@ -396,6 +396,47 @@ __global__ __launch_bounds__(512) void decode_kernel(DecodeParams<T> p) {
     }
 }
 
+// The kernel's rows of a bank and columns of a lane.
+struct DecodeRows {
+    int rows, columns;
+};
+
+DecodeRows decode_rows(const bdm_decode_args &a, bool paged) {
+    // two columns per lane: 64 lanes per slot, more loads in flight per
+    // step (wide heads run as spans of 128 columns)
+    const bool pairs = a.head_width % 2 == 0 && (a.head_width / 2 <= 64 || a.head_width % 128 == 0);
+    // the paged step has banks of four rows, the package's default, without the four more that the dense step pads
+    // them to (a step of four sequences, one head of 128 columns: 9.1 -> 4.6 us)
+    if (paged && a.bank_size <= 4 && pairs) return {4, 2};
+    if (a.bank_size <= 8) {
+        if (pairs) return {8, 2};
+        if (a.head_width % 4 == 0 && a.head_width / 4 <= 64) return {8, 4};
+        return {8, a.head_width % 8 == 0 ? 8 : 1};
+    }
+    if (a.bank_size <= 16) return {16, a.head_width % 4 == 0 ? 4 : 1};
+    return {32, a.head_width % 2 == 0 ? 2 : 1};
+}
+
+// A workgroup of the decode kernel: the widest span of columns (a divisor of
+// the head width, a multiple of a lane's) that fits 512 lanes and 64 KiB of LDS.
+struct DecodeShape {
+    int span, threads;
+    size_t lds;
+    bool fits;
+};
+
+DecodeShape decode_shape(const bdm_decode_args &a, int rows, int columns) {
+    const int slots = a.write_banks > a.read_banks ? a.write_banks : a.read_banks;
+    auto lds_bytes = [&](int span) {
+        return (size_t(a.write_banks) * rows * span + size_t(a.read_banks) * span) * sizeof(float);
+    };
+    int span = a.head_width;
+    while ((slots * (span / columns) > 512 || lds_bytes(span) > 64 * 1024) && span % 2 == 0 && (span / 2) % columns == 0)
+        span /= 2;
+    const int threads = ((slots * (span / columns) + kWave - 1) / kWave) * kWave;
+    return {span, threads, lds_bytes(span), threads <= 512 && lds_bytes(span) <= 64 * 1024};
+}
+
 template <typename T, int S, int CPL, bool PAGED>
 int launch_decode(const bdm_decode_args &a, const PageTables *tables, hipStream_t stream) {
     DecodeParams<T> p{};
@@ -422,15 +463,10 @@ int launch_decode(const bdm_decode_args &a, const PageTables *tables, hipStream_
     p.banks = a.bank_count;
     p.kw = a.write_banks;
     p.kr = a.read_banks;
-    // the widest span (a divisor of the head width, a multiple of CPL) that
-    // fits 512 lanes and 64 KiB of LDS
-    const int slots = a.write_banks > a.read_banks ? a.write_banks : a.read_banks;
-    auto lds_bytes = [&](int span) {
-        return (size_t(a.write_banks) * S * span + size_t(a.read_banks) * span) * sizeof(float);
-    };
-    int span = a.head_width;
-    while ((slots * (span / CPL) > 512 || lds_bytes(span) > 64 * 1024) && span % 2 == 0 && (span / 2) % CPL == 0)
-        span /= 2;
+    const DecodeShape shape = decode_shape(a, S, CPL);
+    if (!shape.fits) return fail(BDM_ERR_UNSUPPORTED, "decode: %d lanes and %zu bytes of LDS a workgroup", shape.threads, shape.lds);
+    const int span = shape.span, threads = shape.threads;
+    const size_t lds = shape.lds;
     p.span = span;
     p.spans = a.head_width / span;
     p.lanes_per_slot = span / CPL;
@@ -442,10 +478,6 @@ int launch_decode(const bdm_decode_args &a, const PageTables *tables, hipStream_
     p.state_dtype = a.state_dtype;
     p.routed_decay = a.routed_decay;
     p.scale = a.scale;
-    const int threads = ((slots * p.lanes_per_slot + kWave - 1) / kWave) * kWave;
-    if (threads > 512) return fail(BDM_ERR_UNSUPPORTED, "decode: %d lanes per workgroup", threads);
-    const size_t lds = lds_bytes(span);
-    if (lds > 64 * 1024) return fail(BDM_ERR_UNSUPPORTED, "decode: %zu bytes of LDS", lds);
     if (a.batch * a.heads * p.spans > int64_t(UINT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "decode: grid too large");
     const unsigned grid = unsigned(a.batch * a.heads * p.spans);
     // the production geometry (8 banks per role, full-width aligned rows) gets
@@ -515,26 +547,21 @@ int launch_decode_fused(const bdm_decode_fused_args &a, hipStream_t stream) {
 
 template <typename T, bool PAGED = false>
 int dispatch_decode(const bdm_decode_args &a, hipStream_t stream, const PageTables *tables = nullptr) {
+    const DecodeRows kind = decode_rows(a, PAGED);
     if constexpr (PAGED) {
-        // banks of four rows, the package's default, without the four more that the dense step pads them to
-        // (a step of four sequences, one head of 128 columns: 9.1 -> 4.6 us)
-        if (a.bank_size <= 4 && a.head_width % 2 == 0 && (a.head_width / 2 <= 64 || a.head_width % 128 == 0))
-            return launch_decode<T, 4, 2, PAGED>(a, tables, stream);
+        if (kind.rows == 4) return launch_decode<T, 4, 2, PAGED>(a, tables, stream);
     }
-    if (a.bank_size <= 8) {
-        // two columns per lane: 64 lanes per slot, more loads in flight per
-        // step (wide heads run as spans of 128 columns)
-        if (a.head_width % 2 == 0 && (a.head_width / 2 <= 64 || a.head_width % 128 == 0))
-            return launch_decode<T, 8, 2, PAGED>(a, tables, stream);
-        if (a.head_width % 4 == 0 && a.head_width / 4 <= 64) return launch_decode<T, 8, 4, PAGED>(a, tables, stream);
-        if (a.head_width % 8 == 0) return launch_decode<T, 8, 8, PAGED>(a, tables, stream);
+    if (kind.rows == 8) {
+        if (kind.columns == 2) return launch_decode<T, 8, 2, PAGED>(a, tables, stream);
+        if (kind.columns == 4) return launch_decode<T, 8, 4, PAGED>(a, tables, stream);
+        if (kind.columns == 8) return launch_decode<T, 8, 8, PAGED>(a, tables, stream);
         return launch_decode<T, 8, 1, PAGED>(a, tables, stream);
     }
-    if (a.bank_size <= 16) {
-        if (a.head_width % 4 == 0) return launch_decode<T, 16, 4, PAGED>(a, tables, stream);
+    if (kind.rows == 16) {
+        if (kind.columns == 4) return launch_decode<T, 16, 4, PAGED>(a, tables, stream);
         return launch_decode<T, 16, 1, PAGED>(a, tables, stream);
     }
-    if (a.head_width % 2 == 0) return launch_decode<T, 32, 2, PAGED>(a, tables, stream);
+    if (kind.columns == 2) return launch_decode<T, 32, 2, PAGED>(a, tables, stream);
     return launch_decode<T, 32, 1, PAGED>(a, tables, stream);
 }
 
@@ -561,6 +588,15 @@ int check_decode(const bdm_decode_args *a) {
     const void *ptrs[] = {a->v, a->w, a->state, a->output};
     for (const void *ptr : ptrs)
         if (!aligned(ptr, 16)) return fail(BDM_ERR_INVALID, "decode: tensors must be 16-byte aligned");
+    return BDM_OK;
+}
+
+int check_decode_pages(const bdm_decode_args *a) {
+    const int rc = check_decode(a);
+    if (rc != BDM_OK) return rc;
+    const DecodeRows kind = decode_rows(*a, true);
+    if (!decode_shape(*a, kind.rows, kind.columns).fits)
+        return fail(BDM_ERR_UNSUPPORTED, "decode: a head of %d columns does not fit a workgroup", a->head_width);
     return BDM_OK;
 }
 

@@ -13,8 +13,8 @@ struct PageTables {
     const int32_t *read;    // [N, KR] page of a read bank; -1: none
 };
 
-// bdm_decode's checks of its arguments (decode.hip).
-int check_decode(const bdm_decode_args *a);
+// What bdm_decode would refuse of a step over pages (decode.hip); nothing is refused behind it.
+int check_decode_pages(const bdm_decode_args *a);
 // The decode step over the pages: bdm_decode's kernel with its states addressed by `tables`.
 int launch_decode_pages(const bdm_decode_args &a, const PageTables &tables, hipStream_t stream);
 

@@ -877,8 +877,8 @@ extern "C" int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm
     if (!aligned(workspace, 16)) return fail(BDM_ERR_INVALID, "pages_decode: workspace must be 16-byte aligned");
     bdm_decode_args args = *a;
     args.state = p.pool;
-    const int checked_args = check_decode(&args);
-    if (checked_args != BDM_OK) return checked_args;
+    const int step = check_decode_pages(&args);  // before the tables change
+    if (step != BDM_OK) return step;
     const int rows = int(a->batch), writes = rows * a->write_banks;
     int32_t *source = static_cast<int32_t *>(workspace), *target = source + writes, *read = target + writes;
     hipStream_t s = as_stream(stream);

@@ -112,8 +112,10 @@ class BankPages:
         return (self.references > 0).sum()
 
     def check(self) -> None:
-        """Raises if a call found no free page.  Synchronises the host."""
+        """Raises if a call since the last check found no free page.
+        Synchronises the host."""
         if int(self.status):
+            self.status.zero_()
             raise RuntimeError(f'BankPages: no free page was left of {self.pages}')
 
     def _rows(self, sequences) -> list[int]:

@@ -585,6 +585,12 @@ def test_calls_refuse(device):
     refused(BankPages.over, pages.pool, pages.table, pages.references[1:])
     refused(BankPages.over, pages.pool[:, :, ::2], pages.table, pages.references)
     refused(BankPages.over, pages.pool.half(), pages.table, pages.references)
+    odd, _, _ = make(device, n=3, banks=8, layers=1, s=8, width=521)  # no span of a workgroup divides the head
+    odd.load(0, [0], torch.zeros(1, 8, 1, 8, 521, dtype=torch.bfloat16, device=device))
+    odd.fork(torch.zeros(3, dtype=torch.int64, device=device))
+    with pytest.raises(NotImplementedError):
+        odd.decode(0, *token(3, 1, 8, 521, 8, 4, 4, torch.bfloat16, gen, device), scale=1.0, routed_decay=True)
+    assert torch.equal(odd.table[0, 0], odd.table[0, 2]) and int(odd.used()) == 8
     with pytest.raises(NotImplementedError):
         wide = [t.repeat(1, 5) if i > 5 else t for i, t in enumerate(step)]
         pages.decode(0, *wide, scale=1.0, routed_decay=True)
