@@ -215,8 +215,7 @@ __device__ __forceinline__ void team_rank(const TeamShared<WAVES> &sh, int count
 template <typename T> struct Vec;
 template <> struct Vec<bf16_t> {
     static constexpr int kSize = 8;
-    static __device__ __forceinline__ void load(const bf16_t *p, float *out) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    static __device__ __forceinline__ void widen(const uint4 &u, float *out) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -227,11 +226,30 @@ template <> struct Vec<bf16_t> {
 };
 template <> struct Vec<float> {
     static constexpr int kSize = 4;
-    static __device__ __forceinline__ void load(const float *p, float *out) {
-        const float4 u = *reinterpret_cast<const float4 *>(p);
-        out[0] = u.x, out[1] = u.y, out[2] = u.z, out[3] = u.w;
+    static __device__ __forceinline__ void widen(const uint4 &u, float *out) {
+        out[0] = __uint_as_float(u.x), out[1] = __uint_as_float(u.y);
+        out[2] = __uint_as_float(u.z), out[3] = __uint_as_float(u.w);
     }
 };
+
+// NV vectors of a row's `vectors`, `step` apart from `begin` on, -inf where the row has none.  All are asked for at
+// once, the last one in the place of those (a load under a condition of its own is waited for before the next).
+template <typename T, int NV>
+__device__ __forceinline__ void load_part(const T *x, int vectors, int begin, int step, float *out) {
+    constexpr int VE = Vec<T>::kSize;
+    uint4 raw[NV];
+    if (vectors > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = *reinterpret_cast<const uint4 *>(x + int64_t(min(begin + i * step, vectors - 1)) * VE);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        Vec<T>::widen(raw[i], out + i * VE);
+        const bool held = begin + i * step < vectors;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) out[i * VE + j] = held ? out[i * VE + j] : -INFINITY;
+    }
+}
 
 struct BeamParams {
     const void *logits;
@@ -271,16 +289,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     const int vectors = (p.vocab - head) / VE;
     float v[E];
     const int begin = split * NV * 256 + int(threadIdx.x);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = begin + i * 256;
-        if (at < vectors) {
-            Vec<T>::load(x + head + at * VE, v + i * VE);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) v[i * VE + j] = -INFINITY;
-        }
-    }
+    load_part<T, NV>(x + head, vectors, begin, 256, v);
     // the row's odd ends: fewer than 2 * VE values
     const int odd = int(threadIdx.x) < head ? int(threadIdx.x) : vectors * VE + int(threadIdx.x);
     v[E - 1] = split == 0 && odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
@@ -309,7 +318,16 @@ struct JoinShared {
     uint64_t chosen[kBeamMax];
     double chosen_total[kBeamMax];
     uint32_t bound[THREADS / kWave];
-    int count;
+    int list[kRoom];  // lists whose best reaches the bound
+    int count, reaching;
+};
+
+struct JoinCandidate {
+    uint64_t key, place;  // ordered compared value; beam * vocab + token
+    double total;
+
+    __device__ __forceinline__ uint32_t high() const { return uint32_t(key >> 32); }
+    __device__ __forceinline__ bool reaches(uint32_t bound) const { return key && high() >= bound; }
 };
 
 // A beam's score and the divisor of its candidates.
@@ -320,111 +338,146 @@ __device__ __forceinline__ void join_beam(const BeamParams &p, JoinShared<THREAD
     sh.norm[beam] = p.penalty != 0.0 ? pow(double(p.lengths[row] + (ended ? 0 : 1)), p.penalty) : 1.0;
 }
 
-// The `width` best of a prompt's candidates: entries [0, entries) of its
-// beams' lists, entry(i, beam) being entry i's list value (0: none; a beam
-// without totals has the log_sum NaN), then the ended beams' own.  Called by the whole workgroup, behind a barrier that made
-// log_sum, norm and score of every beam visible.
-template <int THREADS, typename Entry>
-__device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t prompt, int entries, Entry entry) {
+// The `width` best of a prompt's candidates.  Each of its beams' `lists` lists
+// (entry(list, rank): the list's rank-th value, descending, 0 behind the last;
+// beam_of(list): its beam, which has the log_sum NaN where it has no totals) and
+// each ended beam has candidates in descending order.  A lower bound of the
+// width-th best one is found first, from all of them where a thread has few,
+// else from the lists' first ones; those that reach it are few.  Called by the
+// whole workgroup, behind a barrier that made log_sum, norm and score of every
+// beam visible.
+template <int THREADS, typename Entry, typename BeamOf>
+__device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t prompt, int lists, Entry entry,
+                           BeamOf beam_of) {
     constexpr int kRoom = JoinShared<THREADS>::kRoom;
+    constexpr int kKept = 4;  // candidates that a thread keeps
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
-    const int all = entries + (p.finished ? p.beams : 0);
-    // candidate i's ordered compared value (0: it has none), its place and total
-    auto candidate = [&](int i, uint64_t &place, double &total) -> uint64_t {
-        int beam;
-        if (i < entries) {
-            const uint64_t item = entry(i, beam);
-            if (!item) return 0;
-            place = uint64_t(beam) * uint32_t(p.vocab) + uint32_t(~uint32_t(item));
-            total = sh.score[beam] + (double(unordered(uint32_t(item >> 32))) - sh.log_sum[beam]);
-        } else {
-            beam = i - entries;
-            if (!p.finished[prompt * p.beams + beam]) return 0;
-            place = uint64_t(beam) * uint32_t(p.vocab) + uint64_t(p.eos);
-            total = sh.score[beam];
-        }
-        const double compared = total / sh.norm[beam];
-        return isfinite(compared) ? ordered(compared) : 0;
+    const int ended = p.finished ? p.beams : 0, all = lists + ended;
+    // the candidate of a list value, or an ended beam's own (key 0: there is none)
+    auto made = [&](int beam, uint64_t token, double total) {
+        const double value = p.penalty != 0.0 ? total / sh.norm[beam] : total;
+        return JoinCandidate{isfinite(value) ? ordered(value) : 0, uint64_t(beam) * uint32_t(p.vocab) + token, total};
     };
-    // a thread's first candidates stay in registers between the bound and the list
-    constexpr int kKept = 2;
-    uint64_t kept[kKept], kept_place[kKept], place = 0;
-    double kept_total[kKept], total = 0;
-    uint32_t mine = 0;
-#pragma unroll
-    for (int n = 0; n < kKept; ++n) {
-        kept[n] = 0;
-        if (thread + n * THREADS < all) kept[n] = candidate(thread + n * THREADS, kept_place[n], kept_total[n]);
-        mine = max(mine, uint32_t(kept[n] >> 32));
-    }
-    for (int i = thread + kKept * THREADS; i < all; i += THREADS) mine = max(mine, uint32_t(candidate(i, place, total) >> 32));
-    const uint32_t part = nth_of_lanes<24>(mine >> 8, p.width) << 8;
-    if (lane == 0) sh.bound[wave] = part;
-    if (thread == 0) sh.count = 0;
-    __syncthreads();
+    auto listed = [&](int list, uint64_t item) {
+        const int beam = beam_of(list);
+        JoinCandidate c = made(beam, uint32_t(~uint32_t(item)),
+                               sh.score[beam] + (double(unordered(uint32_t(item >> 32))) - sh.log_sum[beam]));
+        if (!item) c.key = 0;
+        return c;
+    };
+    auto candidate = [&](int list, int rank) {
+        if (list < lists) return listed(list, entry(list, rank));
+        const int beam = list - lists;
+        JoinCandidate c = made(beam, uint64_t(p.eos), sh.score[beam]);
+        if (rank || !p.finished[prompt * p.beams + beam]) c.key = 0;
+        return c;
+    };
     uint32_t bound = 0;
+    // the bound from each thread's best; empties the list
+    auto find_bound = [&](uint32_t best) {
+        const uint32_t part = nth_of_lanes<24>(best >> 8, p.width) << 8;
+        if (lane == 0) sh.bound[wave] = part;
+        if (thread == 0) sh.count = sh.reaching = 0;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / kWave; ++w) bound = max(bound, sh.bound[w]);
-    auto take = [&](uint64_t key) {
+        for (int w = 0; w < THREADS / kWave; ++w) bound = max(bound, sh.bound[w]);
+    };
+    auto take = [&](const JoinCandidate &c) {
         const int at = atomicAdd(&sh.count, 1);
         if (at < kRoom) {
-            sh.key[at] = key;
-            sh.place[at] = place;
-            sh.total[at] = total;
+            sh.key[at] = c.key;
+            sh.place[at] = c.place;
+            sh.total[at] = c.total;
         }
     };
+    uint32_t best = 0;
+    bool complete = true;
+    const int entries = lists * p.width;
+    if (entries <= kKept * THREADS) {
+        // the lists' first ones first, so that one wave holds many of the best
+        uint64_t item[kKept];
+        JoinCandidate kept[kKept + 1];
 #pragma unroll
-    for (int n = 0; n < kKept; ++n) {
-        if (kept[n] && uint32_t(kept[n] >> 32) >= bound) {
-            place = kept_place[n];
-            total = kept_total[n];
-            take(kept[n]);
+        for (int n = 0; n < kKept; ++n) {
+            if (n * THREADS >= entries) break;
+            const uint32_t i = uint32_t(min(thread + n * THREADS, entries - 1));
+            item[n] = entry(int(i % uint32_t(lists)), int(i / uint32_t(lists)));
         }
-    }
-    for (int i = thread + kKept * THREADS; i < all; i += THREADS) {
-        const uint64_t key = candidate(i, place, total);
-        if (key && uint32_t(key >> 32) >= bound) take(key);
+#pragma unroll
+        for (int n = 0; n <= kKept; ++n) {
+            kept[n] = JoinCandidate{0, 0, 0};
+            if (n == kKept && thread < ended) kept[n] = candidate(lists + thread, 0);
+            if (n < kKept && thread + n * THREADS < entries)
+                kept[n] = listed(int(uint32_t(thread + n * THREADS) % uint32_t(lists)), item[n]);
+            best = max(best, kept[n].high());
+        }
+        find_bound(best);
+#pragma unroll
+        for (int n = 0; n <= kKept; ++n)
+            if (kept[n].reaches(bound)) take(kept[n]);
+    } else {
+        // the lists whose best reaches the bound, then all of these
+        const uint32_t ranks = min(uint32_t(p.width), uint32_t(4 * p.width + lists - 1) / uint32_t(lists));
+        for (uint32_t i = thread; i < uint32_t(lists) * ranks; i += THREADS)
+            best = max(best, candidate(int(i % uint32_t(lists)), int(i / uint32_t(lists))).high());
+        find_bound(best);
+        for (int list = thread; list < all; list += THREADS)
+            if (candidate(list, 0).reaches(bound)) {
+                const int at = atomicAdd(&sh.reaching, 1);
+                if (at < kRoom) sh.list[at] = list;
+            }
+        __syncthreads();
+        complete = sh.reaching <= kRoom;
+        if (complete)
+            for (uint32_t i = thread; i < uint32_t(sh.reaching * p.width); i += THREADS) {
+                const uint32_t at = i / uint32_t(p.width);
+                const JoinCandidate c = candidate(sh.list[at], int(i - at * uint32_t(p.width)));
+                if (c.reaches(bound)) take(c);
+            }
     }
     __syncthreads();
-    if (sh.count > kRoom) {
+    if (!complete || sh.count > kRoom) {
         // more than LDS holds: the exact width-th value, then the lowest places of those equal to it
-        auto counted = [&](auto test) {
+        uint64_t value = 0, last = 0;
+        // how many candidates reach `next`, are above `value`, or equal it at a place below `next`; or takes them
+        auto go_through = [&](int what, uint64_t next) {
             __syncthreads();
             if (thread == 0) sh.count = 0;
             __syncthreads();
             int found = 0;
-            for (int i = thread; i < all; i += THREADS) {
-                const uint64_t key = candidate(i, place, total);
-                if (key && test(key, place)) ++found;
-            }
+            for (int list = thread; list < all; list += THREADS)
+                for (int rank = 0; rank < p.width; ++rank) {
+                    const JoinCandidate c = candidate(list, rank);
+                    if (!c.key) break;
+                    if (what == 0) found += c.key >= next;
+                    if (what == 1) found += c.key > value;
+                    if (what == 2) found += c.key == value && c.place < next;
+                    if (what == 3 && (c.key > value || (c.key == value && c.place <= last))) take(c);
+                }
             if (found) atomicAdd(&sh.count, found);
             __syncthreads();
             return sh.count;
         };
-        uint64_t value = 0, last = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const uint64_t next = value | (1ull << bit);
-            if (counted([&](uint64_t key, uint64_t) { return key >= next; }) >= p.width) value = next;
-        }
-        const int above = counted([&](uint64_t key, uint64_t) { return key > value; });
-        for (int bit = 63; bit >= 0; --bit) {
-            const uint64_t next = last | (1ull << bit);
-            if (counted([&](uint64_t key, uint64_t at) { return key == value && at < next; }) < p.width - above)
-                last = next;
-        }
-        __syncthreads();
-        if (thread == 0) sh.count = 0;
-        __syncthreads();
-        for (int i = thread; i < all; i += THREADS) {
-            const uint64_t key = candidate(i, place, total);
-            if (key && (key > value || (key == value && place <= last))) take(key);
-        }
-        __syncthreads();
+        for (int bit = 63; bit >= 0; --bit)
+            if (go_through(0, value | (1ull << bit)) >= p.width) value |= 1ull << bit;
+        const int above = go_through(1, 0);
+        for (int bit = 63; bit >= 0; --bit)
+            if (go_through(2, last | (1ull << bit)) < p.width - above) last |= 1ull << bit;
+        go_through(3, 0);
     }
     const int count = sh.count;
+    if (count > kWave) {
+        // as where one beam of a prompt has all the best: a bound from the candidates themselves leaves few to
+        // rank (300 of them took 30 us)
+        best = 0;
+        for (int i = thread; i < count; i += THREADS) best = max(best, uint32_t(sh.key[i] >> 32));
+        __syncthreads();
+        find_bound(best);
+    }
     // candidate i's rank, 64 others at a time (one at a time, 56 of them took 5.5 us)
     for (int i = wave; i < count; i += THREADS / kWave) {
         const uint64_t key = sh.key[i], at = sh.place[i];
+        if (uint32_t(key >> 32) < bound) continue;
         int rank = 0;
         for (int j = 0; j < count; j += kWave) {
             const int other = min(j + lane, count - 1);
@@ -492,14 +545,12 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamParams p) {
         if (lane == 0) sh.log_sum[beam] = double(high) + log(sum);
     }
     __syncthreads();
-    const int per_beam = p.splits * p.width;
-    const uint64_t *lists = p.lists + prompt * p.beams * per_beam;
-    const uint32_t rows = uint32_t(p.beams * p.splits);  // the lists' best first, so that one wave holds many of the best
-    join_beams<kJoinThreads>(p, sh, prompt, p.beams * per_beam, [&](int i, int &beam) {
-        const uint32_t rank = uint32_t(i) / rows, list = uint32_t(i) % rows;
-        beam = int(list / uint32_t(p.splits));
-        return lists[list * uint32_t(p.width) + rank];
-    });
+    const int rows = p.beams * p.splits;
+    const uint64_t *lists = p.lists + prompt * rows * p.width;
+    join_beams<kJoinThreads>(
+        p, sh, prompt, rows,
+        [&](int list, int rank) { return lists[uint32_t(list) * uint32_t(p.width) + uint32_t(rank)]; },
+        [&](int list) { return int(uint32_t(list) / uint32_t(p.splits)); });
 }
 
 // Small vocabularies, one launch: one workgroup a prompt, a wave a row.
@@ -525,16 +576,7 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
         const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
         const int vectors = (p.vocab - head) / VE;
         float v[E];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int at = i * kWave + lane;
-            if (at < vectors) {
-                Vec<T>::load(x + head + at * VE, v + i * VE);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VE; ++j) v[i * VE + j] = -INFINITY;
-            }
-        }
+        load_part<T, NV>(x + head, vectors, lane, kWave, v);
         const int odd = lane < head ? lane : vectors * VE + lane;
         v[E - 1] = odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
         auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
@@ -552,11 +594,10 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
     }
     if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
     __syncthreads();
-    join_beams<kRowWaves * kWave>(p, sh, prompt, p.beams * p.width, [&](int i, int &beam) {
-        const uint32_t rank = uint32_t(i) / uint32_t(p.beams);
-        beam = int(uint32_t(i) % uint32_t(p.beams));
-        return lists[uint32_t(beam) * uint32_t(p.width) + rank];
-    });
+    join_beams<kRowWaves * kWave>(
+        p, sh, prompt, p.beams,
+        [&](int list, int rank) { return lists[uint32_t(list) * uint32_t(p.width) + uint32_t(rank)]; },
+        [](int list) { return list; });
 }
 
 // How a call is cut: whole rows by a wave each (splits 0), or parts of `vectors` 16-byte vectors a thread.
