@@ -20,6 +20,8 @@
 // The exponentials and their sums are FP32 (each exponent relative to its
 // part's maximum), everything behind them is FP64: candidates of different
 // beams are compared by totals, which lie near each other.
+#include <cfloat>
+
 #include "bdm_common.h"
 
 namespace bdm {
@@ -151,13 +153,13 @@ __device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index
     if constexpr (WAVES > 1) {
         if (lane == 0) sh.sum[wave] = sum;
     }
-    if (mine >= bound && mine) {
+    const float least = bound ? unordered(bound << 16) : -FLT_MAX;
+    if (top >= least) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const uint32_t key = ordered(x[e]);
-            if (x[e] > -INFINITY && key >> 16 >= bound) {
+            if (x[e] >= least) {
                 const int at = atomicAdd(&sh.count, 1);
-                if (at < TeamShared<WAVES>::kRoom) sh.list[at] = uint64_t(key) << 32 | uint32_t(~index(e));
+                if (at < TeamShared<WAVES>::kRoom) sh.list[at] = uint64_t(ordered(x[e])) << 32 | uint32_t(~index(e));
             }
         }
     }
