@@ -137,6 +137,61 @@ def test_select_masked_rows(device, vocab, dtype):
     check(logits, scores, 3)
 
 
+@pytest.mark.parametrize('vocab', [1500, 12000, 50257])
+def test_select_contiguous_masks(device, vocab):
+    # the lowest value, zero and huge values in blocks, so that some lanes hold nothing else
+    logits, scores, _ = inputs(device, 4, 6, vocab, torch.float32, vocab + 2)
+    logits[0, :, : vocab // 2] = torch.finfo(torch.float32).min
+    logits[1, :, vocab // 3:] = -math.inf
+    logits[2, :, : vocab // 2] = -0.0
+    logits[2, :, vocab // 2: vocab // 2 + 40] = 0.0
+    logits[3, 2, 7] = 3e38
+    logits[3, 3] = -torch.rand(vocab, device=device) * 1e-30
+    check(logits, scores, 12)
+    check(logits.bfloat16(), scores, 12)
+
+
+JOINS = [
+    # batch, beams, vocabulary, width: each with more listed values than a workgroup's threads keep
+    (1, 16, 50257, 64), (1, 64, 50257, 12), (5, 64, 9000, 64), (9, 16, 50257, 50),
+]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+@pytest.mark.parametrize('size', JOINS, ids=lambda s: 'x'.join(map(str, s)))
+def test_select_joins_many_lists(device, size, dtype):
+    batch, beams, vocab, width = size
+    logits, scores, gen = inputs(device, batch, beams, vocab, dtype, sum(size))
+    check(logits, scores, width)
+    finished = torch.rand(batch, beams, generator=gen) < 0.3
+    lengths = torch.randint(1, 30, (batch, beams), generator=gen, dtype=torch.int32).to(device)
+    check(logits, scores, width, finished=finished.to(device), eos=11, lengths=lengths, length_penalty=0.8)
+
+
+@pytest.mark.parametrize('size', [(2, 8, 1000, 8), (2, 16, 50257, 16), (1, 16, 50257, 64), (2, 64, 9000, 48),
+                                  (1, 64, 131072, 8)],
+                         ids=lambda s: 'x'.join(map(str, s)))
+def test_select_one_beam_has_all_the_best(device, size):
+    # every other beam is far behind, or level with it in all its values: first few candidates near the bound, then
+    # more of them than are ranked at once, then more than are kept
+    batch, beams, vocab, width = size
+    logits, scores, _ = inputs(device, batch, beams, vocab, torch.float32, sum(size) + 1)
+    ahead = scores - 300
+    ahead[:, beams // 2] += 290
+    check(logits, ahead, width)
+    check(logits[:, :1].expand(-1, beams, -1), scores[:, :1].expand(-1, beams).contiguous(), width)
+    flat = torch.zeros_like(logits)
+    check(flat, scores[:, :1].expand(-1, beams).contiguous(), width)
+    near = flat.clone()
+    near[..., : 3 * width] = 1.0
+    finished = torch.zeros(batch, beams, dtype=torch.bool, device=device)
+    finished[:, beams // 3] = True
+    level = scores[:, :1].expand(-1, beams).contiguous()
+    level[:, beams // 3] -= math.log(vocab)
+    lengths = torch.full((batch, beams), 9, dtype=torch.int32, device=device)
+    check(near, level, width, finished=finished, eos=5, lengths=lengths, length_penalty=0.7)
+
+
 @pytest.mark.parametrize('vocab', [100, 2048, 2049, 30001])
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
 def test_select_ties(device, vocab, dtype):
