@@ -14,8 +14,14 @@
 // is near the W-th best of the lanes' own maxima, found by bisection with one
 // ballot a bit; the few values at or above the bound go to LDS and are ranked
 // there by counting.  Where ties or an unlucky layout put more there than it
-// holds, the exact W-th value and index are found by bisection over all their
-// bits instead.
+// holds, the exact W-th value is found instead, and of those equal to it the
+// first (equal logits, 64 prompts of 16 beams: 94 us).
+//
+// What bounds it: one read of the logits for large calls (64 prompts of 16
+// beams over 50,257: FP32 44.6 us of which the scan 36, 4.6 TB/s; BF16 41 us,
+// there the arithmetic of a value, the widening, maximum and exponential), for
+// small ones the chain of a load, two selections and their barriers (4 beams
+// over 192 tokens: 5.6 us).
 //
 // The exponentials and their sums are FP32 (each exponent relative to its
 // part's maximum), everything behind them is FP64: candidates of different
@@ -76,35 +82,59 @@ __device__ __forceinline__ float wave_sum(float x) {
         return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
     }));
 }
+// The sum of the first row's 16 lanes.
+__device__ __forceinline__ uint32_t row_sum(uint32_t x) {
+    auto with = [&](auto step) {
+        x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), decltype(step)::value, 0xf, 0xf, false));
+    };
+    with(std::integral_constant<int, 0x111>{});
+    with(std::integral_constant<int, 0x112>{});
+    with(std::integral_constant<int, 0x114>{});
+    with(std::integral_constant<int, 0x118>{});
+    return uint32_t(__builtin_amdgcn_readlane(int(x), 15));
+}
 __device__ __forceinline__ int popcount(uint64_t m) { return __popcll(m); }
 
-// A lower bound of the nth largest of the lanes' ordered values (0: the lane
-// has none), one of them itself; 0 where fewer lanes have one.  Bisected, a
-// ballot a bit, over where the values lie between the lowest and the highest
-// of them, in 256 parts: 9 ballots in the place of the 16 of the patterns' top
-// half, and as near where the lanes are like each other (8 prompts of 8 beams
-// over 50,257 BF16 logits: 13.6 -> 12.1 us, 64 of 16: 45.4 -> 40.9).
-__device__ __forceinline__ uint32_t nth_of_lanes(uint32_t value, int nth) {
+// Lower bounds of the nth largest of the lanes' ordered values (0: the lane has
+// none) for several n, each one of them itself; 0 where fewer lanes have one.
+// Bisected, a ballot a bit, over where the values lie between the lowest and
+// the highest of them, in 256 parts: 9 ballots in the place of the 16 of the
+// patterns' top half, and as near where the lanes are like each other (8
+// prompts of 8 beams over 50,257 BF16 logits: 13.6 -> 12.1 us, 64 of 16: 45.4
+// -> 40.9).
+template <int N>
+struct Bounds {
+    uint32_t at[N];
+};
+template <int N>
+__device__ __forceinline__ Bounds<N> nth_of_lanes(uint32_t value, Bounds<N> nth) {
     const uint32_t high = wave_max(value), low = wave_min(value ? value : UINT32_MAX), range = high - low;
     const int shift = max(0, 24 - __clz(int(range | 1)));
     const uint32_t part = value ? ((value - low) >> shift) + 1 : 0;
-    uint32_t bound = 0;
+    Bounds<N> bound{};
 #pragma unroll
     for (int bit = 8; bit >= 0; --bit) {
-        const uint32_t next = bound | (1u << bit);
-        if (popcount(__ballot(part >= next)) >= nth) bound = next;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint32_t next = bound.at[n] | (1u << bit);
+            if (uint32_t(popcount(__ballot(part >= next))) >= nth.at[n]) bound.at[n] = next;
+        }
     }
-    return bound ? wave_min(part >= bound ? value : UINT32_MAX) : 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) bound.at[n] = bound.at[n] ? wave_min(part >= bound.at[n] ? value : UINT32_MAX) : 0;
+    return bound;
 }
 
 // ------------------------------------------------------------------ a team's part of a row
-// A team of WAVES waves holds E values a lane: its shared memory.
+// A team of WAVES waves holds NV vectors of VE values a lane, and one more: its shared memory.
 template <int WAVES>
 struct TeamShared {
     static constexpr int kRoom = 256 * WAVES;
     uint64_t list[kRoom];  // ordered value, then ~index: descending order is value, then lowest index
     float high[WAVES], sum[WAVES];
-    uint32_t bound[WAVES];
+    uint32_t bound[WAVES], share[WAVES];
+    int found[WAVES];
+    int ties[WAVES][10];
     int count;
 };
 
@@ -119,54 +149,135 @@ __device__ __forceinline__ void team_sync() {
     }
 }
 
-// How many of the team's values satisfy test(value, index), in every lane; read(e, index) loads value e again.
-template <int WAVES, int E, typename Read, typename F>
-__device__ int team_count(TeamShared<WAVES> &sh, int lane, Read read, F test) {
+// How many of the team's values are above `than`, or at least that.
+template <int WAVES, int E>
+__device__ __forceinline__ int team_count(TeamShared<WAVES> &sh, const float (&x)[E], float than, bool level, int wave,
+                                          int lane) {
     int mine = 0;
-#pragma unroll 1
-    for (int e = 0; e < E; ++e) {
-        uint32_t index;
-        const float x = read(e, index);
-        mine += popcount(__ballot(x > -INFINITY && test(ordered(x), index)));
-    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine += popcount(__ballot(level ? x[e] >= than : x[e] > than));
     if constexpr (WAVES > 1) {
-        if (threadIdx.x == 0) sh.count = 0;
+        if (lane == 0) sh.found[wave] = mine;
         __syncthreads();
-        if (lane == 0) atomicAdd(&sh.count, mine);
-        __syncthreads();
-        mine = sh.count;
+        mine = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) mine += sh.found[i];
         __syncthreads();
     }
     return mine;
 }
 
+// The exact `width` best of the team's values to sh.list, where more than it
+// holds reach `least`: those above the width-th, then of those equal to it the
+// ones of lowest index, which lie in the order of vectors, lanes, places in the
+// vector; the odd ones before or behind all of these.  Where fewer than width
+// are above `least` (equal logits, or a mask of the type's lowest value over
+// most of the row) it is the width-th itself; else that is bisected.
+template <int WAVES, int NV, int VE, typename Index>
+__device__ __forceinline__ int team_ties(TeamShared<WAVES> &sh, const float (&x)[NV * VE + 1], Index index,
+                                         bool odd_first, float least, int width, int wave, int lane) {
+    constexpr int E = NV * VE + 1, kGroups = NV + 2;
+    static_assert(kGroups <= 10);
+    float value = least;
+    int above = team_count<WAVES, E>(sh, x, value, false, wave, lane);
+    if (above >= width) {
+        uint32_t found = 0;
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; --bit) {
+            // patterns beyond the infinities are NaN: no value reaches them
+            const uint32_t next = found | (1u << bit);
+            if (team_count<WAVES, E>(sh, x, unordered(next), true, wave, lane) >= width) found = next;
+        }
+        value = unordered(found);
+        above = team_count<WAVES, E>(sh, x, value, false, wave, lane);
+    }
+    const bool odd = x[E - 1] == value;
+    int ties[kGroups];
+    ties[0] = popcount(__ballot(odd && odd_first));
+    ties[NV + 1] = popcount(__ballot(odd && !odd_first));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        ties[i + 1] = 0;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) ties[i + 1] += popcount(__ballot(x[i * VE + j] == value));
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) sh.ties[wave][g] = ties[g];
+    }
+    if (wave == 0 && lane == 0) sh.count = 0;
+    team_sync<WAVES>();
+    auto take = [&](int e) {
+        sh.list[atomicAdd(&sh.count, 1)] = uint64_t(ordered(x[e])) << 32 | uint32_t(~index(e));
+    };
+    int before = above;  // candidates ahead of the group's, in this wave's order
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        int at = before;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            at += w < wave ? sh.ties[w][g] : 0;
+            before += sh.ties[w][g];
+        }
+        if (at >= width) continue;
+        if (g == 0 || g == NV + 1) {
+            const bool mine = odd && odd_first == (g == 0);
+            const uint64_t lanes = __ballot(mine);
+            if (mine && at + popcount(lanes & ((1ull << lane) - 1)) < width) take(E - 1);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) at += popcount(__ballot(x[(g - 1) * VE + j] == value) & ((1ull << lane) - 1));
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if (x[(g - 1) * VE + j] == value && at++ < width) take((g - 1) * VE + j);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (x[e] > value) take(e);
+    team_sync<WAVES>();
+    return sh.count;
+}
+
 // Maximum, sum of exponentials and the `width` best of the team's values
-// (index(e) is value e's index): sets high and sum in every lane, leaves the
+// (load(x) gets them, index(e) is value e's index, odd_first whether the last
+// one's is lower than the vectors'): sets high and sum in every lane, leaves the
 // candidates in sh.list and returns how many there are.  Values of -inf are no
-// candidates.  read(e, index) loads a value and its index once more, for the
-// few parts with too many ties: kept alive for those, the values and their
-// patterns took 108 registers of a lane with 33, and half the waves.
-template <int WAVES, int E, typename Index, typename Read>
-__device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index, Read read, int width, int wave,
-                         int lane, float &high, float &sum) {
+// candidates.  The few parts with too many ties load their values once more:
+// kept alive for those, the values and their patterns took 108 registers of a
+// lane with 33, and half the waves.
+template <int WAVES, int NV, int VE, typename Load, typename Index>
+__device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index index, bool odd_first, int width,
+                                         int wave, int lane, float &high, float &sum) {
+    constexpr int E = NV * VE + 1;
+    float x[E];
+    load(x);
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
-    uint32_t bound = nth_of_lanes(top > -INFINITY ? ordered(top) : 0u, width);
+    const uint32_t mine = top > -INFINITY ? ordered(top) : 0u;
+    uint32_t bound;
     high = wave_max(top);
     if constexpr (WAVES > 1) {
+        // width lanes of one wave, or as many of all of them together, reach the bound
+        const Bounds<2> bounds = nth_of_lanes<2>(mine, {{uint32_t(width), uint32_t(width + WAVES - 1) / WAVES}});
         if (lane == 0) {
             sh.high[wave] = high;
-            sh.bound[wave] = bound;
+            sh.bound[wave] = bounds.at[0];
+            sh.share[wave] = bounds.at[1];
         }
         if (threadIdx.x == 0) sh.count = 0;
         __syncthreads();
+        bound = sh.share[0];
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) bound = min(bound, sh.share[i]);
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) {
             high = fmaxf(high, sh.high[i]);
             bound = max(bound, sh.bound[i]);
         }
     } else {
+        bound = nth_of_lanes<1>(mine, {{uint32_t(width)}}).at[0];
         if (lane == 0) sh.count = 0;
         team_sync<WAVES>();
     }
@@ -191,40 +302,17 @@ __device__ int team_scan(TeamShared<WAVES> &sh, const float (&x)[E], Index index
         }
     }
     team_sync<WAVES>();
-    int count = sh.count;
+    const int count = sh.count;
     if constexpr (WAVES > 1) {
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) sum += sh.sum[i];
     }
     if (count <= TeamShared<WAVES>::kRoom) return count;
-    // too many at or above the bound: the exact width-th value, then the lowest indices of those equal to it
     team_sync<WAVES>();
-    uint32_t value = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t next = value | (1u << bit);
-        if (team_count<WAVES, E>(sh, lane, read, [&](uint32_t key, uint32_t) { return key >= next; }) >= width) value = next;
-    }
-    const int above = team_count<WAVES, E>(sh, lane, read, [&](uint32_t key, uint32_t) { return key > value; });
-    uint32_t last = 0;  // the largest bound with fewer than width - above of the equal ones below it
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t next = last | (1u << bit);
-        if (team_count<WAVES, E>(sh, lane, read, [&](uint32_t key, uint32_t at) { return key == value && at < next; }) <
-            width - above)
-            last = next;
-    }
-    if (WAVES > 1 ? threadIdx.x == 0 : lane == 0) sh.count = 0;
-    team_sync<WAVES>();
-#pragma unroll 1
-    for (int e = 0; e < E; ++e) {
-        uint32_t at;
-        const float v = read(e, at);
-        const uint32_t key = ordered(v);
-        if (v > -INFINITY && (key > value || (key == value && at <= last)))
-            sh.list[atomicAdd(&sh.count, 1)] = uint64_t(key) << 32 | uint32_t(~at);
-    }
-    team_sync<WAVES>();
-    return sh.count;
+    float again[E];
+    load(again);
+    return team_ties<WAVES, NV, VE>(sh, again, index, odd_first, least, width, wave, lane);
 }
 
 // The team's candidates in descending order, the first `width` of them to out, 0 behind the last.
@@ -316,20 +404,16 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
                  int64_t(row % uint32_t(p.beams)) * p.beam_stride;
     const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
     const int vectors = (p.vocab - head) / VE;
-    float v[E];
     const int begin = split * NV * 256 + int(threadIdx.x);
-    load_part<T, NV>(x + head, vectors, begin, 256, v);
     // the row's odd ends: fewer than 2 * VE values
     const int odd = int(threadIdx.x) < head ? int(threadIdx.x) : vectors * VE + int(threadIdx.x);
-    v[E - 1] = split == 0 && odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
-    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (begin + e / VE * 256) * VE + e % VE); };
-    auto read = [&](int e, uint32_t &at) {
-        at = index(e);
-        const bool held = e == E - 1 ? split == 0 && odd < p.vocab : begin + e / VE * 256 < vectors;
-        return held ? to_f32(x[at]) : -INFINITY;
+    auto load = [&](float(&v)[E]) {
+        load_part<T, NV>(x + head, vectors, begin, 256, v);
+        v[E - 1] = split == 0 && odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
     };
+    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (begin + e / VE * 256) * VE + e % VE); };
     float high, sum;
-    const int count = team_scan<4, E>(sh, v, index, read, p.width, wave, lane, high, sum);
+    const int count = team_scan<4, NV, VE>(sh, load, index, odd < head, p.width, wave, lane, high, sum);
     const int64_t part = int64_t(row) * p.splits + split;
     if (threadIdx.x == 0) p.parts[part] = make_float2(high, sum);
     uint64_t *out = p.lists + part * p.width;
@@ -339,25 +423,91 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
 // ------------------------------------------------------------------ joining a prompt's beams
 template <int THREADS>
 struct JoinShared {
-    static constexpr int kRoom = 1024;
+    static constexpr int kRoom = THREADS, kWaves = THREADS / kWave;
     double log_sum[kBeamMax], norm[kBeamMax], score[kBeamMax];
     uint64_t key[kRoom];    // ordered compared value
     uint64_t place[kRoom];  // beam * vocab + token
     double total[kRoom];
     uint64_t chosen[kBeamMax];
     double chosen_total[kBeamMax];
-    uint32_t bound[THREADS / kWave];
+    uint32_t bound[3][kWaves];
+    uint2 found[2][kWaves];
     int list[kRoom];  // lists whose best reaches the bound
     int count, reaching;
 };
 
+// What a candidate has to reach: a compared value, and among those equal to it a place.
+struct JoinBound {
+    uint64_t key, place;
+};
+
 struct JoinCandidate {
-    uint64_t key, place;  // ordered compared value; beam * vocab + token
+    uint64_t key, place;  // ordered compared value, 0: there is none; beam * vocab + token
     double total;
 
     __device__ __forceinline__ uint32_t high() const { return uint32_t(key >> 32); }
-    __device__ __forceinline__ bool reaches(uint32_t bound) const { return key && high() >= bound; }
+    __device__ __forceinline__ bool reaches(const JoinBound &b) const {
+        return key && (key > b.key || (key == b.key && place <= b.place));
+    }
 };
+
+// The `width` best of the `count` > width candidates that sh holds, a thread
+// each: the others are dropped.  The width-th value is found two bits at a time
+// from the top, until exactly width are left, then among equal ones the
+// width-th place, which has place_bits bits; a step is three ballots and a
+// barrier.  Returns what the last one reaches.
+template <int THREADS>
+__device__ JoinBound join_cut(JoinShared<THREADS> &sh, int count, int width, int place_bits) {
+    constexpr int kWaves = JoinShared<THREADS>::kWaves;
+    const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
+    const uint64_t key = thread < count ? sh.key[thread] : 0, place = thread < count ? sh.place[thread] : 0;
+    const double total = thread < count ? sh.total[thread] : 0;
+    int turn = 0;
+    // how many threads satisfy each of three conditions, the waves' counts summed in a row of lanes
+    auto counts = [&](bool a, bool b, bool c, int (&sum)[3]) {
+        const uint32_t low = uint32_t(popcount(__ballot(a))) | uint32_t(popcount(__ballot(b))) << 16;
+        const uint32_t high = uint32_t(popcount(__ballot(c)));
+        if (lane == 0) sh.found[turn][wave] = make_uint2(low, high);
+        __syncthreads();
+        uint2 all = sh.found[turn][lane % kWaves];
+        if (lane >= kWaves) all = make_uint2(0, 0);
+        const uint32_t pair = row_sum(all.x);
+        sum[0] = int(pair & 0xffff), sum[1] = int(pair >> 16), sum[2] = int(row_sum(all.y));
+        turn ^= 1;
+    };
+    JoinBound bound{0, UINT64_MAX};
+    int reach = count, sum[3];
+    for (int shift = 62; shift >= 0 && reach > width; shift -= 2) {
+        const uint64_t one = uint64_t(1) << shift, next = bound.key;
+        counts(key >= next + one, key >= next + 2 * one, key >= next + 3 * one, sum);
+#pragma unroll
+        for (int s = 0; s < 3; ++s)
+            if (sum[s] >= width) bound.key = next + uint64_t(s + 1) * one, reach = sum[s];
+    }
+    if (reach > width) {
+        counts(key > bound.key, false, false, sum);
+        const int need = width - sum[0];
+        const bool level = key == bound.key;
+        bound.place = 0;  // the largest with fewer than `need` places below it
+        for (int shift = place_bits & ~1; shift >= 0; shift -= 2) {
+            const uint64_t one = uint64_t(1) << shift, next = bound.place;
+            counts(level && place < next + one, level && place < next + 2 * one, level && place < next + 3 * one, sum);
+#pragma unroll
+            for (int s = 0; s < 3; ++s)
+                if (sum[s] < need) bound.place = next + uint64_t(s + 1) * one;
+        }
+    }
+    if (thread == 0) sh.count = 0;
+    __syncthreads();
+    if (key > bound.key || (key && key == bound.key && place <= bound.place)) {
+        const int at = atomicAdd(&sh.count, 1);
+        sh.key[at] = key;
+        sh.place[at] = place;
+        sh.total[at] = total;
+    }
+    __syncthreads();
+    return bound;
+}
 
 // A beam's score and the divisor of its candidates.
 template <int THREADS>
@@ -372,17 +522,22 @@ __device__ __forceinline__ void join_beam(const BeamParams &p, JoinShared<THREAD
 // beam_of(list): its beam, which has the log_sum NaN where it has no totals) and
 // each ended beam has candidates in descending order.  A lower bound of the
 // width-th best one is found first, from all of them where a thread has few,
-// else from the lists' first ones; those that reach it are few.  Called by the
-// whole workgroup, behind a barrier that made log_sum, norm and score of every
-// beam visible.
-template <int THREADS, typename Entry, typename BeamOf>
+// else from the lists' first ones; those that reach it go to LDS.  Where they
+// are more than a wave, the width best of what LDS took are cut out, and where
+// they are more than LDS holds, the last of these is the next bound: each turn
+// leaves fewer.  FEW: a thread always has few.  Called by the whole workgroup, behind a barrier that made
+// log_sum, norm and score of every beam visible.
+template <int THREADS, bool FEW, typename Entry, typename BeamOf>
 __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t prompt, int lists, Entry entry,
                            BeamOf beam_of) {
-    constexpr int kRoom = JoinShared<THREADS>::kRoom;
+    constexpr int kRoom = JoinShared<THREADS>::kRoom, kWaves = THREADS / kWave;
     constexpr int kKept = 4;  // candidates that a thread keeps
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
+    // few of the best: one wave has them all; more: neighbours, as the lists of one beam, lie in different waves
+    const bool wide = !FEW && p.width > 16;
+    const int slot = wide ? lane * kWaves + wave : thread;
     const int ended = p.finished ? p.beams : 0, all = lists + ended;
-    // the candidate of a list value, or an ended beam's own (key 0: there is none)
+    // the candidate of a list value, or an ended beam's own
     auto made = [&](int beam, uint64_t token, double total) {
         const double value = p.penalty != 0.0 ? total / sh.norm[beam] : total;
         return JoinCandidate{isfinite(value) ? ordered(value) : 0, uint64_t(beam) * uint32_t(p.vocab) + token, total};
@@ -401,15 +556,40 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
         if (rank || !p.finished[prompt * p.beams + beam]) c.key = 0;
         return c;
     };
-    uint32_t bound = 0;
-    // the bound from each thread's best; empties the list
-    auto find_bound = [&](uint32_t best) {
-        const uint32_t part = nth_of_lanes(best, p.width);
-        if (lane == 0) sh.bound[wave] = part;
+    // the bound from each thread's best: width lanes of a wave reach it, or, for the wider ones, a quarter of that
+    // in each of four waves, or as many in all of them together
+    auto first_bound = [&](uint32_t best) {
+        const uint32_t w = uint32_t(p.width);
+        uint32_t bound = 0;
         if (thread == 0) sh.count = sh.reaching = 0;
-        __syncthreads();
+        if (!wide) {
+            const Bounds<1> part = nth_of_lanes<1>(best, {{w}});
+            if (lane == 0) sh.bound[0][wave] = part.at[0];
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < THREADS / kWave; ++w) bound = max(bound, sh.bound[w]);
+            for (int i = 0; i < kWaves; ++i) bound = max(bound, sh.bound[0][i]);
+        } else {
+            const Bounds<3> part = nth_of_lanes<3>(best, {{w, (w + 3) / 4, (w + kWaves - 1) / kWaves}});
+            if (lane == 0) {
+#pragma unroll
+                for (int n = 0; n < 3; ++n) sh.bound[n][wave] = part.at[n];
+            }
+            __syncthreads();
+            uint32_t every = UINT32_MAX;
+#pragma unroll
+            for (int i = 0; i < kWaves; i += 4) {
+                uint32_t group = UINT32_MAX;
+#pragma unroll
+                for (int j = i; j < i + 4; ++j) {
+                    bound = max(bound, sh.bound[0][j]);
+                    group = min(group, sh.bound[1][j]);
+                    every = min(every, sh.bound[2][j]);
+                }
+                bound = max(bound, group);
+            }
+            bound = max(bound, every);
+        }
+        return JoinBound{uint64_t(bound) << 32, UINT64_MAX};
     };
     auto take = [&](const JoinCandidate &c) {
         const int at = atomicAdd(&sh.count, 1);
@@ -419,100 +599,79 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
             sh.total[at] = c.total;
         }
     };
+    // cuts what LDS took down to a wave: by a bound from it, then exactly; whether there was more
+    auto cut = [&](JoinBound &bound) {
+        __syncthreads();
+        const int reached = sh.count;
+        if (reached <= kWave) return false;
+        JoinCandidate mine{0, 0, 0};
+        if (thread < min(reached, kRoom)) mine = JoinCandidate{sh.key[thread], sh.place[thread], sh.total[thread]};
+        __syncthreads();
+        const JoinBound next = first_bound(mine.high());
+        if (next.key > bound.key) bound = next;
+        if (mine.reaches(next)) take(mine);
+        __syncthreads();
+        const int left = sh.count;
+        if (left > kWave) bound = join_cut(sh, left, p.width, 64 - __clzll(uint64_t(p.beams) * uint32_t(p.vocab)));
+        if (reached <= kRoom) return false;
+        __syncthreads();
+        if (thread == 0) sh.count = sh.reaching = 0;
+        __syncthreads();
+        return true;
+    };
     uint32_t best = 0;
-    bool complete = true;
     const int entries = lists * p.width;
-    if (entries <= kKept * THREADS) {
-        // the lists' first ones first, so that one wave holds many of the best
+    if (FEW || entries <= kKept * THREADS) {
+        // the lists' first ones first, so that the best of many threads are high
         uint64_t item[kKept];
         JoinCandidate kept[kKept + 1];
 #pragma unroll
         for (int n = 0; n < kKept; ++n) {
             if (n * THREADS >= entries) break;
-            const uint32_t i = uint32_t(min(thread + n * THREADS, entries - 1));
+            const uint32_t i = uint32_t(min(slot + n * THREADS, entries - 1));
             item[n] = entry(int(i % uint32_t(lists)), int(i / uint32_t(lists)));
         }
 #pragma unroll
         for (int n = 0; n <= kKept; ++n) {
             kept[n] = JoinCandidate{0, 0, 0};
-            if (n == kKept && thread < ended) kept[n] = candidate(lists + thread, 0);
-            if (n < kKept && thread + n * THREADS < entries)
-                kept[n] = listed(int(uint32_t(thread + n * THREADS) % uint32_t(lists)), item[n]);
+            if (n == kKept && slot < ended) kept[n] = candidate(lists + slot, 0);
+            if (n < kKept && slot + n * THREADS < entries)
+                kept[n] = listed(int(uint32_t(slot + n * THREADS) % uint32_t(lists)), item[n]);
             best = max(best, kept[n].high());
         }
-        find_bound(best);
+        JoinBound bound = first_bound(best);
+        do {
 #pragma unroll
-        for (int n = 0; n <= kKept; ++n)
-            if (kept[n].reaches(bound)) take(kept[n]);
+            for (int n = 0; n <= kKept; ++n)
+                if (kept[n].reaches(bound)) take(kept[n]);
+        } while (cut(bound));
     } else {
-        // the lists whose best reaches the bound, then all of these
-        const uint32_t ranks = min(uint32_t(p.width), uint32_t(4 * p.width + lists - 1) / uint32_t(lists));
-        for (uint32_t i = thread; i < uint32_t(lists) * ranks; i += THREADS)
+        const uint32_t ranks = min(uint32_t(p.width), uint32_t(THREADS + lists - 1) / uint32_t(lists));
+        for (uint32_t i = slot; i < uint32_t(lists) * ranks; i += THREADS)
             best = max(best, candidate(int(i % uint32_t(lists)), int(i / uint32_t(lists))).high());
-        find_bound(best);
-        for (int list = thread; list < all; list += THREADS)
-            if (candidate(list, 0).reaches(bound)) {
-                const int at = atomicAdd(&sh.reaching, 1);
-                if (at < kRoom) sh.list[at] = list;
-            }
-        __syncthreads();
-        complete = sh.reaching <= kRoom;
-        if (complete)
-            for (uint32_t i = thread; i < uint32_t(sh.reaching * p.width); i += THREADS) {
+        JoinBound bound = first_bound(best);
+        do {
+            // the lists whose best reaches the bound, then all of these (more than LDS holds: all of all)
+            for (int list = thread; list < all; list += THREADS)
+                if (candidate(list, 0).reaches(bound)) {
+                    const int at = atomicAdd(&sh.reaching, 1);
+                    if (at < kRoom) sh.list[at] = list;
+                }
+            __syncthreads();
+            const bool held = sh.reaching <= kRoom;
+            const uint32_t most = uint32_t(held ? sh.reaching : all) * uint32_t(p.width);
+            for (uint32_t i = thread; i < most; i += THREADS) {
                 const uint32_t at = i / uint32_t(p.width);
-                const JoinCandidate c = candidate(sh.list[at], int(i - at * uint32_t(p.width)));
+                const JoinCandidate c = candidate(held ? sh.list[at] : int(at), int(i - at * uint32_t(p.width)));
                 if (c.reaches(bound)) take(c);
             }
+        } while (cut(bound));
     }
-    __syncthreads();
-    if (!complete || sh.count > kRoom) {
-        // more than LDS holds: the exact width-th value, then the lowest places of those equal to it
-        uint64_t value = 0, last = 0;
-        // how many candidates reach `next`, are above `value`, or equal it at a place below `next`; or takes them
-        auto go_through = [&](int what, uint64_t next) {
-            __syncthreads();
-            if (thread == 0) sh.count = 0;
-            __syncthreads();
-            int found = 0;
-            for (int list = thread; list < all; list += THREADS)
-                for (int rank = 0; rank < p.width; ++rank) {
-                    const JoinCandidate c = candidate(list, rank);
-                    if (!c.key) break;
-                    if (what == 0) found += c.key >= next;
-                    if (what == 1) found += c.key > value;
-                    if (what == 2) found += c.key == value && c.place < next;
-                    if (what == 3 && (c.key > value || (c.key == value && c.place <= last))) take(c);
-                }
-            if (found) atomicAdd(&sh.count, found);
-            __syncthreads();
-            return sh.count;
-        };
-        for (int bit = 63; bit >= 0; --bit)
-            if (go_through(0, value | (1ull << bit)) >= p.width) value |= 1ull << bit;
-        const int above = go_through(1, 0);
-        for (int bit = 63; bit >= 0; --bit)
-            if (go_through(2, last | (1ull << bit)) < p.width - above) last |= 1ull << bit;
-        go_through(3, 0);
-    }
-    const int count = sh.count;
-    if (count > kWave) {
-        // as where one beam of a prompt has all the best: a bound from the candidates themselves leaves few to
-        // rank (300 of them took 30 us)
-        best = 0;
-        for (int i = thread; i < count; i += THREADS) best = max(best, uint32_t(sh.key[i] >> 32));
-        __syncthreads();
-        find_bound(best);
-    }
-    // candidate i's rank, 64 others at a time (one at a time, 56 of them took 5.5 us)
-    for (int i = wave; i < count; i += THREADS / kWave) {
-        const uint64_t key = sh.key[i], at = sh.place[i];
-        if (uint32_t(key >> 32) < bound) continue;
-        int rank = 0;
-        for (int j = 0; j < count; j += kWave) {
-            const int other = min(j + lane, count - 1);
-            const uint64_t k = sh.key[other], place_of = sh.place[other];
-            rank += popcount(__ballot(j + lane < count && (k > key || (k == key && place_of < at))));
-        }
+    const int count = sh.count;  // a wave of them at most
+    for (int i = wave; i < count; i += kWaves) {
+        const uint64_t key = sh.key[i], at = sh.place[i], k = sh.key[min(lane, count - 1)],
+                       place_of = sh.place[min(lane, count - 1)];
+        const int rank = popcount(__ballot(lane < count && (k > key || (k == key && place_of < at))));
         if (lane == 0 && rank < p.width) {
             sh.chosen[rank] = at;
             sh.chosen_total[rank] = sh.total[i];
@@ -576,7 +735,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamParams p) {
     __syncthreads();
     const int rows = p.beams * p.splits;
     const uint64_t *lists = p.lists + prompt * rows * p.width;
-    join_beams<kJoinThreads>(
+    join_beams<kJoinThreads, false>(
         p, sh, prompt, rows,
         [&](int list, int rank) { return lists[uint32_t(list) * uint32_t(p.width) + uint32_t(rank)]; },
         [&](int list) { return int(uint32_t(list) / uint32_t(p.splits)); });
@@ -584,14 +743,14 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamParams p) {
 
 // Small vocabularies, one launch: one workgroup a prompt, a wave a row.
 constexpr int kRowWaves = 8;
-constexpr int kRowLists = 1024;  // beams * width
+constexpr int kRowWidth = 16;
 
 template <typename T, int NV>
 __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams p) {
     constexpr int VE = Vec<T>::kSize, E = NV * VE + 1;
     __shared__ TeamShared<1> teams[kRowWaves];
     __shared__ JoinShared<kRowWaves * kWave> sh;
-    __shared__ uint64_t lists[kRowLists];
+    __shared__ uint64_t lists[2 * kRowWaves * kRowWidth];
     const int64_t prompt = blockIdx.x;
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     TeamShared<1> &team = teams[wave];
@@ -604,18 +763,14 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
         const T *x = static_cast<const T *>(p.logits) + prompt * p.batch_stride + beam * p.beam_stride;
         const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
         const int vectors = (p.vocab - head) / VE;
-        float v[E];
-        load_part<T, NV>(x + head, vectors, lane, kWave, v);
         const int odd = lane < head ? lane : vectors * VE + lane;
-        v[E - 1] = odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
-        auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
-        auto read = [&](int e, uint32_t &at) {
-            at = index(e);
-            const bool held = e == E - 1 ? odd < p.vocab : e / VE * kWave + lane < vectors;
-            return held ? to_f32(x[at]) : -INFINITY;
+        auto load = [&](float(&v)[E]) {
+            load_part<T, NV>(x + head, vectors, lane, kWave, v);
+            v[E - 1] = odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
         };
+        auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
         float high, sum;
-        const int count = team_scan<1, E>(team, v, index, read, p.width, 0, lane, high, sum);
+        const int count = team_scan<1, NV, VE>(team, load, index, odd < head, p.width, 0, lane, high, sum);
         uint64_t *out = lists + beam * p.width;
         team_rank<1>(team, count, p.width, 0, lane, out);
         if (lane == 0) sh.log_sum[beam] = double(high) + log(double(sum));
@@ -623,7 +778,8 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
     }
     if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
     __syncthreads();
-    join_beams<kRowWaves * kWave>(
+    static_assert(2 * kRowWaves * kRowWidth <= 4 * kRowWaves * kWave);
+    join_beams<kRowWaves * kWave, true>(
         p, sh, prompt, p.beams,
         [&](int list, int rank) { return lists[uint32_t(list) * uint32_t(p.width) + uint32_t(rank)]; },
         [](int list) { return list; });
@@ -634,9 +790,16 @@ struct BeamPlan {
     int vectors, splits;
 };
 
+// One launch for small vocabularies: 4 beams over 192 tokens 5.6 us, 8.8 as
+// two; 8 over 2048 7.7 and 9.8; 16 over 2048, of which a wave has two, 12.8 and
+// 11.3 for one prompt, 13.4 and 14.8 for 64.  Not for more than 16 of a row: a
+// lane's best bounds them badly (64 of 16 beams over 2048: 106 us, 33 as two).
+// The parts of a row are made smaller until there are 512 of them, two a
+// compute unit: 8 prompts of 8 beams over 50,257 BF16 logits take 12.3 us so,
+// 12.8 and 13.5 with 256 and 1024.
 BeamPlan beam_plan(const bdm_beam_args &a) {
     const int ve = a.dtype == BDM_BF16 ? Vec<bf16_t>::kSize : Vec<float>::kSize;
-    if (a.vocab <= 2048 && a.beams <= 2 * kRowWaves && a.beams * a.width <= kRowLists)
+    if (a.vocab <= 2048 && a.beams <= 2 * kRowWaves && a.width <= kRowWidth)
         return {a.vocab <= 512 ? 512 / (kWave * ve) : 2048 / (kWave * ve), 0};
     int vectors = 32 / ve;
     const int64_t rows = a.batch * a.beams;
