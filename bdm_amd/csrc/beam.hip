@@ -21,7 +21,7 @@
 // beams over 50,257: FP32 44.6 us of which the scan 36, 4.6 TB/s; BF16 41 us,
 // there the arithmetic of a value, the widening, maximum and exponential), for
 // small ones the chain of a load, two selections and their barriers (4 beams
-// over 192 tokens: 5.6 us).
+// over 192 tokens: 5.4 us).
 //
 // The exponentials and their sums are FP32 (each exponent relative to its
 // part's maximum), everything behind them is FP64: candidates of different
@@ -278,8 +278,6 @@ __device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index
         }
     } else {
         bound = nth_of_lanes<1>(mine, {{uint32_t(width)}}).at[0];
-        if (lane == 0) sh.count = 0;
-        team_sync<WAVES>();
     }
     // the sum relative to the part's maximum; a part without a finite value has the sum 0, one with a NaN
     // or +inf (inf - inf) a NaN
@@ -292,14 +290,33 @@ __device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index
         if (lane == 0) sh.sum[wave] = sum;
     }
     const float least = bound ? unordered(bound) : -FLT_MAX;
-    if (top >= least) {
+    if constexpr (WAVES > 1) {
+        if (top >= least) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (x[e] >= least) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < TeamShared<WAVES>::kRoom) sh.list[at] = uint64_t(ordered(x[e])) << 32 | uint32_t(~index(e));
+            for (int e = 0; e < E; ++e) {
+                if (x[e] >= least) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < TeamShared<WAVES>::kRoom)
+                        sh.list[at] = uint64_t(ordered(x[e])) << 32 | uint32_t(~index(e));
+                }
             }
         }
+    } else {
+        // without atomics, whose trips one row cannot hide (16 beams over 192 tokens: 9.7 us with them, 9.2 so; in
+        // large calls other rows hide them, and waves without candidates pass this by: 40.6 us, 43 so)
+        int found = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool reaches = x[e] >= least;
+            const uint64_t lanes = __ballot(reaches);
+            if (lanes) {
+                const int at = found + popcount(lanes & ((1ull << lane) - 1));
+                if (reaches && at < TeamShared<WAVES>::kRoom)
+                    sh.list[at] = uint64_t(ordered(x[e])) << 32 | uint32_t(~index(e));
+                found += popcount(lanes);
+            }
+        }
+        if (lane == 0) sh.count = found;
     }
     team_sync<WAVES>();
     const int count = sh.count;
@@ -790,9 +807,9 @@ struct BeamPlan {
     int vectors, splits;
 };
 
-// One launch for small vocabularies: 4 beams over 192 tokens 5.6 us, 8.8 as
-// two; 8 over 2048 7.7 and 9.8; 16 over 2048, of which a wave has two, 12.8 and
-// 11.3 for one prompt, 13.4 and 14.8 for 64.  Not for more than 16 of a row: a
+// One launch for small vocabularies: 4 beams over 192 tokens 5.4 us, 8.8 as
+// two; 8 over 2048 7.7 and 9.8; 16 over 2048, of which a wave has two, 12.1 and
+// 11.3 for one prompt, 12.7 and 14.8 for 64.  Not for more than 16 of a row: a
 // lane's best bounds them badly (64 of 16 beams over 2048: 106 us, 33 as two).
 // The parts of a row are made smaller until there are 512 of them, two a
 // compute unit: 8 prompts of 8 beams over 50,257 BF16 logits take 12.3 us so,
