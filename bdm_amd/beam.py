@@ -132,6 +132,8 @@ def beam_search(model, prompt: Tensor, *, beams: int, length: int, eos: int | No
             beam = parents[t].gather(1, beam) % beams
         result = BeamResult(out, search.scores, search.lengths)
     torch.cuda.current_stream(device).wait_stream(stream)
+    if captured is not None:
+        stream.synchronize()  # the last replay, before the graph and its memory go
     if graph:
         for t in result:
             t.record_stream(torch.cuda.current_stream(device))
