@@ -120,8 +120,26 @@ __device__ __forceinline__ Bounds<N> nth_of_lanes(uint32_t value, Bounds<N> nth)
             if (uint32_t(popcount(__ballot(part >= next))) >= nth.at[n]) bound.at[n] = next;
         }
     }
+    // parts of more than an eighth of their values, as where the lanes lie on both sides of zero: the one of the bound
+    // in 256 parts again (64 prompts of 8 beams over 1,024 tokens around zero: 19.8 -> 7.4 us)
+    const bool coarse = shift > 20;
 #pragma unroll
-    for (int n = 0; n < N; ++n) bound.at[n] = bound.at[n] ? wave_min(part >= bound.at[n] ? value : UINT32_MAX) : 0;
+    for (int n = 0; n < N; ++n) {
+        if (!bound.at[n]) continue;
+        bool reaches = part >= bound.at[n];
+        if (coarse) {
+            const uint32_t within = value - (low + ((bound.at[n] - 1) << shift));
+            const uint32_t finer = part > bound.at[n] ? 512 : reaches ? (within >> (shift - 8)) + 1 : 0;
+            uint32_t found = 0;
+#pragma unroll
+            for (int bit = 8; bit >= 0; --bit) {
+                const uint32_t next = found | (1u << bit);
+                if (uint32_t(popcount(__ballot(finer >= next))) >= nth.at[n]) found = next;
+            }
+            reaches = finer >= found;
+        }
+        bound.at[n] = wave_min(reaches ? value : UINT32_MAX);
+    }
     return bound;
 }
 
@@ -302,7 +320,7 @@ __device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index
             }
         }
     } else {
-        // without atomics, whose trips one row cannot hide (16 beams over 192 tokens: 9.7 us with them, 9.2 so; in
+        // without atomics, whose trips one row cannot hide (16 beams over 192 tokens: 9.6 us with them, 9.2 so; in
         // large calls other rows hide them, and waves without candidates pass this by: 40.6 us, 43 so)
         int found = 0;
 #pragma unroll
@@ -764,26 +782,22 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamParams p) {
 }
 
 // Small vocabularies, one launch: one workgroup a prompt, a wave a row.  Bound
-// by latency as the join is: 4 beams over 192 tokens 5.3 us.
-constexpr int kRowWaves = 8;
-constexpr int kRowWidth = 16;
+// by latency as the join is: 4 beams over 192 tokens 5.3 us.  A wave of its own
+// for each of 16 beams, not two beams for each of 8: 12.1 -> 9.9 us over 2048.
+constexpr int kRowBeams = 16, kRowWidth = 16;
 
-template <typename T, int NV>
-__global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams p) {
+template <typename T, int NV, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave) void beam_rows_kernel(BeamParams p) {
     constexpr int VE = Vec<T>::kSize, E = NV * VE + 1;
-    __shared__ TeamShared<1> teams[kRowWaves];
-    __shared__ JoinShared<kRowWaves * kWave> sh;
-    __shared__ uint64_t lists[2 * kRowWaves * kRowWidth];
+    __shared__ TeamShared<1> teams[WAVES];
+    __shared__ JoinShared<WAVES * kWave> sh;
+    __shared__ uint64_t lists[WAVES * kRowWidth];
     const int64_t prompt = blockIdx.x;
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     TeamShared<1> &team = teams[wave];
-    for (int beam = wave; beam < p.beams; beam += kRowWaves) {
-        const int64_t row = prompt * p.beams + beam;
-        if (!beam_live(p, row)) {  // no totals: its list is not written
-            if (lane == 0) sh.log_sum[beam] = NAN;
-            continue;
-        }
-        const T *x = static_cast<const T *>(p.logits) + prompt * p.batch_stride + beam * p.beam_stride;
+    const int64_t row = prompt * p.beams + wave;
+    if (wave < p.beams && beam_live(p, row)) {
+        const T *x = static_cast<const T *>(p.logits) + prompt * p.batch_stride + wave * p.beam_stride;
         const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
         const int vectors = (p.vocab - head) / VE;
         const int odd = lane < head ? lane : vectors * VE + lane;
@@ -794,15 +808,14 @@ __global__ __launch_bounds__(kRowWaves *kWave) void beam_rows_kernel(BeamParams 
         auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
         float high, sum;
         const int count = team_scan<1, NV, VE>(team, load, index, odd < head, p.width, 0, lane, high, sum);
-        uint64_t *out = lists + beam * p.width;
-        team_rank<1>(team, count, p.width, 0, lane, out);
-        if (lane == 0) sh.log_sum[beam] = double(high) + log(double(sum));
-        team_sync<1>();
+        team_rank<1>(team, count, p.width, 0, lane, lists + wave * p.width);
+        if (lane == 0) sh.log_sum[wave] = double(high) + log(double(sum));
+    } else if (wave < p.beams && lane == 0) {
+        sh.log_sum[wave] = NAN;  // no totals: its list is not written
     }
     if (int(threadIdx.x) < p.beams) join_beam(p, sh, prompt * p.beams + threadIdx.x, threadIdx.x);
     __syncthreads();
-    static_assert(2 * kRowWaves * kRowWidth <= 4 * kRowWaves * kWave);
-    join_beams<kRowWaves * kWave, true>(
+    join_beams<WAVES * kWave, true>(
         p, sh, prompt, p.beams,
         [&](int list, int rank) { return lists[uint32_t(list) * uint32_t(p.width) + uint32_t(rank)]; },
         [](int list) { return list; });
@@ -814,15 +827,15 @@ struct BeamPlan {
 };
 
 // One launch for small vocabularies: 4 beams over 192 tokens 5.4 us, 8.8 as
-// two; 8 over 2048 7.7 and 9.8; 16 over 2048, of which a wave has two, 12.1 and
-// 11.3 for one prompt, 12.7 and 14.8 for 64.  Not for more than 16 of a row: a
-// lane's best bounds them badly (64 of 16 beams over 2048: 106 us, 33 as two).
+// two; 8 over 2048 7.1 and 9.8; 16 over 2048 9.9 and 11.3 for one prompt, 10.5
+// and 14.8 for 64.  Not for more than 16 of a row: a lane's best bounds them
+// badly (64 of 16 beams over 2048: 106 us, 33 as two).
 // The parts of a row are made smaller until there are 512 of them, two a
 // compute unit: 8 prompts of 8 beams over 50,257 BF16 logits take 12.3 us so,
 // 12.8 and 13.5 with 256 and 1024.
 BeamPlan beam_plan(const bdm_beam_args &a) {
     const int ve = a.dtype == BDM_BF16 ? Vec<bf16_t>::kSize : Vec<float>::kSize;
-    if (a.vocab <= 2048 && a.beams <= 2 * kRowWaves && a.width <= kRowWidth)
+    if (a.vocab <= 2048 && a.beams <= kRowBeams && a.width <= kRowWidth)
         return {a.vocab <= 512 ? 512 / (kWave * ve) : 2048 / (kWave * ve), 0};
     int vectors = 32 / ve;
     const int64_t rows = a.batch * a.beams;
@@ -996,18 +1009,24 @@ extern "C" int bdm_beam_select(const bdm_beam_args *a, void *workspace, size_t w
     hipStream_t s = as_stream(stream);
     const unsigned prompts = unsigned(a->batch);
     if (plan.splits == 0) {
-        constexpr int threads = kRowWaves * kWave;
-        if (a->dtype == BDM_BF16) {
-            if (plan.vectors == 1)
-                beam_rows_kernel<bf16_t, 1><<<prompts, threads, 0, s>>>(p);
-            else
-                beam_rows_kernel<bf16_t, 4><<<prompts, threads, 0, s>>>(p);
-        } else {
-            if (plan.vectors == 2)
-                beam_rows_kernel<float, 2><<<prompts, threads, 0, s>>>(p);
-            else
-                beam_rows_kernel<float, 8><<<prompts, threads, 0, s>>>(p);
-        }
+        auto rows = [&](auto waves) {
+            constexpr int W = decltype(waves)::value;
+            if (a->dtype == BDM_BF16) {
+                if (plan.vectors == 1)
+                    beam_rows_kernel<bf16_t, 1, W><<<prompts, W * kWave, 0, s>>>(p);
+                else
+                    beam_rows_kernel<bf16_t, 4, W><<<prompts, W * kWave, 0, s>>>(p);
+            } else {
+                if (plan.vectors == 2)
+                    beam_rows_kernel<float, 2, W><<<prompts, W * kWave, 0, s>>>(p);
+                else
+                    beam_rows_kernel<float, 8, W><<<prompts, W * kWave, 0, s>>>(p);
+            }
+        };
+        if (a->beams <= 8)
+            rows(std::integral_constant<int, 8>{});
+        else
+            rows(std::integral_constant<int, 16>{});
         return check_launch("beam_rows_kernel");
     }
     if (a->dtype == BDM_BF16) {
