@@ -15,7 +15,7 @@
 // ballot a bit; the few values at or above the bound go to LDS and are ranked
 // there by counting.  Where ties or an unlucky layout put more there than it
 // holds, the exact W-th value is found instead, and of those equal to it the
-// first (equal logits, 64 prompts of 16 beams: 94 us).
+// first (equal logits, 64 prompts of 16 beams over 50,257: 85 us).
 //
 // What bounds it: one read of the logits for large calls (64 prompts of 16
 // beams over 50,257: FP32 44.6 us of which the scan 36, 4.6 TB/s; BF16 41 us,
@@ -490,22 +490,27 @@ struct JoinCandidate {
 };
 
 // The `width` best of the `count` > width candidates that sh holds, a thread
-// each: the others are dropped.  The width-th value is found two bits at a time
-// from the top, until exactly width are left, then among equal ones the
-// width-th place, which has place_bits bits; a step is three ballots and a
-// barrier.  Returns what the last one reaches.
+// each: the others are dropped.  The width-th one is found two bits at a time
+// from the top, a step three ballots and a barrier: by the upper half of its
+// key, among those equal in that by the lower half, and then by the place (of
+// place_bits bits), as far as more than width are left.  Returns what the last
+// one reaches.
 template <int THREADS>
 __device__ JoinBound join_cut(JoinShared<THREADS> &sh, int count, int width, int place_bits) {
     constexpr int kWaves = JoinShared<THREADS>::kWaves;
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
+    const bool held = wave * kWave < count;  // a wave without candidates only keeps the barriers
     const uint64_t key = thread < count ? sh.key[thread] : 0, place = thread < count ? sh.place[thread] : 0;
     const double total = thread < count ? sh.total[thread] : 0;
     int turn = 0;
     // how many threads satisfy each of three conditions, the waves' counts summed in a row of lanes
     auto counts = [&](bool a, bool b, bool c, int (&sum)[3]) {
-        const uint32_t low = uint32_t(popcount(__ballot(a))) | uint32_t(popcount(__ballot(b))) << 16;
-        const uint32_t high = uint32_t(popcount(__ballot(c)));
-        if (lane == 0) sh.found[turn][wave] = make_uint2(low, high);
+        uint2 mine = make_uint2(0, 0);
+        if (held) {
+            mine.x = uint32_t(popcount(__ballot(a))) | uint32_t(popcount(__ballot(b))) << 16;
+            mine.y = uint32_t(popcount(__ballot(c)));
+        }
+        if (lane == 0) sh.found[turn][wave] = mine;
         __syncthreads();
         uint2 all = sh.found[turn][lane % kWaves];
         if (lane >= kWaves) all = make_uint2(0, 0);
@@ -513,31 +518,48 @@ __device__ JoinBound join_cut(JoinShared<THREADS> &sh, int count, int width, int
         sum[0] = int(pair & 0xffff), sum[1] = int(pair >> 16), sum[2] = int(row_sum(all.y));
         turn ^= 1;
     };
-    JoinBound bound{0, UINT64_MAX};
-    int reach = count, sum[3];
-    for (int shift = 62; shift >= 0 && reach > width; shift -= 2) {
-        const uint64_t one = uint64_t(1) << shift, next = bound.key;
-        counts(key >= next + one, key >= next + 2 * one, key >= next + 3 * one, sum);
-#pragma unroll
-        for (int s = 0; s < 3; ++s)
-            if (sum[s] >= width) bound.key = next + uint64_t(s + 1) * one, reach = sum[s];
-    }
-    if (reach > width) {
-        counts(key > bound.key, false, false, sum);
-        const int need = width - sum[0];
-        const bool level = key == bound.key;
-        bound.place = 0;  // the largest with fewer than `need` places below it
-        for (int shift = place_bits & ~1; shift >= 0; shift -= 2) {
-            const uint64_t one = uint64_t(1) << shift, next = bound.place;
-            counts(level && place < next + one, level && place < next + 2 * one, level && place < next + 3 * one, sum);
+    // the largest bound that `want` of the candidates of `among` reach with `value`; narrows `among` to those equal to
+    // it, and `want` to what is left to find between them.  True: no more than `want` of them reach it.
+    bool among = thread < count, above = false;
+    int want = width;
+    auto narrow = [&](uint32_t value, int bits, uint32_t &bound) {
+        bound = 0;
+        int reach = INT32_MAX, sum[3];
+        for (int shift = (bits - 1) & ~1; shift >= 0 && reach > want; shift -= 2) {
+            const uint32_t one = 1u << shift, next = bound;
+            counts(among && value >= next + one, among && value >= next + 2 * one, among && value >= next + 3 * one, sum);
 #pragma unroll
             for (int s = 0; s < 3; ++s)
-                if (sum[s] < need) bound.place = next + uint64_t(s + 1) * one;
+                if (sum[s] >= want) bound = next + uint32_t(s + 1) * one, reach = sum[s];
         }
+        if (reach == want) {
+            above |= among && value >= bound;
+            return true;
+        }
+        counts(among && value > bound, false, false, sum);
+        want -= sum[0];
+        above |= among && value > bound;
+        among = among && value == bound;
+        return false;
+    };
+    uint32_t high = 0, low = 0;
+    JoinBound bound{0, UINT64_MAX};
+    if (!narrow(uint32_t(key >> 32), 32, high) && !narrow(uint32_t(key), 32, low)) {
+        // lower places are the better ones
+        uint32_t upper = 0, lower = 0;
+        bool done = false;
+        const uint32_t most = place_bits > 32 ? (1u << (place_bits - 32)) - 1 : 0;
+        if (place_bits > 32) done = narrow(most - uint32_t(place >> 32), place_bits - 32, upper);
+        if (!done) done = narrow(~uint32_t(place) << (32 - min(place_bits, 32)) >> (32 - min(place_bits, 32)),
+                                 min(place_bits, 32), lower);
+        above |= among && !done;  // one at most: places differ
+        const uint32_t ones = place_bits >= 32 ? UINT32_MAX : (1u << place_bits) - 1;
+        bound.place = uint64_t(most - upper) << 32 | (ones - lower);
     }
+    bound.key = uint64_t(high) << 32 | low;
     if (thread == 0) sh.count = 0;
     __syncthreads();
-    if (key > bound.key || (key && key == bound.key && place <= bound.place)) {
+    if (above) {
         const int at = atomicAdd(&sh.count, 1);
         sh.key[at] = key;
         sh.place[at] = place;
