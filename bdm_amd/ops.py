@@ -1027,10 +1027,11 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, fin
     continuation, token ``eos`` with its score unchanged.  With
     ``length_penalty`` a, continuations compare by score / length**a, where
     ``lengths`` [B, K] int32 are the beams' lengths and a continuation of an
-    unfinished beam is one longer.  Ties go to the lower beam, then the lower
-    token.  A logit of -inf is no candidate, nor is any of a beam whose score is
-    not finite or whose logits hold a NaN, +inf or nothing finite; where fewer
-    than ``width`` remain, the rest of the prompt's rows has the score -inf."""
+    unfinished beam is one longer.  They compare in FP64, and of a beam only its
+    best logits do.  Ties go to the lower beam, then the lower token.  A logit of
+    -inf is no candidate, nor is any of a beam whose score is not finite or whose
+    logits hold a NaN, +inf or nothing finite; where fewer than ``width`` remain,
+    the rest of the prompt's rows has the score -inf."""
     if logits.ndim != 3 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError('logits must be BF16 or FP32 [batch, beams, vocab]')
     batch, beams, vocab = logits.shape

@@ -539,6 +539,32 @@ def test_on_a_side_stream(device):
     check_step(pages, 0, step, 1.0, True, y, before)
 
 
+def test_two_caches_on_two_streams(device):
+    """Steps and forks of two caches at once, each equal to the same calls alone."""
+    ends = []
+    for at_once in (False, True):
+        caches, streams = [], []
+        for n in range(2):
+            pages, _, gen = make(device, n=6, banks=16, layers=1, s=8, width=32, seed=60 + n)
+            states = torch.randn(6, 16, 1, 8, 32, generator=gen).bfloat16().to(device)
+            steps = [token(6, 1, 8, 32, 16, 8, 8, torch.bfloat16, gen, device) for _ in range(6)]
+            orders = [torch.randint(0, 6, (6,), generator=gen).to(device) for _ in steps]
+            caches.append((pages, states, steps, orders, []))
+            streams.append(torch.cuda.Stream() if at_once else torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        for t in range(6):
+            for (pages, states, steps, orders, out), stream in zip(caches, streams):
+                with torch.cuda.stream(stream):
+                    if t == 0:
+                        pages.load(0, range(6), states)
+                    pages.fork(orders[t])
+                    out.append(pages.decode(0, *steps[t], scale=0.5, routed_decay=True))
+        torch.cuda.synchronize()
+        ends.append([(pages.dense(0, range(6)), pages.table.clone(), *out) for pages, _, _, _, out in caches])
+    for one, two in zip(*ends):
+        assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
 def test_one_head_caches_of_the_layer(device):
     pages, book, gen = make(device, n=2, banks=4, layers=1, s=4, width=8)
     states = torch.randn(2, 4, 4, 8, generator=gen).bfloat16()
