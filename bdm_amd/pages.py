@@ -84,6 +84,7 @@ class BankPages:
             raise NotImplementedError(f'BankPages takes at most {MAX_SEQUENCES} sequences')
         self.pages, self.heads, self.bank_size, self.head_width = pool.shape
         self.dtype, self.device = pool.dtype, pool.device
+        self._index = pool.get_device()
         # one bit a page: set where nothing references it, 64 pages a word
         free = torch.zeros((self.pages + 63) // 64 * 64, dtype=torch.int64, device=self.device)
         free[:self.pages] = references == 0
@@ -204,39 +205,40 @@ class BankPages:
         banks are FP32 here and y is rounded once: with FP32 controllers the
         result is ``decode_step``'s bit for bit, with BF16 ones it is nearer to
         the exact one.  Sequences without pages give 0 and stay without."""
-        layer, device, dtype = self._layer(layer), self.device, q.dtype
-        n, heads, s, width = q.shape[0] if q.ndim else 0, self.heads, self.bank_size, self.head_width
+        # each look at a tensor's attribute is 0.1 to 0.3 us of the host, which a step of few sequences waits for: every
+        # one is asked for once
+        layer, device, dtype, shape = self._layer(layer), self.device, q.dtype, q.shape
+        n, heads, s, width = shape[0] if shape else 0, self.heads, self.bank_size, self.head_width
         if not 1 <= n <= self.sequences:
             raise ValueError(f'decode takes 1 to {self.sequences} sequences')
         rows, columns = (n, heads, s), (n, heads, width)
-        if (q.shape != rows or k.shape != rows or g.shape != rows or b.shape != rows or v.shape != columns
+        if (shape != rows or k.shape != rows or g.shape != rows or b.shape != rows or v.shape != columns
                 or w.shape != columns):
             raise ValueError(f'q, k, g, b must be {rows} and v, w {columns}')
-        if wi.ndim != 2 or ri.ndim != 2 or wi.shape[0] != n or ri.shape[0] != n or wi.shape != ww.shape or (
-                ri.shape != rw.shape):
+        writes, reads = wi.shape, ri.shape
+        if len(writes) != 2 or len(reads) != 2 or writes[0] != n or reads[0] != n or ww.shape != writes or (
+                rw.shape != reads):
             raise ValueError('routes must be [sequences, selected banks]')
         if wi.dtype is not torch.int64 or ri.dtype is not torch.int64:
             raise ValueError('bank indices must be int64')
-        held, pointers = [], []
-        for t in (q, k, b, g, v, w, ww, rw, wi, ri):
-            if t.device != device:
+        if not (k.dtype is b.dtype is v.dtype is w.dtype is ww.dtype is rw.dtype is dtype):
+            raise ValueError('controllers and route weights must share a dtype')
+        if g.dtype is not torch.float32:
+            g = g.float()
+        index, pointers, copies = self._index, [], []
+        for t in (q, k, b, v, w, ww, rw, g, wi, ri):
+            if t.get_device() != index:
                 raise ValueError('all tensors must be on the device of the pages')
-            if t is g and g.dtype is not torch.float32:
-                t = g.float()
-            elif t.dtype is not dtype and t is not g and t is not wi and t is not ri:
-                raise ValueError('controllers and route weights must share a dtype')
-            if not t.is_contiguous():
-                t = t.contiguous()
             pointer = t.data_ptr()
-            if pointer % 16:
-                t = t.clone()
+            if pointer % 16 or not t.is_contiguous():
+                t = t.clone(memory_format=torch.contiguous_format)
+                copies.append(t)  # alive until the launch is enqueued
                 pointer = t.data_ptr()
-            held.append(t)  # copies live until the launch is enqueued
             pointers.append(pointer)
-        kw, kr = wi.shape[1], ri.shape[1]
+        kw, kr = writes[1], reads[1]
         output = torch.empty((n, heads * width), device=device, dtype=dtype)
         args = self._step
-        (args.q, args.k, args.b, args.g, args.v, args.w, args.write_weights, args.read_weights, args.write_indices,
+        (args.q, args.k, args.b, args.v, args.w, args.write_weights, args.read_weights, args.g, args.write_indices,
          args.read_indices) = pointers
         args.output, args.batch, args.write_banks, args.read_banks = output.data_ptr(), n, kw, kr
         args.ctrl_dtype, args.routed_decay, args.scale = ops._dtype_code(dtype), bool(routed_decay), scale

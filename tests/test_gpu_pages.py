@@ -565,6 +565,33 @@ def test_two_caches_on_two_streams(device):
         assert all(torch.equal(a, b) for a, b in zip(one, two))
 
 
+def test_controllers_of_any_layout(device):
+    """Views that start anywhere, with strides, and one tensor in two places: the results of plain ones."""
+    results = []
+    for plain in (True, False):
+        pages, _, gen = make(device, n=4, banks=8, layers=1, s=8, width=16, dtype=torch.float32, seed=70)
+        pages.load(0, range(4), torch.randn(4, 8, 1, 8, 16, generator=gen).to(device))
+        step = token(4, 1, 8, 16, 8, 4, 4, torch.float32, gen, device)
+        q, k, v, g, b, w, wi, ww, ri, rw = step
+        g, rw = b, ww
+        if not plain:
+            q = torch.cat([q.new_zeros(1), q.flatten()])[1:].view(q.shape)
+            v = torch.stack([v, v], -1)[..., 0]
+            b = b.transpose(0, 2).contiguous().transpose(0, 2)
+            g = b
+            wi = torch.cat([wi, wi], 1)[:, :4]
+            ri = torch.cat([ri.new_zeros(1), ri.flatten()])[1:].view(ri.shape)
+            ww = ww.t().contiguous().t()
+        y = pages.decode(0, q, k, v, g, b, w, wi, ww, ri, rw, scale=1.0, routed_decay=True)
+        results.append((y, pages.dense(0, range(4))))
+        with pytest.raises(ValueError):  # g may be FP32 beside others, b may not
+            pages.decode(0, q.bfloat16(), k.bfloat16(), v.bfloat16(), g, b, w.bfloat16(), wi, ww.bfloat16(), ri,
+                         rw.bfloat16(), scale=1.0, routed_decay=True)
+        with pytest.raises(ValueError):
+            pages.decode(0, q, k, v.bfloat16(), g, b, w, wi, ww, ri, rw, scale=1.0, routed_decay=True)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_one_head_caches_of_the_layer(device):
     pages, book, gen = make(device, n=2, banks=4, layers=1, s=4, width=8)
     states = torch.randn(2, 4, 4, 8, generator=gen).bfloat16()
