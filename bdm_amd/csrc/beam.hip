@@ -711,12 +711,15 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
             best = max(best, candidate(int(i % uint32_t(lists)), int(i / uint32_t(lists))).high());
         JoinBound bound = first_bound(best);
         do {
-            // the lists whose best reaches the bound, then all of these (more than LDS holds: all of all)
-            for (int list = thread; list < all; list += THREADS)
-                if (candidate(list, 0).reaches(bound)) {
+            // the lists whose best reaches the bound's key, whatever its place (entries behind it with an equal key can
+            // have lower ones), then all of these (more than LDS holds: all of all)
+            for (int list = thread; list < all; list += THREADS) {
+                const uint64_t key = candidate(list, 0).key;
+                if (key && key >= bound.key) {
                     const int at = atomicAdd(&sh.reaching, 1);
                     if (at < kRoom) sh.list[at] = list;
                 }
+            }
             __syncthreads();
             const bool held = sh.reaching <= kRoom;
             const uint32_t most = uint32_t(held ? sh.reaching : all) * uint32_t(p.width);

@@ -349,3 +349,25 @@ def test_reorder_clamps_parents_into_their_group(device):
     state = torch.arange(8, device=device).view(8, 1).clone()
     ops.reorder_states([state], torch.tensor([-5, 9, 2, 1, 99, 0, 5, 6], device=device), beams=4)
     assert state.flatten().tolist() == [0, 3, 2, 1, 7, 4, 5, 6]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+@pytest.mark.parametrize('first', [0, 1], ids=['first-beam', 'second-beam'])
+def test_select_joins_lists_whose_best_has_a_late_place(device, first, dtype):
+    # more candidates level with each other than LDS holds, in lists whose first entries are not their lowest tokens: a
+    # logit of 1e-20 leads its part of the row but has the total of the zeros
+    vocab, width = 9000, 64
+    logits = torch.zeros(1, 64, vocab, device=device, dtype=dtype)
+    logits[..., 2047::2048] = 1e-20
+    logits[..., -1] = 1e-20
+    logits[..., :2008] = -math.inf
+    logits[:, :first] = -math.inf
+    scores = torch.full((1, 64), -3.0, device=device)
+    out = check(logits, scores, width)
+    assert torch.isfinite(out.scores).all()
+    # totals that are equal in 64 bits go to the lower token, of the lowest beam that has any
+    assert (out.parents == first).all()
+    assert torch.equal(out.tokens.cpu(), torch.arange(2008, 2008 + width)[None])
+    for _ in range(3):
+        again = check(logits, scores, width)
+        assert all(torch.equal(a, b) for a, b in zip(out[:3], again[:3]))
