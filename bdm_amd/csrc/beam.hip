@@ -152,7 +152,7 @@ struct TeamShared {
     float high[WAVES], sum[WAVES];
     uint32_t bound[WAVES], share[WAVES];
     int found[WAVES];
-    int ties[WAVES][10];
+    int ties[WAVES][9];
     int count;
 };
 
@@ -188,14 +188,14 @@ __device__ __forceinline__ int team_count(TeamShared<WAVES> &sh, const float (&x
 // The exact `width` best of the team's values to sh.list, where more than it
 // holds reach `least`: those above the width-th, then of those equal to it the
 // ones of lowest index, which lie in the order of vectors, lanes, places in the
-// vector; the odd ones before or behind all of these.  Where fewer than width
+// vector, the odd ones behind all of these.  Where fewer than width
 // are above `least` (equal logits, or a mask of the type's lowest value over
 // most of the row) it is the width-th itself; else that is bisected.
 template <int WAVES, int NV, int VE, typename Index>
-__device__ __forceinline__ int team_ties(TeamShared<WAVES> &sh, const float (&x)[NV * VE + 1], Index index,
-                                         bool odd_first, float least, int width, int wave, int lane) {
-    constexpr int E = NV * VE + 1, kGroups = NV + 2;
-    static_assert(kGroups <= 10);
+__device__ __forceinline__ int team_ties(TeamShared<WAVES> &sh, const float (&x)[NV * VE + 1], Index index, float least,
+                                         int width, int wave, int lane) {
+    constexpr int E = NV * VE + 1, kGroups = NV + 1;
+    static_assert(kGroups <= 9);
     float value = least;
     int above = team_count<WAVES, E>(sh, x, value, false, wave, lane);
     if (above >= width) {
@@ -211,13 +211,12 @@ __device__ __forceinline__ int team_ties(TeamShared<WAVES> &sh, const float (&x)
     }
     const bool odd = x[E - 1] == value;
     int ties[kGroups];
-    ties[0] = popcount(__ballot(odd && odd_first));
-    ties[NV + 1] = popcount(__ballot(odd && !odd_first));
+    ties[NV] = popcount(__ballot(odd));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        ties[i + 1] = 0;
+        ties[i] = 0;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) ties[i + 1] += popcount(__ballot(x[i * VE + j] == value));
+        for (int j = 0; j < VE; ++j) ties[i] += popcount(__ballot(x[i * VE + j] == value));
     }
     if (lane == 0) {
 #pragma unroll
@@ -238,16 +237,15 @@ __device__ __forceinline__ int team_ties(TeamShared<WAVES> &sh, const float (&x)
             before += sh.ties[w][g];
         }
         if (at >= width) continue;
-        if (g == 0 || g == NV + 1) {
-            const bool mine = odd && odd_first == (g == 0);
-            const uint64_t lanes = __ballot(mine);
-            if (mine && at + popcount(lanes & ((1ull << lane) - 1)) < width) take(E - 1);
+        if (g == NV) {
+            const uint64_t lanes = __ballot(odd);
+            if (odd && at + popcount(lanes & ((1ull << lane) - 1)) < width) take(E - 1);
         } else {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) at += popcount(__ballot(x[(g - 1) * VE + j] == value) & ((1ull << lane) - 1));
+            for (int j = 0; j < VE; ++j) at += popcount(__ballot(x[g * VE + j] == value) & ((1ull << lane) - 1));
 #pragma unroll
             for (int j = 0; j < VE; ++j)
-                if (x[(g - 1) * VE + j] == value && at++ < width) take((g - 1) * VE + j);
+                if (x[g * VE + j] == value && at++ < width) take(g * VE + j);
         }
     }
 #pragma unroll
@@ -258,15 +256,14 @@ __device__ __forceinline__ int team_ties(TeamShared<WAVES> &sh, const float (&x)
 }
 
 // Maximum, sum of exponentials and the `width` best of the team's values
-// (load(x) gets them, index(e) is value e's index, odd_first whether the last
-// one's is lower than the vectors'): sets high and sum in every lane, leaves the
+// (load(x) gets them, index(e) is value e's index): sets high and sum in every lane, leaves the
 // candidates in sh.list and returns how many there are.  Values of -inf are no
 // candidates.  The few parts with too many ties load their values once more:
 // kept alive for those, the values and their patterns took 108 registers of a
 // lane with 33, and half the waves.
 template <int WAVES, int NV, int VE, typename Load, typename Index>
-__device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index index, bool odd_first, int width,
-                                         int wave, int lane, float &high, float &sum) {
+__device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index index, int width, int wave, int lane,
+                                         float &high, float &sum) {
     constexpr int E = NV * VE + 1;
     float x[E];
     load(x);
@@ -347,7 +344,7 @@ __device__ __forceinline__ int team_scan(TeamShared<WAVES> &sh, Load load, Index
     team_sync<WAVES>();
     float again[E];
     load(again);
-    return team_ties<WAVES, NV, VE>(sh, again, index, odd_first, least, width, wave, lane);
+    return team_ties<WAVES, NV, VE>(sh, again, index, least, width, wave, lane);
 }
 
 // The team's candidates in descending order, the first `width` of them to out, 0 behind the last.
@@ -384,6 +381,15 @@ template <> struct Vec<float> {
     }
 };
 
+// 16 bytes that start at any element.  A row's values are dealt to lanes by their tokens, wherever the row starts: the
+// sum of exponentials, whose last bits follow its order, is the same for equal rows, so that beams with equal logits
+// and scores tie.  (64 prompts of 16 beams over 50,257 BF16 logits, half the rows at odd addresses: 39.7 us; dealt from
+// each row's own boundary 39.7, over 50,256, all of them aligned, 39.5.)
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) AnyVector {
+    uint4 bits;
+};
+
 // NV vectors of a row's `vectors`, `step` apart from `begin` on, -inf where the row has none.  All are asked for at
 // once, the last one in the place of those (a load under a condition of its own is waited for before the next).
 template <typename T, int NV>
@@ -392,7 +398,7 @@ __device__ __forceinline__ void load_part(const T *x, int vectors, int begin, in
     uint4 raw[NV];
     if (vectors > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) raw[i] = *reinterpret_cast<const uint4 *>(x + int64_t(min(begin + i * step, vectors - 1)) * VE);
+        for (int i = 0; i < NV; ++i) raw[i] = reinterpret_cast<const AnyVector<T> *>(x + int64_t(min(begin + i * step, vectors - 1)) * VE)->bits;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -424,9 +430,8 @@ __device__ __forceinline__ bool beam_live(const BeamParams &p, int64_t row) {
     return !(p.finished && p.finished[row]) && isfinite(p.scores[row]);
 }
 
-// One part of one row.  The row starts anywhere: the values before its first
-// 16-byte boundary and those behind its last whole vector are a tail that the
-// first part takes one by one.  33 values a lane: with 17 the bounds and ranks
+// One part of one row.  The values behind the row's last whole vector are a
+// tail that the first part takes one by one.  33 values a lane: with 17 the bounds and ranks
 // weigh twice as much, with 65 of BF16 fewer waves hide each other's waits (64
 // prompts of 16 beams over 50,257: 40.5 us, 42.8 with 65; over 131,072, whose
 // parts are all full, 75 and 71).
@@ -440,18 +445,16 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     const T *x = static_cast<const T *>(p.logits) + int64_t(row / uint32_t(p.beams)) * p.batch_stride +
                  int64_t(row % uint32_t(p.beams)) * p.beam_stride;
-    const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
-    const int vectors = (p.vocab - head) / VE;
+    const int vectors = p.vocab / VE;
     const int begin = split * NV * 256 + int(threadIdx.x);
-    // the row's odd ends: fewer than 2 * VE values
-    const int odd = int(threadIdx.x) < head ? int(threadIdx.x) : vectors * VE + int(threadIdx.x);
+    const int odd = vectors * VE + int(threadIdx.x);
     auto load = [&](float(&v)[E]) {
-        load_part<T, NV>(x + head, vectors, begin, 256, v);
+        load_part<T, NV>(x, vectors, begin, 256, v);
         v[E - 1] = split == 0 && odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
     };
-    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (begin + e / VE * 256) * VE + e % VE); };
+    auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : (begin + e / VE * 256) * VE + e % VE); };
     float high, sum;
-    const int count = team_scan<4, NV, VE>(sh, load, index, odd < head, p.width, wave, lane, high, sum);
+    const int count = team_scan<4, NV, VE>(sh, load, index, p.width, wave, lane, high, sum);
     const int64_t part = int64_t(row) * p.splits + split;
     if (threadIdx.x == 0) p.parts[part] = make_float2(high, sum);
     uint64_t *out = p.lists + part * p.width;
@@ -823,16 +826,14 @@ __global__ __launch_bounds__(WAVES *kWave) void beam_rows_kernel(BeamParams p) {
     const int64_t row = prompt * p.beams + wave;
     if (wave < p.beams && beam_live(p, row)) {
         const T *x = static_cast<const T *>(p.logits) + prompt * p.batch_stride + wave * p.beam_stride;
-        const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
-        const int vectors = (p.vocab - head) / VE;
-        const int odd = lane < head ? lane : vectors * VE + lane;
+        const int vectors = p.vocab / VE, odd = vectors * VE + lane;
         auto load = [&](float(&v)[E]) {
-            load_part<T, NV>(x + head, vectors, lane, kWave, v);
+            load_part<T, NV>(x, vectors, lane, kWave, v);
             v[E - 1] = odd < p.vocab ? to_f32(x[odd]) : -INFINITY;
         };
-        auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : head + (e / VE * kWave + lane) * VE + e % VE); };
+        auto index = [&](int e) { return uint32_t(e == E - 1 ? odd : (e / VE * kWave + lane) * VE + e % VE); };
         float high, sum;
-        const int count = team_scan<1, NV, VE>(team, load, index, odd < head, p.width, 0, lane, high, sum);
+        const int count = team_scan<1, NV, VE>(team, load, index, p.width, 0, lane, high, sum);
         team_rank<1>(team, count, p.width, 0, lane, lists + wave * p.width);
         if (lane == 0) sh.log_sum[wave] = double(high) + log(double(sum));
     } else if (wave < p.beams && lane == 0) {

@@ -1028,7 +1028,9 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, fin
     ``length_penalty`` a, continuations compare by score / length**a, where
     ``lengths`` [B, K] int32 are the beams' lengths and a continuation of an
     unfinished beam is one longer.  They compare in FP64, and of a beam only its
-    best logits do.  Ties go to the lower beam, then the lower token.  A logit of
+    best logits do.  Ties go to the lower beam, then the lower token; beams with
+    equal logits and scores tie in any layout (logits of one beam too near for
+    FP64 totals to tell apart count as tied or by their order).  A logit of
     -inf is no candidate, nor is any of a beam whose score is not finite or whose
     logits hold a NaN, +inf or nothing finite; where fewer than ``width`` remain,
     the rest of the prompt's rows has the score -inf."""

@@ -611,8 +611,10 @@ int bdm_adamw_step(const bdm_adamw_args *args, void *stream);
  * (eos, s) alone.  The `width` best totals of each prompt are chosen, compared
  * as total / length^length_penalty (length: the beam's, plus one unless it is
  * finished), ties to the lower k * vocab + t.  Totals and compared values are
- * formed in FP64 from FP32 sums of exponentials; within a beam the order is
- * that of the logits.  A logit of -inf is no candidate; a beam whose
+ * formed in FP64 from FP32 sums of exponentials, which are the same for equal
+ * rows wherever they start.  Within a beam the order is that of the logits;
+ * those too near for their totals to differ count as tied or by their order.
+ * A logit of -inf is no candidate; a beam whose
  * score or sum is not finite (a NaN or +inf logit, no finite logit) has none.
  * Where a prompt has fewer than `width` candidates the lowest places without
  * one fill the rest, each with the score -inf.

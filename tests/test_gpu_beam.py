@@ -371,3 +371,70 @@ def test_select_joins_lists_whose_best_has_a_late_place(device, first, dtype):
     for _ in range(3):
         again = check(logits, scores, width)
         assert all(torch.equal(a, b) for a, b in zip(out[:3], again[:3]))
+
+
+def places(out, beams, vocab):
+    base = torch.arange(out.parents.shape[0])[:, None] * beams
+    return (out.parents.cpu() - base) * vocab + out.tokens.cpu()
+
+
+EQUAL = [
+    # batch, beams, vocabulary, width: one launch and two, rows that start at every offset from a vector's boundary, beams
+    # times vocabulary around a power of two, more lists than threads keep
+    (3, 4, 193, 4), (2, 16, 2047, 16), (2, 8, 2049, 8), (2, 5, 5001, 16), (1, 64, 1023, 64), (1, 64, 1024, 64),
+    (1, 64, 1025, 64), (1, 64, 9003, 64), (1, 16, 50257, 64),
+]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+@pytest.mark.parametrize('size', EQUAL, ids=lambda s: 'x'.join(map(str, s)))
+def test_select_beams_that_are_equal(device, size, dtype):
+    # equal rows and scores have equal totals, wherever a row starts in memory: the lower beam, then the lower token
+    from bdm_amd import ops
+    batch, beams, vocab, width = size
+    print('CASE equal beams', size, dtype, flush=True)
+    gen = torch.Generator().manual_seed(sum(size))
+    for kind in range(4):
+        rows = torch.randn(batch, 1, vocab, generator=gen) * 2.5
+        if kind == 1:
+            rows = torch.randint(0, 3, rows.shape, generator=gen).float()
+        elif kind > 1:
+            rows = torch.zeros_like(rows)
+        rows = rows.to(dtype).to(device)
+        scores = torch.full((batch, beams), -20.0, device=device)
+        if kind == 3:
+            scores[:, :beams // 2] = -math.inf
+        first = beams // 2 if kind == 3 else 0
+        level = rows.expand(batch, beams - first, vocab).flatten(1).float().cpu()
+        want = level.sort(dim=-1, descending=True, stable=True).indices[:, :width] + first * vocab
+        spaced = torch.empty(batch, beams, vocab + 3, device=device, dtype=dtype)[..., 2:vocab + 2]
+        for logits in (rows.expand(batch, beams, vocab), rows.expand(batch, beams, vocab).contiguous(),
+                       spaced.copy_(rows.expand(batch, beams, vocab))):
+            out = ops.beam_select(logits, scores, width=width)
+            assert torch.equal(places(out, beams, vocab), want), (kind, logits.stride())
+            fine = out.scores[:, :min(width, (beams - first) * vocab)]
+            assert torch.isfinite(fine).all() and (fine.diff(dim=-1) <= 0).all()
+
+
+def test_select_a_view_is_its_copy(device):
+    from bdm_amd import ops
+    wide, scores, _ = inputs(device, 6, 4, 5000, torch.bfloat16, 17)
+    for first in range(9):
+        view = wide[:, :, first:first + 4001]
+        a, b = ops.beam_select(view, scores), ops.beam_select(view.contiguous(), scores)
+        assert all(torch.equal(x, y) for x, y in zip(a[:3], b[:3])), first
+
+
+def test_select_places_beyond_32_bits(device):
+    # 64 beams over 2^26 + 3 tokens, one of them live: its best tokens, all level, lie on both sides of place 2^32
+    from bdm_amd import ops
+    vocab, width = 2 ** 26 + 3, 64
+    row = torch.full((1, 1, vocab), -math.inf, dtype=torch.bfloat16, device=device)
+    first = 2 ** 32 - 63 * vocab - 40
+    row[..., first:] = 0.5
+    scores = torch.full((1, 64), -math.inf, device=device)
+    scores[:, 63] = -2.0
+    print('CASE places beyond 32 bits', flush=True)
+    out = ops.beam_select(row.expand(1, 64, vocab), scores, width=width)
+    assert (out.parents == 63).all() and torch.isfinite(out.scores).all()
+    assert torch.equal(out.tokens.cpu(), torch.arange(first, first + width)[None])
