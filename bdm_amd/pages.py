@@ -12,7 +12,8 @@ reads the shared page and stores to the new one.
 
 Every call enqueues its kernels on the current stream of the pool's device and
 returns without synchronising; calls on one cache from several streams are the
-caller's to order.  All of them but ``check`` may be captured in a HIP graph.
+caller's to order.  All of them but ``check`` may be captured in a HIP graph,
+whose replays need the handle kept alive.
 New pages are the lowest-numbered free ones in the order of the requests, so
 tables do not change from run to run.
 """
@@ -106,15 +107,29 @@ class BankPages:
         nbytes = _lib.library().bdm_pages_decode_workspace_size(self._ref, MAX_SELECTED, MAX_SELECTED)
         self._tables = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._library = _lib.library()
+        self._streams = set()
+
+    def _on_stream(self) -> int:
+        """The current stream.  The tensors are recorded on each that a call uses: their memory is not given back
+        while one of them still runs, also where the handle is dropped before."""
+        stream = ops._stream(self.device)
+        if stream not in self._streams:
+            current = torch.cuda.current_stream(self.device)
+            for t in (self.pool, self.table, self.references, self.free_bits, self.status, self._tables):
+                t.record_stream(current)
+            self._streams.add(stream)
+        return stream
 
     # -- bookkeeping ------------------------------------------------------------------
     def used(self) -> Tensor:
         """The number of pages in use, a device scalar."""
+        self._on_stream()
         return (self.references > 0).sum()
 
     def check(self) -> None:
         """Raises if a call since the last check found no free page.
         Synchronises the host."""
+        self._on_stream()
         if int(self.status):
             self.status.zero_()
             raise RuntimeError(f'BankPages: no free page was left of {self.pages}')
@@ -131,12 +146,12 @@ class BankPages:
         return int(layer)
 
     def _call(self, name: str, *arguments) -> None:
-        device = self.device
+        device, stream = self.device, self._on_stream()
         if device.index == torch.cuda.current_device():
-            status = getattr(self._library, name)(self._ref, *arguments, ops._stream(device))
+            status = getattr(self._library, name)(self._ref, *arguments, stream)
         else:
             with torch.cuda.device(device):
-                status = getattr(self._library, name)(self._ref, *arguments, ops._stream(device))
+                status = getattr(self._library, name)(self._ref, *arguments, stream)
         if status:
             _lib.check(status, name)
 

@@ -649,3 +649,30 @@ def test_calls_refuse(device):
         pages.decode(0, *wide, scale=1.0, routed_decay=True)
     torch.cuda.synchronize()
     assert torch.equal(before, pages.table)
+
+
+def test_a_handle_dropped_while_a_stream_runs(device):
+    """Memory of a handle goes to nobody else while a call on another stream than its own still has it."""
+    pages, book, gen = make(device, n=4, banks=8, layers=1, s=8, width=16, dtype=torch.float32, seed=90)
+    states = torch.randn(4, 8, 1, 8, 16, generator=gen)
+    pages.load(0, range(4), states.to(device))
+    book.load(0, range(4), states)
+    parents = torch.tensor([0, 0, 2, 1], device=device)
+    held = (pages.pool, pages.table, pages.references, pages.free_bits, pages.status, pages._tables)
+    spans = [(t.data_ptr(), t.data_ptr() + t.nbytes) for t in held]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        pages.fork(parents)
+        out = pages.dense(0, range(4))
+    del pages, held
+    others = [torch.empty(end - start, dtype=torch.uint8, device=device) for start, end in spans for _ in range(16)]
+    assert not side.query(), 'the stream is done already'
+    taken = [(t.data_ptr(), t.data_ptr() + t.nbytes) for t in others]
+    assert not any(a < end and start < b for a, b in taken for start, end in spans)
+    for t in others:
+        t.zero_()
+    side.synchronize()
+    book.fork(parents.tolist())
+    assert torch.equal(out.cpu(), torch.stack([book.dense(0, i) for i in range(4)]))
