@@ -1087,8 +1087,8 @@ def reorder_states(states, parents: Tensor, *, beams: int) -> None:
     states: contiguous tensors [N, ...] of any dtype, N = prompts * beams (the
     per-layer caches of a model, for instance); parents: int64, N rows (or
     [prompts, beams], as ``beam_select`` returns them), each a row of the same
-    prompt's group of ``beams``.  Rows that keep their place are not touched; no
-    second copy of a cache is made."""
+    prompt's group of ``beams``.  No two of the tensors may share memory.  Rows
+    that keep their place are not touched; no second copy of a cache is made."""
     states = list(states)
     if not states:
         return
@@ -1107,12 +1107,13 @@ def reorder_states(states, parents: Tensor, *, beams: int) -> None:
         sizes.append(t.nbytes)
     if rows == 0:
         return
-    end = 0
-    for start, size in sorted(zip(spans, sizes)):
-        if start < end:
-            raise ValueError('states must not share memory')
-        end = max(end, start + size)
     parents = parents.contiguous()
+    # the parents too: a workgroup reads them while another one moves its rows
+    end = 0
+    for start, size in sorted([*zip(spans, sizes), (parents.data_ptr(), parents.nbytes)]):
+        if start < end:
+            raise ValueError('states must not share memory with each other or the parents')
+        end = max(end, start + size)
     count = len(states)
     pointers, lengths = (ctypes.c_void_p * count)(*spans), (ctypes.c_int64 * count)(*[n // rows for n in sizes])
     with _on(device):

@@ -644,8 +644,9 @@ int bdm_beam_select(const bdm_beam_args *args, void *workspace, size_t workspace
  * states[i][r] <- states[i][parents[r]] for the batch * beams rows of each of
  * `count` tensors, in place.  A row of tensor i has row_bytes[i] bytes, rows
  * follow each other; parents [batch * beams] are rows of the same prompt's
- * group of `beams` (others are clamped into it).  `states` and `row_bytes` are
- * host arrays, read before the call returns.  At most 64 beams.
+ * group of `beams` (others are clamped into it).  No two of the tensors, parents
+ * among them, may share memory.  `states` and `row_bytes` are host arrays, read
+ * before the call returns.  At most 64 beams.
  */
 int bdm_reorder_states(void *const *states, const int64_t *row_bytes, int32_t count, const int64_t *parents,
                        int64_t batch, int32_t beams, void *stream);

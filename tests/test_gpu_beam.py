@@ -438,3 +438,20 @@ def test_select_places_beyond_32_bits(device):
     out = ops.beam_select(row.expand(1, 64, vocab), scores, width=width)
     assert (out.parents == 63).all() and torch.isfinite(out.scores).all()
     assert torch.equal(out.tokens.cpu(), torch.arange(first, first + width)[None])
+
+
+def test_reorder_refuses_shared_memory(device):
+    from bdm_amd import ops
+    parents = torch.tensor([1, 0, 3, 2], device=device)
+    history = torch.arange(12, device=device).view(4, 3) % 4
+    before = history.clone()
+    for states, rows in (([parents], parents), ([history.view(-1)[:4], history.view(-1)[2:6]], parents),
+                         ([history.view(-1)[4:8]], history.view(-1)[7:11])):
+        with pytest.raises(ValueError):
+            ops.reorder_states(states, rows, beams=2)
+    torch.cuda.synchronize()
+    assert parents.tolist() == [1, 0, 3, 2] and torch.equal(history, before)
+    history[:, 1] = parents
+    want = history[parents]
+    ops.reorder_states([history], history[:, 1], beams=2)   # a column of a state is copied first
+    assert torch.equal(history, want)
