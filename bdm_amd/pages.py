@@ -173,6 +173,10 @@ class BankPages:
         if states.device != self.device:
             raise ValueError('all tensors must be on the device of the pages')
         states = states.contiguous()
+        # pages that the sequences leave can be given to the banks of others, ahead of a read of them
+        if self.pool.data_ptr() < states.data_ptr() + states.nbytes and (
+                states.data_ptr() < self.pool.data_ptr() + self.pool.nbytes):
+            states = states.clone()
         nbytes = _lib.library().bdm_pages_load_workspace_size(self._ref, len(rows))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._call('bdm_pages_load', layer, (ctypes.c_int32 * len(rows))(*rows), len(rows),

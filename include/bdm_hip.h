@@ -683,7 +683,8 @@ int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, const int32_t
                    void *stream);
 /* Dense states [count, banks, H, S, v] become the banks of the sequences of the
  * host array `sequences` (distinct), in place of what they held.  A bank that
- * equals sequence `base`'s bit for bit shares its page (base < 0: none). */
+ * equals sequence `base`'s bit for bit shares its page (base < 0: none).  The
+ * states may not overlap the pool. */
 size_t bdm_pages_load_workspace_size(const bdm_pages *pages, int32_t count);
 int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32_t *sequences, int32_t count, int32_t base,
                    const void *states, void *workspace, size_t workspace_bytes, void *stream);

@@ -676,3 +676,22 @@ def test_a_handle_dropped_while_a_stream_runs(device):
     side.synchronize()
     book.fork(parents.tolist())
     assert torch.equal(out.cpu(), torch.stack([book.dense(0, i) for i in range(4)]))
+
+
+def test_load_a_part_of_the_pool(device):
+    """States that are pages of the pool itself: the sequences' own, which are free behind the first kernel, and others'."""
+    for turn in range(3):
+        pages, book, gen = make(device, n=3, banks=64, layers=1, s=8, width=16, pages=200, dtype=torch.float32, seed=91)
+        states = torch.randn(2, 64, 1, 8, 16, generator=gen)
+        pages.load(0, [0, 1], states.to(device))
+        book.load(0, [0, 1], states)
+        first = (0, 63, 64)[turn]
+        part = torch.stack(book.content[first:first + 64]).flip(0)[None]
+        pages.pool[first:first + 64] = part[0].to(device)
+        for i in range(64):
+            book.content[first + i] = part[0, i]
+        for row in (1, 2, 0):
+            pages.load(0, [row], pages.pool[first:first + 64][None])
+            book.load(0, [row], part)
+            agree(pages, book)
+            part = torch.stack(book.content[first:first + 64])[None].clone()
