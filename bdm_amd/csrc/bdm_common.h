@@ -154,4 +154,7 @@ inline bool aligned(const void *p, size_t bytes) {
     return (reinterpret_cast<uintptr_t>(p) % bytes) == 0;
 }
 
+// A launch has fewer than 2^32 threads.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= int64_t(UINT32_MAX) / threads; }
+
 }  // namespace bdm

@@ -26,6 +26,7 @@
 // The exponentials and their sums are FP32 (each exponent relative to its
 // part's maximum), everything behind them is FP64: candidates of different
 // beams are compared by totals, which lie near each other.
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -936,17 +937,18 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
     }
 }
 
+// `check`: nothing is launched, only what a launch would refuse.
 template <typename V>
-int launch_reorder(ReorderParams &p, int64_t batch, hipStream_t stream) {
+int launch_reorder(ReorderParams &p, int64_t batch, bool check, hipStream_t stream) {
     unsigned blocks = 0;
     for (int i = 0; i < p.count; ++i) {
         p.tensors[i].first_block = blocks;
         const int64_t need = (p.tensors[i].row_bytes / int64_t(sizeof(V)) + kReorderRun - 1) / kReorderRun;
-        if (need + blocks > int64_t(UINT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: rows too long");
+        if (!grid_fits(need + blocks, 256)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: rows too long");
         blocks += unsigned(need);
     }
-    if (blocks == 0) return BDM_OK;
-    if (batch * int64_t(blocks) > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: grid too large");
+    if (blocks && !grid_fits(batch, 256 * int64_t(blocks))) return fail(BDM_ERR_UNSUPPORTED, "reorder_states: grid too large");
+    if (blocks == 0 || check) return BDM_OK;
     p.blocks = blocks;
     const unsigned grid = unsigned(batch * blocks);
     constexpr int kMost = sizeof(V) == 16 ? 16 : sizeof(V) == 8 ? 32 : kBeamMax;  // rows that registers hold
@@ -1010,7 +1012,7 @@ extern "C" int bdm_beam_select(const bdm_beam_args *a, void *workspace, size_t w
     if (need && (!workspace || workspace_bytes < need)) return fail(BDM_ERR_WORKSPACE, "beam_select: workspace of %zu bytes", need);
     if (need && !aligned(workspace, 8)) return fail(BDM_ERR_INVALID, "beam_select: workspace must be 8-byte aligned");
     const BeamPlan plan = beam_plan(*a);
-    if (a->batch * a->beams * (plan.splits ? plan.splits : 1) > int64_t(INT32_MAX))
+    if (!grid_fits(a->batch, std::max<int64_t>(kJoinThreads, 256 * int64_t(a->beams) * plan.splits)))
         return fail(BDM_ERR_UNSUPPORTED, "beam_select: grid too large");
     BeamParams p{};
     p.logits = a->logits;
@@ -1087,7 +1089,10 @@ extern "C" int bdm_reorder_states(void *const *states, const int64_t *row_bytes,
         if (row_bytes[i] < 0) return fail(BDM_ERR_INVALID, "reorder_states: bad geometry");
         if (row_bytes[i] && !states[i]) return fail(BDM_ERR_INVALID, "reorder_states: null pointer");
     }
-    for (int done = 0; done < count; done += kReorderTensors) {
+    const int launches = (count + kReorderTensors - 1) / kReorderTensors;
+    for (int turn = 0; turn < 2 * launches; ++turn) {  // every launch checked before the first one
+        const int done = turn % launches * kReorderTensors;
+        const bool check = turn < launches;
         ReorderParams p{};
         p.parents = parents;
         p.beams = beams;
@@ -1102,15 +1107,15 @@ extern "C" int bdm_reorder_states(void *const *states, const int64_t *row_bytes,
         // a thread holds two vectors of each row in registers: 16 bytes of 16 rows are 128 of them, and beyond
         // that the vectors are shorter
         if (bits % 16 == 0 && beams <= 16)
-            rc = launch_reorder<u32x4>(p, batch, as_stream(stream));
+            rc = launch_reorder<u32x4>(p, batch, check, as_stream(stream));
         else if (bits % 8 == 0 && beams <= 32)
-            rc = launch_reorder<u32x2>(p, batch, as_stream(stream));
+            rc = launch_reorder<u32x2>(p, batch, check, as_stream(stream));
         else if (bits % 4 == 0)
-            rc = launch_reorder<uint32_t>(p, batch, as_stream(stream));
+            rc = launch_reorder<uint32_t>(p, batch, check, as_stream(stream));
         else if (bits % 2 == 0)
-            rc = launch_reorder<uint16_t>(p, batch, as_stream(stream));
+            rc = launch_reorder<uint16_t>(p, batch, check, as_stream(stream));
         else
-            rc = launch_reorder<uint8_t>(p, batch, as_stream(stream));
+            rc = launch_reorder<uint8_t>(p, batch, check, as_stream(stream));
         if (rc != BDM_OK) return rc;
     }
     return BDM_OK;

@@ -602,8 +602,10 @@ int check_decode_pages(const bdm_decode_args *a) {
     const int rc = check_decode(a);
     if (rc != BDM_OK) return rc;
     const DecodeRows kind = decode_rows(*a, true);
-    if (!decode_shape(*a, kind.rows, kind.columns).fits)
-        return fail(BDM_ERR_UNSUPPORTED, "decode: a head of %d columns does not fit a workgroup", a->head_width);
+    const DecodeShape shape = decode_shape(*a, kind.rows, kind.columns);
+    if (!shape.fits) return fail(BDM_ERR_UNSUPPORTED, "decode: a head of %d columns does not fit a workgroup", a->head_width);
+    if (!grid_fits(a->batch * a->heads, shape.threads * int64_t(a->head_width / shape.span)))
+        return fail(BDM_ERR_UNSUPPORTED, "decode: grid too large");
     return BDM_OK;
 }
 

@@ -765,7 +765,7 @@ extern "C" int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, co
     const bool wide = p.sequences * 32 <= kForkInts && int64_t(p.layers) * p.banks >= 256 * 32;
     const int span = wide ? 32 : kForkInts / kMaxSequences;
     const int64_t grid = int64_t(p.layers) * ((p.banks + span - 1) / span);
-    if (grid > int64_t(INT32_MAX)) return fail(BDM_ERR_UNSUPPORTED, "pages_fork: grid too large");
+    if (!grid_fits(grid, 256)) return fail(BDM_ERR_UNSUPPORTED, "pages_fork: grid too large");
     fork_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(p, parents, count, mask, span);
     return check_launch("fork_kernel");
 }
@@ -803,6 +803,7 @@ extern "C" int bdm_pages_load(const bdm_pages *pages, int32_t layer, const int32
     return with_vector(p.page_bytes, states, [&](auto vector) {
         using V = decltype(vector);
         const int threads = page_threads(p.page_bytes / int64_t(sizeof(V)));
+        if (!grid_fits(banks, threads)) return fail(BDM_ERR_UNSUPPORTED, "pages_load: grid too large");  // store_kernel's
         compare_kernel<V><<<unsigned((banks + kCompareWaves - 1) / kCompareWaves), kCompareWaves * kWave, 0, s>>>(
             p, layer, rows, base, uint32_t(banks), data, differs);
         int code = check_launch("compare_kernel");
@@ -831,7 +832,9 @@ extern "C" int bdm_pages_dense(const bdm_pages *pages, int32_t layer, const int3
     hipStream_t s = as_stream(stream);
     return with_vector(p.page_bytes, states, [&](auto vector) {
         using V = decltype(vector);
-        dense_kernel<V><<<unsigned(banks), page_threads(p.page_bytes / int64_t(sizeof(V))), 0, s>>>(
+        const int threads = page_threads(p.page_bytes / int64_t(sizeof(V)));
+        if (!grid_fits(banks, threads)) return fail(BDM_ERR_UNSUPPORTED, "pages_dense: grid too large");
+        dense_kernel<V><<<unsigned(banks), threads, 0, s>>>(
             p, layer, rows, static_cast<char *>(states));
         return check_launch("dense_kernel");
     });

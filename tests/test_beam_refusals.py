@@ -139,3 +139,40 @@ def test_struct_mirrors(tmp_path):
     for m in mirrors.values():
         want += [ctypes.sizeof(m)] + [getattr(m, f).offset for f, _ in m._fields_]
     assert got == want
+
+
+def test_c_entry_points_refuse_grids_of_more_threads_than_a_launch_has():
+    """2^32 threads and more: nothing is launched, so a load, a step or a reordering is not left half done."""
+    from bdm_amd import _lib
+    lib = _lib.library()
+    pages = _lib.Pages()
+    ref = ctypes.byref(pages)
+    pages.pages, pages.layers, pages.sequences, pages.banks = 1 << 20, 1, 512, 1 << 17
+    pages.heads, pages.bank_size, pages.head_width, pages.dtype = 1, 1, 8, _lib.BDM_BF16
+    for name in ('pool', 'table', 'references', 'free_bits', 'status'):
+        setattr(pages, name, 4096)
+    rows = (ctypes.c_int32 * 512)(*range(512))
+    assert lib.bdm_pages_load(ref, 0, rows, 512, -1, 4096, 4096, 1 << 40, None) == -2
+    assert lib.bdm_pages_dense(ref, 0, rows, 512, 4096, None) == -2
+    pages.layers = 1 << 15
+    assert lib.bdm_pages_fork(ref, 4096, None, 512, None) == -2
+    pages.layers, pages.banks, pages.heads, pages.head_width = 1, 16, 1 << 15, 64
+    step = _lib.DecodeArgs()
+    step.batch, step.heads, step.bank_size, step.head_width, step.bank_count = 512, 1 << 15, 1, 64, 16
+    step.write_banks = step.read_banks = 8
+    step.ctrl_dtype = step.state_dtype = _lib.BDM_BF16
+    for name in ('q', 'k', 'v', 'b', 'g', 'w', 'write_weights', 'read_weights', 'write_indices', 'read_indices', 'output'):
+        setattr(step, name, 4096)
+    assert lib.bdm_pages_decode(ref, 0, ctypes.byref(step), 4096, 1 << 20, None) == -2
+    assert b'grid' in lib.bdm_last_error_string()
+    # the 33rd tensor goes into a second launch
+    pointers, sizes = (ctypes.c_void_p * 33)(*[4096] * 33), (ctypes.c_int64 * 33)(*[0] * 33)
+    sizes[32] = 16
+    assert lib.bdm_reorder_states(pointers, sizes, 33, 4096, 1 << 24, 2, None) == -2
+    sizes[0], sizes[32] = 16, 1 << 45
+    assert lib.bdm_reorder_states(pointers, sizes, 33, 4096, 1, 2, None) == -2
+    args = _lib.BeamArgs()
+    args.batch, args.beams, args.vocab, args.width, args.dtype = 1 << 18, 64, 4, 4, _lib.BDM_BF16
+    for name in ('logits', 'scores', 'out_scores', 'out_tokens', 'out_parents'):
+        setattr(args, name, 4096)
+    assert lib.bdm_beam_select(ctypes.byref(args), 4096, 1 << 40, None) == -2
