@@ -172,3 +172,44 @@ def test_search_refuses(device):
         other = build(device, torch.float32, banks=16)
         with pytest.raises(ValueError):
             other.step_pages(prompt[:, :1], pages)
+
+
+@pytest.mark.parametrize('graph', [False, True])
+@pytest.mark.parametrize('paged', [False, True])
+def test_search_scores_are_the_model_s(device, paged, graph):
+    """BF16, eight heads: every continuation fed to the model again, alone in a row of its own, has the score that the
+    search gives it.
+
+    Steps of one shape give a row the same logits whatever row it is and whatever the others hold, so the scores
+    differ by the selection's arithmetic alone: a step adds an FP32 sum's error (LOG_SUM) and a rounding of the score."""
+    from bdm_amd import beam_search
+    from test_gpu_beam import LOG_SUM
+    print('CASE search scores', paged, graph, flush=True)
+    batch, beams, length, vocab = 2, 4, 12, 192
+    model = build(device, torch.bfloat16, heads=8, banks=256, vocab=vocab, dim=256)
+    prompt = torch.randint(0, vocab, (batch, 17), generator=torch.Generator().manual_seed(8)).to(device)
+    got = beam_search(model, prompt, beams=beams, length=length, paged=paged, graph=graph)
+    rows = batch * beams
+    with torch.no_grad():
+        if paged:
+            pages = model.create_pages(rows + 1, 2 * (rows + 1) * 256 + rows * 4)
+            model.load_initial(pages, rows)
+            logits = model.prefill_pages(prompt, pages, range(0, rows, beams), base=rows)
+            pages.fork(torch.arange(rows, device=device) // beams * beams)
+        else:
+            logits, caches = model.prefill(prompt)
+            caches = [c.repeat_interleave(beams, 0) for c in caches]
+        logits = logits.repeat_interleave(beams, 0)
+        total = torch.zeros(rows, dtype=torch.float64)
+        for t in range(length):
+            tokens = got.tokens[:, :, t].reshape(rows, 1)
+            x = torch.log_softmax(logits.view(rows, vocab).double().cpu(), -1)
+            total += x.gather(1, tokens.cpu()).flatten()
+            logits = model.step_pages(tokens, pages) if paged else model.step(tokens, caches)[0]
+    scores = got.scores.cpu().double().flatten()
+    assert ((scores - total).abs() <= length * (LOG_SUM + total.abs() * 2.0 ** -24)).all()
+    assert (got.scores.diff(dim=1) <= 0).all() and (got.lengths == length).all()
+    for b in range(batch):
+        assert len({tuple(x) for x in got.tokens[b].tolist()}) == beams
+    if not paged:
+        assert torch.equal(plain_search(model, prompt, beams, length, None, 0.0)[0], got.tokens.cpu())

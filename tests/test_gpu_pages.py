@@ -695,3 +695,73 @@ def test_load_a_part_of_the_pool(device):
             book.load(0, [row], part)
             agree(pages, book)
             part = torch.stack(book.content[first:first + 64])[None].clone()
+
+
+MANY = [
+    # written banks of a step: up to 512, up to 1,024, more (in eight rounds of 1,024 at most); read banks: more than the
+    # threads that look them up, with few or no written ones
+    (60, 24, 1, 4, 8, 5, 3, 'bf16', 'bf16'), (64, 24, 1, 4, 8, 8, 8, 'fp32', 'fp32'), (100, 24, 1, 4, 8, 7, 2, 'fp32', 'bf16'),
+    (128, 24, 1, 8, 16, 8, 8, 'bf16', 'bf16'), (129, 24, 1, 4, 8, 8, 1, 'fp32', 'fp32'), (512, 24, 1, 4, 8, 16, 16, 'fp32', 'bf16'),
+    (64, 24, 1, 4, 8, 1, 16, 'fp32', 'fp32'), (64, 24, 1, 4, 8, 0, 16, 'fp32', 'bf16'), (512, 20, 1, 4, 8, 2, 16, 'bf16', 'bf16'),
+    (512, 20, 1, 4, 8, 16, 0, 'bf16', 'bf16'),
+]
+
+
+@pytest.mark.parametrize('geometry', MANY, ids=lambda c: 'x'.join(map(str, c)))
+def test_decode_of_many(device, geometry):
+    test_decode(device, geometry, True)
+
+
+@pytest.mark.parametrize('n', [4, 64, 129, 256, 257])
+def test_fork_of_many_layers(device, n):
+    """Enough layers and banks that a workgroup takes 32 columns (16 of more than 256 sequences)."""
+    from bdm_amd import BankPages
+    print('CASE pages fork of many layers', n, flush=True)
+    layers, banks, gen = 8, 1027, torch.Generator().manual_seed(n)
+    # a page of each bank for every third sequence, which the two behind it share; every seventh has none
+    owner = torch.arange(n) // 3
+    table = (torch.arange(layers)[:, None, None] * (n // 3 + 1) + owner[:, None]) * banks + torch.arange(banks)
+    table[:, ::7] = -1
+    total = layers * (n // 3 + 1) * banks
+
+    def counted(t):
+        return torch.bincount(t[t >= 0], minlength=total).int()
+
+    pool = torch.zeros(total, 1, 1, 4, dtype=torch.float32, device=device)
+    pages = BankPages.over(pool, table.int().to(device), counted(table).to(device))
+    choices = [torch.randint(-1, n, (n,), generator=gen), torch.arange(n) // 4 * 4, torch.randint(-n, n, (n,), generator=gen),
+               torch.arange(n - n // 2).flip(0), torch.full((n,), -1)]
+    for parents in choices:
+        pages.fork(parents.to(device))
+        whole = torch.cat([parents, torch.arange(len(parents), n)])
+        table = torch.where(whole[:, None] >= 0, table[:, whole.clamp(0)], -1)
+        torch.cuda.synchronize()
+        assert torch.equal(pages.table.cpu().long(), table)
+        references = counted(table)
+        assert torch.equal(pages.references.cpu(), references)
+        free = torch.zeros((total + 63) // 64 * 64, dtype=torch.int64)
+        free[:total] = references == 0
+        assert torch.equal(pages.free_bits.cpu(), (free.view(-1, 64) << torch.arange(64)).sum(-1))
+
+
+def test_the_count_of_used_pages_in_a_graph(device):
+    from bdm_amd import BankPages
+    pages = BankPages(3, 300_000, banks=64, heads=1, bank_size=1, head_width=4, device=device)
+    states = torch.randn(1, 64, 1, 1, 4, generator=torch.Generator().manual_seed(1)).bfloat16().to(device)
+    pages.load(0, [0], states)
+    pages.used()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        used = pages.used()
+    for turn in range(5):
+        if turn == 1:
+            pages.load(0, [1], states + 1)
+        if turn == 2:
+            pages.load(0, [2], states + 2)
+        if turn == 3:
+            pages.release([0, 1])
+        torch.ones(1 << 20, device=device).sum()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(used) == int((pages.references > 0).sum().cpu()) == (64, 128, 192, 64, 64)[turn]
