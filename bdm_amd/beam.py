@@ -104,36 +104,39 @@ def beam_search(model, prompt: Tensor, *, beams: int, length: int, eos: int | No
     parents = torch.empty_like(tokens)
     stream = torch.cuda.Stream(device) if graph else torch.cuda.current_stream(device)
     stream.wait_stream(torch.cuda.current_stream(device))
-    with torch.cuda.stream(stream):
-        search = _Search(model, prompt, beams, eos, length_penalty, paged, length)
-        captured, done = None, length
-        for t in range(length):
-            if t == 0:
-                pass  # chosen from the prompt's logits
-            elif not graph or t < 3:
-                search.step()
-            else:
-                if captured is None:
-                    captured = torch.cuda.CUDAGraph()
-                    torch.cuda.synchronize(device)
-                    with torch.cuda.graph(captured, stream=stream):
-                        search.step()
-                captured.replay()
-            tokens[t].copy_(search.tokens)
-            parents[t].copy_(search.parents)
-            if eos is not None and t % 16 == 15 and bool(search.finished.all()):
-                done = t + 1
-                break
-        # each continuation from its last token back to its first
-        out = torch.full((batch, beams, length), 0 if eos is None else eos, dtype=torch.int64, device=device)
-        beam = torch.arange(beams, device=device).expand(batch, beams)
-        for t in range(done - 1, -1, -1):
-            out[:, :, t] = tokens[t].gather(1, beam)
-            beam = parents[t].gather(1, beam) % beams
-        result = BeamResult(out, search.scores, search.lengths)
-    torch.cuda.current_stream(device).wait_stream(stream)
-    if captured is not None:
-        stream.synchronize()  # the last replay, before the graph and its memory go
+    captured = None
+    try:
+        with torch.cuda.stream(stream):
+            search = _Search(model, prompt, beams, eos, length_penalty, paged, length)
+            done = length
+            for t in range(length):
+                if t == 0:
+                    pass  # chosen from the prompt's logits
+                elif not graph or t < 3:
+                    search.step()
+                else:
+                    if captured is None:
+                        captured = torch.cuda.CUDAGraph()
+                        torch.cuda.synchronize(device)
+                        with torch.cuda.graph(captured, stream=stream):
+                            search.step()
+                    captured.replay()
+                tokens[t].copy_(search.tokens)
+                parents[t].copy_(search.parents)
+                if eos is not None and t % 16 == 15 and bool(search.finished.all()):
+                    done = t + 1
+                    break
+            # each continuation from its last token back to its first
+            out = torch.full((batch, beams, length), 0 if eos is None else eos, dtype=torch.int64, device=device)
+            beam = torch.arange(beams, device=device).expand(batch, beams)
+            for t in range(done - 1, -1, -1):
+                out[:, :, t] = tokens[t].gather(1, beam)
+                beam = parents[t].gather(1, beam) % beams
+            result = BeamResult(out, search.scores, search.lengths)
+    finally:  # also where a step fails: what the stream still reads and writes is not given back before it is done
+        torch.cuda.current_stream(device).wait_stream(stream)
+        if captured is not None:
+            stream.synchronize()  # the last replay, before the graph and its memory go
     if graph:
         for t in result:
             t.record_stream(torch.cuda.current_stream(device))

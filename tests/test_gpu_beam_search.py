@@ -213,3 +213,33 @@ def test_search_scores_are_the_model_s(device, paged, graph):
         assert len({tuple(x) for x in got.tokens[b].tolist()}) == beams
     if not paged:
         assert torch.equal(plain_search(model, prompt, beams, length, None, 0.0)[0], got.tokens.cpu())
+
+
+@pytest.mark.parametrize('at', [1, 3])
+def test_a_search_that_fails_is_waited_for(device, at, monkeypatch):
+    """The caller's stream goes on behind the work that a failed search has left on its own."""
+    from bdm_amd import beam
+    model = build(device, torch.float32)
+    prompt = torch.randint(0, 61, (1, 5), generator=torch.Generator().manual_seed(9)).to(device)
+    done = torch.zeros(1, device=device)
+
+    class Failing(beam._Search):
+        steps = 0
+
+        def step(self):
+            super().step()
+            Failing.steps += 1
+            if Failing.steps == at:
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda._sleep(200_000_000)
+                    done.add_(1)
+                raise KeyError('a step that fails')
+
+    monkeypatch.setattr(beam, '_Search', Failing)
+    with pytest.raises(KeyError):
+        beam.beam_search(model, prompt, beams=3, length=6, graph=True)
+    seen = done.clone()
+    assert int(seen) == (1 if at == 1 else 0)
+    monkeypatch.undo()
+    result = beam.beam_search(model, prompt, beams=3, length=6, graph=True)
+    assert torch.equal(result.tokens, beam.beam_search(model, prompt, beams=3, length=6).tokens)
