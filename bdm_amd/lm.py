@@ -281,9 +281,15 @@ class BDMLanguageModel(nn.Module):
                          bank_size=memory.bank_size, head_width=memory.head_value_width, dtype=dtype,
                          device=self.output.weight.device)
 
+    def _check_pages(self, pages: BankPages) -> None:
+        """Ahead of the first layer: a call that a later one refused would have changed the others' pages."""
+        if pages.layers < len(self.layers):
+            raise ValueError('the pages need a layer for each of the model')
+
     def load_initial(self, pages: BankPages, sequence: int) -> None:
         """``sequence`` takes the layers' initial states: the base with which
         ``prefill_pages`` shares the banks that its prompts do not write."""
+        self._check_pages(pages)
         with torch.no_grad():
             for i, block in enumerate(self.layers):
                 pages.load(i, [sequence], block.attention.create_state(1, dtype=pages.dtype))
@@ -298,6 +304,7 @@ class BDMLanguageModel(nn.Module):
         sequences = list(sequences)
         if len(sequences) != tokens.shape[0]:
             raise ValueError('one sequence per prompt is required')
+        self._check_pages(pages)
 
         def run(i, normed):
             out, state = self.layers[i].attention.prefill(normed, state_dtype=pages.dtype)
@@ -313,6 +320,7 @@ class BDMLanguageModel(nn.Module):
             raise RuntimeError('Stateful inference requires no_grad or inference_mode')
         if tokens.ndim != 2 or tokens.shape[1] != 1:
             raise ValueError('step takes [batch, 1] tokens')
+        self._check_pages(pages)
         return self._run_blocks(self.tok_embeddings(tokens),
                                 lambda i, normed: self.layers[i].attention.step_pages(normed, pages, i))
 

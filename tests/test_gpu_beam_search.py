@@ -243,3 +243,19 @@ def test_a_search_that_fails_is_waited_for(device, at, monkeypatch):
     monkeypatch.undo()
     result = beam.beam_search(model, prompt, beams=3, length=6, graph=True)
     assert torch.equal(result.tokens, beam.beam_search(model, prompt, beams=3, length=6).tokens)
+
+
+def test_pages_of_too_few_layers_are_refused_unchanged(device):
+    model, shallow = build(device, torch.float32, layers=2), build(device, torch.float32, layers=1)
+    prompt = torch.randint(0, 61, (2, 5), generator=torch.Generator().manual_seed(10)).to(device)
+    with torch.no_grad():
+        pages = shallow.create_pages(3, 3 * 64 + 16, dtype=torch.float32)
+        shallow.load_initial(pages, 2)
+        shallow.prefill_pages(prompt, pages, range(2), base=2)
+        before = [t.clone() for t in (pages.pool, pages.table, pages.references, pages.free_bits)]
+        for call in (lambda: model.load_initial(pages, 2), lambda: model.prefill_pages(prompt, pages, range(2), base=2),
+                     lambda: model.step_pages(prompt[:, :1], pages)):
+            with pytest.raises(ValueError):
+                call()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (pages.pool, pages.table, pages.references, pages.free_bits)))
