@@ -63,7 +63,10 @@ class BankPages:
         or BF16, table [layers, sequences, banks] int32 (pages of the pool, or
         -1 throughout a sequence), references [P] int32, the number of table
         entries of each page.  The tensors have to agree with each other, and a
-        page may be an entry of one layer and bank only."""
+        page may be an entry of one layer and bank only.  From then on table and
+        references change through this handle alone, which keeps a map of the
+        free pages beside them: behind a change of the caller's own (a restored
+        snapshot, for instance) a new handle is made over the tensors."""
         if pool.ndim != 4 or table.ndim != 3 or references.shape != pool.shape[:1] or 0 in (*pool.shape, *table.shape):
             raise ValueError('pool must be [pages, heads, bank_size, head_width], table [layers, sequences, banks] and '
                              'references [pages]')
@@ -107,11 +110,11 @@ class BankPages:
         nbytes = _lib.library().bdm_pages_decode_workspace_size(self._ref, MAX_SELECTED, MAX_SELECTED)
         self._tables = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._library = _lib.library()
-        self._streams = set()
+        self._streams = {ops._stream(self.device)}  # the one that the tensors belong to
 
     def _on_stream(self) -> int:
-        """The current stream.  The tensors are recorded on each that a call uses: their memory is not given back
-        while one of them still runs, also where the handle is dropped before."""
+        """The current stream.  The tensors are recorded on each but their own that a call uses: their memory is not
+        given back while one of them still runs, also where the handle is dropped before."""
         stream = ops._stream(self.device)
         if stream not in self._streams:
             current = torch.cuda.current_stream(self.device)
@@ -194,7 +197,8 @@ class BankPages:
     def fork(self, parents: Tensor) -> None:
         """Sequence i continues sequence ``parents[i]``, in every layer: int64,
         entries for the first sequences (the others stay).  A negative entry
-        releases the sequence's pages.  Tables and reference counts change, no
+        releases the sequence's pages, one behind the last sequence counts as the
+        last.  Tables and reference counts change, no
         page is copied."""
         if parents.dtype != torch.int64 or not 1 <= parents.numel() <= self.sequences:
             raise ValueError(f'parents must be int64, for 1 to {self.sequences} sequences')
