@@ -90,9 +90,12 @@ def beam_search(model, prompt: Tensor, *, beams: int, length: int, eos: int | No
     ``length_penalty`` a, continuations compare by score / length**a.  ``paged``
     keeps the beams in a ``BankPages`` cache instead of one dense cache a beam
     (the same search; its decode step rounds once where the dense step rounds
-    every product and sum, so near ties can fall the other way).  ``graph``
-    replays the steps behind the third token from one HIP graph.  Every 16 tokens
-    the host looks whether all continuations have ended."""
+    every product and sum, so near ties can fall the other way).  Its pool holds
+    what the search can need whatever the routes are, which for long prompts is
+    as much as the dense caches; a loop over ``create_pages`` with a pool of the
+    caller's own size saves memory where banks stay shared.  ``graph`` replays the
+    steps behind the third token from one HIP graph, captured in each call.  Every
+    16 tokens the host looks whether all continuations have ended."""
     if prompt.ndim != 2 or prompt.dtype != torch.int64 or 0 in prompt.shape:
         raise ValueError('prompt must be int64 [batch, positive time]')
     if not prompt.is_cuda:

@@ -17,11 +17,14 @@
 // holds, the exact W-th value is found instead, and of those equal to it the
 // first (equal logits, 64 prompts of 16 beams over 50,257: 85 us).
 //
-// What bounds it: one read of the logits for large calls (64 prompts of 16
-// beams over 50,257 FP32 logits, 206 MB, take 42.8 us, the scan 32 of them, a
-// part from the cache; in BF16 41 us, which the arithmetic of each value bounds),
-// for small ones the chain of a load, two selections and their barriers (4 beams
-// over 192 tokens: 5.4 us).
+// What bounds it: for large calls in FP32 the read of the logits (64 prompts of
+// 16 beams over 50,257, 206 MB: 42.3 us, the scan 32 to 35 of them, a part from
+// the cache), in BF16 the vector instructions (40 us, the scan 33.6 of them).
+// Both scans issue 14.5 M of these, 15 for each value of a lane, which is 24 us at
+// four cycles each; of BF16's 40 us the candidates' compares, ballots and LDS
+// atomics are 9, the exponentials 3 (copies without them).  For small calls it is
+// the chain of a load, two selections and their barriers (4 beams over 192 tokens:
+// 5.5 us).
 //
 // The exponentials and their sums are FP32 (each exponent relative to its
 // part's maximum), everything behind them is FP64: candidates of different
@@ -101,7 +104,7 @@ __device__ __forceinline__ int popcount(uint64_t m) { return __popcll(m); }
 // Bisected, a ballot a bit, over where the values lie between the lowest and
 // the highest of them, in 256 parts: 9 ballots in the place of the 16 of the
 // patterns' top half, and as near where the lanes are like each other (8
-// prompts of 8 beams over 50,257 BF16 logits: 13.6 -> 12.1 us, 64 of 16: 45.4
+// prompts of 8 beams over 50,257 BF16 logits: 13.6 -> 12.2 us, 64 of 16: 45.4
 // -> 40.9).
 template <int N>
 struct Bounds {
@@ -436,6 +439,11 @@ __device__ __forceinline__ bool beam_live(const BeamParams &p, int64_t row) {
 // weigh twice as much, with 65 of BF16 fewer waves hide each other's waits (64
 // prompts of 16 beams over 50,257: 40.5 us, 42.8 with 65; over 131,072, whose
 // parts are all full, 75 and 71).
+// For wide selections a row's last part weighs: where it fills few of the lanes
+// the waves without values have no share of the bound, one wave's own bound
+// admits most of the part, and ranking them by counting takes its square (width
+// 64, 16 beams, BF16: 25 us over 49,152 or 51,200 tokens, 36 to 54 over 50,257,
+// whose last part fills 138 of 256 lanes; FP32 25, whose vectors are smaller).
 template <typename T, int NV>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     constexpr int VE = Vec<T>::kSize, E = NV * VE + 1;
@@ -598,6 +606,8 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
     constexpr int kKept = 4;  // candidates that a thread keeps
     const int thread = int(threadIdx.x), wave = thread / kWave, lane = thread % kWave;
     // few of the best: one wave has them all; more: neighbours, as the lists of one beam, lie in different waves
+    // (16 beams over 49,152 logits at width 32 17.7 us, one wave's bounds 20.1; at width 64 FP32 25.5 and 37.7, BF16 33.2
+    // and 59.6; 64 beams at width 17 24.0 and 22.6)
     const bool wide = !FEW && p.width > 16;
     const int slot = wide ? lane * kWaves + wave : thread;
     const int ended = p.finished ? p.beams : 0, all = lists + ended;
@@ -858,7 +868,7 @@ struct BeamPlan {
 // and 14.8 for 64.  Not for more than 16 of a row: a lane's best bounds them
 // badly (64 of 16 beams over 2048: 106 us, 33 as two).
 // The parts of a row are made smaller until there are 512 of them, two a
-// compute unit: 8 prompts of 8 beams over 50,257 BF16 logits take 12.3 us so,
+// compute unit: 8 prompts of 8 beams over 50,257 BF16 logits take 12.2 us so,
 // 12.8 and 13.5 with 256 and 1024.
 BeamPlan beam_plan(const bdm_beam_args &a) {
     const int ve = a.dtype == BDM_BF16 ? Vec<bf16_t>::kSize : Vec<float>::kSize;
@@ -897,6 +907,9 @@ struct ReorderParams {
 // HBM's rate bounds it, and that wants long runs: a workgroup takes 512 vectors
 // of each row (4 KiB of a row at a time reached 3.3 TB/s on 64 rows of 4 MiB,
 // 8 KiB 5.2, past the caches, as the rows stream, 5.4; a large copy 4.8).
+// More rows than registers hold as 16-byte vectors are moved in shorter ones: one
+// prompt's rows of 4 MiB in four tensors, host's launch included, 4.1 TB/s for 16
+// beams, 4.1 to 4.3 for 17 to 32 (8 bytes), 3.9 to 4.0 for 33 to 64 (4 bytes).
 constexpr int kReorderRun = 512;  // vectors of a row
 
 template <typename V, int K>

@@ -194,7 +194,10 @@ __device__ __forceinline__ unsigned long long free_word(const Pages &p, int64_t 
 // to by none of them in this step; where none is left it is free for the next.
 // A chain of dependent loads (bank, table, references, free bits), so it is
 // latency that bounds it: 3.1 us for 64 written banks that nobody shares, 5.0
-// for 32 that are shared, 6.1 for 512 of 64 sequences.
+// for 32 that are shared, 6.1 for 512 of 64 sequences, 8.9 for 1,024 of 128.
+// Beyond 1,024 it is another matter: eight rounds of requests, all of them whatever
+// their number, do not fit the registers (932 bytes of scratch a lane): 98 us for
+// 129 sequences of 8 banks, 101 for 256, 107 for 512.
 template <int THREADS, int TILES>
 __global__ __launch_bounds__(THREADS) void resolve_kernel(Pages p, int layer, const int64_t *write, const int64_t *read,
                                                           int rows, int kw, int kr, int32_t *source, int32_t *target,
@@ -318,8 +321,9 @@ struct ReleaseMask {
 // The rows of a thread are neighbours, as beams of one prompt are, and where they
 // share a page their changes are one (none for a prompt whose beams all share it).
 // Latency bounds it too (parents, table, reference counts, free bits): one layer
-// of 4 rows of 1,024 banks takes 5.1 us, of 64 rows of 256 6.9, 16 layers of 64
-// rows of 1,024 banks (8.4 MB of table in and out) 10.
+// of 4 rows of 1,024 banks takes 4.3 us from a graph (5.1 by the profiler), of 64
+// rows of 256 5.4 (6.9), 16 layers of 64 rows of 1,024 banks (8.4 MB of table in
+// and out) 8.1 (10).
 constexpr int kForkRows = 8;
 constexpr int kForkInts = 8192;  // LDS of a column tile: sequences * span
 
@@ -515,7 +519,8 @@ __global__ __launch_bounds__(kCompareWaves *kWave) void compare_kernel(Pages p, 
 
 // Pages for the banks that differ, in their order: target[i], or -1.  One
 // workgroup, since a bank's page follows from how many differ before it: the
-// latency of its counts and searches bounds it (2,048 banks 6.1 us).
+// latency of its counts and searches bounds it (2,048 banks 6.1 us; 32,768, 2,048
+// a round, 53).
 constexpr int kEach = 2;  // banks of a thread: 8 took 3 us more for 2,048
 
 __global__ __launch_bounds__(kBlock) void assign_kernel(Pages p, int layer, Rows rows, int64_t banks,
@@ -760,8 +765,8 @@ extern "C" int bdm_pages_fork(const bdm_pages *pages, const int64_t *parents, co
     if (rc != BDM_OK) return rc;
     ReleaseMask mask{};
     for (int i = 0; !parents && i < count; ++i) mask.bits[rows.at[i] / 64] |= 1ull << (rows.at[i] % 64);
-    // 128 bytes of a table row where that fills the card (16 layers, 64 rows, 1,024 banks: 10.8 us, 16.6 with 64
-    // bytes), else 64 with more rows in flight at once (one layer, 256 banks: 8.3 us, 11.2 with 128)
+    // 128 bytes of a table row where that fills the card (16 layers, 64 rows, 1,024 banks: 8.1 us, 11.3 with 64 bytes;
+    // 8 layers 7.2 and 6.8), else 64 with more rows in flight at once (one layer, 256 banks: 5.4 us, 7.0 with 128)
     const bool wide = p.sequences * 32 <= kForkInts && int64_t(p.layers) * p.banks >= 256 * 32;
     const int span = wide ? 32 : kForkInts / kMaxSequences;
     const int64_t grid = int64_t(p.layers) * ((p.banks + span - 1) / span);
