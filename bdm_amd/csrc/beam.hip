@@ -41,6 +41,9 @@ namespace {
 constexpr int kBeamMax = 64;       // beams in, and candidates out, per prompt
 constexpr int kReorderTensors = 32;  // tensors of one reordering launch
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 // ------------------------------------------------------------------ ordered bit patterns
 // Unsigned integers in the order of the floating values; -0 counts as +0.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -368,18 +371,17 @@ __device__ __forceinline__ void team_rank(const TeamShared<WAVES> &sh, int count
 template <typename T> struct Vec;
 template <> struct Vec<bf16_t> {
     static constexpr int kSize = 8;
-    static __device__ __forceinline__ void widen(const uint4 &u, float *out) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    static __device__ __forceinline__ void widen(u32x4 u, float *out) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            out[2 * i] = __uint_as_float(w[i] << 16);
-            out[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            out[2 * i] = __uint_as_float(u[i] << 16);
+            out[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         }
     }
 };
 template <> struct Vec<float> {
     static constexpr int kSize = 4;
-    static __device__ __forceinline__ void widen(const uint4 &u, float *out) {
+    static __device__ __forceinline__ void widen(u32x4 u, float *out) {
         out[0] = __uint_as_float(u.x), out[1] = __uint_as_float(u.y);
         out[2] = __uint_as_float(u.z), out[3] = __uint_as_float(u.w);
     }
@@ -391,15 +393,16 @@ template <> struct Vec<float> {
 // each row's own boundary 39.7, over 50,256, all of them aligned, 39.5.)
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) AnyVector {
-    uint4 bits;
+    u32x4 bits;
 };
+static_assert(alignof(AnyVector<bf16_t>) == 2 && alignof(AnyVector<float>) == 4 && sizeof(AnyVector<bf16_t>) == 16);
 
 // NV vectors of a row's `vectors`, `step` apart from `begin` on, -inf where the row has none.  All are asked for at
 // once, the last one in the place of those (a load under a condition of its own is waited for before the next).
 template <typename T, int NV>
 __device__ __forceinline__ void load_part(const T *x, int vectors, int begin, int step, float *out) {
     constexpr int VE = Vec<T>::kSize;
-    uint4 raw[NV];
+    u32x4 raw[NV];
     if (vectors > 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) raw[i] = reinterpret_cast<const AnyVector<T> *>(x + int64_t(min(begin + i * step, vectors - 1)) * VE)->bits;
@@ -883,9 +886,6 @@ BeamPlan beam_plan(const bdm_beam_args &a) {
 }
 
 // ------------------------------------------------------------------ reordering
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 struct ReorderTensor {
     char *data;
     int64_t row_bytes;
