@@ -728,11 +728,12 @@ __device__ void join_beams(const BeamParams &p, JoinShared<THREADS> &sh, int64_t
             best = max(best, candidate(int(i % uint32_t(lists)), int(i / uint32_t(lists))).high());
         JoinBound bound = first_bound(best);
         do {
-            // the lists whose best reaches the bound's key, whatever its place (entries behind it with an equal key can
-            // have lower ones), then all of these (more than LDS holds: all of all)
+            // the lists whose best reaches the bound's key and whose beam its place, whatever the best's own (entries
+            // behind it with an equal key can have lower ones), then all of these (more than LDS holds: all of all)
             for (int list = thread; list < all; list += THREADS) {
-                const uint64_t key = candidate(list, 0).key;
-                if (key && key >= bound.key) {
+                JoinCandidate c = candidate(list, 0);
+                c.place = uint64_t(list < lists ? beam_of(list) : list - lists) * uint32_t(p.vocab);
+                if (c.reaches(bound)) {
                     const int at = atomicAdd(&sh.reaching, 1);
                     if (at < kRoom) sh.list[at] = list;
                 }
