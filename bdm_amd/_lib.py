@@ -53,6 +53,16 @@ EXPORTED_SYMBOLS = (
     'bdm_pages_compact',
     'bdm_pages_decode_workspace_size',
     'bdm_pages_decode',
+    'bdm_token_log_probs_workspace_size',
+    'bdm_token_log_probs',
+    'bdm_token_log_probs_backward',
+    'bdm_token_loss',
+    'bdm_gradient_norm_workspace_size',
+    'bdm_gradient_norm',
+    'bdm_clip_gradients',
+    'bdm_layer_norm',
+    'bdm_layer_norm_backward_workspace_size',
+    'bdm_layer_norm_backward',
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -226,6 +236,32 @@ class Pages(ctypes.Structure):
     ]
 
 
+class TokenArgs(ctypes.Structure):
+    """Mirror of ``bdm_token_args``."""
+    _fields_ = [
+        ('logits', _vp), ('tokens', _vp), ('log_probs', _vp), ('entropy', _vp), ('top_log_probs', _vp),
+        ('top_tokens', _vp), ('stats', _vp),
+        ('rows', _i64), ('row_stride', _i64), ('ignore_index', _i64),
+        ('vocab', _i32), ('alternatives', _i32), ('dtype', _i32),
+    ]
+
+
+class TokenGradArgs(ctypes.Structure):
+    """Mirror of ``bdm_token_grad_args``."""
+    _fields_ = [
+        ('logits', _vp), ('tokens', _vp), ('stats', _vp), ('entropy', _vp), ('top_tokens', _vp),
+        ('grad_log_probs', _vp), ('grad_entropy', _vp), ('grad_top_log_probs', _vp),
+        ('grad_loss', _vp), ('inverse_count', _vp), ('grad_logits', _vp),
+        ('rows', _i64), ('row_stride', _i64), ('ignore_index', _i64),
+        ('vocab', _i32), ('alternatives', _i32), ('dtype', _i32),
+    ]
+
+
+class Gradient(ctypes.Structure):
+    """Mirror of ``bdm_gradient``."""
+    _fields_ = [('data', _vp), ('out', _vp), ('numel', _i64), ('dtype', _i32), ('out_dtype', _i32)]
+
+
 class BDMError(RuntimeError):
     """A call into libbdm_hip returned a non-zero status."""
 
@@ -329,6 +365,27 @@ def library() -> ctypes.CDLL:
     lib.bdm_pages_decode_workspace_size.restype = _size_t
     lib.bdm_pages_decode.argtypes = [pages, _i32, ctypes.POINTER(DecodeArgs), _vp, _size_t, _vp]
     lib.bdm_pages_decode.restype = _i32
+    lib.bdm_token_log_probs_workspace_size.argtypes = [ctypes.POINTER(TokenArgs)]
+    lib.bdm_token_log_probs_workspace_size.restype = _size_t
+    lib.bdm_token_log_probs.argtypes = [ctypes.POINTER(TokenArgs), _vp, _size_t, _vp]
+    lib.bdm_token_log_probs.restype = _i32
+    lib.bdm_token_log_probs_backward.argtypes = [ctypes.POINTER(TokenGradArgs), _vp]
+    lib.bdm_token_log_probs_backward.restype = _i32
+    lib.bdm_token_loss.argtypes = [_vp, _vp, _i64, _i64, _vp, _vp, _vp]
+    lib.bdm_token_loss.restype = _i32
+    gradients = ctypes.POINTER(Gradient)
+    lib.bdm_gradient_norm_workspace_size.argtypes = [gradients, _i32]
+    lib.bdm_gradient_norm_workspace_size.restype = _size_t
+    lib.bdm_gradient_norm.argtypes = [gradients, _i32, ctypes.c_double, _vp, _vp, _vp, _size_t, _vp]
+    lib.bdm_gradient_norm.restype = _i32
+    lib.bdm_clip_gradients.argtypes = [gradients, _i32, ctypes.c_double, _vp, _vp, _size_t, _vp]
+    lib.bdm_clip_gradients.restype = _i32
+    lib.bdm_layer_norm.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp]
+    lib.bdm_layer_norm.restype = _i32
+    lib.bdm_layer_norm_backward_workspace_size.argtypes = [_i64, _i32]
+    lib.bdm_layer_norm_backward_workspace_size.restype = _size_t
+    lib.bdm_layer_norm_backward.argtypes = [_vp] * 7 + [_i64, _i32, _i32, _i32, _f32, _vp, _size_t, _vp]
+    lib.bdm_layer_norm_backward.restype = _i32
     return lib
 
 

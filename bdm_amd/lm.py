@@ -14,12 +14,14 @@ Under no_grad the shell's elementwise work runs in ``libbdm_hip.so``
 projections are one GEMM over their concatenated weights.  With autograd on a
 ROCm device RMSNorm runs as ``bdm_rms_norm`` forward and
 ``bdm_rms_norm_backward`` and the feed-forward's SwiGLU as
-``bdm_swiglu_pair`` and ``bdm_swiglu_backward``; the other modules run as the
-reference writes them.
+``bdm_swiglu_pair`` and ``bdm_swiglu_backward``, and the loss as ``token_loss``;
+the other modules run as the reference writes them.  ``normalization='layer'``
+takes ``LayerNorm`` in the place of RMSNorm.
 """
 
 from __future__ import annotations
 
+import functools
 from dataclasses import asdict, dataclass, field
 
 import torch
@@ -28,8 +30,9 @@ from torch import nn
 
 from . import ops
 from .config import BDMConfig
-from .model import BankedDeltaMemory
+from .model import BankedDeltaMemory, _differentiable, _global_hooks, _torch_gradients
 from .pages import BankPages
+from .scoring import TokenLogProbs, token_log_probs, token_loss
 
 Tensor = torch.Tensor
 
@@ -46,6 +49,7 @@ class LanguageModelConfig:
     seed: int = 0
     recompute_ffn: bool = True
     compact_replay: bool | None = None
+    normalization: str = 'rms'  # of the blocks' inputs and the head's: 'rms' (the reference's) or 'layer'
 
     def __post_init__(self):
         sizes = {'vocab_size': self.vocab_size, 'layers': self.layers, 'ffn_multiple_of': self.ffn_multiple_of}
@@ -54,10 +58,15 @@ class LanguageModelConfig:
             raise ValueError(f'language model needs positive {", ".join(bad) or "sizes"} and a seed >= 0')
         if not (self.compact_replay is None or isinstance(self.compact_replay, bool)):
             raise ValueError(f'compact_replay takes None or a bool, not {self.compact_replay!r}')
+        if self.normalization not in _NORMS:
+            raise ValueError(f'normalization {self.normalization!r} is neither rms nor layer')
 
     def record(self):
-        """Plain-dict form, the memory config nested as its own record."""
+        """Plain-dict form, the memory config nested as its own record; the
+        reference's fields alone where the model is the reference's."""
         out = asdict(self)
+        if self.normalization == 'rms':
+            del out['normalization']
         out['memory'] = self.memory.record()
         return out
 
@@ -129,6 +138,112 @@ class RMSNorm(nn.Module):
         nn.init.ones_(self.weight)
 
 
+def _hooked(module: nn.Module) -> bool:
+    """Whether a call of the module does more than its forward."""
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or _global_hooks())
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    """LayerNorm with HIP forward and backward kernels."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        ctx.save_for_backward(x, weight, bias)
+        ctx.eps = eps
+        return ops.layer_norm(x, weight, bias, eps)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        x, weight, bias = ctx.saved_tensors
+        if _differentiable([grad_out]):
+            return (*_torch_gradients(functools.partial(_layer_norm_ops, eps=ctx.eps), (x, weight, bias), grad_out),
+                    None)
+        return (*ops.layer_norm_backward(x, grad_out, weight, bias, ctx.eps), None)
+
+
+class _AddLayerNormFunction(torch.autograd.Function):
+    """(residual + x, its LayerNorm): one kernel forward, and one backward that
+    adds the sum's own gradient to the norm's."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        total, out = ops.layer_norm(x, weight, bias, eps, residual=residual)
+        ctx.save_for_backward(total, weight, bias)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return total, out
+
+    @staticmethod
+    def backward(ctx, grad_total, grad_out):
+        total, weight, bias = ctx.saved_tensors
+        if grad_out is None:
+            return grad_total, grad_total, None, None, None
+        if _differentiable([g for g in (grad_total, grad_out) if g is not None]):
+            grad, *rest = _torch_gradients(functools.partial(_layer_norm_ops, eps=ctx.eps),
+                                           (total.requires_grad_(), weight, bias), grad_out)
+            grad = grad if grad_total is None else grad + grad_total
+        else:
+            grad, *rest = ops.layer_norm_backward(total, grad_out, weight, bias, ctx.eps, grad_sum=grad_total)
+        return grad, grad, *rest, None
+
+
+def _layer_norm_ops(x, weight, bias, eps):
+    weight, bias = (None if t is None else t.float() for t in (weight, bias))
+    return F.layer_norm(x.float(), (x.shape[-1],), weight, bias, eps).to(x.dtype)
+
+
+class LayerNorm(nn.Module):
+    """(x - mean) * rsqrt(variance + eps) * weight + bias over the last dimension
+    in FP32, cast back: RMSNorm's counterpart for blocks that normalize as the
+    memory layer's output does.  On a ROCm device the norm, a residual add before
+    it and their gradients run in HIP kernels (widths to 16,384); elsewhere in
+    torch."""
+
+    def __init__(self, dim: int, eps: float = 1e-5, bias: bool = True):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(dim))
+        else:
+            self.register_parameter('bias', None)
+
+    def _fused(self, x: Tensor) -> bool:
+        parameters = [t for t in (self.weight, self.bias) if t is not None]
+        return (ops.layer_norm_supported(x) and all(t.dtype in (torch.bfloat16, torch.float32) for t in parameters)
+                and len({t.dtype for t in parameters}) == 1)
+
+    def _trained(self, *tensors: Tensor) -> bool:
+        return torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                               for t in (*tensors, self.weight, self.bias))
+
+    def forward(self, x: Tensor) -> Tensor:
+        if not self._fused(x):
+            return _layer_norm_ops(x, self.weight, self.bias, self.eps)
+        if self._trained(x):
+            return _LayerNormFunction.apply(x, self.weight, self.bias, self.eps)
+        return ops.layer_norm(x, self.weight, self.bias, self.eps)
+
+    def add_norm(self, x: Tensor, residual: Tensor):
+        """(residual + x, its norm): a block's residual add and the normalization
+        behind it, one kernel in each direction."""
+        if not self._fused(x) or residual.dtype != x.dtype or residual.shape != x.shape:
+            total = residual + x
+            return total, self(total)
+        if self._trained(x, residual):
+            return _AddLayerNormFunction.apply(x, residual, self.weight, self.bias, self.eps)
+        return ops.layer_norm(x, self.weight, self.bias, self.eps, residual=residual)
+
+    def reset_parameters(self):
+        nn.init.ones_(self.weight)
+        if self.bias is not None:
+            nn.init.zeros_(self.bias)
+
+
+_NORMS = {'rms': RMSNorm, 'layer': LayerNorm}
+
+
 class FeedForward(nn.Module):
     """SwiGLU w2(silu(w1 x) * w3 x) with the reference's hidden width rule
     (_shell.py:37-118)."""
@@ -189,10 +304,14 @@ class BDMBlock(nn.Module):
                                            compact_replay=config.compact_replay)
         self.feed_forward = FeedForward(dim, 4 * dim, config.ffn_multiple_of, None,
                                         recompute_activations=config.recompute_ffn)
-        self.attention_norm = RMSNorm(dim, eps=config.memory.norm_eps)
-        self.ffn_norm = RMSNorm(dim, eps=config.memory.norm_eps)
+        norm = _NORMS[config.normalization]
+        self.attention_norm = norm(dim, eps=config.memory.norm_eps)
+        self.ffn_norm = norm(dim, eps=config.memory.norm_eps)
 
     def forward(self, hidden: Tensor) -> Tensor:
+        if isinstance(self.ffn_norm, LayerNorm) and not _hooked(self.ffn_norm):
+            hidden, normed = self.ffn_norm.add_norm(self.attention(self.attention_norm(hidden)), hidden)
+            return hidden + self.feed_forward(normed)
         hidden = hidden + self.attention(self.attention_norm(hidden))
         return hidden + self.feed_forward(self.ffn_norm(hidden))
 
@@ -209,7 +328,7 @@ class BDMLanguageModel(nn.Module):
         self.dim = config.memory.dim
         self.layers = nn.ModuleList([BDMBlock(config, i, backend) for i in range(config.layers)])
         self.tok_embeddings = nn.Embedding(config.vocab_size, self.dim)
-        self.norm = RMSNorm(self.dim, eps=config.memory.norm_eps)
+        self.norm = _NORMS[config.normalization](self.dim, eps=config.memory.norm_eps)
         self.output = nn.Linear(self.dim, config.vocab_size, bias=False)
         self._seeded_init()
 
@@ -243,9 +362,20 @@ class BDMLanguageModel(nn.Module):
 
     def forward(self, tokens: Tensor, target: Tensor | None = None):
         logits = self.output(self.norm(self._hidden(tokens)))
-        if target is not None:
-            return F.cross_entropy(logits.float().flatten(0, -2), target.flatten())
-        return logits
+        if target is None:
+            return logits
+        if (logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and target.dtype == torch.int64
+                and target.device == logits.device and target.numel() * logits.shape[-1] == logits.numel()):
+            return token_loss(logits.flatten(0, -2), target.flatten())
+        return F.cross_entropy(logits.float().flatten(0, -2), target.flatten())
+
+    def score(self, tokens: Tensor, targets: Tensor, *, alternatives: int = 0,
+              ignore_index: int = -100) -> TokenLogProbs:
+        """Log-probabilities of ``targets`` [B, T] behind ``tokens`` [B, T], the
+        entropies of the model's distributions and their best alternatives
+        (``token_log_probs``); with gradients where autograd records."""
+        logits = self.output(self.norm(self._hidden(tokens)))
+        return token_log_probs(logits, targets, alternatives=alternatives, ignore_index=ignore_index)
 
     # -- stateful inference (perf_inference_case.py:15-56) ---------------------------
     def empty_cache(self) -> list:
@@ -326,7 +456,7 @@ class BDMLanguageModel(nn.Module):
 
     def _fused_decode_supported(self, hidden: Tensor) -> bool:
         ffn = self.layers[0].feed_forward
-        return (hidden.shape[0] <= ops.GEMV_MAX_ROWS and ffn.hidden_dim % 8 == 0 and self.dim % 8 == 0
+        return (isinstance(self.norm, RMSNorm) and hidden.shape[0] <= ops.GEMV_MAX_ROWS and ffn.hidden_dim % 8 == 0 and self.dim % 8 == 0
                 and max(ffn.hidden_dim, self.dim) <= ops.GEMV_PROLOGUE_MAX_K
                 and all(block.attention.step_fused_norm_supported(hidden, block.attention_norm.weight)
                         for block in self.layers))

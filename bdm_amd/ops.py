@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 from typing import NamedTuple
@@ -910,6 +911,76 @@ def rms_norm_backward(x: Tensor, grad_out: Tensor, weight: Tensor, eps: float):
     return grad_x, grad_weight
 
 
+LAYER_NORM_MAX_WIDTH = 16384
+
+
+def layer_norm_supported(x: Tensor) -> bool:
+    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32) and x.ndim >= 1
+            and 1 <= x.shape[-1] <= LAYER_NORM_MAX_WIDTH)
+
+
+def _layer_norm_parameters(x: Tensor, weight: Tensor | None, bias: Tensor | None) -> int:
+    """The parameters' dtype code, behind the checks of rows and parameters."""
+    if x.dtype not in (torch.bfloat16, torch.float32) or x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError('layer_norm takes BF16/FP32 rows [..., width]')
+    if x.shape[-1] > LAYER_NORM_MAX_WIDTH:
+        raise NotImplementedError(f'layer_norm takes rows of at most {LAYER_NORM_MAX_WIDTH} columns')
+    parameters = [t for t in (weight, bias) if t is not None]
+    if any(t.shape != x.shape[-1:] for t in parameters) or len({t.dtype for t in parameters}) > 1:
+        raise ValueError('weight and bias must be [width] of one dtype')
+    return _dtype_code(parameters[0].dtype) if parameters else _lib.BDM_F32
+
+
+def layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, residual: Tensor | None = None):
+    """LayerNorm over the last dimension in one pass, (x - mean) *
+    rsqrt(variance + eps) * weight + bias: FP32 arithmetic, one rounding.
+    Weight and bias [width] are optional.  With ``residual``, returns (x +
+    residual rounded, its norm); otherwise the norm of x."""
+    device = _require_gpu(x, weight, bias, residual)
+    code = _layer_norm_parameters(x, weight, bias)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError('residual must match x')
+    x = x.contiguous()
+    weight, bias, res = (None if t is None else t.contiguous() for t in (weight, bias, residual))
+    out = torch.empty_like(x)
+    total = None if res is None else torch.empty_like(x)
+    width = x.shape[-1]
+    with _on(device):
+        _lib.check(_lib.library().bdm_layer_norm(
+            _addr(x), _addr(res), _addr(weight), _addr(bias), _addr(total), _addr(out), x.numel() // width, width,
+            _dtype_code(x.dtype), code, float(eps), _stream(device)), 'bdm_layer_norm')
+    return out if res is None else (total, out)
+
+
+def layer_norm_backward(x: Tensor, grad_out: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, *,
+                        grad_sum: Tensor | None = None):
+    """Gradients (grad_x, grad_weight, grad_bias) of ``layer_norm(x, weight,
+    bias, eps)``, None for a parameter that is not there.  ``grad_sum`` is added
+    to grad_x: with the sum of a residual add as x, the gradient of that sum
+    itself."""
+    device = _require_gpu(x, grad_out, weight, bias, grad_sum)
+    code = _layer_norm_parameters(x, weight, bias)
+    for t in (grad_out, grad_sum):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError('the gradients must match x')
+    x, grad_out = x.contiguous(), grad_out.contiguous()
+    weight, grad_sum = (None if t is None else t.contiguous() for t in (weight, grad_sum))
+    width = x.shape[-1]
+    rows = x.numel() // width
+    lib = _lib.library()
+    nbytes = lib.bdm_layer_norm_backward_workspace_size(rows, width)
+    workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    grad_x = torch.empty_like(x)
+    grad_weight, grad_bias = (None if t is None else torch.empty(width, device=device, dtype=t.dtype)
+                              for t in (weight, bias))
+    with _on(device):
+        _lib.check(lib.bdm_layer_norm_backward(
+            _addr(x), _addr(grad_out), _addr(grad_sum), _addr(weight), _addr(grad_x), _addr(grad_weight),
+            _addr(grad_bias), rows, width, _dtype_code(x.dtype), code, float(eps), _addr(workspace), nbytes,
+            _stream(device)), 'bdm_layer_norm_backward')
+    return grad_x, grad_weight, grad_bias
+
+
 def swiglu_pair(a: Tensor, b: Tensor) -> Tensor:
     """round(round(silu(a)) * b) elementwise (the shell's SwiGLU with its two
     inputs from separate GEMMs, _shell.py:86-91)."""
@@ -998,6 +1069,202 @@ def written_bank_curve(first_write: Tensor, prefixes) -> Tensor:
         _addr(first), batch, banks, _addr(ends), ends.numel(), _addr(written), _stream(device)),
         'bdm_written_bank_curve')
     return written
+
+
+# ---------------------------------------------------------------------------
+# log-probabilities of given tokens
+
+ALTERNATIVES_MAX = 32
+
+
+def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int]:
+    """(logits, rows, row stride): as they are where their rows are evenly
+    spaced, a contiguous copy otherwise."""
+    vocab = logits.shape[-1]
+    rows = logits.numel() // vocab
+    if logits.is_contiguous():
+        return logits, rows, vocab
+    if logits.stride(-1) != 1 and vocab > 1:
+        return logits.contiguous(), rows, vocab
+    flat = logits.reshape(-1, vocab)  # a view where the leading dimensions allow one
+    return flat, rows, flat.stride(0)
+
+
+def token_statistics(logits: Tensor, tokens: Tensor, *, alternatives: int = 0, ignore_index: int = -100,
+                     entropy: bool = True, stats: bool = False):
+    """(log_probs, entropy, top_log_probs, top_tokens, stats) of given tokens:
+    ``bdm_amd.token_log_probs`` without autograd; None for what is not asked for.
+    ``stats`` [rows, 2] is what ``token_gradient`` needs of the rows."""
+    if logits.ndim < 1 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.shape[-1] < 1:
+        raise ValueError('logits must be BF16 or FP32 [..., vocab]')
+    if tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64:
+        raise ValueError('tokens must be int64 of the logits\' leading shape')
+    vocab, k = logits.shape[-1], int(alternatives)
+    if not 0 <= k <= vocab:
+        raise ValueError('alternatives must be 0 to the size of the vocabulary')
+    if k > ALTERNATIVES_MAX:
+        raise NotImplementedError(f'at most {ALTERNATIVES_MAX} alternatives')
+    device = _require_gpu(logits, tokens)
+    lead = tokens.shape
+    logits, rows, stride = _logit_rows(logits)
+    tokens = tokens.contiguous()
+    new = functools.partial(torch.empty, device=device, dtype=torch.float32)
+    log_probs, entropies = new(lead), new(lead) if entropy else None
+    top = new((*lead, k)) if k else None
+    top_tokens = torch.empty((*lead, k), device=device, dtype=torch.int64) if k else None
+    held = new((rows, 2)) if stats else None
+    args = _lib.TokenArgs(logits.data_ptr(), tokens.data_ptr(), log_probs.data_ptr(), _addr(entropies), _addr(top),
+                          _addr(top_tokens), _addr(held), rows, stride, int(ignore_index), vocab, k,
+                          _dtype_code(logits.dtype))
+    lib, ref = _lib.library(), ctypes.byref(args)
+    nbytes = lib.bdm_token_log_probs_workspace_size(ref)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    with _on(device):
+        _lib.check(lib.bdm_token_log_probs(ref, _addr(workspace), nbytes, _stream(device)), 'bdm_token_log_probs')
+    return log_probs, entropies, top, top_tokens, held
+
+
+def token_loss_mean(log_probs: Tensor, tokens: Tensor, *, ignore_index: int = -100) -> tuple[Tensor, Tensor]:
+    """The mean of -log_probs over the rows whose token is not ignore_index (FP64
+    sum in a fixed order) and the inverse of their number, FP32 scalars."""
+    device = _require_gpu(log_probs, tokens)
+    if log_probs.shape != tokens.shape or log_probs.dtype != torch.float32 or tokens.dtype != torch.int64:
+        raise ValueError('log_probs (FP32) and tokens (int64) must have one shape')
+    log_probs, tokens = log_probs.contiguous(), tokens.contiguous()
+    loss, inverse = (torch.empty((), device=device, dtype=torch.float32) for _ in range(2))
+    with _on(device):
+        _lib.check(_lib.library().bdm_token_loss(
+            _addr(log_probs), _addr(tokens), tokens.numel(), int(ignore_index), _addr(loss), _addr(inverse),
+            _stream(device)), 'bdm_token_loss')
+    return loss, inverse
+
+
+def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Tensor | None = None,
+                   top_tokens: Tensor | None = None, grad_log_probs: Tensor | None = None,
+                   grad_entropy: Tensor | None = None, grad_top_log_probs: Tensor | None = None,
+                   grad_loss: Tensor | None = None, inverse_count: Tensor | None = None,
+                   ignore_index: int = -100) -> Tensor:
+    """The logits' gradient from those of ``token_statistics``' results, or from
+    that of ``token_loss_mean``'s loss."""
+    device = _require_gpu(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs,
+                          grad_loss, inverse_count)
+    if logits.dtype not in (torch.bfloat16, torch.float32) or tokens.dtype != torch.int64 \
+            or tokens.shape != logits.shape[:-1] or stats.shape != (tokens.numel(), 2):
+        raise ValueError('the gradient takes BF16/FP32 logits, their int64 tokens and the rows\' statistics')
+    if (grad_entropy is not None and entropy is None) or (grad_top_log_probs is not None and top_tokens is None) \
+            or (grad_loss is None) != (inverse_count is None):
+        raise ValueError('a gradient comes without the result it belongs to')
+    for t, shape in ((stats, stats.shape), (entropy, tokens.shape), (grad_log_probs, tokens.shape),
+                     (grad_entropy, tokens.shape), (grad_loss, ()), (inverse_count, ()),
+                     (grad_top_log_probs, None if top_tokens is None else top_tokens.shape)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape):
+            raise ValueError('the results and their gradients must be FP32 of the tokens\' shape')
+    grad = torch.empty(logits.shape, device=device, dtype=logits.dtype)
+    logits, rows, stride = _logit_rows(logits)
+    kept = [None if t is None else t.contiguous() for t in (tokens, stats, entropy, top_tokens, grad_log_probs,
+                                                            grad_entropy, grad_top_log_probs, grad_loss, inverse_count)]
+    k = 0 if top_tokens is None else top_tokens.shape[-1]
+    args = _lib.TokenGradArgs(logits.data_ptr(), *(_addr(t) for t in kept), grad.data_ptr(), rows, stride,
+                              int(ignore_index), logits.shape[-1], k, _dtype_code(logits.dtype))
+    with _on(device):
+        _lib.check(_lib.library().bdm_token_log_probs_backward(ctypes.byref(args), _stream(device)),
+                   'bdm_token_log_probs_backward')
+    return grad
+
+
+# ---------------------------------------------------------------------------
+# the gradients' norm and clipping
+
+_ELEMENT = {torch.float32: _lib.BDM_F32, torch.bfloat16: _lib.BDM_BF16}
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether the elements fill their span of memory, each once, in any order."""
+    if t.is_contiguous():
+        return True
+    return t.permute(sorted(range(t.ndim), key=t.stride, reverse=True)).is_contiguous()
+
+
+class _GradientTable:
+    """The ``bdm_gradient`` array of the tensors that are not None, and the
+    copies that it points to."""
+
+    def __init__(self, gradients, out=None, *, written: bool = False) -> None:
+        gradients = list(gradients)
+        out = gradients if out is None else list(out)
+        if len(out) != len(gradients):
+            raise ValueError('out must hold a tensor for each gradient')
+        self.device, self.copies, flat = None, [], []
+        for g, o in zip(gradients, out):
+            if g is None:
+                continue
+            element = _ELEMENT.get(g.dtype)
+            if element is None or g.layout is not torch.strided:
+                raise ValueError('gradients must be dense BF16 or FP32 tensors')
+            if self.device is None:
+                self.device = _require_gpu(g)
+            elif g.device != self.device:
+                raise ValueError('all tensors must be on the same device')
+            size = g.numel()
+            if o is g:
+                if not _dense(g):
+                    if written:
+                        raise ValueError('a gradient whose elements do not fill its memory cannot be clipped in place')
+                    g = g.contiguous()
+                    self.copies.append(g)
+                place = g.data_ptr()
+                flat += (place, place, size, element | element << 32)
+                continue
+            other = None if o is None else _ELEMENT.get(o.dtype)
+            if other is None or o.shape != g.shape or o.layout is not torch.strided or o.device != self.device:
+                raise ValueError('out must hold a BF16 or FP32 tensor of each gradient\'s shape on its device')
+            if not (o.is_contiguous() and g.is_contiguous()) and not (o.stride() == g.stride() and _dense(g)):
+                if not o.is_contiguous():
+                    raise ValueError('out must be contiguous, or dense with its gradient\'s strides')
+                g = g.contiguous()
+                self.copies.append(g)
+            flat += (g.data_ptr(), o.data_ptr(), size, element | other << 32)
+        self.count = len(flat) // 4
+        self._flat = (ctypes.c_int64 * len(flat))(*flat)
+        self.entries = ctypes.cast(self._flat, ctypes.POINTER(_lib.Gradient))
+
+
+def gradient_norm(gradients, *, max_norm: float | None = None):
+    """``bdm_amd.gradient_norm``; with ``max_norm`` also the factor that clips to
+    it, min(1, max_norm / (norm + 1e-6)), as an FP32 scalar: (norm, factor)."""
+    table = _GradientTable(gradients)
+    if max_norm is not None and not max_norm >= 0:
+        raise ValueError('max_norm must not be negative')
+    if table.device is None:
+        return torch.zeros(()) if max_norm is None else (torch.zeros(()), torch.ones(()))
+    norm, factor = (torch.empty((), device=table.device, dtype=torch.float32) for _ in range(2))
+    lib = _lib.library()
+    nbytes = lib.bdm_gradient_norm_workspace_size(table.entries, table.count)
+    workspace = torch.empty(nbytes, device=table.device, dtype=torch.uint8)
+    with _on(table.device):
+        _lib.check(lib.bdm_gradient_norm(
+            table.entries, table.count, 0.0 if max_norm is None else float(max_norm), _addr(norm),
+            None if max_norm is None else _addr(factor), _addr(workspace), nbytes, _stream(table.device)),
+            'bdm_gradient_norm')
+    return norm if max_norm is None else (norm, factor)
+
+
+def clip_gradients(gradients, max_norm: float, *, out=None) -> Tensor:
+    """``bdm_amd.clip_gradients``."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError('max_norm must not be negative')
+    table = _GradientTable(gradients, out, written=True)
+    if table.device is None:
+        return torch.zeros(())
+    norm = torch.empty((), device=table.device, dtype=torch.float32)
+    lib = _lib.library()
+    nbytes = lib.bdm_gradient_norm_workspace_size(table.entries, table.count)
+    workspace = torch.empty(nbytes, device=table.device, dtype=torch.uint8)
+    with _on(table.device):
+        _lib.check(lib.bdm_clip_gradients(table.entries, table.count, max_norm, _addr(norm), _addr(workspace), nbytes,
+                                          _stream(table.device)), 'bdm_clip_gradients')
+    return norm
 
 
 # ---------------------------------------------------------------------------

@@ -28,7 +28,7 @@ import ctypes
 import torch
 from torch import Tensor
 
-from . import _lib
+from . import _lib, ops
 
 _ALIGN = 4  # elements: a tensor's slice of the flat buffers starts 16-byte aligned
 CHUNK = 16384  # elements per workgroup
@@ -41,10 +41,14 @@ class MasterAdamW:
     parameter flagged ``_no_weight_decay`` takes weight decay 0, the others
     ``weight_decay`` (the reference's two groups).  ``step(lr)`` clips to
     ``max_norm`` and applies one AdamW update with learning rate ``lr``.
+
+    The clipping norm is torch's by default, a BF16 number as the gradients are;
+    with ``float32_norm`` it is ``gradient_norm``'s, not rounded to BF16 and
+    formed in two kernels instead of some dozens.
     """
 
     def __init__(self, params, lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.01,
-                 max_norm: float = 1.0) -> None:
+                 max_norm: float = 1.0, float32_norm: bool = False) -> None:
         self.params = list(params)
         if not self.params:
             raise ValueError('MasterAdamW needs parameters')
@@ -54,6 +58,7 @@ class MasterAdamW:
                 raise ValueError('MasterAdamW takes contiguous BF16 parameters on one ROCm device')
         self.lr, self.betas, self.eps, self.max_norm = float(lr), (float(betas[0]), float(betas[1])), float(eps), \
             float(max_norm)
+        self.float32_norm = bool(float32_norm)
         self.device = device
         offsets, total = [], 0
         for p in self.params:
@@ -100,10 +105,13 @@ class MasterAdamW:
         for p, g in zip(self.params, grads):
             if g.dtype != torch.bfloat16 or not g.is_contiguous() or g.shape != p.shape:
                 raise ValueError('MasterAdamW.step: gradients must be contiguous BF16 of the parameter shape')
-        # clip_grad_norm_(params, max_norm): the same norm and BF16 coefficient
-        norm = torch.nn.utils.get_total_norm(grads, 2.0)
-        coef = torch.clamp(self.max_norm / (norm + 1e-6), max=1.0)
-        self._scale.copy_(coef.reshape(1))
+        if self.float32_norm:
+            norm, scale = ops.gradient_norm(grads, max_norm=self.max_norm)
+        else:
+            # clip_grad_norm_(params, max_norm): the same norm and BF16 coefficient
+            norm = torch.nn.utils.get_total_norm(grads, 2.0)
+            coef = torch.clamp(self.max_norm / (norm + 1e-6), max=1.0)
+            scale = self._scale.copy_(coef.reshape(1))
         if lr is not None:
             self.lr = float(lr)
         self.step_count += 1
@@ -123,7 +131,7 @@ class MasterAdamW:
         args.tensor_count, args.blocks, args.chunk = len(self.params), self.blocks, CHUNK
         args.master, args.exp_avg, args.exp_avg_sq = (self.master.data_ptr(), self.exp_avg.data_ptr(),
                                                       self.exp_avg_sq.data_ptr())
-        args.grad_scale = self._scale.data_ptr()
+        args.grad_scale = scale.data_ptr()
         args.lr, args.beta1, args.beta2, args.eps = self.lr, self.betas[0], self.betas[1], self.eps
         args.step = float(self.step_count)
         stream = torch.cuda.current_stream(self.device).cuda_stream

@@ -704,6 +704,99 @@ size_t bdm_pages_decode_workspace_size(const bdm_pages *pages, int32_t write_ban
 int bdm_pages_decode(const bdm_pages *pages, int32_t layer, const bdm_decode_args *args, void *workspace,
                      size_t workspace_bytes, void *stream);
 
+/*
+ * Log-probabilities of given tokens, the entropy of their distributions and the
+ * best alternatives.  No counterpart in the reference, whose shell forms the
+ * mean cross entropy alone (model.py:207-216).
+ *
+ * For a row x of logits with m = max x and s = sum exp(x - m):
+ *   log_probs = x[token] - m - log s,   entropy = -sum p log p,
+ * and the `alternatives` best logits in descending order (a NaN before all
+ * others), equal ones by the lower index.  FP32; logits [rows, vocab] of dtype,
+ * rows `row_stride` elements apart, starting anywhere.  A token equal to
+ * ignore_index has the log-probability 0, one outside the vocabulary NaN.  A
+ * row of -inf alone has log-probabilities -inf, the entropy 0 and no gradient;
+ * one with a NaN or +inf has NaN.  stats holds m and log s of each row for the
+ * backward.  At most 32 alternatives.
+ */
+typedef struct bdm_token_args {
+    const void *logits;
+    const int64_t *tokens;     /* [rows] */
+    float *log_probs;          /* [rows] */
+    float *entropy;            /* optional: [rows] */
+    float *top_log_probs;      /* [rows, alternatives] */
+    int64_t *top_tokens;       /* [rows, alternatives] */
+    float *stats;              /* optional: [rows, 2] */
+    int64_t rows, row_stride, ignore_index;
+    int32_t vocab, alternatives, dtype;
+} bdm_token_args;
+
+size_t bdm_token_log_probs_workspace_size(const bdm_token_args *args);
+int bdm_token_log_probs(const bdm_token_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The gradient of the logits [rows, vocab] (contiguous, of dtype) from those of
+ * the log-probabilities, the entropies and the alternatives' log-probabilities,
+ * each optional; or from that of the mean loss, a scalar, with the inverse of
+ * the rows' number from bdm_token_loss in the place of grad_log_probs.  Rounded
+ * once. */
+typedef struct bdm_token_grad_args {
+    const void *logits;
+    const int64_t *tokens;
+    const float *stats, *entropy;
+    const int64_t *top_tokens;
+    const float *grad_log_probs, *grad_entropy, *grad_top_log_probs;
+    const float *grad_loss, *inverse_count;
+    void *grad_logits;
+    int64_t rows, row_stride, ignore_index;
+    int32_t vocab, alternatives, dtype;
+} bdm_token_grad_args;
+
+int bdm_token_log_probs_backward(const bdm_token_grad_args *args, void *stream);
+/* loss = -sum of the log-probabilities / their number n over the rows whose
+ * token is not ignore_index (NaN where there is none), and 1 / n. */
+int bdm_token_loss(const float *log_probs, const int64_t *tokens, int64_t rows, int64_t ignore_index, float *loss,
+                   float *inverse_count, void *stream);
+
+/*
+ * The global norm of gradients, n = sqrt(sum g^2) over all tensors, and their
+ * clipping, g' = round(g min(1, max_norm / (n + 1e-6))): the arithmetic of the
+ * shell's clip_grad_norm_ (reproduction/experiments/optim.py:33-36) with the
+ * norm and the factor in FP64.  `tensors` is a host array, read before the call
+ * returns.  Clipped values go to `out`, of any of the two dtypes; out = data
+ * with the same dtype clips in place, where no value is written if the factor
+ * is 1.  An output may not overlap another tensor.  bdm_gradient_norm reads the
+ * data alone and with `scale` non-null also stores the factor.  The workspace is
+ * 16-byte aligned.
+ */
+typedef struct bdm_gradient {
+    const void *data;
+    void *out;
+    int64_t numel;
+    int32_t dtype, out_dtype;
+} bdm_gradient;
+
+size_t bdm_gradient_norm_workspace_size(const bdm_gradient *tensors, int32_t count);
+int bdm_gradient_norm(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm, float *scale,
+                      void *workspace, size_t workspace_bytes, void *stream);
+int bdm_clip_gradients(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/*
+ * Layer normalization: out = (x - mean) / sqrt(variance + eps) * weight + bias
+ * over rows [rows, width] of dtype, in FP32, rounded once; weight and bias
+ * [width] of param_dtype, each optional.  With residual non-null, sum_out =
+ * round(x + residual) is written and normalized.  The backward takes the
+ * normalized rows as x; grad_sum (optional) is added to grad_x, grad_weight and
+ * grad_bias are optional, FP32 sums over the rows rounded once.  Any width up to
+ * 16384.
+ */
+int bdm_layer_norm(const void *x, const void *residual, const void *weight, const void *bias, void *sum_out, void *out,
+                   int64_t rows, int32_t width, int32_t dtype, int32_t param_dtype, float eps, void *stream);
+size_t bdm_layer_norm_backward_workspace_size(int64_t rows, int32_t width);
+int bdm_layer_norm_backward(const void *x, const void *grad_out, const void *grad_sum, const void *weight, void *grad_x,
+                            void *grad_weight, void *grad_bias, int64_t rows, int32_t width, int32_t dtype,
+                            int32_t param_dtype, float eps, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

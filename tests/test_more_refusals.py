@@ -1,0 +1,191 @@
+"""What the entry points of the log-probabilities, the clipping and the layer
+norm refuse, before a device is touched."""
+
+import ctypes
+
+import pytest
+import torch
+
+from bdm_amd import LayerNorm, clip_gradients, gradient_norm, token_log_probs, token_loss
+from bdm_amd import _lib, ops
+from bdm_amd.lm import BDMConfig, LanguageModelConfig
+
+
+def tokens(*shape):
+    return torch.zeros(shape, dtype=torch.int64)
+
+
+@pytest.mark.parametrize('logits,given,options,error', [
+    (torch.zeros(3, 8), tokens(3), {}, ValueError),                                    # on the CPU
+    (torch.zeros(3, 8, dtype=torch.float16), tokens(3), {}, ValueError),
+    (torch.zeros(3, 8, dtype=torch.float64), tokens(3), {}, ValueError),
+    (torch.zeros(()), tokens(), {}, ValueError),
+    (torch.zeros(3, 0), tokens(3), {}, ValueError),
+    (torch.zeros(3, 8), tokens(4), {}, ValueError),
+    (torch.zeros(3, 8), tokens(3, 1), {}, ValueError),
+    (torch.zeros(3, 8), tokens(3).int(), {}, ValueError),
+    (torch.zeros(3, 8), tokens(3), dict(alternatives=9), ValueError),
+    (torch.zeros(3, 8), tokens(3), dict(alternatives=-1), ValueError),
+    (torch.zeros(3, 80), tokens(3), dict(alternatives=33), NotImplementedError),
+])
+def test_token_log_probs(logits, given, options, error):
+    with pytest.raises(error):
+        token_log_probs(logits, given, **options)
+    if not options:
+        with pytest.raises(error):
+            token_loss(logits, given)
+
+
+def test_token_gradient():
+    stats = torch.zeros(3, 2)
+    for options in (dict(grad_entropy=torch.zeros(3)), dict(grad_top_log_probs=torch.zeros(3, 1)),
+                    dict(grad_loss=torch.zeros(()))):
+        with pytest.raises(ValueError):
+            ops.token_gradient(torch.zeros(3, 8), tokens(3), stats, **options)
+
+
+@pytest.mark.parametrize('gradients,options', [
+    ([torch.zeros(3)], {}),
+    ([torch.zeros(3, dtype=torch.float16)], {}),
+    ([torch.zeros(3, dtype=torch.int64)], {}),
+    ([torch.zeros(3).to_sparse()], {}),
+    ([torch.zeros(3)], dict(out=[])),
+    ([torch.zeros(3)], dict(out=[None])),
+    ([torch.zeros(3)], dict(out=[torch.zeros(4)])),
+    ([torch.zeros(3)], dict(max_norm=-1.0)),
+    ([torch.zeros(3)], dict(max_norm=float('nan'))),
+])
+def test_clipping(gradients, options):
+    options = {'max_norm': 1.0, **options}
+    with pytest.raises(ValueError):
+        clip_gradients(gradients, **options)
+    if list(options) == ['max_norm'] and options['max_norm'] == 1.0:
+        with pytest.raises(ValueError):
+            gradient_norm(gradients)
+
+
+def test_layer_norm():
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    for call in (lambda: ops.layer_norm(x, w, None, 1e-5),                                 # on the CPU
+                 lambda: ops.layer_norm_backward(x, x, w, None, 1e-5),
+                 lambda: ops._layer_norm_parameters(x.half(), w, None),
+                 lambda: ops._layer_norm_parameters(x, torch.ones(9), None),
+                 lambda: ops._layer_norm_parameters(x, w, torch.ones(8, dtype=torch.bfloat16)),
+                 lambda: ops._layer_norm_parameters(torch.zeros(()), None, None),
+                 lambda: ops._layer_norm_parameters(torch.zeros(3, 0), None, None)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(NotImplementedError):
+        ops._layer_norm_parameters(torch.zeros(1, 16385), None, None)
+
+
+def test_layer_norm_on_the_cpu():
+    """torch's formula, with a residual too."""
+    norm = LayerNorm(12)
+    x, r = torch.randn(5, 12), torch.randn(5, 12)
+    total, y = norm.add_norm(x, r)
+    assert torch.equal(total, r + x)
+    assert torch.allclose(y, torch.nn.functional.layer_norm(total, (12,), norm.weight, norm.bias, norm.eps))
+    norm = LayerNorm(12, bias=False)
+    assert norm.bias is None and torch.allclose(norm(x), torch.nn.functional.layer_norm(x, (12,), norm.weight, None, 1e-5))
+
+
+def test_configuration():
+    assert 'normalization' not in LanguageModelConfig(memory=BDMConfig()).record()
+    assert LanguageModelConfig(memory=BDMConfig(), normalization='layer').record()['normalization'] == 'layer'
+    with pytest.raises(ValueError, match='normalization'):
+        LanguageModelConfig(memory=BDMConfig(), normalization='batch')
+
+
+# ------------------------------------------------------------------ the C entries: pointers are never followed here
+
+HELD = ctypes.c_void_p(4096)
+
+
+def test_token_entries():
+    lib = _lib.library()
+
+    def status(**fields):
+        a = _lib.TokenArgs()
+        a.logits = a.tokens = a.log_probs = 4096
+        a.rows, a.row_stride, a.vocab, a.dtype = 4, 8, 8, _lib.BDM_F32
+        for name, value in fields.items():
+            setattr(a, name, value)
+        return lib.bdm_token_log_probs(ctypes.byref(a), None, 0, None)
+
+    assert lib.bdm_token_log_probs(None, None, 0, None) == -1
+    for fields in (dict(rows=-1), dict(vocab=0), dict(row_stride=-1), dict(dtype=7), dict(logits=None), dict(tokens=None),
+                   dict(log_probs=None), dict(alternatives=9), dict(alternatives=-1), dict(alternatives=2)):
+        assert status(**fields) == -1, fields
+    assert status(alternatives=40, vocab=100) == -2
+    assert status(vocab=2 ** 30 + 1) == -2
+    assert status(rows=2 ** 32) == -2
+    assert status(rows=0, logits=None) == 0
+
+    def backward(**fields):
+        a = _lib.TokenGradArgs()
+        a.logits = a.tokens = a.stats = a.grad_logits = 4096
+        a.rows, a.row_stride, a.vocab, a.dtype = 4, 8, 8, _lib.BDM_F32
+        for name, value in fields.items():
+            setattr(a, name, value)
+        return lib.bdm_token_log_probs_backward(ctypes.byref(a), None)
+
+    assert lib.bdm_token_log_probs_backward(None, None) == -1
+    for fields in (dict(stats=None), dict(grad_logits=None), dict(grad_entropy=4096), dict(grad_top_log_probs=4096),
+                   dict(grad_loss=4096), dict(vocab=-5), dict(dtype=9)):
+        assert backward(**fields) == -1, fields
+    assert lib.bdm_token_loss(HELD, HELD, -1, 0, HELD, HELD, None) == -1
+    assert lib.bdm_token_loss(HELD, HELD, 4, 0, None, HELD, None) == -1
+    assert lib.bdm_token_loss(None, HELD, 4, 0, HELD, HELD, None) == -1
+
+
+def test_gradient_entries():
+    lib = _lib.library()
+    one = (_lib.Gradient * 1)()
+
+    def status(call, **fields):
+        g = one[0]
+        g.data, g.out, g.numel, g.dtype, g.out_dtype = 4096, 4096, 8, _lib.BDM_F32, _lib.BDM_F32
+        for name, value in fields.items():
+            setattr(g, name, value)
+        return call()
+
+    size = lib.bdm_gradient_norm_workspace_size(one, 1)
+    clip = lambda: lib.bdm_clip_gradients(one, 1, 1.0, HELD, HELD, 1 << 20, None)  # noqa: E731
+    norm = lambda: lib.bdm_gradient_norm(one, 1, 1.0, HELD, None, HELD, 1 << 20, None)  # noqa: E731
+    for fields in (dict(numel=-1), dict(dtype=5), dict(data=None)):
+        assert status(clip, **fields) == status(norm, **fields) == -1, fields
+    for fields in (dict(out=None), dict(out_dtype=3), dict(out=4100), dict(out=4096, out_dtype=_lib.BDM_BF16)):
+        assert status(clip, **fields) == -1, fields
+    assert status(clip, numel=2 ** 41) == status(norm, numel=2 ** 41) == -2
+    assert status(lambda: lib.bdm_clip_gradients(one, 1, -1.0, HELD, HELD, 1 << 20, None)) == -1
+    assert status(lambda: lib.bdm_clip_gradients(one, 1, float('nan'), HELD, HELD, 1 << 20, None)) == -1
+    assert status(lambda: lib.bdm_clip_gradients(one, 1, 1.0, HELD, HELD, 8, None)) == -1
+    assert status(lambda: lib.bdm_clip_gradients(one, 1, 1.0, HELD, None, 1 << 20, None)) == -1
+    assert status(lambda: lib.bdm_clip_gradients(None, 1, 1.0, HELD, HELD, 1 << 20, None)) == -1
+    assert status(lambda: lib.bdm_gradient_norm(one, -1, 1.0, HELD, None, HELD, 1 << 20, None)) == -1
+    assert size >= 16
+
+
+def test_layer_norm_entries():
+    lib = _lib.library()
+
+    def forward(x=HELD, residual=None, out=HELD, total=None, rows=4, width=8, dtype=0, param=0):
+        return lib.bdm_layer_norm(x, residual, None, None, total, out, rows, width, dtype, param, 1e-5, None)
+
+    for fields in (dict(x=None), dict(out=None), dict(residual=HELD), dict(rows=-1), dict(width=0), dict(dtype=4),
+                   dict(param=4)):
+        assert forward(**fields) == -1, fields
+    assert forward(width=16385) == forward(rows=2 ** 40) == -2
+    assert forward(rows=0, x=None) == 0
+    size = lib.bdm_layer_norm_backward_workspace_size(4, 8)
+    assert size > 0 and lib.bdm_layer_norm_backward_workspace_size(0, 8) == 0
+
+    def backward(x=HELD, dy=HELD, dx=HELD, rows=4, width=8, workspace=HELD, nbytes=size):
+        return lib.bdm_layer_norm_backward(x, dy, None, None, dx, None, None, rows, width, 0, 0, 1e-5, workspace, nbytes,
+                                           None)
+
+    for fields in (dict(x=None), dict(dy=None), dict(dx=None), dict(workspace=None), dict(nbytes=size - 1),
+                   dict(workspace=ctypes.c_void_p(4100)), dict(width=-1)):
+        assert backward(**fields) == -1, fields
+    assert backward(width=20000) == -2
