@@ -6,24 +6,22 @@
 // and with gradients a of log p_t, h of H and b_k of log p at the alternatives
 //   dx_i = a [i = t] + sum_k b_k [i = top_k] - p_i (a + sum_k b_k + h (log p_i + H)).
 // Everything is FP32.
-#include <cfloat>
+#include <algorithm>
 
 #include "bdm_common.h"
+#include "selection_ops.h"
 
 namespace bdm {
 namespace {
 
 constexpr int kAlternativesMax = 32;
+constexpr int kVocabMax = 1 << 24;
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr uint32_t kNanKey = UINT32_MAX - 1, kEmptyKey = 0x007fffffu;  // a NaN's, and that of -inf
 
-// Unsigned integers in the order of the floating values; -0 counts as +0, a NaN is above all.
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t u = __float_as_uint(x + 0.f);
-    return x != x ? UINT32_MAX - 1 : u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float unordered(uint32_t u) {
-    return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
-}
+// ordered() with a NaN above all others.
+__device__ __forceinline__ uint32_t ordered_all(float x) { return x != x ? kNanKey : ordered(x); }
 
 template <typename V, typename F>
 __device__ __forceinline__ V block_join(V x, F op, V *shared) {
@@ -41,24 +39,331 @@ __device__ __forceinline__ float log_probability(float x, float high, float log_
     return log_sum == -INFINITY ? -INFINITY : (x - high) - log_sum;
 }
 
-// One row per workgroup.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void token_log_probs_kernel(bdm_token_args a) {
-    __shared__ float floats[kWaves];
-    __shared__ unsigned long long keys[kWaves];
-    const int64_t row = blockIdx.x;
-    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
-    float high = -INFINITY;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) high = fmaxf(high, to_f32(x[i]));
-    high = block_join(high, [](float p, float q) { return fmaxf(p, q); }, floats);
-    const float from = high == -INFINITY ? 0.f : high;  // an empty row
-    float sum = 0.f, moment = 0.f;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-        const float d = to_f32(x[i]) - from, e = expf(d);
-        sum += e;
-        moment += e == 0.f ? 0.f : e * d;
+// ------------------------------------------------------------------ a team's part of a row
+template <int WAVES, int NV>
+struct Team {
+    static constexpr int kRoom = WAVES == 1 ? 128 : 64 * (WAVES < 8 ? WAVES : 8);
+    uint64_t list[kRoom];  // ordered value, then ~index: descending order is value, then lowest index
+    float high[WAVES], sum[WAVES], moment[WAVES];
+    uint32_t bound[WAVES], share[WAVES];
+    int found[WAVES];
+    int ties[WAVES][NV];
+    int count;
+};
+
+struct Rows {
+    bdm_token_args a;
+    float4 *parts;    // [rows, splits] maximum, sum of exponentials, their first moment
+    uint64_t *lists;  // [rows, splits, alternatives], 0 behind the last
+    int splits;
+};
+
+// A lane's vectors of a part.  Vector i has the row's values from `start(i)` on.  The last vector of a row starts early
+// enough to end with it; what the one before holds already, and what lies behind the row, is -inf in it.
+template <typename T, int WAVES>
+struct Place {
+    static constexpr int VE = Vec<T>::kSize, kSpan = WAVES * kWave * VE;
+    const T *x;                // the part's first value
+    int first, length, vocab;  // of the lane's first vector in the part; the part's values; the row's
+
+    __device__ __forceinline__ int begin(int i) const { return first + i * kSpan; }
+    __device__ __forceinline__ int start(int i) const { return vocab < VE ? begin(i) : min(begin(i), length - VE); }
+    __device__ __forceinline__ bool valid(int i, int j) const {
+        const int at = start(i) + j;
+        return at >= begin(i) && at < length;
     }
-    const auto add = [](float p, float q) { return p + q; };
+    __device__ __forceinline__ u32x4 load(int i) const { return reinterpret_cast<const AnyVector<T> *>(x + start(i))->bits; }
+    // of a row shorter than a vector
+    __device__ __forceinline__ u32x4 gather() const {
+        u32x4 raw{};
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const uint32_t bits = __float_as_uint(to_f32(x[min(j, vocab - 1)]));
+            if constexpr (VE == 8)
+                raw[j / 2] |= j % 2 ? bits : bits >> 16;
+            else
+                raw[j] = bits;
+        }
+        return raw;
+    }
+    __device__ __forceinline__ void mask(int i, u32x4 &raw) const {
+        if (begin(i) + VE <= length) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (valid(i, j)) continue;
+            if constexpr (VE == 8)
+                raw[j / 2] = j % 2 ? (raw[j / 2] & 0xffffu) | 0xff800000u : (raw[j / 2] & 0xffff0000u) | 0xff80u;
+            else
+                raw[j] = 0xff800000u;
+        }
+    }
+};
+
+// The exact `width` best of the team's values to sh.list where the bound does not serve: those above the width-th, then
+// of those equal to it the ones of lowest index, which lie in the order of vectors, lanes, places in the vector.  `guess`
+// is the width-th's key if no `width` values are above it (equal logits, or a mask over most of the row): three passes
+// over the part; else that is bisected, a pass a bit.  A function of its own, which loads vector by vector: it takes no
+// registers from the ordinary case.
+template <typename T, int WAVES, int NV>
+__device__ __noinline__ int team_exact(Team<WAVES, NV> &sh, const T *x, int length, int vocab, uint32_t guess, int width,
+                                       uint32_t offset, int wave, int lane) {
+    constexpr int VE = Vec<T>::kSize;
+    const Place<T, WAVES> place{x, (wave * kWave + lane) * VE, length, vocab};
+    width = min(width, length);
+    // f(i, keys of vector i, 0 where it has none)
+    const auto each = [&](auto f) {
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+            const u32x4 raw = vocab < VE ? place.gather() : place.load(i);
+            float v[VE];
+            uint32_t keys[VE];
+            Vec<T>::widen(raw, v);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) keys[j] = place.valid(i, j) ? ordered_all(v[j]) : 0;
+            f(i, keys);
+        }
+    };
+    const auto reach = [&](uint32_t least) {
+        int mine = 0;
+        each([&](int, const uint32_t *keys) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) mine += popcount(__ballot(keys[j] >= least));
+        });
+        if constexpr (WAVES > 1) {
+            if (lane == 0) sh.found[wave] = mine;
+            __syncthreads();
+            mine = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) mine += sh.found[i];
+            __syncthreads();
+        }
+        return mine;
+    };
+    team_sync<WAVES>();
+    uint32_t value = guess;
+    int above = reach(value + 1);
+    if (above >= width) {
+        value = 0;
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t next = value | (1u << bit);
+            if (reach(next) >= width) value = next;
+        }
+        above = reach(value + 1);
+    }
+    each([&](int i, const uint32_t *keys) {
+        int ties = 0;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) ties += popcount(__ballot(keys[j] == value));
+        if (lane == 0) sh.ties[wave][i] = ties;
+    });
+    if (wave == 0 && lane == 0) sh.count = 0;
+    team_sync<WAVES>();
+    int before = above;  // candidates ahead of the vector's, in this wave's order
+    each([&](int i, const uint32_t *keys) {
+        const auto take = [&](int j) {
+            sh.list[atomicAdd(&sh.count, 1)] = uint64_t(keys[j]) << 32 | uint32_t(~(offset + uint32_t(place.start(i) + j)));
+        };
+        int at = before;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            at += w < wave ? sh.ties[w][i] : 0;
+            before += sh.ties[w][i];
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) at += popcount(__ballot(keys[j] == value) & ((1ull << lane) - 1));
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+            if (keys[j] > value || (keys[j] == value && at++ < width)) take(j);
+    });
+    team_sync<WAVES>();
+    return sh.count;
+}
+
+// One part of one row, held in registers by a team of WAVES waves.
+template <typename T, int WAVES, int NV, bool TOP>
+__device__ __forceinline__ void score_part(const Rows &p, Team<WAVES, NV> &sh, int64_t row, int split, int wave, int lane) {
+    constexpr int VE = Vec<T>::kSize;
+    const bdm_token_args &a = p.a;
+    constexpr int kPart = NV * Place<T, WAVES>::kSpan;
+    const int offset = split * kPart, thread = wave * kWave + lane;
+    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
+    const Place<T, WAVES> place{x + offset, thread * VE, min(a.vocab - offset, kPart), a.vocab};
+    const int64_t token = a.tokens[row];
+    const bool inside = token >= 0 && token < a.vocab;
+    const float given = to_f32(x[inside ? token : 0]);
+    u32x4 raw[NV];
+    if (a.vocab >= VE) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = place.load(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = place.gather();
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) place.mask(i, raw[i]);
+    // f(i, values of vector i)
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float v[VE];
+            Vec<T>::widen(raw[i], v);
+            f(i, v);
+        }
+    };
+    float top = -INFINITY;
+    each([&](int, const float *v) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) top = fmaxf(top, v[j]);
+    });
+    float high = wave_max(top);
+    uint32_t bound = 0;
+    if constexpr (WAVES > 1) {
+        if constexpr (TOP) {
+            // `alternatives` lanes of one wave, or as many of all of them together, reach the bound
+            const uint32_t width = uint32_t(a.alternatives);
+            const Bounds<2> bounds = nth_of_lanes<2>(top > -INFINITY ? ordered(top) : 0u, {{width, (width + WAVES - 1) / WAVES}});
+            if (lane == 0) {
+                sh.bound[wave] = bounds.at[0];
+                sh.share[wave] = bounds.at[1];
+            }
+            if (thread == 0) sh.count = 0;
+        }
+        if (lane == 0) sh.high[wave] = high;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) high = fmaxf(high, sh.high[i]);
+        if constexpr (TOP) {
+            bound = sh.share[0];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) bound = min(bound, sh.share[i]);
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) bound = max(bound, sh.bound[i]);
+        }
+    } else if constexpr (TOP) {
+        bound = nth_of_lanes<1>(top > -INFINITY ? ordered(top) : 0u, {{uint32_t(a.alternatives)}}).at[0];
+        if (lane == 0) sh.count = 0;
+        team_sync<WAVES>();
+    }
+    const float from = high > -INFINITY ? high : 0.f;  // a part without a finite value has the sum 0
+    float sum = 0.f, moment = 0.f;
+    each([&](int, const float *v) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const float d = v[j] - from, e = __builtin_amdgcn_exp2f(d * kLog2E);
+            sum += e;
+            moment = fmaf(e, fmaxf(d, -1e30f), moment);  // e = 0 there: no 0 * inf
+        }
+    });
+    sum = wave_sum(sum);
+    moment = wave_sum(moment);
+    if constexpr (TOP) {
+        const float least = unordered(bound);
+        if (bound && top >= least) {
+            each([&](int i, const float *v) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    if (v[j] >= least) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < Team<WAVES, NV>::kRoom)
+                            sh.list[at] = uint64_t(ordered(v[j])) << 32 | uint32_t(~uint32_t(offset + place.start(i) + j));
+                    }
+                }
+            });
+        }
+    }
+    if constexpr (WAVES > 1) {
+        if (lane == 0) {
+            sh.sum[wave] = sum;
+            sh.moment[wave] = moment;
+        }
+        __syncthreads();
+        sum = moment = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            sum += sh.sum[i];
+            moment += sh.moment[i];
+        }
+    } else {
+        team_sync<WAVES>();
+    }
+    int count = 0;
+    if constexpr (TOP) {
+        count = sh.count;
+        if (!bound || count > Team<WAVES, NV>::kRoom || sum != sum)
+            count = team_exact<T, WAVES, NV>(sh, place.x, place.length, a.vocab, bound ? bound : kEmptyKey, a.alternatives,
+                                                  uint32_t(offset), wave, lane);
+    }
+    const float log_sum = logf(sum);
+    if (thread == 0) {
+        if (p.splits > 1) {
+            p.parts[row * p.splits + split] = make_float4(high, sum, moment, 0.f);
+        } else {
+            a.log_probs[row] = token == a.ignore_index ? 0.f : inside ? log_probability(given, from, log_sum) : NAN;
+            if (a.entropy) a.entropy[row] = sum == 0.f ? 0.f : log_sum - moment / sum;
+            if (a.stats) {
+                a.stats[2 * row] = from;
+                a.stats[2 * row + 1] = log_sum;
+            }
+        }
+    }
+    if constexpr (TOP) {
+        const int64_t out = (row * p.splits + split) * a.alternatives;
+        for (int i = thread; i < count; i += WAVES * kWave) {
+            const uint64_t mine = sh.list[i];
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < count; ++j) rank += sh.list[j] > mine;
+            if (rank >= a.alternatives) continue;
+            if (p.splits > 1) {
+                p.lists[out + rank] = mine;
+            } else {
+                a.top_tokens[out + rank] = int64_t(~uint32_t(mine));
+                a.top_log_probs[out + rank] = log_probability(unordered(uint32_t(mine >> 32)), from, log_sum);
+            }
+        }
+        if (p.splits > 1)
+            for (int i = count + thread; i < a.alternatives; i += WAVES * kWave) p.lists[out + i] = 0;
+    }
+}
+
+template <typename T, int WAVES, int NV, bool TOP>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void score_kernel(Rows p) {
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    if constexpr (WAVES == 1) {
+        __shared__ Team<1, NV> teams[4];
+        const int64_t row = int64_t(blockIdx.x) * 4 + wave;
+        if (row < p.a.rows) score_part<T, 1, NV, TOP>(p, teams[wave], row, 0, 0, lane);
+    } else {
+        __shared__ Team<WAVES, NV> team;
+        const int64_t row = blockIdx.x / uint32_t(p.splits);
+        score_part<T, WAVES, NV, TOP>(p, team, row, int(blockIdx.x % uint32_t(p.splits)), wave, lane);
+    }
+}
+
+// The parts of a row joined.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(Rows p) {
+    constexpr int kRoom = 512;
+    __shared__ float floats[kWaves];
+    __shared__ uint64_t keys[kWaves];
+    __shared__ uint64_t list[kRoom];
+    const bdm_token_args &a = p.a;
+    const int64_t row = blockIdx.x;
+    const float4 *parts = p.parts + row * p.splits;
+    float high = -INFINITY;
+    for (int i = threadIdx.x; i < p.splits; i += kThreads) high = fmaxf(high, parts[i].x);
+    high = block_join(high, [](float x, float y) { return fmaxf(x, y); }, floats);
+    const float from = high > -INFINITY ? high : 0.f;
+    float sum = 0.f, moment = 0.f;
+    for (int i = threadIdx.x; i < p.splits; i += kThreads) {
+        const float4 part = parts[i];
+        if (part.y == 0.f) continue;
+        const float d = (part.x > -INFINITY ? part.x : 0.f) - from, e = __builtin_amdgcn_exp2f(d * kLog2E);
+        sum += part.y * e;
+        moment += e == 0.f ? 0.f : e * (part.z + part.y * d);  // d may be near the lowest value
+    }
+    const auto add = [](float x, float y) { return x + y; };
     sum = block_join(sum, add, floats);
     moment = block_join(moment, add, floats);
     const float log_sum = logf(sum);
@@ -66,7 +371,9 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(bdm_token_arg
         const int64_t token = a.tokens[row];
         float lp = 0.f;
         if (token != a.ignore_index)
-            lp = token >= 0 && token < a.vocab ? log_probability(to_f32(x[token]), from, log_sum) : NAN;
+            lp = token >= 0 && token < a.vocab
+                     ? log_probability(to_f32(static_cast<const T *>(a.logits)[row * a.row_stride + token]), from, log_sum)
+                     : NAN;
         a.log_probs[row] = lp;
         if (a.entropy) a.entropy[row] = sum == 0.f ? 0.f : log_sum - moment / sum;
         if (a.stats) {
@@ -74,51 +381,129 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(bdm_token_arg
             a.stats[2 * row + 1] = log_sum;
         }
     }
-    unsigned long long last = UINT64_MAX;
+    if (!a.alternatives) return;
+    const int total = p.splits * a.alternatives;
+    const uint64_t *lists = p.lists + row * total;
+    const auto put = [&](int rank, uint64_t key) {
+        a.top_tokens[row * a.alternatives + rank] = int64_t(~uint32_t(key));
+        a.top_log_probs[row * a.alternatives + rank] = log_probability(unordered(uint32_t(key >> 32)), from, log_sum);
+    };
+    if (total <= kRoom) {
+        for (int i = threadIdx.x; i < total; i += kThreads) list[i] = lists[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < total; i += kThreads) {
+            const uint64_t mine = list[i];
+            int rank = 0;
+            for (int j = 0; j < total; ++j) rank += list[j] > mine;
+            if (mine && rank < a.alternatives) put(rank, mine);
+        }
+        return;
+    }
+    uint64_t last = UINT64_MAX;
     for (int k = 0; k < a.alternatives; ++k) {
-        unsigned long long best = 0;
-        for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-            const unsigned long long key = (unsigned long long)(ordered(to_f32(x[i]))) << 32 | uint32_t(~i);
+        uint64_t best = 0;
+        for (int i = threadIdx.x; i < total; i += kThreads) {
+            const uint64_t key = lists[i];
             if (key < last && key > best) best = key;
         }
-        best = block_join(best, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; }, keys);
-        if (threadIdx.x == 0) {
-            const int token = int(~uint32_t(best));
-            a.top_tokens[row * a.alternatives + k] = token;
-            a.top_log_probs[row * a.alternatives + k] = log_probability(to_f32(x[token]), from, log_sum);
-        }
+        best = block_join(best, [](uint64_t x, uint64_t y) { return x > y ? x : y; }, keys);
+        if (threadIdx.x == 0) put(k, best);
         last = best;
     }
 }
 
-// The gradients that reach a row: of its token's log-probability, its entropy and its alternatives.
-struct RowGradient {
-    float given, total, entropy;
-};
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad_args a) {
-    const int64_t row = blockIdx.x;
+// The gradient of a row's logits, one pass over them: a team of LANES lanes takes U vectors a lane of one row.  `TOPS`:
+// gradients of the alternatives arrive too.
+template <typename T, int LANES, int U, bool TOPS>
+__global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad_args a, int parts) {
+    constexpr int VE = Vec<T>::kSize;
+    __shared__ int spots[kThreads / LANES][kAlternativesMax];
+    __shared__ float weights[kThreads / LANES][kAlternativesMax];
+    const int team = int(threadIdx.x) / LANES, lane = int(threadIdx.x) % LANES;
+    const int64_t item = int64_t(blockIdx.x) * (kThreads / LANES) + team, row = item / parts;
+    if (row >= a.rows) return;
+    const int first = int(item % parts) * LANES * U * VE + lane * VE;
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     T *out = static_cast<T *>(a.grad_logits) + row * a.vocab;
+    const bool whole = a.vocab >= VE;
+    u32x4 raw[U];
+    if (whole) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            raw[u] = reinterpret_cast<const AnyVector<T> *>(x + min(first + u * LANES * VE, a.vocab - VE))->bits;
+    }
     const int64_t token = a.tokens[row];
     const float high = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
-    const float h = a.grad_entropy ? a.grad_entropy[row] : 0.f, entropy = a.entropy ? a.entropy[row] : 0.f;
+    const float h = a.grad_entropy ? a.grad_entropy[row] : 0.f, entropy = a.grad_entropy ? a.entropy[row] : 0.f;
     float given = 0.f;
     if (token != a.ignore_index && (a.grad_loss || a.grad_log_probs)) {
         given = a.grad_loss ? -(a.grad_loss[0] * a.inverse_count[0]) : a.grad_log_probs[row];
         if (token < 0 || token >= a.vocab) given = NAN;
     }
     float total = given;
-    const int tops = a.grad_top_log_probs ? a.alternatives : 0;
-    for (int k = 0; k < tops; ++k) total += a.grad_top_log_probs[row * tops + k];
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-        const float lp = (to_f32(x[i]) - high) - log_sum, p = expf(lp);
-        float d = p == 0.f ? 0.f : -p * (total + h * (lp + entropy));
-        if (i == token) d += given;
-        for (int k = 0; k < tops; ++k)
-            if (a.top_tokens[row * tops + k] == i) d += a.grad_top_log_probs[row * tops + k];
-        out[i] = from_f32<T>(log_sum == -INFINITY ? 0.f : d);
+    if constexpr (TOPS) {
+        if (lane < a.alternatives) {
+            spots[team][lane] = int(a.top_tokens[row * a.alternatives + lane]);
+            weights[team][lane] = a.grad_top_log_probs[row * a.alternatives + lane];
+        }
+        team_sync<LANES / kWave>();
+        for (int k = 0; k < a.alternatives; ++k) total += weights[team][k];
+    }
+    const int at = token >= 0 && token < a.vocab ? int(token) : -VE;
+    const bool empty = log_sum == -INFINITY;
+    // the gradient at index i of the row
+    const auto gradient = [&](float v) {
+        const float lp = (v - high) - log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2E);
+        return -p * (total + h * (fmaxf(lp, -1e30f) + entropy));  // p = 0 there: no 0 * inf
+    };
+    const auto spot = [&](int i) {
+        float d = i == at ? given : 0.f;
+        if constexpr (TOPS)
+            for (int k = 0; k < a.alternatives; ++k) d += spots[team][k] == i ? weights[team][k] : 0.f;
+        return d;
+    };
+    if (!whole) {
+        if (lane < a.vocab) out[lane] = from_f32<T>(empty ? 0.f : gradient(to_f32(x[lane])) + spot(lane));
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int begin = first + u * LANES * VE, start = min(begin, a.vocab - VE);
+        if (begin >= a.vocab) break;
+        float v[VE];
+        Vec<T>::widen(raw[u], v);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) v[j] = empty ? 0.f : gradient(v[j]);
+        if (!empty) {
+            if constexpr (TOPS) {
+                for (int k = 0; k < a.alternatives; ++k) {
+                    const int place = spots[team][k] - start;
+                    if (unsigned(place) < unsigned(VE)) {
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) v[j] += j == place ? weights[team][k] : 0.f;
+                    }
+                }
+            }
+            if (unsigned(at - start) < unsigned(VE)) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) v[j] += j == at - start ? given : 0.f;
+            }
+        }
+        if (begin + VE <= a.vocab) {
+            u32x4 bits;
+            if constexpr (VE == 8) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bits[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bits[j] = __float_as_uint(v[j]);
+            }
+            reinterpret_cast<AnyVector<T> *>(out + begin)->bits = bits;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if (start + j >= begin) out[start + j] = from_f32<T>(v[j]);
+        }
     }
 }
 
@@ -147,9 +532,72 @@ int check_rows(const char *what, int64_t rows, int64_t row_stride, int32_t vocab
     if (dtype != BDM_BF16 && dtype != BDM_F32) return fail(BDM_ERR_INVALID, "%s: dtype", what);
     if (alternatives > kAlternativesMax)
         return fail(BDM_ERR_UNSUPPORTED, "%s: more than %d alternatives", what, kAlternativesMax);
-    if (vocab > (1 << 30)) return fail(BDM_ERR_UNSUPPORTED, "%s: vocabulary beyond 2^30", what);
-    if (!grid_fits(rows, kThreads)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (vocab > kVocabMax) return fail(BDM_ERR_UNSUPPORTED, "%s: vocabulary beyond 2^24", what);
+    if (!grid_fits(rows, 1024)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
     return BDM_OK;
+}
+
+// A team's waves and values a lane, and the parts of a row.
+struct Shape {
+    int waves, values, splits;
+};
+
+Shape shape_of(const bdm_token_args &a) {
+    constexpr Shape kShapes[] = {{1, 8, 1}, {1, 16, 1}, {1, 32, 1}, {4, 16, 1}, {4, 32, 1}, {4, 64, 1}, {16, 32, 1}, {16, 48, 1},
+                                 {16, 56, 1}, {16, 64, 1}};
+    for (const Shape &shape : kShapes)
+        if (a.vocab <= shape.waves * kWave * shape.values) return shape;
+    Shape wide{16, 64, 1};
+    wide.splits = (a.vocab + 65535) / 65536;
+    return wide;
+}
+
+template <typename T, int WAVES, int VALUES>
+void launch_scores(const Rows &p, hipStream_t s) {
+    constexpr int NV = VALUES / Vec<T>::kSize, kTeam = WAVES == 1 ? 256 : WAVES * kWave;
+    const int64_t blocks = WAVES == 1 ? (p.a.rows + 3) / 4 : p.a.rows * p.splits;
+    if (p.a.alternatives)
+        score_kernel<T, WAVES, NV, true><<<unsigned(blocks), kTeam, 0, s>>>(p);
+    else
+        score_kernel<T, WAVES, NV, false><<<unsigned(blocks), kTeam, 0, s>>>(p);
+}
+
+template <typename T>
+int launch_scores(const Rows &p, const Shape &shape, hipStream_t s) {
+    if (shape.waves == 1)
+        shape.values == 8 ? launch_scores<T, 1, 8>(p, s) : shape.values == 16 ? launch_scores<T, 1, 16>(p, s) : launch_scores<T, 1, 32>(p, s);
+    else if (shape.waves == 4)
+        shape.values == 16 ? launch_scores<T, 4, 16>(p, s) : shape.values == 32 ? launch_scores<T, 4, 32>(p, s) : launch_scores<T, 4, 64>(p, s);
+    else if (shape.values == 32)
+        launch_scores<T, 16, 32>(p, s);
+    else if (shape.values == 48)
+        launch_scores<T, 16, 48>(p, s);
+    else if (shape.values == 56)
+        launch_scores<T, 16, 56>(p, s);
+    else
+        launch_scores<T, 16, 64>(p, s);
+    if (int rc = check_launch("score_kernel")) return rc;
+    if (p.splits == 1) return BDM_OK;
+    join_kernel<T><<<unsigned(p.a.rows), kThreads, 0, s>>>(p);
+    return check_launch("join_kernel");
+}
+
+template <typename T, int LANES, int U>
+int launch_gradient(const bdm_token_grad_args &a, hipStream_t s) {
+    constexpr int kPart = LANES * U * Vec<T>::kSize, kTeams = kThreads / LANES;
+    const int parts = (a.vocab + kPart - 1) / kPart;
+    const int64_t blocks = (a.rows * parts + kTeams - 1) / kTeams;
+    if (!grid_fits(blocks, kThreads)) return fail(BDM_ERR_UNSUPPORTED, "token_log_probs_backward: too many rows");
+    if (a.grad_top_log_probs)
+        token_gradient_kernel<T, LANES, U, true><<<unsigned(blocks), kThreads, 0, s>>>(a, parts);
+    else
+        token_gradient_kernel<T, LANES, U, false><<<unsigned(blocks), kThreads, 0, s>>>(a, parts);
+    return check_launch("token_gradient_kernel");
+}
+
+template <typename T>
+int launch_gradient(const bdm_token_grad_args &a, hipStream_t s) {
+    return a.vocab <= 1024 ? launch_gradient<T, 64, 4>(a, s) : launch_gradient<T, 256, 4>(a, s);
 }
 
 }  // namespace
@@ -157,21 +605,27 @@ int check_rows(const char *what, int64_t rows, int64_t row_stride, int32_t vocab
 
 using namespace bdm;
 
-extern "C" size_t bdm_token_log_probs_workspace_size(const bdm_token_args *) { return 0; }
+extern "C" size_t bdm_token_log_probs_workspace_size(const bdm_token_args *a) {
+    if (!a || a->rows <= 0 || a->vocab <= 0 || a->alternatives < 0 || a->vocab > kVocabMax) return 0;
+    const size_t splits = size_t(shape_of(*a).splits);
+    if (splits == 1) return 0;
+    return size_t(a->rows) * splits * (sizeof(float4) + size_t(a->alternatives) * sizeof(uint64_t));
+}
 
-extern "C" int bdm_token_log_probs(const bdm_token_args *a, void *, size_t, void *stream) {
+extern "C" int bdm_token_log_probs(const bdm_token_args *a, void *workspace, size_t workspace_bytes, void *stream) {
     if (!a) return fail(BDM_ERR_INVALID, "token_log_probs: null args");
     if (int rc = check_rows("token_log_probs", a->rows, a->row_stride, a->vocab, a->dtype, a->alternatives)) return rc;
     if (a->rows == 0) return BDM_OK;
-    if (!a->logits || !a->tokens || !a->log_probs ||
-        (a->alternatives && (!a->top_log_probs || !a->top_tokens)))
+    if (!a->logits || !a->tokens || !a->log_probs || (a->alternatives && (!a->top_log_probs || !a->top_tokens)))
         return fail(BDM_ERR_INVALID, "token_log_probs: null pointer");
-    hipStream_t s = as_stream(stream);
-    if (a->dtype == BDM_BF16)
-        token_log_probs_kernel<bf16_t><<<unsigned(a->rows), kThreads, 0, s>>>(*a);
-    else
-        token_log_probs_kernel<float><<<unsigned(a->rows), kThreads, 0, s>>>(*a);
-    return check_launch("token_log_probs_kernel");
+    const Shape shape = shape_of(*a);
+    if (!grid_fits(a->rows * shape.splits, 1024)) return fail(BDM_ERR_UNSUPPORTED, "token_log_probs: too many rows");
+    if (shape.splits > 1 && (!workspace || workspace_bytes < bdm_token_log_probs_workspace_size(a) || !aligned(workspace, 16)))
+        return fail(BDM_ERR_INVALID, "token_log_probs: workspace too small or not aligned to 16 bytes");
+    Rows p{*a, static_cast<float4 *>(workspace), nullptr, shape.splits};
+    p.lists = reinterpret_cast<uint64_t *>(p.parts + a->rows * shape.splits);
+    return a->dtype == BDM_BF16 ? launch_scores<bf16_t>(p, shape, as_stream(stream))
+                                : launch_scores<float>(p, shape, as_stream(stream));
 }
 
 extern "C" int bdm_token_log_probs_backward(const bdm_token_grad_args *a, void *stream) {
@@ -184,10 +638,8 @@ extern "C" int bdm_token_log_probs_backward(const bdm_token_grad_args *a, void *
         return fail(BDM_ERR_INVALID, "token_log_probs_backward: null pointer");
     hipStream_t s = as_stream(stream);
     if (a->dtype == BDM_BF16)
-        token_gradient_kernel<bf16_t><<<unsigned(a->rows), kThreads, 0, s>>>(*a);
-    else
-        token_gradient_kernel<float><<<unsigned(a->rows), kThreads, 0, s>>>(*a);
-    return check_launch("token_gradient_kernel");
+        return launch_gradient<bf16_t>(*a, s);
+    return launch_gradient<float>(*a, s);
 }
 
 extern "C" int bdm_token_loss(const float *log_probs, const int64_t *tokens, int64_t rows, int64_t ignore_index,
