@@ -4,25 +4,101 @@
 //   dx = r (dy w - mean(dy w) - xh mean(dy w xh)) + dsum,   dw = sum over rows dy xh,   db = sum over rows dy.
 // With a residual, x is the rounded sum, written beside y.  The statistics and
 // sums are FP32, the variance from the centred values.
+//
+// A row is held in registers by a team of waves, the next one loaded meanwhile; the backward keeps its columns' parts of
+// dw and db there too, over all rows of the team.  Every wave centres its values on its own mean c first, and one
+// exchange joins what all sums need: with d = x - c and n the wave's columns,
+//   mu = (sum over waves n c + sum d) / width,   sum (x - mu)^2 = sum d^2 + 2 (c - mu) sum d + n (c - mu)^2,
+//   sum g (x - mu) = sum g d + (c - mu) sum g       (g = dy w),
+// so that rows far from zero lose nothing, and a team of several waves waits once a row.
+#include <type_traits>
+
 #include "bdm_common.h"
 #include "epilogue_ops.h"
+#include "selection_ops.h"
 
 namespace bdm {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMaxWidth = 16384;
-constexpr int kRowsPerPart = 32;
+constexpr int kSumWaves = 16;
 
-__device__ __forceinline__ float block_sum(float x, float *shared) {
-    x = wave_total<kWave>(x);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) shared[threadIdx.x / kWave] = x;
-    __syncthreads();
-    x = shared[0];
-    for (int i = 1; i < kWaves; ++i) x += shared[i];
-    return x;
-}
+template <int N, typename P>
+struct __attribute__((packed, aligned(sizeof(P)))) Packed {
+    P at[N];
+};
+
+// The columns of a lane: NV vectors of VE, the team's lanes next to each other.  Vector i starts at column `start(i)`:
+// the last one of a row early enough to end with it, the columns that the one before holds already not `valid` in it.
+template <int LANES, int VE>
+struct Columns {
+    int thread, width;
+    __device__ __forceinline__ int begin(int i) const { return (thread + i * LANES) * VE; }
+    __device__ __forceinline__ int start(int i) const { return width < VE ? 0 : min(begin(i), width - VE); }
+    __device__ __forceinline__ bool full(int i) const { return begin(i) + VE <= width; }
+    __device__ __forceinline__ bool valid(int i, int j) const {
+        const int at = start(i) + j;
+        return at >= begin(i) && at < width;
+    }
+    template <typename T>
+    __device__ __forceinline__ u32x4 load(const T *row, int i) const {
+        if (width >= VE) return reinterpret_cast<const AnyVector<T> *>(row + start(i))->bits;
+        u32x4 raw{};
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const uint32_t bits = __float_as_uint(to_f32(row[min(j, width - 1)]));
+            if constexpr (VE == 8)
+                raw[j / 2] |= j % 2 ? bits : bits >> 16;
+            else
+                raw[j] = bits;
+        }
+        return raw;
+    }
+    // values of vector i, 0 where it has none
+    template <typename T>
+    __device__ __forceinline__ void widen(u32x4 raw, int i, float (&out)[VE]) const {
+        Vec<T>::widen(raw, out);
+        clear(i, out);
+    }
+    __device__ __forceinline__ void clear(int i, float (&out)[VE]) const {
+        if (full(i)) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) out[j] = valid(i, j) ? out[j] : 0.f;
+    }
+    template <typename P>
+    __device__ __forceinline__ void parameters(const void *p, int i, float other, float (&out)[VE]) const {
+        const P *from = static_cast<const P *>(p);
+        if (!p) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) out[j] = other;
+        } else if (width >= VE) {
+            const Packed<VE, P> some = *reinterpret_cast<const Packed<VE, P> *>(from + start(i));
+#pragma unroll
+            for (int j = 0; j < VE; ++j) out[j] = to_f32(some.at[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) out[j] = to_f32(from[min(j, width - 1)]);
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T *row, int i, const float (&v)[VE]) const {
+        if (full(i)) {
+            u32x4 bits;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (VE == 8)
+                    bits[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+                else
+                    bits[j] = __float_as_uint(v[j]);
+            }
+            reinterpret_cast<AnyVector<T> *>(row + begin(i))->bits = bits;
+        } else if (begin(i) < width) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if (valid(i, j)) row[start(i) + j] = from_f32<T>(v[j]);
+        }
+    }
+};
 
 template <typename T>
 struct Rows {
@@ -31,85 +107,285 @@ struct Rows {
     T *sum_out, *out;
     float *partials;
     int64_t rows;
-    int width, param_dtype;
+    int width;
     float eps;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_kernel(Rows<T> p) {
-    __shared__ float shared[kWaves];
-    const int64_t base = int64_t(blockIdx.x) * p.width;
-    const auto value = [&](int c) {
-        const float x = to_f32(p.x[base + c]);
-        return p.residual ? round_to<T>(x + to_f32(p.residual[base + c])) : x;
+// A team of 16 waves has 128 registers a lane: it loads a row when its turn comes, and the parameters with every row.
+constexpr int kLeanWaves = 16;
+
+// What a wave gives to its team of a row.
+struct Sums {
+    float count, centre, d, square, g, gd;
+};
+
+// The row's mean as an offset from the wave's own centre, 1 / deviation, mean g and mean g xh.
+struct Statistics {
+    float offset, scale, g, dot;
+};
+
+template <int WAVES, bool GRADIENT>
+__device__ __forceinline__ Statistics join(Sums mine, Sums (&shared)[2][WAVES], int turn, int wave, int lane, int width,
+                                           float eps) {
+    const float inverse = 1.f / float(width);
+    Statistics out{};
+    if constexpr (WAVES == 1) {
+        out.offset = mine.d * inverse;
+        out.scale = rsqrtf(fmaxf(mine.square * inverse - out.offset * out.offset, 0.f) + eps);
+        out.g = mine.g * inverse;
+        out.dot = (mine.gd - out.offset * mine.g) * inverse * out.scale;
+    } else {
+        if (lane == 0) shared[turn][wave] = mine;
+        __syncthreads();
+        const float pivot = shared[turn][0].centre;
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+            total += fmaf(shared[turn][w].count, shared[turn][w].centre - pivot, shared[turn][w].d);
+        const float mean = total * inverse;  // from the pivot
+        float square = 0.f, g = 0.f, gd = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const Sums &s = shared[turn][w];
+            const float from = (s.centre - pivot) - mean;
+            square += s.square + from * (2.f * s.d + s.count * from);
+            if constexpr (GRADIENT) {
+                g += s.g;
+                gd += s.gd + from * s.g;
+            }
+        }
+        out.offset = mean - (mine.centre - pivot);
+        out.scale = rsqrtf(fmaxf(square * inverse, 0.f) + eps);
+        out.g = g * inverse;
+        out.dot = gd * inverse * out.scale;
+    }
+    return out;
+}
+
+template <int LANES, int VE, int NV>
+__device__ __forceinline__ float columns_of_wave(const Columns<LANES, VE> &c, int wave) {
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) count += min(max(c.width - (wave * kWave + i * LANES) * VE, 0), kWave * VE);
+    return float(count);
+}
+
+// Teams of WAVES waves take the rows in turn; a workgroup holds four teams of one wave, or one team.
+template <typename T, typename P, int WAVES, int NV, bool RESIDUAL>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_kernel(Rows<T> p) {
+    constexpr int VE = Vec<T>::kSize, kTeams = WAVES == 1 ? 4 : 1;
+    constexpr bool kLean = WAVES == kLeanWaves;
+    __shared__ Sums shared[2][WAVES];
+    const int lane = int(threadIdx.x) % kWave, wave = WAVES == 1 ? 0 : int(threadIdx.x) / kWave;
+    const Columns<WAVES * kWave, VE> c{wave * kWave + lane, p.width};
+    const int64_t step = int64_t(gridDim.x) * kTeams;
+    int64_t row = int64_t(blockIdx.x) * kTeams + (WAVES == 1 ? int(threadIdx.x) / kWave : 0);
+    if (row >= p.rows) return;
+    u32x4 x[NV], r[NV];
+    const auto load = [&](int64_t at) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] = c.load(p.x + at * p.width, i);
+            if constexpr (RESIDUAL) r[i] = c.load(p.residual + at * p.width, i);
+        }
     };
-    float sum = 0.f, square = 0.f;
-    for (int c = threadIdx.x; c < p.width; c += kThreads) sum += value(c);
-    const float mean = block_sum(sum, shared) / float(p.width);
-    for (int c = threadIdx.x; c < p.width; c += kThreads) {
-        const float d = value(c) - mean;
-        square = fmaf(d, d, square);
+    float weight[NV][VE], bias[NV][VE];
+    if constexpr (!kLean) {
+        load(row);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            c.template parameters<P>(p.weight, i, 1.f, weight[i]);
+            c.template parameters<P>(p.bias, i, 0.f, bias[i]);
+        }
     }
-    const float scale = rsqrtf(block_sum(square, shared) / float(p.width) + p.eps);
-    for (int c = threadIdx.x; c < p.width; c += kThreads) {
-        const float x = value(c);
-        float y = (x - mean) * scale;
-        if (p.weight) y *= param_at(p.weight, p.param_dtype, c);
-        if (p.bias) y += param_at(p.bias, p.param_dtype, c);
-        if (p.residual) p.sum_out[base + c] = from_f32<T>(x);
-        p.out[base + c] = from_f32<T>(y);
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_backward_kernel(Rows<T> p) {
-    __shared__ float shared[kWaves];
-    float *dw = p.partials + int64_t(blockIdx.x) * 2 * p.width, *db = dw + p.width;
-    for (int c = threadIdx.x; c < p.width; c += kThreads) dw[c] = db[c] = 0.f;
-    const int64_t first = int64_t(blockIdx.x) * kRowsPerPart, last = min(p.rows, first + kRowsPerPart);
-    for (int64_t row = first; row < last; ++row) {
+    const float count = columns_of_wave<WAVES * kWave, VE, NV>(c, wave);
+    int turn = 0;
+    for (; row < p.rows; row += step, turn ^= 1) {
         const int64_t base = row * p.width;
-        float sum = 0.f, square = 0.f, dot = 0.f, plain = 0.f;
-        for (int c = threadIdx.x; c < p.width; c += kThreads) sum += to_f32(p.x[base + c]);
-        const float mean = block_sum(sum, shared) / float(p.width);
-        for (int c = threadIdx.x; c < p.width; c += kThreads) {
-            const float d = to_f32(p.x[base + c]) - mean;
-            square = fmaf(d, d, square);
+        if constexpr (kLean) load(row);
+        float v[NV][VE];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            c.template widen<T>(x[i], i, v[i]);
+            if constexpr (RESIDUAL) {
+                float other[VE];
+                c.template widen<T>(r[i], i, other);
+#pragma unroll
+                for (int j = 0; j < VE; ++j) v[i][j] = round_to<T>(v[i][j] + other[j]);
+                c.store(p.sum_out + base, i, v[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < VE; ++j) sum += v[i][j];
         }
-        const float scale = rsqrtf(block_sum(square, shared) / float(p.width) + p.eps);
-        for (int c = threadIdx.x; c < p.width; c += kThreads) {
-            const float dy = to_f32(p.grad_out[base + c]), xh = (to_f32(p.x[base + c]) - mean) * scale;
-            const float g = p.weight ? dy * param_at(p.weight, p.param_dtype, c) : dy;
-            plain += g;
-            dot = fmaf(g, xh, dot);
-            dw[c] = fmaf(dy, xh, dw[c]);
-            db[c] += dy;
+        if (!kLean && row + step < p.rows) load(row + step);
+        Sums s{};
+        s.count = count;
+        s.centre = wave_sum(sum) / fmaxf(count, 1.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[i][j] -= s.centre;
+            c.clear(i, v[i]);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                s.d += v[i][j];
+                s.square = fmaf(v[i][j], v[i][j], s.square);
+            }
         }
-        plain = block_sum(plain, shared) / float(p.width);
-        dot = block_sum(dot, shared) / float(p.width);
-        for (int c = threadIdx.x; c < p.width; c += kThreads) {
-            const float dy = to_f32(p.grad_out[base + c]), xh = (to_f32(p.x[base + c]) - mean) * scale;
-            const float g = p.weight ? dy * param_at(p.weight, p.param_dtype, c) : dy;
-            float dx = (g - plain - xh * dot) * scale;
-            if (p.grad_sum) dx += to_f32(p.grad_sum[base + c]);
-            p.out[base + c] = from_f32<T>(dx);
+        s.d = wave_sum(s.d);
+        s.square = wave_sum(s.square);
+        const Statistics t = join<WAVES, false>(s, shared, turn, wave, lane, p.width, p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (kLean) {
+                c.template parameters<P>(p.weight, i, 1.f, weight[i]);
+                c.template parameters<P>(p.bias, i, 0.f, bias[i]);
+            }
+            float y[VE];
+#pragma unroll
+            for (int j = 0; j < VE; ++j) y[j] = fmaf((v[i][j] - t.offset) * t.scale, weight[i][j], bias[i][j]);
+            c.store(p.out + base, i, y);
         }
     }
 }
 
-__global__ __launch_bounds__(kThreads) void layer_norm_param_kernel(const float *partials, int64_t parts, int width,
-                                                                    void *dw, void *db, int dtype) {
-    const int c = int(blockIdx.x) * kThreads + threadIdx.x;
-    if (c >= 2 * width) return;
+template <typename T, typename P, int WAVES, int NV, bool SUM>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_backward_kernel(Rows<T> p) {
+    constexpr int VE = Vec<T>::kSize, kTeams = WAVES == 1 ? 4 : 1, kColumns = WAVES * kWave * NV * VE;
+    constexpr bool kLean = WAVES == kLeanWaves;
+    __shared__ Sums shared[2][WAVES];
+    __shared__ float slice[WAVES == 1 ? 4 : 1][WAVES == 1 ? kColumns : 1];
+    const int lane = int(threadIdx.x) % kWave, wave = WAVES == 1 ? 0 : int(threadIdx.x) / kWave;
+    const int team = WAVES == 1 ? int(threadIdx.x) / kWave : 0;
+    const Columns<WAVES * kWave, VE> c{wave * kWave + lane, p.width};
+    const int64_t step = int64_t(gridDim.x) * kTeams;
+    int64_t row = int64_t(blockIdx.x) * kTeams + team;
+    u32x4 x[NV], dy[NV], ds[NV];
+    const auto load = [&](int64_t at) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] = c.load(p.x + at * p.width, i);
+            dy[i] = c.load(p.grad_out + at * p.width, i);
+            if constexpr (SUM) ds[i] = c.load(p.grad_sum + at * p.width, i);
+        }
+    };
+    if (!kLean && row < p.rows) load(row);
+    float weight[NV][VE], dw[NV][VE], db[NV][VE];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if constexpr (!kLean) c.template parameters<P>(p.weight, i, 1.f, weight[i]);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) dw[i][j] = db[i][j] = 0.f;
+    }
+    const float count = columns_of_wave<WAVES * kWave, VE, NV>(c, wave);
+    int turn = 0;
+    for (; row < p.rows; row += step, turn ^= 1) {
+        const int64_t base = row * p.width;
+        if constexpr (kLean) load(row);
+        float v[NV][VE], g[NV][VE], more[NV][VE];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            c.template widen<T>(x[i], i, v[i]);
+            c.template widen<T>(dy[i], i, g[i]);
+            if constexpr (SUM) Vec<T>::widen(ds[i], more[i]);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) sum += v[i][j];
+        }
+        if (!kLean && row + step < p.rows) load(row + step);
+        Sums s{};
+        s.count = count;
+        s.centre = wave_sum(sum) / fmaxf(count, 1.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[i][j] -= s.centre;
+            c.clear(i, v[i]);
+            if constexpr (kLean) c.template parameters<P>(p.weight, i, 1.f, weight[i]);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const float gw = g[i][j] * weight[i][j];
+                s.d += v[i][j];
+                s.square = fmaf(v[i][j], v[i][j], s.square);
+                s.g += gw;
+                s.gd = fmaf(gw, v[i][j], s.gd);
+            }
+        }
+        s.d = wave_sum(s.d);
+        s.square = wave_sum(s.square);
+        s.g = wave_sum(s.g);
+        s.gd = wave_sum(s.gd);
+        const Statistics t = join<WAVES, true>(s, shared, turn, wave, lane, p.width, p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (kLean) c.template parameters<P>(p.weight, i, 1.f, weight[i]);
+            float dx[VE];
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const float xh = (v[i][j] - t.offset) * t.scale;
+                dw[i][j] = fmaf(g[i][j], xh, dw[i][j]);
+                db[i][j] += g[i][j];
+                dx[j] = (g[i][j] * weight[i][j] - t.g - xh * t.dot) * t.scale;
+                if constexpr (SUM) dx[j] += more[i][j];
+            }
+            c.store(p.out + base, i, dx);
+        }
+    }
+    float *part = p.partials + int64_t(blockIdx.x) * 2 * p.width;
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                if (!c.valid(i, j)) continue;
+                part[c.start(i) + j] = dw[i][j];
+                part[p.width + c.start(i) + j] = db[i][j];
+            }
+        }
+    } else {
+        // the four teams' sums, in their order
+        const auto put = [&](const float (&from)[NV][VE], float *to) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j)
+                    if (c.valid(i, j)) slice[team][c.start(i) + j] = from[i][j];
+            }
+            __syncthreads();
+            for (int at = threadIdx.x; at < p.width; at += 256)
+                to[at] = ((slice[0][at] + slice[1][at]) + slice[2][at]) + slice[3][at];
+            __syncthreads();
+        };
+        put(dw, part);
+        put(db, part + p.width);
+    }
+}
+
+// The parts' sums, column by column: wave k of a workgroup's 16 takes the parts k, k + 16, ..., and the waves' sums are
+// added in their order.
+__global__ __launch_bounds__(kSumWaves * kWave) void layer_norm_param_kernel(const float *partials, int parts, int width,
+                                                                             void *dw, void *db, int dtype) {
+    __shared__ float slice[kSumWaves][kWave];
+    const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
+    const int c = int(blockIdx.x) * kWave + lane;
     float total = 0.f;
-    for (int64_t i = 0; i < parts; ++i) total += partials[i * 2 * width + c];
+    if (c < 2 * width) {
+#pragma unroll 8
+        for (int i = wave; i < parts; i += kSumWaves) total += partials[int64_t(i) * 2 * width + c];
+    }
+    slice[wave][lane] = total;
+    __syncthreads();
+    if (wave != 0 || c >= 2 * width) return;
+    float sum = slice[0][lane];
+    for (int k = 1; k < kSumWaves; ++k) sum += slice[k][lane];
     void *out = c < width ? dw : db;
     if (!out) return;
     const int at = c < width ? c : c - width;
     if (dtype == BDM_BF16)
-        static_cast<bf16_t *>(out)[at] = from_f32<bf16_t>(total);
+        static_cast<bf16_t *>(out)[at] = from_f32<bf16_t>(sum);
     else
-        static_cast<float *>(out)[at] = total;
+        static_cast<float *>(out)[at] = sum;
 }
 
 int check_rows(const char *what, int64_t rows, int32_t width, int32_t dtype, int32_t param_dtype) {
@@ -117,9 +393,37 @@ int check_rows(const char *what, int64_t rows, int32_t width, int32_t dtype, int
     if (width > kMaxWidth) return fail(BDM_ERR_UNSUPPORTED, "%s: width %d > %d", what, width, kMaxWidth);
     if ((dtype != BDM_BF16 && dtype != BDM_F32) || (param_dtype != BDM_BF16 && param_dtype != BDM_F32))
         return fail(BDM_ERR_INVALID, "%s: dtype", what);
-    if (!grid_fits(rows, kThreads)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (rows > (int64_t(1) << 40)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
     return BDM_OK;
 }
+
+// Waves of a team and vectors of a lane for a width: a wave holds up to 1024 columns, 16 a lane.
+template <typename T, typename F>
+void with_shape(int width, F f) {
+    constexpr int kVectors = 16 / Vec<T>::kSize;
+    const auto shape = [&](auto waves, auto vectors) { f(waves, vectors); };
+    if (width <= 512)
+        shape(std::integral_constant<int, 1>{}, std::integral_constant<int, kVectors / 2>{});
+    else if (width <= 1024)
+        shape(std::integral_constant<int, 1>{}, std::integral_constant<int, kVectors>{});
+    else if (width <= 2048)
+        shape(std::integral_constant<int, 2>{}, std::integral_constant<int, kVectors>{});
+    else if (width <= 4096)
+        shape(std::integral_constant<int, 4>{}, std::integral_constant<int, kVectors>{});
+    else if (width <= 8192)
+        shape(std::integral_constant<int, 8>{}, std::integral_constant<int, kVectors>{});
+    else
+        shape(std::integral_constant<int, 16>{}, std::integral_constant<int, kVectors>{});
+}
+
+// Workgroups of a pass over the rows: as many as there is work for, at most those that the chip holds at once.
+int64_t blocks_of(int64_t rows, int width, int64_t waves) {
+    const int64_t team = width <= 1024 ? 1 : width <= 2048 ? 2 : width <= 4096 ? 4 : width <= 8192 ? 8 : 16;
+    const int64_t teams = team == 1 ? 4 : 1, most = waves / (team * teams);
+    const int64_t blocks = (rows + teams - 1) / teams;
+    return blocks < most ? blocks : most;
+}
+constexpr int64_t kForwardWaves = 256 * 32, kBackwardWaves = 256 * 8;
 
 }  // namespace
 }  // namespace bdm
@@ -132,22 +436,32 @@ extern "C" int bdm_layer_norm(const void *x, const void *residual, const void *w
     if (int rc = check_rows("layer_norm", rows, width, dtype, param_dtype)) return rc;
     if (rows == 0) return BDM_OK;
     if (!x || !out || (residual && !sum_out)) return fail(BDM_ERR_INVALID, "layer_norm: null pointer");
-    const auto run = [&](auto element) {
+    const auto run = [&](auto element, auto parameter) {
         using T = decltype(element);
-        Rows<T> p{static_cast<const T *>(x), static_cast<const T *>(residual), nullptr, nullptr, weight, bias,
-                  static_cast<T *>(sum_out), static_cast<T *>(out), nullptr, rows, width, param_dtype, eps};
-        layer_norm_kernel<T><<<unsigned(rows), kThreads, 0, as_stream(stream)>>>(p);
+        using P = decltype(parameter);
+        const Rows<T> p{static_cast<const T *>(x), static_cast<const T *>(residual), nullptr, nullptr, weight, bias,
+                        static_cast<T *>(sum_out), static_cast<T *>(out), nullptr, rows, width, eps};
+        const unsigned blocks = unsigned(blocks_of(rows, width, kForwardWaves));
+        with_shape<T>(width, [&](auto waves, auto vectors) {
+            constexpr int kTeam = decltype(waves)::value;
+            constexpr int kBlock = kTeam == 1 ? 256 : kTeam * kWave;
+            if (residual)
+                layer_norm_kernel<T, P, kTeam, decltype(vectors)::value, true><<<blocks, kBlock, 0, as_stream(stream)>>>(p);
+            else
+                layer_norm_kernel<T, P, kTeam, decltype(vectors)::value, false><<<blocks, kBlock, 0, as_stream(stream)>>>(p);
+        });
     };
     if (dtype == BDM_BF16)
-        run(bf16_t{});
+        param_dtype == BDM_BF16 ? run(bf16_t{}, bf16_t{}) : run(bf16_t{}, float{});
     else
-        run(float{});
+        param_dtype == BDM_BF16 ? run(float{}, bf16_t{}) : run(float{}, float{});
     return check_launch("layer_norm_kernel");
 }
 
 extern "C" size_t bdm_layer_norm_backward_workspace_size(int64_t rows, int32_t width) {
     if (rows <= 0 || width <= 0) return 0;
-    return size_t((rows + kRowsPerPart - 1) / kRowsPerPart) * 2 * size_t(width) * sizeof(float);
+    if (width > kMaxWidth) return 0;
+    return size_t(blocks_of(rows, width, kBackwardWaves)) * 2 * size_t(width) * sizeof(float);
 }
 
 extern "C" int bdm_layer_norm_backward(const void *x, const void *grad_out, const void *grad_sum, const void *weight,
@@ -160,21 +474,30 @@ extern "C" int bdm_layer_norm_backward(const void *x, const void *grad_out, cons
     if (workspace_bytes < bdm_layer_norm_backward_workspace_size(rows, width) || !aligned(workspace, 16))
         return fail(BDM_ERR_INVALID, "layer_norm_backward: workspace too small or not aligned to 16 bytes");
     hipStream_t s = as_stream(stream);
-    const int64_t parts = (rows + kRowsPerPart - 1) / kRowsPerPart;
-    const auto run = [&](auto element) {
+    const int64_t parts = blocks_of(rows, width, kBackwardWaves);
+    const auto run = [&](auto element, auto parameter) {
         using T = decltype(element);
-        Rows<T> p{static_cast<const T *>(x), nullptr, static_cast<const T *>(grad_out), static_cast<const T *>(grad_sum),
-                  weight, nullptr, nullptr, static_cast<T *>(grad_x), static_cast<float *>(workspace), rows, width,
-                  param_dtype, eps};
-        if (parts) layer_norm_backward_kernel<T><<<unsigned(parts), kThreads, 0, s>>>(p);
+        using P = decltype(parameter);
+        const Rows<T> p{static_cast<const T *>(x), nullptr, static_cast<const T *>(grad_out), static_cast<const T *>(grad_sum),
+                        weight, nullptr, nullptr, static_cast<T *>(grad_x), static_cast<float *>(workspace), rows, width, eps};
+        with_shape<T>(width, [&](auto waves, auto vectors) {
+            constexpr int kTeam = decltype(waves)::value;
+            constexpr int kBlock = kTeam == 1 ? 256 : kTeam * kWave;
+            if (grad_sum)
+                layer_norm_backward_kernel<T, P, kTeam, decltype(vectors)::value, true><<<unsigned(parts), kBlock, 0, s>>>(p);
+            else
+                layer_norm_backward_kernel<T, P, kTeam, decltype(vectors)::value, false><<<unsigned(parts), kBlock, 0, s>>>(p);
+        });
     };
-    if (dtype == BDM_BF16)
-        run(bf16_t{});
-    else
-        run(float{});
+    if (parts) {
+        if (dtype == BDM_BF16)
+            param_dtype == BDM_BF16 ? run(bf16_t{}, bf16_t{}) : run(bf16_t{}, float{});
+        else
+            param_dtype == BDM_BF16 ? run(float{}, bf16_t{}) : run(float{}, float{});
+    }
     if (int rc = check_launch("layer_norm_backward_kernel")) return rc;
     if (!grad_weight && !grad_bias) return BDM_OK;
-    layer_norm_param_kernel<<<unsigned((2 * width + kThreads - 1) / kThreads), kThreads, 0, s>>>(
-        static_cast<const float *>(workspace), parts, width, grad_weight, grad_bias, param_dtype);
+    layer_norm_param_kernel<<<unsigned((2 * width + kWave - 1) / kWave), kSumWaves * kWave, 0, s>>>(
+        static_cast<const float *>(workspace), int(parts), width, grad_weight, grad_bias, param_dtype);
     return check_launch("layer_norm_param_kernel");
 }
