@@ -257,11 +257,6 @@ class TokenGradArgs(ctypes.Structure):
     ]
 
 
-class Gradient(ctypes.Structure):
-    """Mirror of ``bdm_gradient``."""
-    _fields_ = [('data', _vp), ('out', _vp), ('numel', _i64), ('dtype', _i32), ('out_dtype', _i32)]
-
-
 class BDMError(RuntimeError):
     """A call into libbdm_hip returned a non-zero status."""
 
@@ -373,12 +368,11 @@ def library() -> ctypes.CDLL:
     lib.bdm_token_log_probs_backward.restype = _i32
     lib.bdm_token_loss.argtypes = [_vp, _vp, _i64, _i64, _vp, _vp, _vp]
     lib.bdm_token_loss.restype = _i32
-    gradients = ctypes.POINTER(Gradient)
-    lib.bdm_gradient_norm_workspace_size.argtypes = [gradients, _i32]
+    lib.bdm_gradient_norm_workspace_size.argtypes = [_vp, _i32]
     lib.bdm_gradient_norm_workspace_size.restype = _size_t
-    lib.bdm_gradient_norm.argtypes = [gradients, _i32, ctypes.c_double, _vp, _vp, _vp, _size_t, _vp]
+    lib.bdm_gradient_norm.argtypes = [_vp, _vp, _vp, _i32, ctypes.c_double, _vp, _vp, _vp, _size_t, _vp]
     lib.bdm_gradient_norm.restype = _i32
-    lib.bdm_clip_gradients.argtypes = [gradients, _i32, ctypes.c_double, _vp, _vp, _size_t, _vp]
+    lib.bdm_clip_gradients.argtypes = [_vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_double, _vp, _vp, _size_t, _vp]
     lib.bdm_clip_gradients.restype = _i32
     lib.bdm_layer_norm.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp]
     lib.bdm_layer_norm.restype = _i32

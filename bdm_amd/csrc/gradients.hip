@@ -5,26 +5,39 @@
 // Squares and their sums are FP64: those of FP32 overflow from 2e19 on and
 // vanish below 1e-23, and a sum of a billion of them is exact to the last bits
 // of the norm.  Every sum is made in a fixed order.
+//
+// The tensors' addresses are arguments of the launch, so that nothing is copied
+// to the device before it and a captured graph keeps them.  Workgroups take the
+// tensors' chunks in turn, one FP64 sum each; those that scale add up the few
+// thousand sums for themselves, which costs less than a launch between.
 #include <algorithm>
 #include <vector>
 
 #include "bdm_common.h"
+#include "selection_ops.h"
 
 namespace bdm {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kChunk = 16384;  // elements of one tensor that a workgroup takes
-constexpr int kBatch = 100;    // tensors of one launch, in its arguments
+constexpr int kChunk = 16384;       // elements of one tensor that a workgroup takes at a time
+constexpr int64_t kMostParts = 2048;  // sums of a call: eight workgroups a CU
+constexpr uint32_t kSizeMask = (1u << 30) - 1;
 
-struct Batch {
-    bdm_gradient tensors[kBatch];
-    uint32_t end[kBatch];  // chunks of the batch up to and with this tensor's
+// Tensors of one launch: chunk k belongs to the first tensor whose `end` is above it.  The size's upper bits hold the
+// types: bit 31 the data's, bit 30 the output's, set for BF16.
+template <bool OUTPUTS>
+struct Table {
+    static constexpr int kTensors = OUTPUTS ? 160 : 240;
+    const void *data[kTensors];
+    void *out[OUTPUTS ? kTensors : 1];
+    uint32_t size[kTensors], end[kTensors];
     int32_t count;
 };
-static_assert(sizeof(Batch) <= 4000, "the arguments of a launch are at most 4 KiB");
+static_assert(sizeof(Table<true>) <= 4000 && sizeof(Table<false>) <= 4000, "the arguments of a launch are at most 4 KiB");
 
-__device__ __forceinline__ int tensor_of(const Batch &b, uint32_t chunk) {
+template <typename Table>
+__device__ __forceinline__ int tensor_of(const Table &b, uint32_t chunk) {
     int low = 0, high = b.count - 1;
     while (low < high) {
         const int middle = (low + high) / 2;
@@ -46,129 +59,234 @@ __device__ __forceinline__ double block_sum(double x, double *shared) {
     return x;
 }
 
+// The sum of squares of n <= kChunk elements, this thread's share.
 template <typename T>
-__device__ __forceinline__ double squares(const T *g, int64_t begin, int64_t end) {
-    double sum = 0;
-    for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) {
-        const double x = double(to_f32(g[i]));
-        sum = fma(x, x, sum);
+__device__ __forceinline__ double squares(const T *g, int n) {
+    constexpr int VE = Vec<T>::kSize, U = 8;
+    double sums[2] = {0, 0};
+    const int vectors = n / VE;
+    const auto add = [&](u32x4 raw) {
+        float v[VE];
+        Vec<T>::widen(raw, v);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) sums[j % 2] = fma(double(v[j]), double(v[j]), sums[j % 2]);
+    };
+    int at = threadIdx.x;
+    for (; at + (U - 1) * kThreads < vectors; at += U * kThreads) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = reinterpret_cast<const AnyVector<T> *>(g + (at + u * kThreads) * VE)->bits;
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(raw[u]);
     }
-    return sum;
+    for (; at < vectors; at += kThreads) add(reinterpret_cast<const AnyVector<T> *>(g + at * VE)->bits);
+    const int odd = vectors * VE + int(threadIdx.x);
+    if (odd < n) {
+        const double x = double(to_f32(g[odd]));
+        sums[0] = fma(x, x, sums[0]);
+    }
+    return sums[0] + sums[1];
 }
 
-__global__ __launch_bounds__(kThreads) void squares_kernel(Batch b, double *parts) {
+__global__ __launch_bounds__(kThreads) void squares_kernel(Table<false> b, uint32_t chunks, double *parts) {
     __shared__ double shared[kWaves];
-    const int i = tensor_of(b, blockIdx.x);
-    const bdm_gradient &t = b.tensors[i];
-    const int64_t begin = int64_t(blockIdx.x - (i ? b.end[i - 1] : 0)) * kChunk, end = min(t.numel, begin + kChunk);
-    const double sum = block_sum(t.dtype == BDM_BF16 ? squares(static_cast<const bf16_t *>(t.data), begin, end)
-                                                     : squares(static_cast<const float *>(t.data), begin, end), shared);
+    double sum = 0;
+    for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int i = tensor_of(b, chunk);
+        const int64_t begin = int64_t(chunk - (i ? b.end[i - 1] : 0)) * kChunk;
+        const int n = int(min(int64_t(b.size[i] & kSizeMask) - begin, int64_t(kChunk)));
+        sum += b.size[i] >> 31 ? squares(static_cast<const bf16_t *>(b.data[i]) + begin, n)
+                               : squares(static_cast<const float *>(b.data[i]) + begin, n);
+    }
+    sum = block_sum(sum, shared);
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(kThreads) void norm_kernel(const double *parts, int64_t count, double max_norm, float *norm,
-                                                        float *scale) {
+// The norm and the factor from the parts, in every thread of a workgroup.
+__device__ __forceinline__ float factor_of(const double *parts, int count, double max_norm, double &norm) {
     __shared__ double shared[kWaves];
     double sum = 0;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads) sum += parts[i];
-    sum = block_sum(sum, shared);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < count; i += kThreads) sum += parts[i];
+    norm = sqrt(block_sum(sum, shared));
+    const double c = max_norm / (norm + 1e-6);
+    return c > 1 ? 1.f : float(c);
+}
+
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double *parts, int count, double max_norm, float *norm,
+                                                        float *scale) {
+    double n;
+    const float c = factor_of(parts, count, max_norm, n);
     if (threadIdx.x == 0) {
-        const double n = sqrt(sum), c = max_norm / (n + 1e-6);
         *norm = float(n);
-        if (scale) *scale = c > 1 ? 1.f : float(c);
+        if (scale) *scale = c;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *g, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        Vec<bf16_t>::widen(reinterpret_cast<const AnyVector<T> *>(g)->bits, v);
+    } else {
+        Vec<float>::widen(reinterpret_cast<const AnyVector<T> *>(g)->bits, v);
+        Vec<float>::widen(reinterpret_cast<const AnyVector<T> *>(g + 4)->bits, v + 4);
+    }
+}
+
+template <typename O>
+__device__ __forceinline__ void store8(O *out, const float (&v)[8]) {
+    u32x4 bits;
+    if constexpr (sizeof(O) == 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bits[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+        reinterpret_cast<AnyVector<O> *>(out)->bits = bits;
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bits[j] = __float_as_uint(v[4 * h + j]);
+            reinterpret_cast<AnyVector<O> *>(out + 4 * h)->bits = bits;
+        }
     }
 }
 
 template <typename T, typename O>
-__device__ __forceinline__ void scale_part(const bdm_gradient &t, int64_t begin, int64_t end, float scale) {
-    const T *g = static_cast<const T *>(t.data);
-    O *out = static_cast<O *>(t.out);
-    for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) out[i] = from_f32<O>(to_f32(g[i]) * scale);
+__device__ __forceinline__ void scale_part(const T *g, O *out, int n, float scale) {
+    constexpr int U = 4;
+    const int vectors = n / 8;
+    const auto put = [&](int at, float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= scale;
+        store8(out + at * 8, v);
+    };
+    int at = threadIdx.x;
+    for (; at + (U - 1) * kThreads < vectors; at += U * kThreads) {
+        float v[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load8(g + (at + u * kThreads) * 8, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) put(at + u * kThreads, v[u]);
+    }
+    for (; at < vectors; at += kThreads) {
+        float v[8];
+        load8(g + at * 8, v);
+        put(at, v);
+    }
+    const int odd = vectors * 8 + int(threadIdx.x);
+    if (odd < n) out[odd] = from_f32<O>(to_f32(g[odd]) * scale);
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(Batch b, const float *scale) {
-    const int i = tensor_of(b, blockIdx.x);
-    const bdm_gradient &t = b.tensors[i];
-    const int64_t begin = int64_t(blockIdx.x - (i ? b.end[i - 1] : 0)) * kChunk, end = min(t.numel, begin + kChunk);
-    const float c = *scale;
-    if (c == 1.f && t.out == t.data) return;  // as they are
-    if (t.dtype == BDM_BF16) {
-        if (t.out_dtype == BDM_BF16)
-            scale_part<bf16_t, bf16_t>(t, begin, end, c);
+// The chunks are taken from the last to the first: the last ones that the norm has read are still in the cache.
+__global__ __launch_bounds__(kThreads) void scale_kernel(Table<true> b, uint32_t chunks, const double *parts, int count,
+                                                         double max_norm, float *norm) {
+    double n;
+    const float c = factor_of(parts, count, max_norm, n);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = float(n);
+    for (uint32_t turn = blockIdx.x; turn < chunks; turn += gridDim.x) {
+        const uint32_t chunk = chunks - 1 - turn;
+        const int i = tensor_of(b, chunk);
+        const uint32_t size = b.size[i];
+        const int64_t begin = int64_t(chunk - (i ? b.end[i - 1] : 0)) * kChunk;
+        const int left = int(min(int64_t(size & kSizeMask) - begin, int64_t(kChunk)));
+        const void *data = b.data[i];
+        void *out = b.out[i];
+        if (c == 1.f && out == data) continue;  // as they are
+        const bf16_t *half = static_cast<const bf16_t *>(data) + begin;
+        const float *single = static_cast<const float *>(data) + begin;
+        bf16_t *half_out = static_cast<bf16_t *>(out) + begin;
+        float *single_out = static_cast<float *>(out) + begin;
+        if (size >> 31)
+            size >> 30 & 1 ? scale_part(half, half_out, left, c) : scale_part(half, single_out, left, c);
         else
-            scale_part<bf16_t, float>(t, begin, end, c);
-    } else {
-        if (t.out_dtype == BDM_BF16)
-            scale_part<float, bf16_t>(t, begin, end, c);
-        else
-            scale_part<float, float>(t, begin, end, c);
+            size >> 30 & 1 ? scale_part(single, half_out, left, c) : scale_part(single, single_out, left, c);
     }
 }
 
-int64_t chunks_of(int64_t numel) { return (numel + kChunk - 1) / kChunk; }
+// ------------------------------------------------------------------ host
+struct Tensors {
+    const void *const *data;
+    void *const *out;  // null: none
+    const int64_t *size;
+    const int32_t *dtype, *out_dtype;
+    int32_t count;
+};
 
-int check_tensors(const char *what, const bdm_gradient *tensors, int32_t count, bool outputs) {
-    if (count < 0 || (count && !tensors)) return fail(BDM_ERR_INVALID, "%s: bad tensors", what);
-    for (int i = 0; i < count; ++i) {
-        const bdm_gradient &t = tensors[i];
-        if (t.numel < 0 || (t.dtype != BDM_BF16 && t.dtype != BDM_F32) ||
-            (outputs && t.out_dtype != BDM_BF16 && t.out_dtype != BDM_F32))
+int check_tensors(const char *what, const Tensors &t, bool outputs) {
+    if (t.count < 0 || (t.count && (!t.data || !t.size || !t.dtype || (outputs && (!t.out || !t.out_dtype)))))
+        return fail(BDM_ERR_INVALID, "%s: bad tensors", what);
+    for (int i = 0; i < t.count; ++i) {
+        if (t.size[i] < 0 || (t.dtype[i] != BDM_BF16 && t.dtype[i] != BDM_F32) ||
+            (outputs && t.out_dtype[i] != BDM_BF16 && t.out_dtype[i] != BDM_F32))
             return fail(BDM_ERR_INVALID, "%s: tensor %d has a bad size or dtype", what, i);
-        if (t.numel && (!t.data || (outputs && !t.out))) return fail(BDM_ERR_INVALID, "%s: null pointer", what);
-        if (t.numel > (int64_t(1) << 40)) return fail(BDM_ERR_UNSUPPORTED, "%s: tensor %d is too large", what, i);
+        if (t.size[i] && (!t.data[i] || (outputs && !t.out[i]))) return fail(BDM_ERR_INVALID, "%s: null pointer", what);
+        if (t.size[i] > (int64_t(1) << 40)) return fail(BDM_ERR_UNSUPPORTED, "%s: tensor %d is too large", what, i);
     }
     return BDM_OK;
 }
 
-// Batches of tensors, each to launch(batch, its chunks, chunks before it); empty tensors are left out.
-template <typename F>
-int for_batches(const bdm_gradient *tensors, int32_t count, F launch) {
-    Batch b{};
-    int64_t chunks = 0, before = 0;
+// Tables of the tensors, each to launch(table, its chunks); empty tensors are left out, very large ones take several
+// entries.
+template <bool OUTPUTS, typename F>
+int for_tables(const Tensors &t, F launch) {
+    constexpr int64_t kMostEntry = int64_t(1) << 29;  // elements, a multiple of kChunk
+    static_assert(kMostEntry % kChunk == 0 && kMostEntry <= kSizeMask);
+    constexpr int64_t kMostChunks = int64_t(1) << 31;
+    Table<OUTPUTS> b;
+    b.count = 0;
+    int64_t chunks = 0;
     const auto flush = [&]() -> int {
-        if (!b.count) return BDM_OK;
-        const int rc = launch(b, chunks, before);
-        before += chunks;
+        const int rc = b.count ? launch(b, uint32_t(chunks)) : BDM_OK;
         chunks = b.count = 0;
         return rc;
     };
-    for (int i = 0; i < count; ++i) {
-        if (!tensors[i].numel) continue;
-        const int64_t more = chunks_of(tensors[i].numel);
-        if (b.count == kBatch || !grid_fits(chunks + more, kThreads))
-            if (int rc = flush()) return rc;
-        if (!grid_fits(more, kThreads)) return fail(BDM_ERR_UNSUPPORTED, "gradients: tensor %d is too large", i);
-        chunks += more;
-        b.tensors[b.count] = tensors[i];
-        b.end[b.count++] = uint32_t(chunks);
+    for (int i = 0; i < t.count; ++i) {
+        for (int64_t from = 0; from < t.size[i]; from += kMostEntry) {
+            const int64_t size = std::min(t.size[i] - from, kMostEntry), more = (size + kChunk - 1) / kChunk;
+            if (b.count == Table<OUTPUTS>::kTensors || chunks + more > kMostChunks)
+                if (int rc = flush()) return rc;
+            chunks += more;
+            const bool half = t.dtype[i] == BDM_BF16;
+            b.data[b.count] = static_cast<const char *>(t.data[i]) + from * (half ? 2 : 4);
+            b.size[b.count] = uint32_t(size) | uint32_t(half) << 31;
+            if constexpr (OUTPUTS) {
+                const bool half_out = t.out_dtype[i] == BDM_BF16;
+                b.out[b.count] = static_cast<char *>(t.out[i]) + from * (half_out ? 2 : 4);
+                b.size[b.count] |= uint32_t(half_out) << 30;
+            }
+            b.end[b.count++] = uint32_t(chunks);
+        }
     }
     return flush();
 }
 
-int64_t total_chunks(const bdm_gradient *tensors, int32_t count) {
-    int64_t total = 0;
-    for (int i = 0; i < count; ++i) total += tensors[i].numel > 0 ? chunks_of(tensors[i].numel) : 0;
-    return total;
+// Workgroups of a table's launch: one a chunk, up to a bound that the tables of a call share.
+int64_t blocks_of(int64_t chunks, int64_t tables) {
+    return std::min(chunks, std::max<int64_t>(kMostParts / tables, 64));
 }
 
-size_t dtype_bytes(int32_t dtype) { return dtype == BDM_BF16 ? 2 : 4; }
+int64_t tables_of(const Tensors &t) {
+    int64_t tables = 0;
+    for_tables<false>(t, [&](const Table<false> &, uint32_t) { return ++tables, BDM_OK; });
+    return std::max<int64_t>(tables, 1);
+}
 
 // Whether two outputs share memory, or an output shares it with another tensor's gradient or, without being the
 // same in place, with its own.
-bool share_memory(const bdm_gradient *tensors, int32_t count) {
+bool share_memory(const Tensors &t) {
     struct Span {
         uintptr_t begin, end;
-        int32_t tensor;
         bool output;
     };
     std::vector<Span> spans;
-    spans.reserve(size_t(count) * 2);
-    for (int i = 0; i < count; ++i) {
-        const bdm_gradient &t = tensors[i];
-        if (!t.numel) continue;
-        const uintptr_t data = reinterpret_cast<uintptr_t>(t.data), out = reinterpret_cast<uintptr_t>(t.out);
-        spans.push_back({out, out + size_t(t.numel) * dtype_bytes(t.out_dtype), i, true});
-        if (data != out || t.dtype != t.out_dtype) spans.push_back({data, data + size_t(t.numel) * dtype_bytes(t.dtype), i, false});
+    spans.reserve(size_t(t.count) * 2);
+    for (int i = 0; i < t.count; ++i) {
+        if (!t.size[i]) continue;
+        const auto span = [&](const void *p, int32_t dtype, bool output) {
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
+            spans.push_back({begin, begin + size_t(t.size[i]) * (dtype == BDM_BF16 ? 2 : 4), output});
+        };
+        span(t.out[i], t.out_dtype[i], true);
+        if (t.data[i] != t.out[i] || t.dtype[i] != t.out_dtype[i]) span(t.data[i], t.dtype[i], false);
     }
     std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
     uintptr_t outputs_end = 0, all_end = 0;
@@ -180,15 +298,23 @@ bool share_memory(const bdm_gradient *tensors, int32_t count) {
     return false;
 }
 
-int norm_of(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm, float *scale, double *parts,
-            hipStream_t s) {
-    if (int rc = for_batches(tensors, count, [&](const Batch &b, int64_t chunks, int64_t before) {
-            squares_kernel<<<unsigned(chunks), kThreads, 0, s>>>(b, parts + before);
-            return check_launch("squares_kernel");
-        }))
-        return rc;
-    norm_kernel<<<1, kThreads, 0, s>>>(parts, total_chunks(tensors, count), max_norm, norm, scale);
-    return check_launch("norm_kernel");
+// The parts of the sum of squares, `count` of them.
+int launch_squares(const Tensors &t, double *parts, int64_t &count, hipStream_t s) {
+    const int64_t tables = tables_of(t);
+    count = 0;
+    return for_tables<false>(t, [&](const Table<false> &b, uint32_t chunks) {
+        const int64_t blocks = blocks_of(chunks, tables);
+        squares_kernel<<<unsigned(blocks), kThreads, 0, s>>>(b, chunks, parts + count);
+        count += blocks;
+        return check_launch("squares_kernel");
+    });
+}
+
+size_t workspace_of(const Tensors &t) {
+    const int64_t tables = tables_of(t);
+    int64_t parts = 0;
+    for_tables<false>(t, [&](const Table<false> &, uint32_t chunks) { return parts += blocks_of(chunks, tables), BDM_OK; });
+    return size_t(std::max<int64_t>(parts, 1)) * sizeof(double);
 }
 
 }  // namespace
@@ -196,38 +322,61 @@ int norm_of(const bdm_gradient *tensors, int32_t count, double max_norm, float *
 
 using namespace bdm;
 
-extern "C" size_t bdm_gradient_norm_workspace_size(const bdm_gradient *tensors, int32_t count) {
-    if (count <= 0 || !tensors) return 16;
-    return 16 + size_t(total_chunks(tensors, count)) * sizeof(double);
+extern "C" size_t bdm_gradient_norm_workspace_size(const int64_t *sizes, int32_t count) {
+    if (count <= 0 || !sizes) return sizeof(double);
+    try {
+        // the sizes alone count
+        const std::vector<const void *> data(size_t(count), nullptr);
+        const std::vector<int32_t> dtypes(size_t(count), BDM_F32);
+        return workspace_of({data.data(), nullptr, sizes, dtypes.data(), nullptr, count});
+    } catch (...) {
+        return 0;
+    }
 }
 
-extern "C" int bdm_gradient_norm(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm, float *scale,
-                                 void *workspace, size_t workspace_bytes, void *stream) {
-    if (int rc = check_tensors("gradient_norm", tensors, count, false)) return rc;
+extern "C" int bdm_gradient_norm(const void *const *data, const int64_t *sizes, const int32_t *dtypes, int32_t count,
+                                 double max_norm, float *norm, float *scale, void *workspace, size_t workspace_bytes,
+                                 void *stream) {
+    const Tensors t{data, nullptr, sizes, dtypes, nullptr, count};
+    if (int rc = check_tensors("gradient_norm", t, false)) return rc;
     if (!norm || !workspace) return fail(BDM_ERR_INVALID, "gradient_norm: null pointer");
     if (scale && !(max_norm >= 0)) return fail(BDM_ERR_INVALID, "gradient_norm: max_norm is negative or NaN");
-    if (workspace_bytes < bdm_gradient_norm_workspace_size(tensors, count) || !aligned(workspace, 16))
-        return fail(BDM_ERR_INVALID, "gradient_norm: workspace too small or not aligned to 16 bytes");
-    return norm_of(tensors, count, max_norm, norm, scale, static_cast<double *>(workspace) + 2, as_stream(stream));
+    if (workspace_bytes < workspace_of(t) || !aligned(workspace, sizeof(double)))
+        return fail(BDM_ERR_INVALID, "gradient_norm: workspace too small or not aligned to 8 bytes");
+    double *parts = static_cast<double *>(workspace);
+    int64_t used = 0;
+    if (int rc = launch_squares(t, parts, used, as_stream(stream))) return rc;
+    norm_kernel<<<1, kThreads, 0, as_stream(stream)>>>(parts, int(used), max_norm, norm, scale);
+    return check_launch("norm_kernel");
 }
 
-extern "C" int bdm_clip_gradients(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm,
-                                  void *workspace, size_t workspace_bytes, void *stream) {
-    if (int rc = check_tensors("clip_gradients", tensors, count, true)) return rc;
+extern "C" int bdm_clip_gradients(const void *const *data, void *const *out, const int64_t *sizes, const int32_t *dtypes,
+                                  const int32_t *out_dtypes, int32_t count, double max_norm, float *norm, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+    const Tensors t{data, out, sizes, dtypes, out_dtypes, count};
+    if (int rc = check_tensors("clip_gradients", t, true)) return rc;
     if (!norm || !workspace) return fail(BDM_ERR_INVALID, "clip_gradients: null pointer");
     if (!(max_norm >= 0)) return fail(BDM_ERR_INVALID, "clip_gradients: max_norm is negative or NaN");
-    if (workspace_bytes < bdm_gradient_norm_workspace_size(tensors, count) || !aligned(workspace, 16))
-        return fail(BDM_ERR_INVALID, "clip_gradients: workspace too small or not aligned to 16 bytes");
+    if (workspace_bytes < workspace_of(t) || !aligned(workspace, sizeof(double)))
+        return fail(BDM_ERR_INVALID, "clip_gradients: workspace too small or not aligned to 8 bytes");
     try {
-        if (share_memory(tensors, count)) return fail(BDM_ERR_INVALID, "clip_gradients: tensors share memory");
+        if (share_memory(t)) return fail(BDM_ERR_INVALID, "clip_gradients: tensors share memory");
     } catch (...) {
         return fail(BDM_ERR_INVALID, "clip_gradients: out of host memory");
     }
     hipStream_t s = as_stream(stream);
-    float *scale = static_cast<float *>(workspace);
-    if (int rc = norm_of(tensors, count, max_norm, norm, scale, static_cast<double *>(workspace) + 2, s)) return rc;
-    return for_batches(tensors, count, [&](const Batch &b, int64_t chunks, int64_t) {
-        scale_kernel<<<unsigned(chunks), kThreads, 0, s>>>(b, scale);
-        return check_launch("scale_kernel");
-    });
+    double *parts = static_cast<double *>(workspace);
+    int64_t used = 0;
+    if (int rc = launch_squares(t, parts, used, s)) return rc;
+    bool first = true;
+    if (int rc = for_tables<true>(t, [&](const Table<true> &b, uint32_t chunks) {
+            scale_kernel<<<unsigned(std::min<int64_t>(chunks, kMostParts)), kThreads, 0, s>>>(
+                b, chunks, parts, int(used), max_norm, first ? norm : nullptr);
+            first = false;
+            return check_launch("scale_kernel");
+        }))
+        return rc;
+    if (!first) return BDM_OK;
+    norm_kernel<<<1, kThreads, 0, s>>>(parts, 0, max_norm, norm, nullptr);  // no elements
+    return check_launch("norm_kernel");
 }

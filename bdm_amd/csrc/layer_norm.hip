@@ -393,7 +393,7 @@ int check_rows(const char *what, int64_t rows, int32_t width, int32_t dtype, int
     if (width > kMaxWidth) return fail(BDM_ERR_UNSUPPORTED, "%s: width %d > %d", what, width, kMaxWidth);
     if ((dtype != BDM_BF16 && dtype != BDM_F32) || (param_dtype != BDM_BF16 && param_dtype != BDM_F32))
         return fail(BDM_ERR_INVALID, "%s: dtype", what);
-    if (rows > (int64_t(1) << 40)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (rows >= (int64_t(1) << 40)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
     return BDM_OK;
 }
 

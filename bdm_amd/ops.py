@@ -11,7 +11,9 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import operator
 import os
+from array import array
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -1185,67 +1187,86 @@ def _dense(t: Tensor) -> bool:
     return t.permute(sorted(range(t.ndim), key=t.stride, reverse=True)).is_contiguous()
 
 
-class _GradientTable:
-    """The ``bdm_gradient`` array of the tensors that are not None, and the
-    copies that it points to."""
+def _table(tensors, what: str) -> array:
+    """The dtype codes of dense tensors on one device, behind their checks."""
+    device = tensors[0].get_device()
+    if device < 0:
+        raise ValueError('the HIP path requires tensors on a ROCm device')
+    if any(t.get_device() != device for t in tensors):
+        raise ValueError('all tensors must be on the same device')
+    codes = [_ELEMENT.get(t.dtype) for t in tensors]
+    if None in codes or any(t.layout is not torch.strided for t in tensors):
+        raise ValueError(f'{what} must be dense BF16 or FP32 tensors')
+    return array('i', codes)
+
+
+class _Gradients:
+    """The host arrays of gradients and, where they are written, outputs, those of
+    None left out.  ``copies`` keeps what the arrays point to besides the
+    caller's tensors."""
 
     def __init__(self, gradients, out=None, *, written: bool = False) -> None:
-        gradients = list(gradients)
-        out = gradients if out is None else list(out)
-        if len(out) != len(gradients):
+        kept = list(gradients)
+        out = kept if out is None else list(out)
+        if len(out) != len(kept):
             raise ValueError('out must hold a tensor for each gradient')
-        self.device, self.copies, flat = None, [], []
-        for g, o in zip(gradients, out):
-            if g is None:
-                continue
-            element = _ELEMENT.get(g.dtype)
-            if element is None or g.layout is not torch.strided:
-                raise ValueError('gradients must be dense BF16 or FP32 tensors')
-            if self.device is None:
-                self.device = _require_gpu(g)
-            elif g.device != self.device:
+        if any(g is None for g in kept):
+            out = [o for g, o in zip(kept, out) if g is not None]
+            kept = [g for g in kept if g is not None]
+        self.count, self.copies, self.device = len(kept), None, None
+        if not kept:
+            return
+        self.dtypes = _table(kept, 'gradients')
+        self.device = kept[0].device
+        inplace = all(map(operator.is_, kept, out))
+        if inplace:
+            self.out_dtypes = self.dtypes
+        else:
+            if any(o is None for o in out) or [o.shape for o in out] != [g.shape for g in kept]:
+                raise ValueError('out must hold a tensor of each gradient\'s shape')
+            self.out_dtypes = _table(out, 'out')
+            if out[0].device != self.device:
                 raise ValueError('all tensors must be on the same device')
-            size = g.numel()
-            if o is g:
-                if not _dense(g):
-                    if written:
-                        raise ValueError('a gradient whose elements do not fill its memory cannot be clipped in place')
-                    g = g.contiguous()
-                    self.copies.append(g)
-                place = g.data_ptr()
-                flat += (place, place, size, element | element << 32)
-                continue
-            other = None if o is None else _ELEMENT.get(o.dtype)
-            if other is None or o.shape != g.shape or o.layout is not torch.strided or o.device != self.device:
-                raise ValueError('out must hold a BF16 or FP32 tensor of each gradient\'s shape on its device')
-            if not (o.is_contiguous() and g.is_contiguous()) and not (o.stride() == g.stride() and _dense(g)):
-                if not o.is_contiguous():
-                    raise ValueError('out must be contiguous, or dense with its gradient\'s strides')
-                g = g.contiguous()
-                self.copies.append(g)
-            flat += (g.data_ptr(), o.data_ptr(), size, element | other << 32)
-        self.count = len(flat) // 4
-        self._flat = (ctypes.c_int64 * len(flat))(*flat)
-        self.entries = ctypes.cast(self._flat, ctypes.POINTER(_lib.Gradient))
+        if not all(t.is_contiguous() for t in (kept if inplace else kept + out)):
+            kept = self.copies = [self._filled(g, o, written) for g, o in zip(kept, out)]
+        self.data = array('Q', [g.data_ptr() for g in kept])
+        self.out = self.data if inplace else array('Q', [o.data_ptr() for o in out])
+        self.sizes = array('q', [g.numel() for g in kept])
+
+    @staticmethod
+    def _filled(g: Tensor, o: Tensor, written: bool) -> Tensor:
+        """The gradient, or a copy, whose elements lie one behind the other as its output's do."""
+        if (g is o and _dense(g)) or (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _dense(g)):
+            return g
+        if written and g is o:
+            raise ValueError('a gradient whose elements do not fill its memory cannot be clipped in place')
+        if written and not o.is_contiguous():
+            raise ValueError('out must be contiguous, or dense with its gradient\'s strides')
+        return g.contiguous()
+
+
+def _at(values: array) -> int:
+    return values.buffer_info()[0]
 
 
 def gradient_norm(gradients, *, max_norm: float | None = None):
     """``bdm_amd.gradient_norm``; with ``max_norm`` also the factor that clips to
     it, min(1, max_norm / (norm + 1e-6)), as an FP32 scalar: (norm, factor)."""
-    table = _GradientTable(gradients)
+    tensors = _Gradients(gradients)
     if max_norm is not None and not max_norm >= 0:
         raise ValueError('max_norm must not be negative')
-    if table.device is None:
+    if not tensors.count:
         return torch.zeros(()) if max_norm is None else (torch.zeros(()), torch.ones(()))
-    norm, factor = (torch.empty((), device=table.device, dtype=torch.float32) for _ in range(2))
-    lib = _lib.library()
-    nbytes = lib.bdm_gradient_norm_workspace_size(table.entries, table.count)
-    workspace = torch.empty(nbytes, device=table.device, dtype=torch.uint8)
-    with _on(table.device):
+    device, lib = tensors.device, _lib.library()
+    norm = torch.empty((), device=device, dtype=torch.float32)
+    factor = None if max_norm is None else torch.empty_like(norm)
+    sizes, count = _at(tensors.sizes), tensors.count
+    nbytes = lib.bdm_gradient_norm_workspace_size(sizes, count)
+    workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    with _on(device):
         _lib.check(lib.bdm_gradient_norm(
-            table.entries, table.count, 0.0 if max_norm is None else float(max_norm), _addr(norm),
-            None if max_norm is None else _addr(factor), _addr(workspace), nbytes, _stream(table.device)),
-            'bdm_gradient_norm')
+            _at(tensors.data), sizes, _at(tensors.dtypes), count, 0.0 if max_norm is None else float(max_norm),
+            _addr(norm), _addr(factor), _addr(workspace), nbytes, _stream(device)), 'bdm_gradient_norm')
     return norm if max_norm is None else (norm, factor)
 
 
@@ -1254,16 +1275,18 @@ def clip_gradients(gradients, max_norm: float, *, out=None) -> Tensor:
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError('max_norm must not be negative')
-    table = _GradientTable(gradients, out, written=True)
-    if table.device is None:
+    tensors = _Gradients(gradients, out, written=True)
+    if not tensors.count:
         return torch.zeros(())
-    norm = torch.empty((), device=table.device, dtype=torch.float32)
-    lib = _lib.library()
-    nbytes = lib.bdm_gradient_norm_workspace_size(table.entries, table.count)
-    workspace = torch.empty(nbytes, device=table.device, dtype=torch.uint8)
-    with _on(table.device):
-        _lib.check(lib.bdm_clip_gradients(table.entries, table.count, max_norm, _addr(norm), _addr(workspace), nbytes,
-                                          _stream(table.device)), 'bdm_clip_gradients')
+    device, lib = tensors.device, _lib.library()
+    norm = torch.empty((), device=device, dtype=torch.float32)
+    sizes, count = _at(tensors.sizes), tensors.count
+    nbytes = lib.bdm_gradient_norm_workspace_size(sizes, count)
+    workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    with _on(device):
+        _lib.check(lib.bdm_clip_gradients(
+            _at(tensors.data), _at(tensors.out), sizes, _at(tensors.dtypes), _at(tensors.out_dtypes), count, max_norm,
+            _addr(norm), _addr(workspace), nbytes, _stream(device)), 'bdm_clip_gradients')
     return norm
 
 

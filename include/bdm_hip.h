@@ -761,24 +761,18 @@ int bdm_token_loss(const float *log_probs, const int64_t *tokens, int64_t rows, 
  * The global norm of gradients, n = sqrt(sum g^2) over all tensors, and their
  * clipping, g' = round(g min(1, max_norm / (n + 1e-6))): the arithmetic of the
  * shell's clip_grad_norm_ (reproduction/experiments/optim.py:33-36) with the
- * norm and the factor in FP64.  `tensors` is a host array, read before the call
- * returns.  Clipped values go to `out`, of any of the two dtypes; out = data
- * with the same dtype clips in place, where no value is written if the factor
- * is 1.  An output may not overlap another tensor.  bdm_gradient_norm reads the
- * data alone and with `scale` non-null also stores the factor.  The workspace is
- * 16-byte aligned.
+ * norm and the factor in FP64.  The `count` tensors are given by host arrays of
+ * their addresses, sizes in elements and dtypes, read before the call returns.
+ * bdm_gradient_norm also stores the factor where `scale` is not null.
+ * bdm_clip_gradients writes the clipped values to `out`, of either dtype; out =
+ * data with the same dtype clips in place, where no value is written if the
+ * factor is 1.  An output may not overlap another tensor.
  */
-typedef struct bdm_gradient {
-    const void *data;
-    void *out;
-    int64_t numel;
-    int32_t dtype, out_dtype;
-} bdm_gradient;
-
-size_t bdm_gradient_norm_workspace_size(const bdm_gradient *tensors, int32_t count);
-int bdm_gradient_norm(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm, float *scale,
-                      void *workspace, size_t workspace_bytes, void *stream);
-int bdm_clip_gradients(const bdm_gradient *tensors, int32_t count, double max_norm, float *norm, void *workspace,
+size_t bdm_gradient_norm_workspace_size(const int64_t *sizes, int32_t count);
+int bdm_gradient_norm(const void *const *data, const int64_t *sizes, const int32_t *dtypes, int32_t count,
+                      double max_norm, float *norm, float *scale, void *workspace, size_t workspace_bytes, void *stream);
+int bdm_clip_gradients(const void *const *data, void *const *out, const int64_t *sizes, const int32_t *dtypes,
+                       const int32_t *out_dtypes, int32_t count, double max_norm, float *norm, void *workspace,
                        size_t workspace_bytes, void *stream);
 
 /*

@@ -141,30 +141,38 @@ def test_token_entries():
 
 def test_gradient_entries():
     lib = _lib.library()
-    one = (_lib.Gradient * 1)()
+    keep = []
 
-    def status(call, **fields):
-        g = one[0]
-        g.data, g.out, g.numel, g.dtype, g.out_dtype = 4096, 4096, 8, _lib.BDM_F32, _lib.BDM_F32
-        for name, value in fields.items():
-            setattr(g, name, value)
-        return call()
+    def arrays(data=4096, out=4096, size=8, dtype=_lib.BDM_F32, out_dtype=_lib.BDM_F32):
+        made = ((ctypes.c_uint64 * 1)(data), (ctypes.c_uint64 * 1)(out), (ctypes.c_int64 * 1)(size),
+                (ctypes.c_int32 * 1)(dtype), (ctypes.c_int32 * 1)(out_dtype))
+        keep.append(made)
+        return made
 
-    size = lib.bdm_gradient_norm_workspace_size(one, 1)
-    clip = lambda: lib.bdm_clip_gradients(one, 1, 1.0, HELD, HELD, 1 << 20, None)  # noqa: E731
-    norm = lambda: lib.bdm_gradient_norm(one, 1, 1.0, HELD, None, HELD, 1 << 20, None)  # noqa: E731
-    for fields in (dict(numel=-1), dict(dtype=5), dict(data=None)):
-        assert status(clip, **fields) == status(norm, **fields) == -1, fields
-    for fields in (dict(out=None), dict(out_dtype=3), dict(out=4100), dict(out=4096, out_dtype=_lib.BDM_BF16)):
-        assert status(clip, **fields) == -1, fields
-    assert status(clip, numel=2 ** 41) == status(norm, numel=2 ** 41) == -2
-    assert status(lambda: lib.bdm_clip_gradients(one, 1, -1.0, HELD, HELD, 1 << 20, None)) == -1
-    assert status(lambda: lib.bdm_clip_gradients(one, 1, float('nan'), HELD, HELD, 1 << 20, None)) == -1
-    assert status(lambda: lib.bdm_clip_gradients(one, 1, 1.0, HELD, HELD, 8, None)) == -1
-    assert status(lambda: lib.bdm_clip_gradients(one, 1, 1.0, HELD, None, 1 << 20, None)) == -1
-    assert status(lambda: lib.bdm_clip_gradients(None, 1, 1.0, HELD, HELD, 1 << 20, None)) == -1
-    assert status(lambda: lib.bdm_gradient_norm(one, -1, 1.0, HELD, None, HELD, 1 << 20, None)) == -1
-    assert size >= 16
+    def clip(count=1, max_norm=1.0, norm=HELD, workspace=HELD, nbytes=1 << 20, **fields):
+        data, out, size, dtype, out_dtype = arrays(**fields)
+        return lib.bdm_clip_gradients(data, out, size, dtype, out_dtype, count, max_norm, norm, workspace, nbytes, None)
+
+    def norm(count=1, max_norm=1.0, norm=HELD, scale=None, workspace=HELD, nbytes=1 << 20, **fields):
+        data, _, size, dtype, _ = arrays(**fields)
+        return lib.bdm_gradient_norm(data, size, dtype, count, max_norm, norm, scale, workspace, nbytes, None)
+
+    for fields in (dict(size=-1), dict(dtype=5), dict(data=0), dict(count=-1), dict(norm=None), dict(workspace=None),
+                   dict(nbytes=4), dict(workspace=ctypes.c_void_p(4100))):
+        assert clip(**fields) == norm(**fields) == -1, fields
+    for fields in (dict(out=0), dict(out_dtype=3), dict(out=4100), dict(out=4096, out_dtype=_lib.BDM_BF16),
+                   dict(max_norm=-1.0), dict(max_norm=float('nan'))):
+        assert clip(**fields) == -1, fields
+    assert norm(max_norm=-1.0, scale=HELD) == -1
+    assert clip(size=2 ** 40 + 1) == norm(size=2 ** 40 + 1) == -2
+    assert lib.bdm_clip_gradients(None, None, None, None, None, 1, 1.0, HELD, HELD, 1 << 20, None) == -1
+    assert lib.bdm_gradient_norm(None, None, None, 1, 1.0, HELD, None, HELD, 1 << 20, None) == -1
+    # a sum for each workgroup: one a chunk of 16384 elements, 2048 at most in all
+    sizes = (ctypes.c_int64 * 3)(1, 16385, 0)
+    assert lib.bdm_gradient_norm_workspace_size(sizes, 3) == 3 * 8
+    many = (ctypes.c_int64 * 500)(*[2 ** 31] * 500)
+    assert lib.bdm_gradient_norm_workspace_size(many, 500) <= (2048 + 64) * 8
+    assert lib.bdm_gradient_norm_workspace_size(None, 0) == 8
 
 
 def test_layer_norm_entries():
