@@ -29,8 +29,8 @@ def clip_gradients(gradients, max_norm: float, *, out=None) -> Tensor:
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)) and returns their
     norm before that, ``gradient_norm(gradients)``.
 
-    In place by default; ``out`` gives a tensor for each gradient instead, of its
-    shape, BF16 or FP32 (an optimizer's FP32 gradients, for instance).  Each value
+    In place by default; ``out`` gives a tensor for each gradient instead, of as
+    many elements in the same order, BF16 or FP32 (an optimizer's FP32 gradients, for instance).  Each value
     is rounded once.  A norm of infinity gives the factor 0 and one of NaN the
     factor NaN, as torch's clipping does without its check.  A tensor written may
     not share memory with another one of the call (ValueError), so that none is

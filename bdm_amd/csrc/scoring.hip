@@ -7,6 +7,7 @@
 //   dx_i = a [i = t] + sum_k b_k [i = top_k] - p_i (a + sum_k b_k + h (log p_i + H)).
 // Everything is FP32.
 #include <algorithm>
+#include <cfloat>
 
 #include "bdm_common.h"
 #include "selection_ops.h"
@@ -39,10 +40,22 @@ __device__ __forceinline__ float log_probability(float x, float high, float log_
     return log_sum == -INFINITY ? -INFINITY : (x - high) - log_sum;
 }
 
+// The results of one row from its statistics: by one thread.
+__device__ __forceinline__ void put_row(const bdm_token_args &a, int64_t row, int64_t token, float given, float from,
+                                        float log_sum, float entropy) {
+    const bool inside = token >= 0 && token < a.vocab;
+    a.log_probs[row] = token == a.ignore_index ? 0.f : inside ? log_probability(given, from, log_sum) : NAN;
+    if (a.entropy) a.entropy[row] = log_sum == -INFINITY ? 0.f : entropy;
+    if (a.stats) {
+        a.stats[2 * row] = from;
+        a.stats[2 * row + 1] = log_sum;
+    }
+}
+
 // ------------------------------------------------------------------ a team's part of a row
 template <int WAVES, int NV>
 struct Team {
-    static constexpr int kRoom = WAVES == 1 ? 128 : 64 * (WAVES < 8 ? WAVES : 8);
+    static constexpr int kRoom = WAVES == 1 ? 128 : 256;
     uint64_t list[kRoom];  // ordered value, then ~index: descending order is value, then lowest index
     float high[WAVES], sum[WAVES], moment[WAVES];
     uint32_t bound[WAVES], share[WAVES];
@@ -102,10 +115,10 @@ struct Place {
 // The exact `width` best of the team's values to sh.list where the bound does not serve: those above the width-th, then
 // of those equal to it the ones of lowest index, which lie in the order of vectors, lanes, places in the vector.  `guess`
 // is the width-th's key if no `width` values are above it (equal logits, or a mask over most of the row): three passes
-// over the part; else that is bisected, a pass a bit.  A function of its own, which loads vector by vector: it takes no
-// registers from the ordinary case.
+// over the part; else that is bisected, a pass a bit.  Vector by vector from memory: it takes no registers from the
+// ordinary case.
 template <typename T, int WAVES, int NV>
-__device__ __noinline__ int team_exact(Team<WAVES, NV> &sh, const T *x, int length, int vocab, uint32_t guess, int width,
+__device__ __forceinline__ int team_exact(Team<WAVES, NV> &sh, const T *x, int length, int vocab, uint32_t guess, int width,
                                        uint32_t offset, int wave, int lane) {
     constexpr int VE = Vec<T>::kSize;
     const Place<T, WAVES> place{x, (wave * kWave + lane) * VE, length, vocab};
@@ -162,7 +175,10 @@ __device__ __noinline__ int team_exact(Team<WAVES, NV> &sh, const T *x, int leng
     int before = above;  // candidates ahead of the vector's, in this wave's order
     each([&](int i, const uint32_t *keys) {
         const auto take = [&](int j) {
-            sh.list[atomicAdd(&sh.count, 1)] = uint64_t(keys[j]) << 32 | uint32_t(~(offset + uint32_t(place.start(i) + j)));
+            // `width` of them, unless another stream changes the logits between two passes
+            const int to = atomicAdd(&sh.count, 1);
+            if (to < Team<WAVES, NV>::kRoom)
+                sh.list[to] = uint64_t(keys[j]) << 32 | uint32_t(~(offset + uint32_t(place.start(i) + j)));
         };
         int at = before;
 #pragma unroll
@@ -177,7 +193,7 @@ __device__ __noinline__ int team_exact(Team<WAVES, NV> &sh, const T *x, int leng
             if (keys[j] > value || (keys[j] == value && at++ < width)) take(j);
     });
     team_sync<WAVES>();
-    return sh.count;
+    return min(sh.count, Team<WAVES, NV>::kRoom);
 }
 
 // One part of one row, held in registers by a team of WAVES waves.
@@ -190,8 +206,7 @@ __device__ __forceinline__ void score_part(const Rows &p, Team<WAVES, NV> &sh, i
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Place<T, WAVES> place{x + offset, thread * VE, min(a.vocab - offset, kPart), a.vocab};
     const int64_t token = a.tokens[row];
-    const bool inside = token >= 0 && token < a.vocab;
-    const float given = to_f32(x[inside ? token : 0]);
+    const float given = to_f32(x[token >= 0 && token < a.vocab ? token : 0]);
     u32x4 raw[NV];
     if (a.vocab >= VE) {
 #pragma unroll
@@ -299,12 +314,7 @@ __device__ __forceinline__ void score_part(const Rows &p, Team<WAVES, NV> &sh, i
         if (p.splits > 1) {
             p.parts[row * p.splits + split] = make_float4(high, sum, moment, 0.f);
         } else {
-            a.log_probs[row] = token == a.ignore_index ? 0.f : inside ? log_probability(given, from, log_sum) : NAN;
-            if (a.entropy) a.entropy[row] = sum == 0.f ? 0.f : log_sum - moment / sum;
-            if (a.stats) {
-                a.stats[2 * row] = from;
-                a.stats[2 * row + 1] = log_sum;
-            }
+            put_row(a, row, token, given, from, log_sum, log_sum - moment / sum);
         }
     }
     if constexpr (TOP) {
@@ -328,7 +338,7 @@ __device__ __forceinline__ void score_part(const Rows &p, Team<WAVES, NV> &sh, i
 }
 
 template <typename T, int WAVES, int NV, bool TOP>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void score_kernel(Rows p) {
+__global__ __launch_bounds__(kThreads) void score_kernel(Rows p) {
     const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     if constexpr (WAVES == 1) {
         __shared__ Team<1, NV> teams[4];
@@ -341,6 +351,91 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void score_kernel
     }
 }
 
+// Statistics without alternatives, for calls of many rows: a workgroup streams one row through a running maximum, sum
+// and moment in every lane, rescaled once for U vectors.  Vectors start at 16-byte boundaries; the few values in front
+// of the first and behind the last one go to a lane each.
+template <typename T, int U>
+__global__ __launch_bounds__(kThreads) void stream_kernel(Rows p) {
+    constexpr int VE = Vec<T>::kSize;
+    __shared__ float highs[kWaves], sums[kWaves], moments[kWaves];
+    const bdm_token_args &a = p.a;
+    const int64_t row = blockIdx.x;
+    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
+    const int64_t token = a.tokens[row];
+    const float given = to_f32(x[token >= 0 && token < a.vocab ? token : 0]);
+    const int lead = int((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T));
+    const int vectors = (a.vocab - lead) / VE, tail = lead + vectors * VE, thread = int(threadIdx.x);
+    const u32x4 *from = reinterpret_cast<const u32x4 *>(x + lead);
+    // lanes 0 to 7 take the values in front, lanes 8 to 15 those behind
+    const int odd = thread < VE ? (thread < lead ? thread : -1) : (thread < 2 * VE && tail + thread - VE < a.vocab ? tail + thread - VE : -1);
+    float high = odd >= 0 ? to_f32(x[odd]) : -INFINITY, sum = 0.f, moment = 0.f;
+    const auto add = [&](float v) {
+        const float d = v - high, e = __builtin_amdgcn_exp2f(d * kLog2E);
+        sum += e;
+        moment = fmaf(e, fmaxf(d, -1e30f), moment);  // e = 0 there: no 0 * inf
+    };
+    {
+        const float v = high;
+        high = fmaxf(high, -FLT_MAX);
+        add(v);
+    }
+    const auto rescale = [&](float to) {
+        const float d = fmaxf(high - to, -1e30f), e = __builtin_amdgcn_exp2f(d * kLog2E);
+        moment = e * fmaf(sum, d, moment);
+        sum *= e;
+        high = to;
+    };
+    int at = thread;
+    for (; at + (U - 1) * kThreads < vectors; at += U * kThreads) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = from[at + u * kThreads];
+        float v[U][VE], top = high;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Vec<T>::widen(raw[u], v[u]);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) top = fmaxf(top, v[u][j]);
+        }
+        rescale(top);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) add(v[u][j]);
+    }
+    for (; at < vectors; at += kThreads) {
+        float v[VE], top = high;
+        Vec<T>::widen(from[at], v);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) top = fmaxf(top, v[j]);
+        rescale(top);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) add(v[j]);
+    }
+    const int wave = thread / kWave;
+    rescale(wave_max(high));
+    sum = wave_sum(sum);
+    moment = wave_sum(moment);
+    if (thread % kWave == 0) {
+        highs[wave] = high;
+        sums[wave] = sum;
+        moments[wave] = moment;
+    }
+    __syncthreads();
+    if (thread) return;
+    float top = highs[0];
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, highs[i]);
+    float total = 0.f, first = 0.f;
+    for (int i = 0; i < kWaves; ++i) {
+        high = highs[i], sum = sums[i], moment = moments[i];
+        rescale(top);
+        total += sum;
+        first += moment;
+    }
+    const float log_sum = logf(total);
+    put_row(a, row, token, given, top, log_sum, log_sum - first / total);
+}
+
 // The parts of a row joined.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(Rows p) {
@@ -348,6 +443,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Rows p) {
     __shared__ float floats[kWaves];
     __shared__ uint64_t keys[kWaves];
     __shared__ uint64_t list[kRoom];
+    __shared__ int count;
     const bdm_token_args &a = p.a;
     const int64_t row = blockIdx.x;
     const float4 *parts = p.parts + row * p.splits;
@@ -369,51 +465,63 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Rows p) {
     const float log_sum = logf(sum);
     if (threadIdx.x == 0) {
         const int64_t token = a.tokens[row];
-        float lp = 0.f;
-        if (token != a.ignore_index)
-            lp = token >= 0 && token < a.vocab
-                     ? log_probability(to_f32(static_cast<const T *>(a.logits)[row * a.row_stride + token]), from, log_sum)
-                     : NAN;
-        a.log_probs[row] = lp;
-        if (a.entropy) a.entropy[row] = sum == 0.f ? 0.f : log_sum - moment / sum;
-        if (a.stats) {
-            a.stats[2 * row] = from;
-            a.stats[2 * row + 1] = log_sum;
-        }
+        const bool inside = token >= 0 && token < a.vocab;
+        const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
+        put_row(a, row, token, to_f32(x[inside ? token : 0]), from, log_sum, log_sum - moment / sum);
     }
     if (!a.alternatives) return;
-    const int total = p.splits * a.alternatives;
+    // every part's list is in descending order: as many entries as are wanted reach the largest last one of them, and
+    // the least of all parts' n-th ones, n the share of a part
+    const int k = a.alternatives, total = p.splits * k, share = (k + p.splits - 1) / p.splits - 1;
     const uint64_t *lists = p.lists + row * total;
+    uint64_t last = 0, least = UINT64_MAX;
+    for (int i = threadIdx.x; i < p.splits; i += kThreads) {
+        last = max(last, lists[i * k + k - 1]);
+        least = min(least, lists[i * k + share]);
+    }
+    last = block_join(last, [](uint64_t x, uint64_t y) { return x > y ? x : y; }, keys);
+    least = block_join(least, [](uint64_t x, uint64_t y) { return x < y ? x : y; }, keys);
+    const uint64_t bound = max(max(last, least), uint64_t(1));
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        const uint64_t key = lists[i];
+        if (key < bound) continue;
+        const int at = atomicAdd(&count, 1);
+        if (at < kRoom) list[at] = key;
+    }
+    __syncthreads();
     const auto put = [&](int rank, uint64_t key) {
-        a.top_tokens[row * a.alternatives + rank] = int64_t(~uint32_t(key));
-        a.top_log_probs[row * a.alternatives + rank] = log_probability(unordered(uint32_t(key >> 32)), from, log_sum);
+        a.top_tokens[row * k + rank] = int64_t(~uint32_t(key));
+        a.top_log_probs[row * k + rank] = log_probability(unordered(uint32_t(key >> 32)), from, log_sum);
     };
-    if (total <= kRoom) {
-        for (int i = threadIdx.x; i < total; i += kThreads) list[i] = lists[i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < total; i += kThreads) {
+    if (count <= kRoom) {
+        for (int i = threadIdx.x; i < count; i += kThreads) {
             const uint64_t mine = list[i];
             int rank = 0;
-            for (int j = 0; j < total; ++j) rank += list[j] > mine;
-            if (mine && rank < a.alternatives) put(rank, mine);
+#pragma unroll 8
+            for (int j = 0; j < count; ++j) rank += list[j] > mine;
+            if (rank < k) put(rank, mine);
         }
         return;
     }
-    uint64_t last = UINT64_MAX;
-    for (int k = 0; k < a.alternatives; ++k) {
+    uint64_t above = UINT64_MAX;
+    for (int rank = 0; rank < k; ++rank) {
         uint64_t best = 0;
         for (int i = threadIdx.x; i < total; i += kThreads) {
             const uint64_t key = lists[i];
-            if (key < last && key > best) best = key;
+            if (key < above && key > best) best = key;
         }
         best = block_join(best, [](uint64_t x, uint64_t y) { return x > y ? x : y; }, keys);
-        if (threadIdx.x == 0) put(k, best);
-        last = best;
+        if (threadIdx.x == 0) put(rank, best);
+        above = best;
     }
 }
 
-// The gradient of a row's logits, one pass over them: a team of LANES lanes takes U vectors a lane of one row.  `TOPS`:
-// gradients of the alternatives arrive too.
+// The gradient of a row's logits, one pass over them: a team of LANES lanes takes U vectors a lane of one row, which
+// start at the gradient's 16-byte boundaries (the logits' too, where both are as torch allocates them); the few values
+// in front of the first and behind the last go to a lane each of the row's first team.  `TOPS`: gradients of the
+// alternatives arrive too.
 template <typename T, int LANES, int U, bool TOPS>
 __global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad_args a, int parts) {
     constexpr int VE = Vec<T>::kSize;
@@ -422,15 +530,16 @@ __global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad
     const int team = int(threadIdx.x) / LANES, lane = int(threadIdx.x) % LANES;
     const int64_t item = int64_t(blockIdx.x) * (kThreads / LANES) + team, row = item / parts;
     if (row >= a.rows) return;
-    const int first = int(item % parts) * LANES * U * VE + lane * VE;
+    const int part = int(item % parts);
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     T *out = static_cast<T *>(a.grad_logits) + row * a.vocab;
-    const bool whole = a.vocab >= VE;
+    const int lead = min(int((16 - reinterpret_cast<uintptr_t>(out) % 16) % 16 / sizeof(T)), a.vocab);
+    const int vectors = (a.vocab - lead) / VE, tail = lead + vectors * VE, first = part * LANES * U + lane;
     u32x4 raw[U];
-    if (whole) {
+    if (vectors > 0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            raw[u] = reinterpret_cast<const AnyVector<T> *>(x + min(first + u * LANES * VE, a.vocab - VE))->bits;
+            raw[u] = reinterpret_cast<const AnyVector<T> *>(x + lead + min(first + u * LANES, vectors - 1) * VE)->bits;
     }
     const int64_t token = a.tokens[row];
     const float high = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
@@ -451,59 +560,47 @@ __global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad
     }
     const int at = token >= 0 && token < a.vocab ? int(token) : -VE;
     const bool empty = log_sum == -INFINITY;
-    // the gradient at index i of the row
-    const auto gradient = [&](float v) {
-        const float lp = (v - high) - log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2E);
-        return -p * (total + h * (fmaxf(lp, -1e30f) + entropy));  // p = 0 there: no 0 * inf
-    };
-    const auto spot = [&](int i) {
-        float d = i == at ? given : 0.f;
+    // N values from index `start` on
+    const auto gradient = [&](int start, float *v, auto count) {
+        constexpr int N = decltype(count)::value;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float lp = (v[j] - high) - log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2E);
+            v[j] = empty ? 0.f : -p * (total + h * (fmaxf(lp, -1e30f) + entropy));  // p = 0 there: no 0 * inf
+        }
+        if (empty) return;
+        const auto add = [&](int place, float weight) {
+            if (unsigned(place) >= unsigned(N)) return;
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] += j == place ? weight : 0.f;
+        };
         if constexpr (TOPS)
-            for (int k = 0; k < a.alternatives; ++k) d += spots[team][k] == i ? weights[team][k] : 0.f;
-        return d;
+            for (int k = 0; k < a.alternatives; ++k) add(spots[team][k] - start, weights[team][k]);
+        add(at - start, given);
     };
-    if (!whole) {
-        if (lane < a.vocab) out[lane] = from_f32<T>(empty ? 0.f : gradient(to_f32(x[lane])) + spot(lane));
-        return;
+    const int odd = part ? -1 : lane < VE ? (lane < lead ? lane : -1)
+                              : (lane < 2 * VE && tail + lane - VE < a.vocab ? tail + lane - VE : -1);
+    if (odd >= 0) {
+        float v = to_f32(x[odd]);
+        gradient(odd, &v, std::integral_constant<int, 1>{});
+        out[odd] = from_f32<T>(v);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int begin = first + u * LANES * VE, start = min(begin, a.vocab - VE);
-        if (begin >= a.vocab) break;
+        const int vector = first + u * LANES;
+        if (vector >= vectors) break;
         float v[VE];
         Vec<T>::widen(raw[u], v);
+        gradient(lead + vector * VE, v, std::integral_constant<int, VE>{});
+        u32x4 bits;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = empty ? 0.f : gradient(v[j]);
-        if (!empty) {
-            if constexpr (TOPS) {
-                for (int k = 0; k < a.alternatives; ++k) {
-                    const int place = spots[team][k] - start;
-                    if (unsigned(place) < unsigned(VE)) {
-#pragma unroll
-                        for (int j = 0; j < VE; ++j) v[j] += j == place ? weights[team][k] : 0.f;
-                    }
-                }
-            }
-            if (unsigned(at - start) < unsigned(VE)) {
-#pragma unroll
-                for (int j = 0; j < VE; ++j) v[j] += j == at - start ? given : 0.f;
-            }
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (VE == 8)
+                bits[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            else
+                bits[j] = __float_as_uint(v[j]);
         }
-        if (begin + VE <= a.vocab) {
-            u32x4 bits;
-            if constexpr (VE == 8) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) bits[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) bits[j] = __float_as_uint(v[j]);
-            }
-            reinterpret_cast<AnyVector<T> *>(out + begin)->bits = bits;
-        } else {
-#pragma unroll
-            for (int j = 0; j < VE; ++j)
-                if (start + j >= begin) out[start + j] = from_f32<T>(v[j]);
-        }
+        reinterpret_cast<AnyVector<T> *>(out + lead + vector * VE)->bits = bits;
     }
 }
 
@@ -533,7 +630,7 @@ int check_rows(const char *what, int64_t rows, int64_t row_stride, int32_t vocab
     if (alternatives > kAlternativesMax)
         return fail(BDM_ERR_UNSUPPORTED, "%s: more than %d alternatives", what, kAlternativesMax);
     if (vocab > kVocabMax) return fail(BDM_ERR_UNSUPPORTED, "%s: vocabulary beyond 2^24", what);
-    if (!grid_fits(rows, 1024)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (!grid_fits(rows, kThreads)) return fail(BDM_ERR_UNSUPPORTED, "%s: too many rows", what);
     return BDM_OK;
 }
 
@@ -542,44 +639,48 @@ struct Shape {
     int waves, values, splits;
 };
 
+#ifndef FEW
+#define FEW 256
+#endif
 Shape shape_of(const bdm_token_args &a) {
-    constexpr Shape kShapes[] = {{1, 8, 1}, {1, 16, 1}, {1, 32, 1}, {4, 16, 1}, {4, 32, 1}, {4, 64, 1}, {16, 32, 1}, {16, 48, 1},
-                                 {16, 56, 1}, {16, 64, 1}};
-    for (const Shape &shape : kShapes)
-        if (a.vocab <= shape.waves * kWave * shape.values) return shape;
-    Shape wide{16, 64, 1};
-    wide.splits = (a.vocab + 65535) / 65536;
-    return wide;
+    for (const int values : {8, 16, 32})
+        if (a.vocab <= kWave * values) return {1, values, 1};
+    for (const int values : {16, 32})
+        if (a.vocab <= 256 * values) return {4, values, 1};
+    const int splits = (a.vocab + 16383) / 16384;
+    if (splits > 1 && a.rows * splits < FEW) return {4, 32, (a.vocab + 8191) / 8192};
+    for (const int values : {48, 56})
+        if (a.vocab <= 256 * values * splits) return {4, values, splits};
+    return {4, 64, splits};
 }
 
 template <typename T, int WAVES, int VALUES>
 void launch_scores(const Rows &p, hipStream_t s) {
-    constexpr int NV = VALUES / Vec<T>::kSize, kTeam = WAVES == 1 ? 256 : WAVES * kWave;
+    constexpr int NV = VALUES / Vec<T>::kSize;
     const int64_t blocks = WAVES == 1 ? (p.a.rows + 3) / 4 : p.a.rows * p.splits;
     if (p.a.alternatives)
-        score_kernel<T, WAVES, NV, true><<<unsigned(blocks), kTeam, 0, s>>>(p);
+        score_kernel<T, WAVES, NV, true><<<unsigned(blocks), kThreads, 0, s>>>(p);
     else
-        score_kernel<T, WAVES, NV, false><<<unsigned(blocks), kTeam, 0, s>>>(p);
+        score_kernel<T, WAVES, NV, false><<<unsigned(blocks), kThreads, 0, s>>>(p);
 }
 
 template <typename T>
 int launch_scores(const Rows &p, const Shape &shape, hipStream_t s) {
     if (shape.waves == 1)
         shape.values == 8 ? launch_scores<T, 1, 8>(p, s) : shape.values == 16 ? launch_scores<T, 1, 16>(p, s) : launch_scores<T, 1, 32>(p, s);
-    else if (shape.waves == 4)
-        shape.values == 16 ? launch_scores<T, 4, 16>(p, s) : shape.values == 32 ? launch_scores<T, 4, 32>(p, s) : launch_scores<T, 4, 64>(p, s);
-    else if (shape.values == 32)
-        launch_scores<T, 16, 32>(p, s);
-    else if (shape.values == 48)
-        launch_scores<T, 16, 48>(p, s);
-    else if (shape.values == 56)
-        launch_scores<T, 16, 56>(p, s);
+    else if (shape.values <= 32)
+        shape.values == 16 ? launch_scores<T, 4, 16>(p, s) : launch_scores<T, 4, 32>(p, s);
     else
-        launch_scores<T, 16, 64>(p, s);
+        shape.values == 48 ? launch_scores<T, 4, 48>(p, s) : shape.values == 56 ? launch_scores<T, 4, 56>(p, s) : launch_scores<T, 4, 64>(p, s);
     if (int rc = check_launch("score_kernel")) return rc;
     if (p.splits == 1) return BDM_OK;
     join_kernel<T><<<unsigned(p.a.rows), kThreads, 0, s>>>(p);
     return check_launch("join_kernel");
+}
+
+// Whether a call without alternatives streams its rows.
+bool streams(const bdm_token_args &a) {
+    return !a.alternatives && a.vocab > 4096 && (a.rows >= 256 || a.vocab <= 65536);
 }
 
 template <typename T, int LANES, int U>
@@ -607,7 +708,7 @@ using namespace bdm;
 
 extern "C" size_t bdm_token_log_probs_workspace_size(const bdm_token_args *a) {
     if (!a || a->rows <= 0 || a->vocab <= 0 || a->alternatives < 0 || a->vocab > kVocabMax) return 0;
-    const size_t splits = size_t(shape_of(*a).splits);
+    const size_t splits = streams(*a) ? 1 : size_t(shape_of(*a).splits);
     if (splits == 1) return 0;
     return size_t(a->rows) * splits * (sizeof(float4) + size_t(a->alternatives) * sizeof(uint64_t));
 }
@@ -618,8 +719,16 @@ extern "C" int bdm_token_log_probs(const bdm_token_args *a, void *workspace, siz
     if (a->rows == 0) return BDM_OK;
     if (!a->logits || !a->tokens || !a->log_probs || (a->alternatives && (!a->top_log_probs || !a->top_tokens)))
         return fail(BDM_ERR_INVALID, "token_log_probs: null pointer");
+    if (streams(*a)) {
+        const Rows p{*a, nullptr, nullptr, 1};
+        if (a->dtype == BDM_BF16)
+            stream_kernel<bf16_t, 4><<<unsigned(a->rows), kThreads, 0, as_stream(stream)>>>(p);
+        else
+            stream_kernel<float, 4><<<unsigned(a->rows), kThreads, 0, as_stream(stream)>>>(p);
+        return check_launch("stream_kernel");
+    }
     const Shape shape = shape_of(*a);
-    if (!grid_fits(a->rows * shape.splits, 1024)) return fail(BDM_ERR_UNSUPPORTED, "token_log_probs: too many rows");
+    if (!grid_fits(a->rows * shape.splits, kThreads)) return fail(BDM_ERR_UNSUPPORTED, "token_log_probs: too many rows");
     if (shape.splits > 1 && (!workspace || workspace_bytes < bdm_token_log_probs_workspace_size(a) || !aligned(workspace, 16)))
         return fail(BDM_ERR_INVALID, "token_log_probs: workspace too small or not aligned to 16 bytes");
     Rows p{*a, static_cast<float4 *>(workspace), nullptr, shape.splits};

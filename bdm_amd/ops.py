@@ -1187,56 +1187,61 @@ def _dense(t: Tensor) -> bool:
     return t.permute(sorted(range(t.ndim), key=t.stride, reverse=True)).is_contiguous()
 
 
-def _table(tensors, what: str) -> array:
-    """The dtype codes of dense tensors on one device, behind their checks."""
-    device = tensors[0].get_device()
-    if device < 0:
-        raise ValueError('the HIP path requires tensors on a ROCm device')
-    if any(t.get_device() != device for t in tensors):
-        raise ValueError('all tensors must be on the same device')
-    codes = [_ELEMENT.get(t.dtype) for t in tensors]
-    if None in codes or any(t.layout is not torch.strided for t in tensors):
-        raise ValueError(f'{what} must be dense BF16 or FP32 tensors')
-    return array('i', codes)
-
-
 class _Gradients:
     """The host arrays of gradients and, where they are written, outputs, those of
     None left out.  ``copies`` keeps what the arrays point to besides the
-    caller's tensors."""
+    caller's tensors.  A model has hundreds of them: each attribute is looked at
+    once, over all tensors at a time."""
 
     def __init__(self, gradients, out=None, *, written: bool = False) -> None:
         kept = list(gradients)
         out = kept if out is None else list(out)
         if len(out) != len(kept):
             raise ValueError('out must hold a tensor for each gradient')
-        if any(g is None for g in kept):
+        if any([g is None for g in kept]):
             out = [o for g, o in zip(kept, out) if g is not None]
             kept = [g for g in kept if g is not None]
         self.count, self.copies, self.device = len(kept), None, None
         if not kept:
             return
-        self.dtypes = _table(kept, 'gradients')
-        self.device = kept[0].device
         inplace = all(map(operator.is_, kept, out))
-        if inplace:
-            self.out_dtypes = self.dtypes
-        else:
-            if any(o is None for o in out) or [o.shape for o in out] != [g.shape for g in kept]:
-                raise ValueError('out must hold a tensor of each gradient\'s shape')
-            self.out_dtypes = _table(out, 'out')
-            if out[0].device != self.device:
-                raise ValueError('all tensors must be on the same device')
-        if not all(t.is_contiguous() for t in (kept if inplace else kept + out)):
-            kept = self.copies = [self._filled(g, o, written) for g, o in zip(kept, out)]
-        self.data = array('Q', [g.data_ptr() for g in kept])
-        self.out = self.data if inplace else array('Q', [o.data_ptr() for o in out])
-        self.sizes = array('q', [g.numel() for g in kept])
+        if not inplace and any([o is None for o in out]):
+            raise ValueError('out must hold a tensor for each gradient')
+        self.dtypes = self._codes(kept, 'gradients')
+        self.out_dtypes = self.dtypes if inplace else self._codes(out, 'out')
+        indices = {t.get_device() for t in kept} | (set() if inplace else {t.get_device() for t in out})
+        if min(indices) < 0:
+            raise ValueError('the HIP path requires tensors on a ROCm device')
+        if len(indices) > 1:
+            raise ValueError('all tensors must be on the same device')
+        self.device = kept[0].device
+        sizes = [g.numel() for g in kept]
+        if not inplace and [o.numel() for o in out] != sizes:
+            raise ValueError('out must hold as many elements as each gradient')
+        try:
+            if not all(map(Tensor.is_contiguous, kept)) or not (inplace or all(map(Tensor.is_contiguous, out))):
+                kept = self.copies = [self._filled(g, o, written) for g, o in zip(kept, out)]
+            self.data = array('Q', [g.data_ptr() for g in kept])
+            self.out = self.data if inplace else array('Q', [o.data_ptr() for o in out])
+        except RuntimeError as e:  # a tensor without a storage, a sparse one for instance
+            raise ValueError('gradients and out must be dense BF16 or FP32 tensors') from e
+        self.sizes = array('q', sizes)
+
+    @staticmethod
+    def _codes(tensors, what: str) -> array:
+        dtypes = [t.dtype for t in tensors]
+        first = _ELEMENT.get(dtypes[0])
+        same = dtypes.count(dtypes[0]) == len(dtypes)
+        codes = [first] * len(dtypes) if same else [_ELEMENT.get(d) for d in dtypes]
+        if None in codes:
+            raise ValueError(f'{what} must be dense BF16 or FP32 tensors')
+        return array('i', codes)
 
     @staticmethod
     def _filled(g: Tensor, o: Tensor, written: bool) -> Tensor:
         """The gradient, or a copy, whose elements lie one behind the other as its output's do."""
-        if (g is o and _dense(g)) or (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _dense(g)):
+        if (g is o and _dense(g)) or (g.is_contiguous() and o.is_contiguous()) or (
+                g.shape == o.shape and g.stride() == o.stride() and _dense(g)):
             return g
         if written and g is o:
             raise ValueError('a gradient whose elements do not fill its memory cannot be clipped in place')

@@ -51,8 +51,31 @@ def test_vocabularies(vocab, dtype):
 @pytest.mark.parametrize('dtype', [BF16, FP32])
 @pytest.mark.parametrize('rows', [1, 2, 63, 64, 255, 256, 257, 1023, 2049])
 def test_rows(rows, dtype):
-    check(logits_of(rows, 192, dtype, rows), tokens_of(rows, 192), 5)
-    check(logits_of(rows, 5003, dtype, rows), tokens_of(rows, 5003), 5)
+    for vocab in (192, 5003, 9001):
+        check(logits_of(rows, vocab, dtype, rows), tokens_of(rows, vocab))
+        check(logits_of(rows, vocab, dtype, rows), tokens_of(rows, vocab), 5)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP32])
+@pytest.mark.parametrize('vocab', [9001, 50257])
+def test_many_rows(vocab, dtype):
+    """Rows of every alignment, masked, empty, level, not finite ones among many."""
+    rows = 600
+    logits, tokens = logits_of(rows, vocab, dtype), tokens_of(rows, vocab)
+    lowest = torch.finfo(dtype).min
+    for first, change in ((0, -torch.inf), (1, lowest), (2, torch.finfo(dtype).max), (3, 7.0)):
+        logits[first::16] = change
+    logits[4::16, 5:] = -torch.inf
+    logits[5::16, :-5] = lowest
+    logits[6::16, vocab // 3] = torch.nan
+    logits[7::16, vocab // 2] = torch.inf
+    logits[8::16, ::2] = -torch.inf
+    logits[9::16] *= 1000
+    logits[10::16] = torch.linspace(-90, 90, vocab, device='cuda').to(dtype)
+    logits[11::16] = torch.linspace(90, -90, vocab, device='cuda').to(dtype)
+    check(logits, tokens)
+    check(logits, tokens, 3)
+    check(logits[:, 1:], tokens_of(rows, vocab - 1))
 
 
 @pytest.mark.parametrize('vocab', [5, 192, 3001, 20000, 50257])
@@ -65,7 +88,7 @@ def test_alternatives(k, vocab):
 
 
 @pytest.mark.parametrize('dtype', [BF16, FP32])
-@pytest.mark.parametrize('vocab', [192, 4099, 50257, 70000])
+@pytest.mark.parametrize('vocab', [192, 700, 1500, 3000, 4099, 10000, 20000, 40000, 50257, 60000, 70000])
 def test_masks(vocab, dtype):
     """Rows that keep a few tokens, one, or none; masks of -inf and of the type's lowest value."""
     for mask in (-torch.inf, torch.finfo(dtype).min):
@@ -85,7 +108,7 @@ def test_masks(vocab, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, FP32])
-@pytest.mark.parametrize('vocab', [192, 4099, 50257, 70001])
+@pytest.mark.parametrize('vocab', [192, 700, 1500, 3000, 4099, 10000, 20000, 40000, 50257, 60000, 70001])
 def test_ties_and_orders(vocab, dtype):
     """Level rows, ascending and descending ones, two values, both zeros, most of the best in one place."""
     ramp = torch.linspace(-20, 20, vocab, device='cuda')
@@ -100,7 +123,7 @@ def test_ties_and_orders(vocab, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, FP32])
-@pytest.mark.parametrize('vocab', [192, 50257, 70001])
+@pytest.mark.parametrize('vocab', [192, 700, 1500, 3000, 4099, 10000, 20000, 40000, 50257, 60000, 70001])
 def test_not_finite(vocab, dtype):
     """A NaN or +inf makes its row NaN, and only that row; the alternatives keep their order, a NaN first."""
     logits, tokens = logits_of(6, vocab, dtype), tokens_of(6, vocab)
