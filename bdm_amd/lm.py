@@ -159,7 +159,7 @@ class _LayerNormFunction(torch.autograd.Function):
         if _differentiable([grad_out]):
             return (*_torch_gradients(functools.partial(_layer_norm_ops, eps=ctx.eps), (x, weight, bias), grad_out),
                     None)
-        return (*ops.layer_norm_backward(x, grad_out, weight, bias, ctx.eps), None)
+        return (*ops.layer_norm_gradients(x, grad_out, weight, bias, ctx.eps), None)
 
 
 class _AddLayerNormFunction(torch.autograd.Function):
@@ -184,7 +184,7 @@ class _AddLayerNormFunction(torch.autograd.Function):
                                            (total.requires_grad_(), weight, bias), grad_out)
             grad = grad if grad_total is None else grad + grad_total
         else:
-            grad, *rest = ops.layer_norm_backward(total, grad_out, weight, bias, ctx.eps, grad_sum=grad_total)
+            grad, *rest = ops.layer_norm_gradients(total, grad_out, weight, bias, ctx.eps, grad_total)
         return grad, grad, *rest, None
 
 
@@ -210,9 +210,9 @@ class LayerNorm(nn.Module):
             self.register_parameter('bias', None)
 
     def _fused(self, x: Tensor) -> bool:
-        parameters = [t for t in (self.weight, self.bias) if t is not None]
-        return (ops.layer_norm_supported(x) and all(t.dtype in (torch.bfloat16, torch.float32) for t in parameters)
-                and len({t.dtype for t in parameters}) == 1)
+        weight, bias = self.weight, self.bias
+        return (ops.layer_norm_supported(x) and weight.dtype in (torch.bfloat16, torch.float32)
+                and (bias is None or bias.dtype == weight.dtype))
 
     def _trained(self, *tensors: Tensor) -> bool:
         return torch.is_grad_enabled() and any(t is not None and t.requires_grad

@@ -26,6 +26,9 @@ from .config import near_square_factors
 Tensor = torch.Tensor
 
 
+_ELEMENT = {torch.float32: _lib.BDM_F32, torch.bfloat16: _lib.BDM_BF16}
+
+
 def _dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.bfloat16:
         return _lib.BDM_BF16
@@ -960,25 +963,34 @@ def layer_norm_backward(x: Tensor, grad_out: Tensor, weight: Tensor | None, bias
     bias, eps)``, None for a parameter that is not there.  ``grad_sum`` is added
     to grad_x: with the sum of a residual add as x, the gradient of that sum
     itself."""
-    device = _require_gpu(x, grad_out, weight, bias, grad_sum)
-    code = _layer_norm_parameters(x, weight, bias)
+    _require_gpu(x, grad_out, weight, bias, grad_sum)
+    _layer_norm_parameters(x, weight, bias)
     for t in (grad_out, grad_sum):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise ValueError('the gradients must match x')
+    return layer_norm_gradients(x, grad_out, weight, bias, eps, grad_sum)
+
+
+def layer_norm_gradients(x, grad_out, weight, bias, eps, grad_sum=None):
+    """``layer_norm_backward`` of tensors that a forward and autograd have
+    checked: its thread runs a backward's Python at half the speed."""
     x, grad_out = x.contiguous(), grad_out.contiguous()
-    weight, grad_sum = (None if t is None else t.contiguous() for t in (weight, grad_sum))
-    width = x.shape[-1]
+    parameter = bias if weight is None else weight
+    grad_x = torch.empty_like(x)
+    grad_weight = None if weight is None else torch.empty_like(weight, memory_format=torch.contiguous_format)
+    grad_bias = None if bias is None else torch.empty_like(bias, memory_format=torch.contiguous_format)
+    weight = None if weight is None else weight.contiguous()
+    grad_sum = None if grad_sum is None else grad_sum.contiguous()
+    device, width = x.device, x.shape[-1]
     rows = x.numel() // width
     lib = _lib.library()
     nbytes = lib.bdm_layer_norm_backward_workspace_size(rows, width)
     workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
-    grad_x = torch.empty_like(x)
-    grad_weight, grad_bias = (None if t is None else torch.empty(width, device=device, dtype=t.dtype)
-                              for t in (weight, bias))
     with _on(device):
         _lib.check(lib.bdm_layer_norm_backward(
-            _addr(x), _addr(grad_out), _addr(grad_sum), _addr(weight), _addr(grad_x), _addr(grad_weight),
-            _addr(grad_bias), rows, width, _dtype_code(x.dtype), code, float(eps), _addr(workspace), nbytes,
+            x.data_ptr(), grad_out.data_ptr(), _addr(grad_sum), _addr(weight), grad_x.data_ptr(), _addr(grad_weight),
+            _addr(grad_bias), rows, width, _ELEMENT[x.dtype],
+            _lib.BDM_F32 if parameter is None else _ELEMENT[parameter.dtype], eps, workspace.data_ptr(), nbytes,
             _stream(device)), 'bdm_layer_norm_backward')
     return grad_x, grad_weight, grad_bias
 
@@ -1148,8 +1160,8 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
                    ignore_index: int = -100) -> Tensor:
     """The logits' gradient from those of ``token_statistics``' results, or from
     that of ``token_loss_mean``'s loss."""
-    device = _require_gpu(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs,
-                          grad_loss, inverse_count)
+    _require_gpu(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs, grad_loss,
+                 inverse_count)
     if logits.dtype not in (torch.bfloat16, torch.float32) or tokens.dtype != torch.int64 \
             or tokens.shape != logits.shape[:-1] or stats.shape != (tokens.numel(), 2):
         raise ValueError('the gradient takes BF16/FP32 logits, their int64 tokens and the rows\' statistics')
@@ -1161,13 +1173,21 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
                      (grad_top_log_probs, None if top_tokens is None else top_tokens.shape)):
         if t is not None and (t.dtype != torch.float32 or t.shape != shape):
             raise ValueError('the results and their gradients must be FP32 of the tokens\' shape')
+    return token_gradients(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs,
+                           grad_loss, inverse_count, int(ignore_index))
+
+
+def token_gradients(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs,
+                    grad_loss, inverse_count, ignore_index):
+    """``token_gradient`` of tensors that a forward and autograd have checked."""
+    device = logits.device
     grad = torch.empty(logits.shape, device=device, dtype=logits.dtype)
     logits, rows, stride = _logit_rows(logits)
     kept = [None if t is None else t.contiguous() for t in (tokens, stats, entropy, top_tokens, grad_log_probs,
                                                             grad_entropy, grad_top_log_probs, grad_loss, inverse_count)]
-    k = 0 if top_tokens is None else top_tokens.shape[-1]
-    args = _lib.TokenGradArgs(logits.data_ptr(), *(_addr(t) for t in kept), grad.data_ptr(), rows, stride,
-                              int(ignore_index), logits.shape[-1], k, _dtype_code(logits.dtype))
+    args = _lib.TokenGradArgs(logits.data_ptr(), *[None if t is None else t.data_ptr() for t in kept], grad.data_ptr(),
+                              rows, stride, ignore_index, logits.shape[-1],
+                              0 if top_tokens is None else top_tokens.shape[-1], _ELEMENT[logits.dtype])
     with _on(device):
         _lib.check(_lib.library().bdm_token_log_probs_backward(ctypes.byref(args), _stream(device)),
                    'bdm_token_log_probs_backward')
@@ -1176,9 +1196,6 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
 
 # ---------------------------------------------------------------------------
 # the gradients' norm and clipping
-
-_ELEMENT = {torch.float32: _lib.BDM_F32, torch.bfloat16: _lib.BDM_BF16}
-
 
 def _dense(t: Tensor) -> bool:
     """Whether the elements fill their span of memory, each once, in any order."""

@@ -73,16 +73,15 @@ class _TokenLogProbs(torch.autograd.Function):
     def backward(ctx, *grads):
         logits, tokens, stats, entropy, top_tokens = ctx.saved_tensors
         grads = [*grads[:3], None][:3]
-        if all(g is None for g in grads):
+        present = [g for g in grads if g is not None]
+        if not present:
             return None, None, None, None
-        if _differentiable([g for g in grads if g is not None]):
+        if _differentiable(present):
             def form(x):
                 results = _log_probs_ops(x, tokens, top_tokens, ctx.ignore_index)
                 return [r for r, g in zip(results, grads) if g is not None]
-            return (*_torch_gradients(form, (logits,), [g for g in grads if g is not None]), None, None, None)
-        grad = ops.token_gradient(logits, tokens, stats, entropy=entropy, top_tokens=top_tokens,
-                                  grad_log_probs=grads[0], grad_entropy=grads[1], grad_top_log_probs=grads[2],
-                                  ignore_index=ctx.ignore_index)
+            return (*_torch_gradients(form, (logits,), present), None, None, None)
+        grad = ops.token_gradients(logits, tokens, stats, entropy, top_tokens, *grads, None, None, ctx.ignore_index)
         return grad, None, None, None
 
 
@@ -102,8 +101,8 @@ class _TokenLoss(torch.autograd.Function):
         if _differentiable([grad_loss]):
             form = functools.partial(_loss_ops, tokens=tokens, ignore_index=ctx.ignore_index)
             return (*_torch_gradients(form, (logits,), grad_loss), None, None)
-        grad = ops.token_gradient(logits, tokens, stats, grad_loss=grad_loss, inverse_count=inverse_count,
-                                  ignore_index=ctx.ignore_index)
+        grad = ops.token_gradients(logits, tokens, stats, None, None, None, None, None, grad_loss, inverse_count,
+                                   ctx.ignore_index)
         return grad, None, None
 
 
