@@ -112,7 +112,31 @@ struct Rows {
 };
 
 // A team of 16 waves has 128 registers a lane: it loads a row when its turn comes, and the parameters with every row.
-constexpr int kLeanWaves = 16;
+constexpr int kLeanLanes = 1024;
+
+template <int CONTROL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(uint32_t(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(x)), CONTROL, 0xf, 0xf, false)));
+}
+// The sum over each 16 lanes, in all of them: neighbours, pairs, then the mirrored half and row.
+__device__ __forceinline__ float row_total(float x) {
+    x += dpp<0xb1>(x);   // quad_perm 1 0 3 2
+    x += dpp<0x4e>(x);   // quad_perm 2 3 0 1
+    x += dpp<0x141>(x);  // row_half_mirror
+    x += dpp<0x140>(x);  // row_mirror
+    return x;
+}
+// The sum over the lanes of a row's team, or over its wave where the team has several.
+template <int LANES>
+__device__ __forceinline__ float lanes_total(float x) {
+    if constexpr (LANES >= kWave) {
+        return wave_sum(x);
+    } else {
+        x = row_total(x);
+        if constexpr (LANES == 32) x += __shfl_xor(x, 16, kWave);
+        return x;
+    }
+}
 
 // What a wave gives to its team of a row.
 struct Sums {
@@ -135,51 +159,47 @@ __device__ __forceinline__ Statistics join(Sums mine, Sums (&shared)[2][WAVES], 
         out.g = mine.g * inverse;
         out.dot = (mine.gd - out.offset * mine.g) * inverse * out.scale;
     } else {
+        // lane i of 16 takes wave i
+        static_assert(WAVES <= 16);
         if (lane == 0) shared[turn][wave] = mine;
         __syncthreads();
+        const int from = lane % 16;
+        Sums s = shared[turn][min(from, WAVES - 1)];
         const float pivot = shared[turn][0].centre;
-        float total = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-            total += fmaf(shared[turn][w].count, shared[turn][w].centre - pivot, shared[turn][w].d);
-        const float mean = total * inverse;  // from the pivot
-        float square = 0.f, g = 0.f, gd = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const Sums &s = shared[turn][w];
-            const float from = (s.centre - pivot) - mean;
-            square += s.square + from * (2.f * s.d + s.count * from);
-            if constexpr (GRADIENT) {
-                g += s.g;
-                gd += s.gd + from * s.g;
-            }
-        }
+        if (from >= WAVES) s = Sums{0.f, pivot, 0.f, 0.f, 0.f, 0.f};
+        const float mean = row_total(fmaf(s.count, s.centre - pivot, s.d)) * inverse;  // from the pivot
+        const float away = (s.centre - pivot) - mean;
+        const float square = row_total(s.square + away * (2.f * s.d + s.count * away));
         out.offset = mean - (mine.centre - pivot);
         out.scale = rsqrtf(fmaxf(square * inverse, 0.f) + eps);
-        out.g = g * inverse;
-        out.dot = gd * inverse * out.scale;
+        if constexpr (GRADIENT) {
+            out.g = row_total(s.g) * inverse;
+            out.dot = row_total(s.gd + away * s.g) * inverse * out.scale;
+        }
     }
     return out;
 }
 
 template <int LANES, int VE, int NV>
 __device__ __forceinline__ float columns_of_wave(const Columns<LANES, VE> &c, int wave) {
+    constexpr int kMine = LANES < kWave ? LANES : kWave;
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) count += min(max(c.width - (wave * kWave + i * LANES) * VE, 0), kWave * VE);
+    for (int i = 0; i < NV; ++i) count += min(max(c.width - (wave * kWave + i * LANES) * VE, 0), kMine * VE);
     return float(count);
 }
 
-// Teams of WAVES waves take the rows in turn; a workgroup holds four teams of one wave, or one team.
-template <typename T, typename P, int WAVES, int NV, bool RESIDUAL>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_kernel(Rows<T> p) {
-    constexpr int VE = Vec<T>::kSize, kTeams = WAVES == 1 ? 4 : 1;
-    constexpr bool kLean = WAVES == kLeanWaves;
+// Teams of LANES lanes take the rows in turn; a workgroup of 256 lanes holds several teams of a wave or less, one of
+// several waves is a workgroup.
+template <typename T, typename P, int LANES, int NV, bool RESIDUAL>
+__global__ __launch_bounds__(LANES <= 256 ? 256 : LANES) void layer_norm_kernel(Rows<T> p) {
+    constexpr int VE = Vec<T>::kSize, WAVES = LANES <= kWave ? 1 : LANES / kWave, kTeams = WAVES == 1 ? 256 / LANES : 1;
+    constexpr bool kLean = LANES == kLeanLanes;
     __shared__ Sums shared[2][WAVES];
     const int lane = int(threadIdx.x) % kWave, wave = WAVES == 1 ? 0 : int(threadIdx.x) / kWave;
-    const Columns<WAVES * kWave, VE> c{wave * kWave + lane, p.width};
+    const Columns<LANES, VE> c{int(threadIdx.x) % LANES, p.width};
     const int64_t step = int64_t(gridDim.x) * kTeams;
-    int64_t row = int64_t(blockIdx.x) * kTeams + (WAVES == 1 ? int(threadIdx.x) / kWave : 0);
+    int64_t row = int64_t(blockIdx.x) * kTeams + (WAVES == 1 ? int(threadIdx.x) / LANES : 0);
     if (row >= p.rows) return;
     u32x4 x[NV], r[NV];
     const auto load = [&](int64_t at) {
@@ -198,7 +218,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_k
             c.template parameters<P>(p.bias, i, 0.f, bias[i]);
         }
     }
-    const float count = columns_of_wave<WAVES * kWave, VE, NV>(c, wave);
+    const float count = columns_of_wave<LANES, VE, NV>(c, wave);
     int turn = 0;
     for (; row < p.rows; row += step, turn ^= 1) {
         const int64_t base = row * p.width;
@@ -221,7 +241,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_k
         if (!kLean && row + step < p.rows) load(row + step);
         Sums s{};
         s.count = count;
-        s.centre = wave_sum(sum) / fmaxf(count, 1.f);
+        s.centre = lanes_total<LANES>(sum) / fmaxf(count, 1.f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -233,8 +253,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_k
                 s.square = fmaf(v[i][j], v[i][j], s.square);
             }
         }
-        s.d = wave_sum(s.d);
-        s.square = wave_sum(s.square);
+        s.d = lanes_total<LANES>(s.d);
+        s.square = lanes_total<LANES>(s.square);
         const Statistics t = join<WAVES, false>(s, shared, turn, wave, lane, p.width, p.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -250,15 +270,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_k
     }
 }
 
-template <typename T, typename P, int WAVES, int NV, bool SUM>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_backward_kernel(Rows<T> p) {
-    constexpr int VE = Vec<T>::kSize, kTeams = WAVES == 1 ? 4 : 1, kColumns = WAVES * kWave * NV * VE;
-    constexpr bool kLean = WAVES == kLeanWaves;
+template <typename T, typename P, int LANES, int NV, bool SUM>
+__global__ __launch_bounds__(LANES <= 256 ? 256 : LANES) void layer_norm_backward_kernel(Rows<T> p) {
+    constexpr int VE = Vec<T>::kSize, WAVES = LANES <= kWave ? 1 : LANES / kWave, kTeams = WAVES == 1 ? 256 / LANES : 1;
+    constexpr int kColumns = LANES * NV * VE;
+    constexpr bool kLean = LANES == kLeanLanes;
     __shared__ Sums shared[2][WAVES];
-    __shared__ float slice[WAVES == 1 ? 4 : 1][WAVES == 1 ? kColumns : 1];
+    __shared__ float slice[kTeams][WAVES == 1 ? kColumns : 1];
     const int lane = int(threadIdx.x) % kWave, wave = WAVES == 1 ? 0 : int(threadIdx.x) / kWave;
-    const int team = WAVES == 1 ? int(threadIdx.x) / kWave : 0;
-    const Columns<WAVES * kWave, VE> c{wave * kWave + lane, p.width};
+    const int team = WAVES == 1 ? int(threadIdx.x) / LANES : 0;
+    const Columns<LANES, VE> c{int(threadIdx.x) % LANES, p.width};
     const int64_t step = int64_t(gridDim.x) * kTeams;
     int64_t row = int64_t(blockIdx.x) * kTeams + team;
     u32x4 x[NV], dy[NV], ds[NV];
@@ -278,7 +299,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_b
 #pragma unroll
         for (int j = 0; j < VE; ++j) dw[i][j] = db[i][j] = 0.f;
     }
-    const float count = columns_of_wave<WAVES * kWave, VE, NV>(c, wave);
+    const float count = columns_of_wave<LANES, VE, NV>(c, wave);
     int turn = 0;
     for (; row < p.rows; row += step, turn ^= 1) {
         const int64_t base = row * p.width;
@@ -296,7 +317,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_b
         if (!kLean && row + step < p.rows) load(row + step);
         Sums s{};
         s.count = count;
-        s.centre = wave_sum(sum) / fmaxf(count, 1.f);
+        s.centre = lanes_total<LANES>(sum) / fmaxf(count, 1.f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -312,10 +333,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_b
                 s.gd = fmaf(gw, v[i][j], s.gd);
             }
         }
-        s.d = wave_sum(s.d);
-        s.square = wave_sum(s.square);
-        s.g = wave_sum(s.g);
-        s.gd = wave_sum(s.gd);
+        s.d = lanes_total<LANES>(s.d);
+        s.square = lanes_total<LANES>(s.square);
+        s.g = lanes_total<LANES>(s.g);
+        s.gd = lanes_total<LANES>(s.gd);
         const Statistics t = join<WAVES, true>(s, shared, turn, wave, lane, p.width, p.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -344,7 +365,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_b
             }
         }
     } else {
-        // the four teams' sums, in their order
+        // the teams' sums, in their order
         const auto put = [&](const float (&from)[NV][VE], float *to) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -353,8 +374,12 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void layer_norm_b
                     if (c.valid(i, j)) slice[team][c.start(i) + j] = from[i][j];
             }
             __syncthreads();
-            for (int at = threadIdx.x; at < p.width; at += 256)
-                to[at] = ((slice[0][at] + slice[1][at]) + slice[2][at]) + slice[3][at];
+            for (int at = threadIdx.x; at < p.width; at += 256) {
+                float total = slice[0][at];
+#pragma unroll
+                for (int i = 1; i < kTeams; ++i) total += slice[i][at];
+                to[at] = total;
+            }
             __syncthreads();
         };
         put(dw, part);
@@ -397,33 +422,50 @@ int check_rows(const char *what, int64_t rows, int32_t width, int32_t dtype, int
     return BDM_OK;
 }
 
-// Waves of a team and vectors of a lane for a width: a wave holds up to 1024 columns, 16 a lane.
+// Lanes of a team and vectors of a lane for a width.
 template <typename T, typename F>
 void with_shape(int width, F f) {
-    constexpr int kVectors = 16 / Vec<T>::kSize;
-    const auto shape = [&](auto waves, auto vectors) { f(waves, vectors); };
-    if (width <= 512)
-        shape(std::integral_constant<int, 1>{}, std::integral_constant<int, kVectors / 2>{});
+    constexpr int kVectors = 8 / Vec<T>::kSize;
+    const auto shape = [&](auto lanes, auto vectors) { f(lanes, vectors); };
+    const auto eight = std::integral_constant<int, kVectors>{};
+    const auto sixteen = std::integral_constant<int, 2 * kVectors>{};
+    if (width <= 128)
+        shape(std::integral_constant<int, 16>{}, eight);
+    else if (width <= 256)
+        shape(std::integral_constant<int, 32>{}, eight);
+    else if (width <= 512)
+        shape(std::integral_constant<int, 64>{}, eight);
     else if (width <= 1024)
-        shape(std::integral_constant<int, 1>{}, std::integral_constant<int, kVectors>{});
+        shape(std::integral_constant<int, 64>{}, sixteen);
     else if (width <= 2048)
-        shape(std::integral_constant<int, 2>{}, std::integral_constant<int, kVectors>{});
+        shape(std::integral_constant<int, 128>{}, sixteen);
     else if (width <= 4096)
-        shape(std::integral_constant<int, 4>{}, std::integral_constant<int, kVectors>{});
+        shape(std::integral_constant<int, 256>{}, sixteen);
     else if (width <= 8192)
-        shape(std::integral_constant<int, 8>{}, std::integral_constant<int, kVectors>{});
+        shape(std::integral_constant<int, 512>{}, sixteen);
     else
-        shape(std::integral_constant<int, 16>{}, std::integral_constant<int, kVectors>{});
+        shape(std::integral_constant<int, 1024>{}, sixteen);
 }
 
-// Workgroups of a pass over the rows: as many as there is work for, at most those that the chip holds at once.
-int64_t blocks_of(int64_t rows, int width, int64_t waves) {
-    const int64_t team = width <= 1024 ? 1 : width <= 2048 ? 2 : width <= 4096 ? 4 : width <= 8192 ? 8 : 16;
-    const int64_t teams = team == 1 ? 4 : 1, most = waves / (team * teams);
-    const int64_t blocks = (rows + teams - 1) / teams;
+// Workgroups of a pass over the rows by teams of `lanes` lanes: as many as there is work for, at most `waves` waves.
+int64_t blocks_of(int64_t rows, int lanes, int64_t waves) {
+    const int64_t block = lanes <= kWave ? 256 : lanes, teams = lanes <= kWave ? 256 / lanes : 1;
+    const int64_t blocks = (rows + teams - 1) / teams, most = waves * kWave / block;
     return blocks < most ? blocks : most;
 }
-constexpr int64_t kForwardWaves = 256 * 32, kBackwardWaves = 256 * 8;
+constexpr int64_t kForwardWaves = 256 * 32;
+
+// The backward's workgroups, each of which leaves its columns' sums: as many waves as the registers of 16 values a lane
+// admit, twice as many with 8 values or without a row loaded ahead (more of 16 wait for the first ones: 32,768 rows of
+// 1,024 BF16 43 us with 2,048 waves, 53 with 3,072; 2,048 rows of 16,384 95 with 2,048, 73 with 4,096).
+int64_t backward_parts(int64_t rows, int width) {
+    int64_t parts = 0;
+    with_shape<bf16_t>(width, [&](auto lanes, auto vectors) {
+        constexpr bool kMany = decltype(vectors)::value == 1 || decltype(lanes)::value == kLeanLanes;
+        parts = blocks_of(rows, decltype(lanes)::value, kMany ? 4096 : 2048);
+    });
+    return parts;
+}
 
 }  // namespace
 }  // namespace bdm
@@ -441,10 +483,9 @@ extern "C" int bdm_layer_norm(const void *x, const void *residual, const void *w
         using P = decltype(parameter);
         const Rows<T> p{static_cast<const T *>(x), static_cast<const T *>(residual), nullptr, nullptr, weight, bias,
                         static_cast<T *>(sum_out), static_cast<T *>(out), nullptr, rows, width, eps};
-        const unsigned blocks = unsigned(blocks_of(rows, width, kForwardWaves));
-        with_shape<T>(width, [&](auto waves, auto vectors) {
-            constexpr int kTeam = decltype(waves)::value;
-            constexpr int kBlock = kTeam == 1 ? 256 : kTeam * kWave;
+        with_shape<T>(width, [&](auto lanes, auto vectors) {
+            constexpr int kTeam = decltype(lanes)::value, kBlock = kTeam <= kWave ? 256 : kTeam;
+            const unsigned blocks = unsigned(blocks_of(rows, kTeam, kForwardWaves));
             if (residual)
                 layer_norm_kernel<T, P, kTeam, decltype(vectors)::value, true><<<blocks, kBlock, 0, as_stream(stream)>>>(p);
             else
@@ -461,7 +502,7 @@ extern "C" int bdm_layer_norm(const void *x, const void *residual, const void *w
 extern "C" size_t bdm_layer_norm_backward_workspace_size(int64_t rows, int32_t width) {
     if (rows <= 0 || width <= 0) return 0;
     if (width > kMaxWidth) return 0;
-    return size_t(blocks_of(rows, width, kBackwardWaves)) * 2 * size_t(width) * sizeof(float);
+    return size_t(backward_parts(rows, width)) * 2 * size_t(width) * sizeof(float);
 }
 
 extern "C" int bdm_layer_norm_backward(const void *x, const void *grad_out, const void *grad_sum, const void *weight,
@@ -474,15 +515,14 @@ extern "C" int bdm_layer_norm_backward(const void *x, const void *grad_out, cons
     if (workspace_bytes < bdm_layer_norm_backward_workspace_size(rows, width) || !aligned(workspace, 16))
         return fail(BDM_ERR_INVALID, "layer_norm_backward: workspace too small or not aligned to 16 bytes");
     hipStream_t s = as_stream(stream);
-    const int64_t parts = blocks_of(rows, width, kBackwardWaves);
+    const int64_t parts = backward_parts(rows, width);
     const auto run = [&](auto element, auto parameter) {
         using T = decltype(element);
         using P = decltype(parameter);
         const Rows<T> p{static_cast<const T *>(x), nullptr, static_cast<const T *>(grad_out), static_cast<const T *>(grad_sum),
                         weight, nullptr, nullptr, static_cast<T *>(grad_x), static_cast<float *>(workspace), rows, width, eps};
-        with_shape<T>(width, [&](auto waves, auto vectors) {
-            constexpr int kTeam = decltype(waves)::value;
-            constexpr int kBlock = kTeam == 1 ? 256 : kTeam * kWave;
+        with_shape<T>(width, [&](auto lanes, auto vectors) {
+            constexpr int kTeam = decltype(lanes)::value, kBlock = kTeam <= kWave ? 256 : kTeam;
             if (grad_sum)
                 layer_norm_backward_kernel<T, P, kTeam, decltype(vectors)::value, true><<<unsigned(parts), kBlock, 0, s>>>(p);
             else
