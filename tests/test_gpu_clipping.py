@@ -88,6 +88,20 @@ def test_unaligned(dtype):
     check_clip(views, 1.0)
 
 
+def test_very_large():
+    """A tensor of more than 2^30 elements, in several entries of a launch."""
+    from bdm_amd import clip_gradients, gradient_norm
+    n = (1 << 30) + 17
+    g = torch.full((n,), 0.5, device='cuda', dtype=BF16)
+    g[-1] = 2.0 ** 14
+    want = math.sqrt(0.25 * (n - 1) + 2.0 ** 28)
+    assert abs(float(gradient_norm([g])) - want) <= 2 * STEP * want
+    clip_gradients([g], want / 4)
+    ends = torch.cat([g[:3], g[(1 << 29) - 2:(1 << 29) + 2], g[-3:]]).double().cpu()
+    close(ends, torch.tensor([0.125] * 9 + [2.0 ** 12], dtype=torch.float64), 2.0 ** -8 * torch.ones(10) * ends.abs())
+    assert float((g[:-1].float() - 0.125).abs().max()) <= 2.0 ** -8 * 0.125
+
+
 def test_layouts():
     """Transposed gradients are clipped in place; those with holes have a norm, and go to out."""
     from bdm_amd import clip_gradients

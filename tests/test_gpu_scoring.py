@@ -344,6 +344,21 @@ def test_rows_beyond_32_bits():
     close(grad[-3:], *expected_gradient(logits.detach()[-3:], tokens[-3:], given=torch.ones(3, device='cuda')))
 
 
+def test_widest_vocabularies():
+    """Joins of many parts: level lists in every part, whose bounds admit more candidates than fit, and the largest size."""
+    from bdm_amd import ops
+    vocab = 64 * 16384
+    logits = logits_of(2, 16384, FP32).repeat(1, 64)
+    for k in (1, 31, 32):
+        check(logits, tokens_of(2, vocab), k)
+    logits = logits_of(1, 1 << 24, BF16)
+    check(logits, tokens_of(1, 1 << 24))
+    check(logits, tokens_of(1, 1 << 24), 32)
+    check(torch.zeros_like(logits), tokens_of(1, 1 << 24), 32)
+    with pytest.raises(NotImplementedError):
+        ops.token_statistics(torch.zeros(1, (1 << 24) + 1, device='cuda', dtype=BF16), tokens_of(1, 5))
+
+
 def test_repeats_and_streams():
     """The same call gives the same bits, on any stream and beside another call."""
     from bdm_amd import token_log_probs
