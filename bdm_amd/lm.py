@@ -149,17 +149,18 @@ class _LayerNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
+        out = ops.layer_norm(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, bias)
-        ctx.eps = eps
-        return ops.layer_norm(x, weight, bias, eps)
+        ctx.eps, ctx.plan = eps, ops.layer_norm_plan(x, weight, bias, eps)
+        return out
 
     @staticmethod
     def backward(ctx, grad_out):
         x, weight, bias = ctx.saved_tensors
-        if _differentiable([grad_out]):
+        if _differentiable((grad_out,)):
             return (*_torch_gradients(functools.partial(_layer_norm_ops, eps=ctx.eps), (x, weight, bias), grad_out),
                     None)
-        return (*ops.layer_norm_gradients(x, grad_out, weight, bias, ctx.eps), None)
+        return (*ops.layer_norm_gradients(x, grad_out, weight, bias, None, ctx.plan), None)
 
 
 class _AddLayerNormFunction(torch.autograd.Function):
@@ -170,7 +171,7 @@ class _AddLayerNormFunction(torch.autograd.Function):
     def forward(ctx, x, residual, weight, bias, eps):
         total, out = ops.layer_norm(x, weight, bias, eps, residual=residual)
         ctx.save_for_backward(total, weight, bias)
-        ctx.eps = eps
+        ctx.eps, ctx.plan = eps, ops.layer_norm_plan(x, weight, bias, eps)
         ctx.set_materialize_grads(False)
         return total, out
 
@@ -179,12 +180,12 @@ class _AddLayerNormFunction(torch.autograd.Function):
         total, weight, bias = ctx.saved_tensors
         if grad_out is None:
             return grad_total, grad_total, None, None, None
-        if _differentiable([g for g in (grad_total, grad_out) if g is not None]):
+        if _differentiable((grad_out,) if grad_total is None else (grad_total, grad_out)):
             grad, *rest = _torch_gradients(functools.partial(_layer_norm_ops, eps=ctx.eps),
                                            (total.requires_grad_(), weight, bias), grad_out)
             grad = grad if grad_total is None else grad + grad_total
         else:
-            grad, *rest = ops.layer_norm_gradients(total, grad_out, weight, bias, ctx.eps, grad_total)
+            grad, *rest = ops.layer_norm_gradients(total, grad_out, weight, bias, grad_total, ctx.plan)
         return grad, grad, *rest, None
 
 

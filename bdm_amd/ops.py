@@ -968,30 +968,38 @@ def layer_norm_backward(x: Tensor, grad_out: Tensor, weight: Tensor | None, bias
     for t in (grad_out, grad_sum):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise ValueError('the gradients must match x')
-    return layer_norm_gradients(x, grad_out, weight, bias, eps, grad_sum)
+    plan = layer_norm_plan(x, weight, bias, eps)
+    with _on(x.device):
+        return layer_norm_gradients(x, grad_out, weight, bias, grad_sum, plan)
 
 
-def layer_norm_gradients(x, grad_out, weight, bias, eps, grad_sum=None):
-    """``layer_norm_backward`` of tensors that a forward and autograd have
-    checked: its thread runs a backward's Python at half the speed."""
-    x, grad_out = x.contiguous(), grad_out.contiguous()
+def layer_norm_plan(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float) -> tuple:
+    """What ``layer_norm_gradients`` asks of shapes and types that the forward has
+    checked."""
+    width = x.shape[-1]
+    rows = x.numel() // width
     parameter = bias if weight is None else weight
+    code = _lib.BDM_F32 if parameter is None else _ELEMENT[parameter.dtype]
+    lib = _lib.library()
+    return (lib.bdm_layer_norm_backward, rows, width, _ELEMENT[x.dtype], code, float(eps),
+            lib.bdm_layer_norm_backward_workspace_size(rows, width), x.device)
+
+
+def layer_norm_gradients(x, grad_out, weight, bias, grad_sum, plan):
+    """``layer_norm_backward`` by a plan of the forward, on the current device:
+    autograd's thread, which may run Python several times slower than its
+    caller's, finds it set."""
+    call, rows, width, code, parameter_code, eps, nbytes, device = plan
+    x, grad_out = x.contiguous(), grad_out.contiguous()
     grad_x = torch.empty_like(x)
-    grad_weight = None if weight is None else torch.empty_like(weight, memory_format=torch.contiguous_format)
-    grad_bias = None if bias is None else torch.empty_like(bias, memory_format=torch.contiguous_format)
+    grad_weight = None if weight is None else torch.empty(width, device=device, dtype=weight.dtype)
+    grad_bias = None if bias is None else torch.empty(width, device=device, dtype=bias.dtype)
     weight = None if weight is None else weight.contiguous()
     grad_sum = None if grad_sum is None else grad_sum.contiguous()
-    device, width = x.device, x.shape[-1]
-    rows = x.numel() // width
-    lib = _lib.library()
-    nbytes = lib.bdm_layer_norm_backward_workspace_size(rows, width)
     workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
-    with _on(device):
-        _lib.check(lib.bdm_layer_norm_backward(
-            x.data_ptr(), grad_out.data_ptr(), _addr(grad_sum), _addr(weight), grad_x.data_ptr(), _addr(grad_weight),
-            _addr(grad_bias), rows, width, _ELEMENT[x.dtype],
-            _lib.BDM_F32 if parameter is None else _ELEMENT[parameter.dtype], eps, workspace.data_ptr(), nbytes,
-            _stream(device)), 'bdm_layer_norm_backward')
+    _lib.check(call(x.data_ptr(), grad_out.data_ptr(), _addr(grad_sum), _addr(weight), grad_x.data_ptr(),
+                    _addr(grad_weight), _addr(grad_bias), rows, width, code, parameter_code, eps, workspace.data_ptr(),
+                    nbytes, _stream(device)), 'bdm_layer_norm_backward')
     return grad_x, grad_weight, grad_bias
 
 
@@ -1173,24 +1181,27 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
                      (grad_top_log_probs, None if top_tokens is None else top_tokens.shape)):
         if t is not None and (t.dtype != torch.float32 or t.shape != shape):
             raise ValueError('the results and their gradients must be FP32 of the tokens\' shape')
-    return token_gradients(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs,
-                           grad_loss, inverse_count, int(ignore_index))
+    with _on(logits.device):
+        return token_gradients(logits, tokens.contiguous(), stats.contiguous(),
+                               None if entropy is None else entropy.contiguous(),
+                               None if top_tokens is None else top_tokens.contiguous(), grad_log_probs, grad_entropy,
+                               grad_top_log_probs, grad_loss, inverse_count, int(ignore_index))
 
 
 def token_gradients(logits, tokens, stats, entropy, top_tokens, grad_log_probs, grad_entropy, grad_top_log_probs,
                     grad_loss, inverse_count, ignore_index):
-    """``token_gradient`` of tensors that a forward and autograd have checked."""
+    """``token_gradient`` of tensors that a forward has checked, contiguous but for
+    the logits and the gradients, on the current device."""
     device = logits.device
     grad = torch.empty(logits.shape, device=device, dtype=logits.dtype)
     logits, rows, stride = _logit_rows(logits)
-    kept = [None if t is None else t.contiguous() for t in (tokens, stats, entropy, top_tokens, grad_log_probs,
-                                                            grad_entropy, grad_top_log_probs, grad_loss, inverse_count)]
-    args = _lib.TokenGradArgs(logits.data_ptr(), *[None if t is None else t.data_ptr() for t in kept], grad.data_ptr(),
-                              rows, stride, ignore_index, logits.shape[-1],
-                              0 if top_tokens is None else top_tokens.shape[-1], _ELEMENT[logits.dtype])
-    with _on(device):
-        _lib.check(_lib.library().bdm_token_log_probs_backward(ctypes.byref(args), _stream(device)),
-                   'bdm_token_log_probs_backward')
+    grads = [None if t is None else t.contiguous() for t in (grad_log_probs, grad_entropy, grad_top_log_probs)]
+    args = _lib.TokenGradArgs(logits.data_ptr(), tokens.data_ptr(), stats.data_ptr(), _addr(entropy), _addr(top_tokens),
+                              *map(_addr, grads), _addr(grad_loss), _addr(inverse_count), grad.data_ptr(), rows, stride,
+                              ignore_index, logits.shape[-1], 0 if top_tokens is None else top_tokens.shape[-1],
+                              _ELEMENT[logits.dtype])
+    _lib.check(_lib.library().bdm_token_log_probs_backward(ctypes.byref(args), _stream(device)),
+               'bdm_token_log_probs_backward')
     return grad
 
 

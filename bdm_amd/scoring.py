@@ -59,6 +59,7 @@ def _loss_ops(logits, tokens, ignore_index):
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, alternatives, ignore_index):
+        tokens = tokens.contiguous()
         log_probs, entropy, top, top_tokens, stats = ops.token_statistics(
             logits, tokens, alternatives=alternatives, ignore_index=ignore_index, stats=True)
         ctx.save_for_backward(logits, tokens, stats, entropy, top_tokens)
@@ -88,6 +89,7 @@ class _TokenLogProbs(torch.autograd.Function):
 class _TokenLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, ignore_index):
+        tokens = tokens.contiguous()
         log_probs, _, _, _, stats = ops.token_statistics(logits, tokens, ignore_index=ignore_index, entropy=False,
                                                          stats=True)
         loss, inverse_count = ops.token_loss_mean(log_probs, tokens, ignore_index=ignore_index)
