@@ -197,3 +197,28 @@ def test_layer_norm_entries():
                    dict(workspace=ctypes.c_void_p(4100)), dict(width=-1)):
         assert backward(**fields) == -1, fields
     assert backward(width=20000) == -2
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    """sizeof and offsetof of the two argument structs, compiled from the header with gcc, equal the ctypes mirrors."""
+    import os
+    import shutil
+    import subprocess
+    from conftest import ROOT
+    gcc = shutil.which('gcc')
+    if gcc is None:
+        pytest.skip('no host C compiler')
+    mirrors = {'bdm_token_args': _lib.TokenArgs, 'bdm_token_grad_args': _lib.TokenGradArgs}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{os.path.join(ROOT, "include", "bdm_hip.h")}"',
+             'int main(void) {']
+    for struct, mirror in mirrors.items():
+        lines.append(f'printf("%zu\\n", sizeof({struct}));')
+        lines += [f'printf("%zu\\n", offsetof({struct}, {field}));' for field, _ in mirror._fields_]
+    source, program = tmp_path / 'layout.c', tmp_path / 'layout'
+    source.write_text('\n'.join([*lines, 'return 0; }']))
+    subprocess.run([gcc, str(source), '-o', str(program)], check=True)
+    got = [int(x) for x in subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout.split()]
+    want = []
+    for mirror in mirrors.values():
+        want += [ctypes.sizeof(mirror), *(getattr(mirror, field).offset for field, _ in mirror._fields_)]
+    assert got == want
