@@ -446,8 +446,8 @@ int check_rows(const char *what, int64_t rows, int32_t width, int32_t dtype, int
 }
 
 // Lanes of a team and vectors of a lane for a width: eight values a lane up to a wave's 512 columns, so that narrow rows
-// share a wave (65,536 rows of 64 BF16: 8.4 us forward, 19.8 with a wave a row), then sixteen, which halve the exchanges
-// (32,768 rows of 1,024 BF16, backward: 43 us, 49 by two waves with eight values; 4,096 of 8,192: 50 and 68).
+// share a wave (65,536 rows of 64 BF16: 8.7 us forward, 20.7 with a wave a row), then sixteen, which halve the exchanges
+// (32,768 rows of 1,024 BF16, backward: 43 us, 49 by two waves with eight values; 4,096 of 8,192: 50 and 63).
 template <typename T, typename F>
 void with_shape(int width, F f) {
     constexpr int kVectors = 8 / Vec<T>::kSize;

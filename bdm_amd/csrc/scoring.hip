@@ -759,11 +759,12 @@ int launch_gradient(const bdm_token_grad_args &a, hipStream_t s) {
     return check_launch("token_gradient_kernel");
 }
 
-// A wave a part for short rows (8,192 of 192 BF16 5.3 us, 10.8 by workgroups; of 2,048 12.9 and 18.4; 4,096 of 4,096 12.9
-// and 15.4), a workgroup for long ones (8,192 of 50,257 290 us, 300 by waves).
+// A wave a part for short rows (8,192 of 192 BF16 5.3 us, 10.8 by workgroups; of 2,048 12.4 and 18.1; 4,096 of 4,096 13.0
+// and 15.3), a workgroup for long ones (4,096 of 6,000: 19.9 us, 20.7 by waves; of 8,192 with 8 alternatives 27.4 either
+// way; 8,192 of 50,257 290 and 300).
 template <typename T>
 int launch_gradient(const bdm_token_grad_args &a, hipStream_t s) {
-    return a.vocab <= 8192 ? launch_gradient<T, 64, 4>(a, s) : launch_gradient<T, 256, 4>(a, s);
+    return a.vocab <= 4096 ? launch_gradient<T, 64, 4>(a, s) : launch_gradient<T, 256, 4>(a, s);
 }
 
 }  // namespace
