@@ -136,6 +136,8 @@ class MasterAdamW:
         args.step = float(self.step_count)
         stream = torch.cuda.current_stream(self.device).cuda_stream
         _lib.check(_lib.library().bdm_adamw_step(ctypes.byref(args), ctypes.c_void_p(stream)), 'bdm_adamw_step')
+        # as an in-place operation of torch does: what inference has prepared of the weights is keyed by their version
+        torch.autograd.graph.increment_version(self.params)
         return norm
 
     def state_dict(self) -> dict:

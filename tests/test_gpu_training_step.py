@@ -160,3 +160,23 @@ def test_steps_together():
         assert abs(float(optimizer.step()) - largest) <= 1.01 * half_step(BF16) * largest
         assert any(not torch.equal(p, b) for p, b in zip(params, before))
         assert all(torch.isfinite(p).all() for p in params)
+
+
+@pytest.mark.parametrize('normalization', ['rms', 'layer'])
+def test_logits_behind_a_step(normalization):
+    """Logits without gradients before and behind an update: the second ones are those of a new model with the updated
+    weights, whatever the first call has prepared of the old ones."""
+    from bdm_amd.optim import MasterAdamW
+    model = model_of(BF16, normalization)
+    tokens, target = batch_of()
+    optimizer = MasterAdamW(list(model.parameters()), lr=0.05)
+    with torch.no_grad():
+        before = model(tokens)
+    model(tokens, target).backward()
+    optimizer.step()
+    other = model_of(BF16, normalization)
+    other.load_state_dict(model.state_dict())
+    with torch.no_grad():
+        after, want = model(tokens), other(tokens)
+    assert not torch.equal(before, want)
+    assert torch.equal(after, want)
