@@ -1216,8 +1216,8 @@ def _dense(t: Tensor) -> bool:
 
 
 class _Gradients:
-    """The host arrays of gradients and, where they are written, outputs, those of
-    None left out.  ``copies`` keeps what the arrays point to besides the
+    """The host arrays of gradients and, where they are written, ``outputs``, those
+    of None left out.  ``copies`` keeps what the arrays point to besides the
     caller's tensors.  A model has hundreds of them: each attribute is looked at
     once, over all tensors at a time."""
 
@@ -1229,7 +1229,7 @@ class _Gradients:
         if any([g is None for g in kept]):
             out = [o for g, o in zip(kept, out) if g is not None]
             kept = [g for g in kept if g is not None]
-        self.count, self.copies, self.device = len(kept), None, None
+        self.count, self.copies, self.device, self.outputs = len(kept), None, None, out
         if not kept:
             return
         inplace = all(map(operator.is_, kept, out))
@@ -1320,6 +1320,7 @@ def clip_gradients(gradients, max_norm: float, *, out=None) -> Tensor:
         _lib.check(lib.bdm_clip_gradients(
             _at(tensors.data), _at(tensors.out), sizes, _at(tensors.dtypes), _at(tensors.out_dtypes), count, max_norm,
             _addr(norm), _addr(workspace), nbytes, _stream(device)), 'bdm_clip_gradients')
+    torch.autograd.graph.increment_version(tensors.outputs)  # as an in-place operation of torch does
     return norm
 
 

@@ -246,3 +246,18 @@ def test_optimizer():
         p.grad = torch.ones_like(p)
     with pytest.raises(ValueError, match='negative'):
         torch_norm.step()
+
+
+@pytest.mark.parametrize('inplace', [True, False])
+def test_autograd_sees_the_write(inplace):
+    """A tensor that a backward pass has saved and that is clipped, or written as an output, is refused by it."""
+    from bdm_amd import clip_gradients
+    gen = torch.Generator(device='cuda').manual_seed(4)
+    g, other = (torch.randn(50, generator=gen, device='cuda') for _ in range(2))
+    leaf = torch.ones(50, device='cuda', requires_grad=True)
+    y = leaf * g
+    read = other._version
+    clip_gradients([None, g if inplace else other], 0.5, out=None if inplace else [None, g])
+    assert other._version == read
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
