@@ -310,7 +310,7 @@ class BDMBlock(nn.Module):
         self.ffn_norm = norm(dim, eps=config.memory.norm_eps)
 
     def forward(self, hidden: Tensor) -> Tensor:
-        if isinstance(self.ffn_norm, LayerNorm) and not _hooked(self.ffn_norm):
+        if type(self.ffn_norm) is LayerNorm and not _hooked(self.ffn_norm):  # one of another class may do more
             hidden, normed = self.ffn_norm.add_norm(self.attention(self.attention_norm(hidden)), hidden)
             return hidden + self.feed_forward(normed)
         hidden = hidden + self.attention(self.attention_norm(hidden))

@@ -222,3 +222,26 @@ def test_struct_layouts_match_the_header(tmp_path):
     for mirror in mirrors.values():
         want += [ctypes.sizeof(mirror), *(getattr(mirror, field).offset for field, _ in mirror._fields_)]
     assert got == want
+
+
+def test_block_calls_an_own_norm():
+    """A block's norm that has a forward of its own is called, not passed over by the residual add before it."""
+    from bdm_amd import BSDMConfig
+    from bdm_amd.lm import BDMLanguageModel, LanguageModelConfig
+
+    class Halved(LayerNorm):
+        def forward(self, x):
+            return super().forward(x) * 0.5
+
+    memory = BSDMConfig(dim=64, bank_count=16, bank_size=8, selected_banks=4, value_width=64, num_heads=2)
+    block = BDMLanguageModel(LanguageModelConfig(memory=memory, vocab_size=50, layers=1, ffn_multiple_of=32,
+                                                 normalization='layer')).layers[0]
+    block.attention_norm = block.attention = torch.nn.Identity()
+    block.feed_forward = torch.nn.Identity()
+    block.ffn_norm = Halved(64)
+    called = []
+    block.ffn_norm.add_norm = lambda *a: called.append(a) or LayerNorm.add_norm(block.ffn_norm, *a)
+    hidden = torch.randn(2, 3, 64)
+    total = hidden + hidden
+    assert torch.equal(block(hidden), total + block.ffn_norm(total))
+    assert not called
