@@ -32,7 +32,8 @@ def clip_gradients(gradients, max_norm: float, *, out=None) -> Tensor:
     In place by default; ``out`` gives a tensor for each gradient instead, of as
     many elements in the same order, BF16 or FP32 (an optimizer's FP32 gradients, for instance).  Each value
     is rounded once.  A norm of infinity gives the factor 0 and one of NaN the
-    factor NaN, as torch's clipping does without its check.  A tensor written may
+    factor NaN, as torch's clipping does without its check.  To autograd it is an
+    in-place operation on the tensors written.  A tensor written may
     not share memory with another one of the call (ValueError), so that none is
     given twice.  The host is not synchronised."""
     return ops.clip_gradients(gradients, max_norm, out=out)

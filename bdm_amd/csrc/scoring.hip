@@ -5,7 +5,7 @@
 //   log p_i = (x_i - m) - log s,   H = log s - sum exp(x - m) (x - m) / s,
 // and with gradients a of log p_t, h of H and b_k of log p at the alternatives
 //   dx_i = a [i = t] + sum_k b_k [i = top_k] - p_i (a + sum_k b_k + h (log p_i + H)).
-// Everything is FP32.
+// Arithmetic and sums are FP32, those of the loss' mean FP64; a BF16 gradient is rounded once.
 //
 // Forward.  A call without alternatives over many or long rows streams them (stream_kernel): bound by the read of the
 // logits (8,192 rows of 50,257 BF16, 823 MB: 144 us, 5.7 TB/s).  Others hold a row, or a part of a long one, in
