@@ -1173,6 +1173,9 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
     if logits.dtype not in (torch.bfloat16, torch.float32) or tokens.dtype != torch.int64 \
             or tokens.shape != logits.shape[:-1] or stats.shape != (tokens.numel(), 2):
         raise ValueError('the gradient takes BF16/FP32 logits, their int64 tokens and the rows\' statistics')
+    if top_tokens is not None and (top_tokens.dtype != torch.int64 or top_tokens.ndim != logits.ndim
+                                   or top_tokens.shape[:-1] != tokens.shape):
+        raise ValueError('top_tokens must be int64 of the tokens\' shape and the alternatives')
     if (grad_entropy is not None and entropy is None) or (grad_top_log_probs is not None and top_tokens is None) \
             or (grad_loss is None) != (inverse_count is None):
         raise ValueError('a gradient comes without the result it belongs to')
