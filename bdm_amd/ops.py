@@ -1179,6 +1179,8 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
     if (grad_entropy is not None and entropy is None) or (grad_top_log_probs is not None and top_tokens is None) \
             or (grad_loss is None) != (inverse_count is None):
         raise ValueError('a gradient comes without the result it belongs to')
+    if grad_loss is not None and grad_log_probs is not None:
+        raise ValueError('the gradient of the loss takes the place of that of the log-probabilities')
     for t, shape in ((stats, stats.shape), (entropy, tokens.shape), (grad_log_probs, tokens.shape),
                      (grad_entropy, tokens.shape), (grad_loss, ()), (inverse_count, ()),
                      (grad_top_log_probs, None if top_tokens is None else top_tokens.shape)):

@@ -42,3 +42,14 @@ def test_token_gradient_checks_the_alternatives(no_device, top_tokens, top):
     assert not no_device
     gradient(top_tokens=tokens(3, 2), grad_top_log_probs=torch.zeros(3, 2))
     assert no_device
+
+
+def test_token_gradient_of_a_loss_and_log_probs(no_device):
+    """The loss' gradient takes the place of the log-probabilities': both at once are refused, none is dropped."""
+    scalar = torch.zeros(())
+    with pytest.raises(ValueError, match='loss'):
+        gradient(grad_loss=scalar, inverse_count=scalar, grad_log_probs=torch.zeros(3))
+    assert not no_device
+    gradient(grad_loss=scalar, inverse_count=scalar)
+    gradient(grad_log_probs=torch.zeros(3))
+    assert len(no_device) == 2
