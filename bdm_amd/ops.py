@@ -1097,6 +1097,13 @@ def written_bank_curve(first_write: Tensor, prefixes) -> Tensor:
 # log-probabilities of given tokens
 
 ALTERNATIVES_MAX = 32
+VOCAB_MAX = 1 << 24
+
+
+def _check_vocabulary(logits: Tensor) -> None:
+    """Ahead of the argument structs, whose field of 32 bits holds another number for the longest rows."""
+    if logits.shape[-1] > VOCAB_MAX:
+        raise NotImplementedError(f'token scores take vocabularies of at most {VOCAB_MAX}')
 
 
 def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int]:
@@ -1126,6 +1133,7 @@ def token_statistics(logits: Tensor, tokens: Tensor, *, alternatives: int = 0, i
         raise ValueError('alternatives must be 0 to the size of the vocabulary')
     if k > ALTERNATIVES_MAX:
         raise NotImplementedError(f'at most {ALTERNATIVES_MAX} alternatives')
+    _check_vocabulary(logits)
     device = _require_gpu(logits, tokens)
     lead = tokens.shape
     logits, rows, stride = _logit_rows(logits)
@@ -1173,6 +1181,7 @@ def token_gradient(logits: Tensor, tokens: Tensor, stats: Tensor, *, entropy: Te
     if logits.dtype not in (torch.bfloat16, torch.float32) or tokens.dtype != torch.int64 \
             or tokens.shape != logits.shape[:-1] or stats.shape != (tokens.numel(), 2):
         raise ValueError('the gradient takes BF16/FP32 logits, their int64 tokens and the rows\' statistics')
+    _check_vocabulary(logits)
     if top_tokens is not None and (top_tokens.dtype != torch.int64 or top_tokens.ndim != logits.ndim
                                    or top_tokens.shape[:-1] != tokens.shape):
         raise ValueError('top_tokens must be int64 of the tokens\' shape and the alternatives')

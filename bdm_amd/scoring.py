@@ -113,8 +113,8 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, alternatives: int = 0,
     """Log-probabilities of given tokens under the logits' distributions, the
     entropies of these, and their ``alternatives`` best tokens with theirs.
 
-    logits [..., vocab] BF16 or FP32 on a ROCm device, rows evenly spaced or not;
-    tokens int64 [...].  All results are FP32 (statistics too), and all three take
+    logits [..., vocab] BF16 or FP32 on a ROCm device, rows evenly spaced or not,
+    vocabularies to 2^24 and fewer than 2^24 rows; tokens int64 [...].  All results are FP32 (statistics too), and all three take
     gradients.  Alternatives come best first, equal logits by the lower token; at
     most 32.
 

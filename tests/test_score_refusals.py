@@ -53,3 +53,15 @@ def test_token_gradient_of_a_loss_and_log_probs(no_device):
     gradient(grad_loss=scalar, inverse_count=scalar)
     gradient(grad_log_probs=torch.zeros(3))
     assert len(no_device) == 2
+
+
+@pytest.mark.parametrize('vocab', [2 ** 24 + 1, 2 ** 31 + 5, 2 ** 32 + 192])
+def test_vocabularies_beyond_the_limit(no_device, vocab):
+    """Sizes that a field of 32 bits holds as other ones are refused like any beyond 2^24 (the logits here take four
+    bytes)."""
+    logits = torch.zeros(1).expand(vocab)
+    with pytest.raises(NotImplementedError, match='16777216'):
+        ops.token_statistics(logits, tokens())
+    with pytest.raises(NotImplementedError, match='16777216'):
+        ops.token_gradient(logits, tokens(), torch.zeros(1, 2), grad_log_probs=torch.zeros(()))
+    assert not no_device
