@@ -365,7 +365,7 @@ class BDMLanguageModel(nn.Module):
         logits = self.output(self.norm(self._hidden(tokens)))
         if target is None:
             return logits
-        if (logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and target.dtype == torch.int64
+        if (logits.is_cuda and ops.token_scores_supported(logits) and target.dtype == torch.int64
                 and target.device == logits.device and target.numel() * logits.shape[-1] == logits.numel()):
             return token_loss(logits.flatten(0, -2), target.flatten())
         return F.cross_entropy(logits.float().flatten(0, -2), target.flatten())

@@ -1098,6 +1098,14 @@ def written_bank_curve(first_write: Tensor, prefixes) -> Tensor:
 
 ALTERNATIVES_MAX = 32
 VOCAB_MAX = 1 << 24
+ROWS_LIMIT = 1 << 24  # a launch has at most 2^32 - 1 threads, 256 a row
+
+
+def token_scores_supported(logits: Tensor) -> bool:
+    """Whether ``token_statistics`` takes such logits, were they on a ROCm device: a workgroup a row and 32-bit indexes
+    in a row bound both sizes."""
+    return (logits.dtype in _ELEMENT and logits.ndim >= 1 and 1 <= logits.shape[-1] <= VOCAB_MAX
+            and logits.shape[:-1].numel() < ROWS_LIMIT)
 
 
 def _check_vocabulary(logits: Tensor) -> None:
