@@ -351,9 +351,15 @@ __global__ __launch_bounds__(kThreads) void score_kernel(Rows p) {
 // Statistics without alternatives, for calls of many rows: a workgroup streams one row through a running maximum, sum
 // and moment in every lane, rescaled once for U vectors.  Vectors start at 16-byte boundaries; the few values in front
 // of the first and behind the last one go to a lane each.
+// A lane meets vocab / 256 values.  U vectors' are summed by themselves, kGroups such sums one after the other, and what
+// that gives goes to a sum in FP64, so that no chain of FP32 additions grows with the vocabulary (one of all values, a best
+// token and level others 5 below it, 262,144: log s off by 1.5e-5).  The FP64 sums keep their reference until the maximum
+// is kFar above it: what is added is scaled to it, and a row that creeps up does not round all that came before each time.
+constexpr float kFar = 4.f;
+
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void stream_kernel(Rows p) {
-    constexpr int VE = Vec<T>::kSize;
+    constexpr int VE = Vec<T>::kSize, kGroups = 64 / VE;  // chains of at most 32 additions, then of 8 or 16
     __shared__ float highs[kWaves], sums[kWaves], moments[kWaves];
     const bdm_token_args &a = p.a;
     const int64_t row = blockIdx.x;
@@ -366,15 +372,15 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(Rows p) {
     // lanes 0 to 7 take the values in front, lanes 8 to 15 those behind
     const int odd = thread < VE ? (thread < lead ? thread : -1) : (thread < 2 * VE && tail + thread - VE < a.vocab ? tail + thread - VE : -1);
     float high = odd >= 0 ? to_f32(x[odd]) : -INFINITY, sum = 0.f, moment = 0.f;
-    const auto add = [&](float v) {
+    const auto add = [&](float v, float &s, float &m) {
         const float d = v - high, e = __builtin_amdgcn_exp2f(d * kLog2E);
-        sum += e;
-        moment = fmaf(e, fmaxf(d, -1e30f), moment);  // e = 0 there: no 0 * inf
+        s += e;
+        m = fmaf(e, fmaxf(d, -1e30f), m);  // e = 0 there: no 0 * inf
     };
     {
         const float v = high;
         high = fmaxf(high, -FLT_MAX);
-        add(v);
+        add(v, sum, moment);
     }
     const auto rescale = [&](float to) {
         const float d = fmaxf(high - to, -1e30f), e = __builtin_amdgcn_exp2f(d * kLog2E);
@@ -382,32 +388,57 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(Rows p) {
         sum *= e;
         high = to;
     };
-    int at = thread;
-    for (; at + (U - 1) * kThreads < vectors; at += U * kThreads) {
-        u32x4 raw[U];
+    // N vectors
+    const auto take = [&](const u32x4 *raw, auto count) {
+        constexpr int N = decltype(count)::value;
+        float v[N][VE], top = high, s = 0.f, m = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = from[at + u * kThreads];
-        float v[U][VE], top = high;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < N; ++u) {
             Vec<T>::widen(raw[u], v[u]);
 #pragma unroll
             for (int j = 0; j < VE; ++j) top = fmaxf(top, v[u][j]);
         }
         rescale(top);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < N; ++u)
 #pragma unroll
-            for (int j = 0; j < VE; ++j) add(v[u][j]);
+            for (int j = 0; j < VE; ++j) add(v[u][j], s, m);
+        sum += s;
+        moment += m;
+    };
+    double far_sum = 0, far_moment = 0;
+    float base = -FLT_MAX;
+    int at = thread;
+    for (int stop = min(vectors, kGroups * U * kThreads);; stop = min(vectors, stop + kGroups * U * kThreads)) {
+        for (; at + (U - 1) * kThreads < stop; at += U * kThreads) {
+            u32x4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = from[at + u * kThreads];
+            take(raw, std::integral_constant<int, U>{});
+        }
+        if (stop == vectors) break;
+        if (high > base + kFar) {
+            const float d = fmaxf(base - high, -1e30f);
+            const double e = double(__builtin_amdgcn_exp2f(d * kLog2E));
+            far_moment = e * fma(far_sum, double(d), far_moment);
+            far_sum *= e;
+            base = high;
+        }
+        const float d = fmaxf(high - base, 0.f);  // both infinite: the sum is NaN
+        const double e = double(__builtin_amdgcn_exp2f(d * kLog2E));
+        far_moment = fma(e, fma(double(sum), double(d), double(moment)), far_moment);
+        far_sum = fma(e, double(sum), far_sum);
+        sum = moment = 0.f;
     }
     for (; at < vectors; at += kThreads) {
-        float v[VE], top = high;
-        Vec<T>::widen(from[at], v);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) top = fmaxf(top, v[j]);
-        rescale(top);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) add(v[j]);
+        const u32x4 raw = from[at];
+        take(&raw, std::integral_constant<int, 1>{});
+    }
+    if (vectors > kGroups * U * kThreads) {
+        const float d = fmaxf(base - high, -1e30f);
+        const double e = double(__builtin_amdgcn_exp2f(d * kLog2E));
+        moment = float(fma(e, fma(far_sum, double(d), far_moment), double(moment)));
+        sum = float(fma(e, far_sum, double(sum)));
     }
     const int wave = thread / kWave;
     rescale(wave_max(high));
