@@ -107,6 +107,14 @@ def _rms_norm_trainable(x: Tensor, weight: Tensor) -> bool:
     return ops.rms_norm_supported(x) and x.shape[-1] <= 4096 and weight.dtype in (torch.bfloat16, torch.float32)
 
 
+def _plain(module: nn.Module, kind: type) -> bool:
+    """Whether a call of the module is ``kind``'s forward and nothing else: neither a forward of a derived class or of
+    the instance nor hooks, its own or global ones."""
+    return (type(module).forward is kind.forward and 'forward' not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                     or module._backward_pre_hooks or _global_hooks()))
+
+
 class RMSNorm(nn.Module):
     """x * rsqrt(mean(x^2) + eps) * weight in FP32, cast back (_shell.py:10-35).
     On a ROCm device the norm and, under autograd, its gradients run in HIP
@@ -128,20 +136,15 @@ class RMSNorm(nn.Module):
 
     def add_norm(self, x: Tensor, residual: Tensor):
         """(residual + x, its norm): a block's residual add followed by the
-        next normalization, one kernel under no_grad."""
-        if not torch.is_grad_enabled() and ops.rms_norm_supported(x):
+        next normalization, one kernel under no_grad where a call of the module
+        is no more than this class' forward."""
+        if not torch.is_grad_enabled() and ops.rms_norm_supported(x) and _plain(self, RMSNorm):
             return ops.rms_norm(x, self.weight, self.eps, residual=residual)
         total = residual + x
         return total, self(total)
 
     def reset_parameters(self):
         nn.init.ones_(self.weight)
-
-
-def _hooked(module: nn.Module) -> bool:
-    """Whether a call of the module does more than its forward."""
-    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
-                or module._backward_pre_hooks or _global_hooks())
 
 
 class _LayerNormFunction(torch.autograd.Function):
@@ -228,8 +231,10 @@ class LayerNorm(nn.Module):
 
     def add_norm(self, x: Tensor, residual: Tensor):
         """(residual + x, its norm): a block's residual add and the normalization
-        behind it, one kernel in each direction."""
-        if not self._fused(x) or residual.dtype != x.dtype or residual.shape != x.shape:
+        behind it, one kernel in each direction where a call of the module is no
+        more than this class' forward."""
+        if (not self._fused(x) or residual.dtype != x.dtype or residual.shape != x.shape
+                or not _plain(self, LayerNorm)):
             total = residual + x
             return total, self(total)
         if self._trained(x, residual):
@@ -310,7 +315,7 @@ class BDMBlock(nn.Module):
         self.ffn_norm = norm(dim, eps=config.memory.norm_eps)
 
     def forward(self, hidden: Tensor) -> Tensor:
-        if type(self.ffn_norm) is LayerNorm and not _hooked(self.ffn_norm):  # one of another class may do more
+        if type(self.ffn_norm) is LayerNorm:  # one of another class may do more
             hidden, normed = self.ffn_norm.add_norm(self.attention(self.attention_norm(hidden)), hidden)
             return hidden + self.feed_forward(normed)
         hidden = hidden + self.attention(self.attention_norm(hidden))
