@@ -110,9 +110,13 @@ def _rms_norm_trainable(x: Tensor, weight: Tensor) -> bool:
 def _plain(module: nn.Module, kind: type) -> bool:
     """Whether a call of the module is ``kind``'s forward and nothing else: neither a forward of a derived class or of
     the instance nor hooks, its own or global ones."""
+    return _plain_module(module, kind) and not _global_hooks()
+
+
+def _plain_module(module: nn.Module, kind: type) -> bool:
     return (type(module).forward is kind.forward and 'forward' not in module.__dict__
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
-                     or module._backward_pre_hooks or _global_hooks()))
+                     or module._backward_pre_hooks))
 
 
 class RMSNorm(nn.Module):
@@ -462,10 +466,22 @@ class BDMLanguageModel(nn.Module):
 
     def _fused_decode_supported(self, hidden: Tensor) -> bool:
         ffn = self.layers[0].feed_forward
-        return (isinstance(self.norm, RMSNorm) and hidden.shape[0] <= ops.GEMV_MAX_ROWS and ffn.hidden_dim % 8 == 0 and self.dim % 8 == 0
-                and max(ffn.hidden_dim, self.dim) <= ops.GEMV_PROLOGUE_MAX_K
+        return (hidden.shape[0] <= ops.GEMV_MAX_ROWS and ffn.hidden_dim % 8 == 0 and self.dim % 8 == 0
+                and max(ffn.hidden_dim, self.dim) <= ops.GEMV_PROLOGUE_MAX_K and self._fused_norms()
                 and all(block.attention.step_fused_norm_supported(hidden, block.attention_norm.weight)
                         for block in self.layers))
+
+    def _fused_norms(self) -> bool:
+        """Whether the decode step's products may form every norm of the model, and
+        the sum before it, by themselves: RMSNorms of which neither call is more
+        than that.  Looked at for each step: their tables of modules directly."""
+        norms = [self._modules['norm']]
+        for block in self.layers:
+            modules = block._modules
+            norms += modules['attention_norm'], modules['ffn_norm']
+        return not _global_hooks() and all([
+            isinstance(n, RMSNorm) and type(n).add_norm is RMSNorm.add_norm and 'add_norm' not in n.__dict__
+            and _plain_module(n, RMSNorm) for n in norms])
 
     def _decode_fused(self, hidden: Tensor, caches: list):
         # One decode token with every one-row elementwise kernel formed inside

@@ -79,3 +79,24 @@ def check_tokens(model, tokens):
 def test_layer_norm_tokens(place, change):
     model, tokens, _ = changed('layer', place, change)
     check_tokens(model, tokens)
+
+
+@pytest.mark.parametrize('change', CHANGES)
+@pytest.mark.parametrize('place', ['attention_norm', 'ffn_norm', 'norm'])
+@torch.no_grad()
+def test_rms_norm_tokens(place, change):
+    """The fused decode step leaves such a model to the modules."""
+    model, tokens, _ = changed('rms', place, change)
+    check_tokens(model, tokens)
+
+
+@pytest.mark.parametrize('place', ['attention_norm', 'ffn_norm', 'norm'])
+@torch.no_grad()
+def test_tokens_of_mixed_norms(place):
+    """One layer norm among RMS norms."""
+    from bdm_amd import LayerNorm
+    model = model_of(BF16, 'rms').eval()
+    norm = LayerNorm(64).to(device='cuda', dtype=BF16)
+    norm.bias.add_(0.5)
+    setattr(model if place == 'norm' else model.layers[1], place, norm)
+    check_tokens(model, batch_of(time=9)[0])

@@ -115,3 +115,35 @@ def test_training(kernels, monkeypatch, change):
     hidden = torch.randn(2, 3, 64)
     total = hidden + hidden
     assert torch.equal(block(hidden), total + block.ffn_norm(total))
+
+
+@pytest.fixture
+def fused_step(monkeypatch):
+    """The memory layer's part of the decode step taken for granted."""
+    from bdm_amd import BankedDeltaMemory
+    monkeypatch.setattr(BankedDeltaMemory, 'step_fused_norm_supported', lambda self, hidden, weight: True)
+
+
+@pytest.mark.parametrize('place', ['attention_norm', 'ffn_norm', 'norm'])
+@pytest.mark.parametrize('change', [*CHANGES, 'layer'])
+def test_fused_step_takes_plain_norms_alone(fused_step, place, change):
+    """The decode step's kernels form RMSNorm before a product: any other norm, in any place, is not theirs."""
+    model = model_of('rms')
+    hidden = torch.zeros(1, 1, 64)
+    assert model._fused_decode_supported(hidden)
+    owner = model if place == 'norm' else model.layers[1]
+    if change == 'layer':
+        setattr(owner, place, LayerNorm(64))
+    else:
+        CHANGES[change](getattr(owner, place))
+    assert not model._fused_decode_supported(hidden)
+
+
+def test_fused_step_takes_a_derived_class_without_a_forward(fused_step):
+    class Named(RMSNorm):
+        pass
+
+    model = model_of('rms')
+    for owner, place in ((model, 'norm'), (model.layers[0], 'attention_norm'), (model.layers[1], 'ffn_norm')):
+        getattr(owner, place).__class__ = Named
+    assert model._fused_decode_supported(torch.zeros(1, 1, 64))
