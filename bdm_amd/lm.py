@@ -30,7 +30,7 @@ from torch import nn
 
 from . import ops
 from .config import BDMConfig
-from .model import BankedDeltaMemory, _differentiable, _global_hooks, _torch_gradients
+from .model import BankedDeltaMemory, _differentiable, _dual, _global_hooks, _torch_gradients
 from .pages import BankPages
 from .scoring import TokenLogProbs, token_log_probs, token_loss
 
@@ -220,7 +220,7 @@ class LayerNorm(nn.Module):
     def _fused(self, x: Tensor) -> bool:
         weight, bias = self.weight, self.bias
         return (ops.layer_norm_supported(x) and weight.dtype in (torch.bfloat16, torch.float32)
-                and (bias is None or bias.dtype == weight.dtype))
+                and (bias is None or bias.dtype == weight.dtype) and not _dual(x, weight, bias))
 
     def _trained(self, *tensors: Tensor) -> bool:
         return torch.is_grad_enabled() and any(t is not None and t.requires_grad
@@ -238,7 +238,7 @@ class LayerNorm(nn.Module):
         behind it, one kernel in each direction where a call of the module is no
         more than this class' forward."""
         if (not self._fused(x) or residual.dtype != x.dtype or residual.shape != x.shape
-                or not _plain(self, LayerNorm)):
+                or not _plain(self, LayerNorm) or _dual(residual)):
             total = residual + x
             return total, self(total)
         if self._trained(x, residual):

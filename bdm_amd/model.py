@@ -20,6 +20,7 @@ import math
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import ops
 from .config import BDMConfig, near_square_factors
@@ -75,6 +76,13 @@ def _differentiable(grads) -> bool:
     again (create_graph; a kernel's would end the graph), or the gradients are
     batched (is_grads_batched)."""
     return torch.is_grad_enabled() or any(wrapped(t) for t in grads for wrapped in _WRAPPED)
+
+
+def _dual(*tensors) -> bool:
+    """Whether one of the tensors carries a tangent of forward-mode differentiation: a kernel's result would have none,
+    and no error."""
+    return getattr(forward_ad, '_current_level', 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _torch_gradients(form, inputs, grads):

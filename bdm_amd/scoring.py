@@ -12,9 +12,10 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
-from .model import _differentiable, _torch_gradients
+from .model import _differentiable, _dual, _torch_gradients
 
 Tensor = torch.Tensor
 
@@ -49,6 +50,10 @@ def _log_probs_ops(logits, tokens, top_tokens, ignore_index):
     moment = (e * torch.where(e == 0, 0.0, d)).sum(-1)
     entropy = total.squeeze(-1).log() - moment / total.squeeze(-1)
     return given, entropy, None if top_tokens is None else at(top_tokens)
+
+
+def _primal(dual):
+    return forward_ad.unpack_dual(dual).primal.detach()
 
 
 def _loss_ops(logits, tokens, ignore_index):
@@ -114,9 +119,10 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, alternatives: int = 0,
     entropies of these, and their ``alternatives`` best tokens with theirs.
 
     logits [..., vocab] BF16 or FP32 on a ROCm device, rows evenly spaced or not,
-    vocabularies to 2^24 and fewer than 2^24 rows; tokens int64 [...].  All results are FP32 (statistics too), and all three take
-    gradients.  Alternatives come best first, equal logits by the lower token; at
-    most 32.
+    vocabularies to 2^24 and fewer than 2^24 rows; tokens int64 [...].  All
+    results are FP32 (statistics too), and all three take gradients; tangents of
+    forward-mode differentiation go through torch ops.  Alternatives come best
+    first, equal logits by the lower token; at most 32.
 
     A logit of -inf has the probability 0.  A row of nothing else has no
     distribution: log-probabilities -inf, entropy 0, gradient 0.  A NaN or +inf
@@ -124,6 +130,10 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, alternatives: int = 0,
     token equal to ``ignore_index`` has the log-probability 0 and passes no
     gradient; one outside the vocabulary has the log-probability NaN, and its
     row's gradient is NaN where that of the log-probability arrives."""
+    if _dual(logits):
+        # the call's checks and the alternatives by the kernel, the results and their tangents in torch ops
+        top_tokens = ops.token_statistics(_primal(logits), tokens, alternatives=alternatives, ignore_index=ignore_index)[3]
+        return TokenLogProbs(*_log_probs_ops(logits, tokens, top_tokens, ignore_index), top_tokens)
     if torch.is_grad_enabled() and logits.requires_grad:
         out = _TokenLogProbs.apply(logits, tokens, int(alternatives), int(ignore_index))
         return TokenLogProbs(*(*out, None, None)[:4])
@@ -136,6 +146,9 @@ def token_loss(logits: Tensor, tokens: Tensor, *, ignore_index: int = -100) -> T
     that are not ``ignore_index``, an FP32 scalar (NaN where there is none): the
     cross entropy of the shell's training step.  The mean is formed in FP64 and in
     a fixed order."""
+    if _dual(logits):
+        ops.token_statistics(_primal(logits), tokens, ignore_index=ignore_index, entropy=False)  # the call's checks
+        return _loss_ops(logits, tokens, ignore_index)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TokenLoss.apply(logits, tokens, int(ignore_index))
     log_probs = ops.token_statistics(logits, tokens, ignore_index=ignore_index, entropy=False)[0]
