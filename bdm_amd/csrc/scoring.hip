@@ -624,16 +624,17 @@ __global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad
         for (int k = 0; k < a.alternatives; ++k) total += weights[team][k];
     }
     const int at = token >= 0 && token < a.vocab ? int(token) : -VE;
-    const bool empty = log_sum == -INFINITY;
+    // no distribution, or no gradient: an ignored token's row may hold a NaN, and 0 * NaN is not 0
+    const bool none = log_sum == -INFINITY || (!TOPS && !a.grad_entropy && token == a.ignore_index);
     // N values from index `start` on
     const auto gradient = [&](int start, float *v, auto count) {
         constexpr int N = decltype(count)::value;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const float lp = (v[j] - high) - log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2E);
-            v[j] = empty ? 0.f : -p * (total + h * (fmaxf(lp, -1e30f) + entropy));  // p = 0 there: no 0 * inf
+            v[j] = none ? 0.f : -p * (total + h * (fmaxf(lp, -1e30f) + entropy));  // p = 0 there: no 0 * inf
         }
-        if (empty) return;
+        if (none) return;
         const auto add = [&](int place, float weight) {
             if (unsigned(place) >= unsigned(N)) return;
 #pragma unroll

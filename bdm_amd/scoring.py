@@ -56,8 +56,14 @@ def _primal(dual):
     return forward_ad.unpack_dual(dual).primal.detach()
 
 
+def _counted_rows(logits, tokens, ignore_index):
+    """The logits with zeros in the ignored tokens' rows, whose NaN would reach their gradient."""
+    return logits.masked_fill((tokens == ignore_index).unsqueeze(-1), 0)
+
+
 def _loss_ops(logits, tokens, ignore_index):
     counted = tokens != ignore_index
+    logits = _counted_rows(logits, tokens, ignore_index)
     return -_log_probs_ops(logits, tokens, None, ignore_index)[0].sum() / counted.sum()
 
 
@@ -84,6 +90,8 @@ class _TokenLogProbs(torch.autograd.Function):
             return None, None, None, None
         if _differentiable(present):
             def form(x):
+                if grads[1] is None and grads[2] is None:
+                    x = _counted_rows(x, tokens, ctx.ignore_index)
                 results = _log_probs_ops(x, tokens, top_tokens, ctx.ignore_index)
                 return [r for r, g in zip(results, grads) if g is not None]
             return (*_torch_gradients(form, (logits,), present), None, None, None)
@@ -127,8 +135,8 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, alternatives: int = 0,
     A logit of -inf has the probability 0.  A row of nothing else has no
     distribution: log-probabilities -inf, entropy 0, gradient 0.  A NaN or +inf
     makes its row's results NaN (and a NaN comes first of the alternatives).  A
-    token equal to ``ignore_index`` has the log-probability 0 and passes no
-    gradient; one outside the vocabulary has the log-probability NaN, and its
+    token equal to ``ignore_index`` has the log-probability 0, which passes no
+    gradient, whatever its row holds; one outside the vocabulary has the log-probability NaN, and its
     row's gradient is NaN where that of the log-probability arrives."""
     if _dual(logits):
         # the call's checks and the alternatives by the kernel, the results and their tangents in torch ops

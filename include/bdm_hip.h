@@ -738,7 +738,8 @@ int bdm_token_log_probs(const bdm_token_args *args, void *workspace, size_t work
  * the log-probabilities, the entropies and the alternatives' log-probabilities,
  * each optional; or from that of the mean loss, a scalar, with the inverse of
  * the rows' number from bdm_token_loss in the place of grad_log_probs.  Rounded
- * once. */
+ * once.  The row of an ignored token has the gradient 0, whatever it holds, where
+ * neither entropies nor alternatives have one. */
 typedef struct bdm_token_grad_args {
     const void *logits;
     const int64_t *tokens;
