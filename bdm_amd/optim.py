@@ -151,7 +151,7 @@ class MasterAdamW:
                 'exp_avg': [self.moments_of(i)[0].detach().cpu().clone() for i in range(count)],
                 'exp_avg_sq': [self.moments_of(i)[1].detach().cpu().clone() for i in range(count)],
                 'step': self.step_count, 'lr': self.lr, 'betas': self.betas, 'eps': self.eps,
-                'max_norm': self.max_norm, 'weight_decay': list(self.decay)}
+                'max_norm': self.max_norm, 'float32_norm': self.float32_norm, 'weight_decay': list(self.decay)}
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
@@ -182,6 +182,7 @@ class MasterAdamW:
         self.betas = tuple(float(b) for b in state.get('betas', self.betas))
         self.eps = float(state.get('eps', self.eps))
         self.max_norm = float(state.get('max_norm', self.max_norm))
+        self.float32_norm = bool(state.get('float32_norm', self.float32_norm))
 
     @torch.no_grad()
     def reload_masters(self) -> None:
