@@ -13,8 +13,10 @@
 // so that rows far from zero lose nothing, and a team of several waves waits once a row.
 //
 // Bound by HBM where rows are many (32,768 of 1,024 BF16 behind a residual add, 268 MB each way: forward 46 us, backward
-// 46 and 4 for the parts' sums, 5.8 TB/s), by the chain of a row's sums where the registers admit two waves a SIMD
-// (backward of 8,192 rows of 2,048 BF16: 27 us, 3.7 TB/s), by latency where they are few (64 of 1,024: 4 and 7 us).
+// 46 and 4 for the parts' sums, 5.8 TB/s); by the instructions of a row's sums, issued by the two waves a SIMD that the
+// registers admit, in the backward of wider BF16 rows (8,192 of 2,048: 27 us, 3.7 TB/s, the SIMDs issue vector
+// instructions 73% of the time) and of narrow ones (65,536 of 64: 18 us, 83%); by latency where rows are few (64 of 1,024:
+// 4 and 7 us).
 #include <type_traits>
 
 #include "bdm_common.h"
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(LANES <= 256 ? 256 : LANES) void layer_norm_kernel(
 }
 
 // Lanes of a backward's workgroup: several teams share one, and its LDS adds up their columns' sums (8,192 rows of 2,048
-// BF16: 38 us with one team of two waves, 29 with four).
+// BF16: 32 us with one team of two waves, 28 with four).
 constexpr int backward_block(int lanes) { return lanes <= kWave ? 256 : lanes <= 512 ? 512 : lanes; }
 
 template <typename T, typename P, int LANES, int NV, bool SUM>
@@ -446,8 +448,8 @@ int check_rows(const char *what, int64_t rows, int32_t width, int32_t dtype, int
 }
 
 // Lanes of a team and vectors of a lane for a width: eight values a lane up to a wave's 512 columns, so that narrow rows
-// share a wave (65,536 rows of 64 BF16: 8.7 us forward, 20.7 with a wave a row), then sixteen, which halve the exchanges
-// (32,768 rows of 1,024 BF16, backward: 43 us, 49 by two waves with eight values; 4,096 of 8,192: 50 and 63).
+// share a wave (65,536 rows of 64 BF16: 8.7 us forward, 20.8 with a wave a row), then sixteen, which halve the exchanges
+// (32,768 rows of 1,024 BF16, backward: 43 us, 49 by two waves with eight values; 4,096 of 8,192: 50 and 61).
 template <typename T, typename F>
 void with_shape(int width, F f) {
     constexpr int kVectors = 8 / Vec<T>::kSize;
@@ -481,8 +483,9 @@ int64_t blocks_of(int64_t rows, int lanes, int block, int64_t waves) {
 constexpr int64_t kForwardWaves = 256 * 32;
 
 // The backward's workgroups, each of which leaves its columns' sums: as many waves as the registers of 16 values a lane
-// admit, twice as many with 8 values or without a row loaded ahead (more of 16 wait for the first ones: 32,768 rows of
-// 1,024 BF16 43 us with 2,048 waves, 53 with 3,072; 2,048 rows of 16,384 95 with 2,048, 73 with 4,096).
+// admit, twice as many with 8 values or without a row loaded ahead (more of 16 wait for the first ones: 8,192 rows of
+// 2,048 BF16 28 us with 2,048 waves, 34 with 3,072, 32 with 4,096, 32,768 of 1,024 43, 42 and 48; 2,048 rows of 16,384 83
+// with 2,048, 60 with 4,096, 65,536 of 256 29 and 28).
 int64_t backward_parts(int64_t rows, int width) {
     int64_t parts = 0;
     with_shape<bf16_t>(width, [&](auto lanes, auto vectors) {

@@ -5,16 +5,18 @@
 //   log p_i = (x_i - m) - log s,   H = log s - sum exp(x - m) (x - m) / s,
 // and with gradients a of log p_t, h of H and b_k of log p at the alternatives
 //   dx_i = a [i = t] + sum_k b_k [i = top_k] - p_i (a + sum_k b_k + h (log p_i + H)).
-// Arithmetic and sums are FP32, those of the loss' mean FP64; a BF16 gradient is rounded once.
+// Arithmetic and sums are FP32, those of the loss' mean FP64 and of long rows' parts too; a BF16 gradient is rounded once.
+// Times, here and below: of a call in a graph over two to eight tensors of logits in turn; "alone" those of a kernel under
+// the profiler.
 //
 // Forward.  A call without alternatives over many or long rows streams them (stream_kernel): bound by the read of the
-// logits (8,192 rows of 50,257 BF16, 823 MB: 144 us, 5.7 TB/s).  Others hold a row, or a part of a long one, in
+// logits (8,192 rows of 50,257 BF16, 823 MB: 149 us, 5.5 TB/s; alone 144).  Others hold a row, or a part of a long one, in
 // registers (score_kernel): every value is read once, and the alternatives are found without a second read, by a bound
 // that as many lanes' own maxima reach and a ranking of the few values above it.  The parts of a row are joined by a
-// second launch (join_kernel).  Bound by latency for few rows (64 of 50,257 with 8 alternatives: 8.7 and 4.0 us), by the
-// instructions of the selection for many (4,096: 113 us, 3.6 TB/s).
+// second launch (join_kernel).  Bound by latency for few rows (64 of 50,257 with 8 alternatives: 12.1 us; alone 8.7 and
+// 4.0), by the instructions of the selection for many (4,096: 113 us, 3.6 TB/s).
 // Backward (token_gradient_kernel).  The logits are read again and the gradient is written: HBM (8,192 rows of 50,257
-// BF16: 267 us behind the forward, 6.2 TB/s).
+// BF16: 290 us, 5.7 TB/s; alone, behind the forward of the same logits, 267).
 #include <algorithm>
 #include <cfloat>
 
@@ -112,8 +114,10 @@ struct Place {
 // The exact `width` best of the team's values to sh.list where the bound does not serve: those above the width-th, then
 // of those equal to it the ones of lowest index, which lie in the order of vectors, lanes, places in the vector.  `guess`
 // is the width-th's key if no `width` values are above it (equal logits, or a mask over most of the row): three passes
-// over the part; else that is bisected, a pass a bit.  Vector by vector from memory: it takes no registers from the
-// ordinary case.
+// over the part (4,096 level rows of 50,257 BF16 with 8: 409 us, 113 of others); else that is bisected, a pass a bit.  So
+// it is where fewer lanes than `width` hold a value, which gives no bound: vocabularies, or a row's last part, of fewer
+// than `width` vectors (8,192 rows of 192 BF16, 24 vectors: 30 us with 24 alternatives, 55 with 25 to 32; of 64 with 16
+// 54, 8.4 with 8).  Vector by vector from memory: it takes no registers from the ordinary case.
 template <typename T, int WAVES, int NV>
 __device__ __forceinline__ int team_exact(Team<WAVES, NV> &sh, const T *x, int length, int vocab, uint32_t guess, int width,
                                        uint32_t offset, int wave, int lane) {
@@ -470,8 +474,8 @@ __device__ __forceinline__ uint64_t largest_key(uint64_t x) {
 }
 
 // The parts of a row joined: two exchanges between the waves, and the candidates ranked by counting (parts and join of 64
-// rows of 50,257 BF16 logits with 8 alternatives: 12.2 us, 3 rows of 262,144 FP32 with 20 13.4; by one wave, which meets no
-// barrier but ranks alone, 12.0 and 19).
+// rows of 50,257 BF16 logits with 8 alternatives: 12.1 us, 3 rows of 262,144 FP32 with 20 12.9; joined by one wave, which
+// meets no barrier but ranks alone, 12.0 and 19).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(Rows p) {
     constexpr int kRoom = 512;
@@ -583,7 +587,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Rows p) {
 // start at the gradient's 16-byte boundaries (the logits' too, where both are as torch allocates them); the few values
 // in front of the first and behind the last go to a lane each of the row's first team.  Loads and stores pass by the
 // caches: kept there, what was written made the next forward slower (its loss and gradient, 8,192 rows of 50,257 BF16
-// logits: 479 us, 426 so).  `TOPS`: gradients of the
+// logits: 477 us, 430 so).  `TOPS`: gradients of the
 // alternatives arrive too.
 template <typename T, int LANES, int U, bool TOPS>
 __global__ __launch_bounds__(kThreads) void token_gradient_kernel(bdm_token_grad_args a, int parts) {
@@ -728,9 +732,9 @@ int check_rows(const char *what, int64_t rows, int64_t row_stride, int32_t vocab
 }
 
 // A team's waves and values a lane, and the parts of a row.  One wave a row as long as it holds it (8,192 rows of 2,000
-// BF16 logits with 4 alternatives: 12.9 us, 28.2 by four waves), then four; parts of at most 16,384, all alike, which
-// leave several workgroups to a CU (4,096 rows of 50,257 with 8: 122 us, 199 by sixteen waves over whole rows); half as
-// long ones where there are few workgroups (a row of 50,257 with 8: 10.6 us, 11.4 otherwise).
+// BF16 logits with 4 alternatives: 12.6 us, 28.3 by four waves), then four; parts of at most 16,384, all alike, which
+// leave several workgroups to a CU (4,096 rows of 50,257 with 8: 113 us, 127 in parts of at most 8,192); half as long ones
+// where there are few workgroups (a row of 50,257 with 8: 9.5 us, 10.1 otherwise; 64 rows 12.1 and 12.0).
 struct Shape {
     int waves, values, splits;
 };
@@ -771,9 +775,12 @@ int launch_scores(const Rows &p, const Shape &shape, hipStream_t s) {
     return check_launch("join_kernel");
 }
 
-// Whether a call without alternatives streams its rows (8,192 rows of 50,257 BF16: 148 us, 285 from registers; 2,048 of
-// 4,099 6.4 and 8.7): not short rows (8,192 of 4,096: 18.0 us, 15.9 from registers), nor few long ones, whose parts work
-// side by side (a row of 131,072: 11.7 us, 5.8 in parts).
+// Whether a call without alternatives streams its rows (8,192 rows of 50,257 BF16: 149 us, 196 from registers; 2,048 of
+// 4,099 6.5 and 8.7; 255 of 65,536 10.7 and 12.3): not short rows (8,192 of 4,096: 17.6 us, 15.4 from registers), nor few
+// long ones, whose parts work side by side (a row of 131,072: 12.1 us, 5.6 in parts; 255 22.9 and 17.8).  Both bounds are
+// rough: some 64 rows of 50,000 to 65,536 tokens would gain by parts (of 65,536: 9.3 us, 7.7 in parts; 128 rows 9.9 and
+// 9.3), and so would few hundred of 131,072 and more (256: 22.8 us, 17.9 in parts; 1,024 53 either way; 512 of 262,144 51
+// and 53).
 bool streams(const bdm_token_args &a) {
     return !a.alternatives && a.vocab > 4096 && (a.rows >= 256 || a.vocab <= 65536);
 }
@@ -791,9 +798,9 @@ int launch_gradient(const bdm_token_grad_args &a, hipStream_t s) {
     return check_launch("token_gradient_kernel");
 }
 
-// A wave a part for short rows (8,192 of 192 BF16 5.3 us, 10.8 by workgroups; of 2,048 12.4 and 18.1; 4,096 of 4,096 13.0
-// and 15.3), a workgroup for long ones (4,096 of 6,000: 19.9 us, 20.7 by waves; of 8,192 with 8 alternatives 27.4 either
-// way; 8,192 of 50,257 290 and 300).
+// A wave a part for short rows (8,192 of 192 BF16 5.2 us, 10.9 by workgroups; of 2,048 12.9 and 17.9; 4,096 of 4,096 13.0
+// and 15.3), a workgroup for long ones (4,096 of 6,000: 19.9 us, 21.2 by waves; of 8,192 with 8 alternatives 27.5 either
+// way; 8,192 of 50,257 290 and 298).
 template <typename T>
 int launch_gradient(const bdm_token_grad_args &a, hipStream_t s) {
     return a.vocab <= 4096 ? launch_gradient<T, 64, 4>(a, s) : launch_gradient<T, 256, 4>(a, s);
