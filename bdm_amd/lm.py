@@ -474,11 +474,13 @@ class BDMLanguageModel(nn.Module):
     def _fused_norms(self) -> bool:
         """Whether the decode step's products may form every norm of the model, and
         the sum before it, by themselves: RMSNorms of which neither call is more
-        than that.  Looked at for each step: their tables of modules directly."""
-        norms = [self._modules['norm']]
+        than that."""
+        norms = [self.norm]
         for block in self.layers:
-            modules = block._modules
-            norms += modules['attention_norm'], modules['ffn_norm']
+            if type(block) is BDMBlock:  # its table directly: every step asks
+                norms += block._modules['attention_norm'], block._modules['ffn_norm']
+            else:
+                norms += block.attention_norm, block.ffn_norm
         return not _global_hooks() and all([
             isinstance(n, RMSNorm) and type(n).add_norm is RMSNorm.add_norm and 'add_norm' not in n.__dict__
             and _plain_module(n, RMSNorm) for n in norms])

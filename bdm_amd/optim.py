@@ -44,7 +44,7 @@ class MasterAdamW:
 
     The clipping norm is torch's by default, a BF16 number as the gradients are;
     with ``float32_norm`` it is ``gradient_norm``'s, not rounded to BF16 and
-    formed in two kernels instead of some dozens.
+    formed in two kernels instead of some dozens.  A saved state holds which.
     """
 
     def __init__(self, params, lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.01,

@@ -147,3 +147,26 @@ def test_fused_step_takes_a_derived_class_without_a_forward(fused_step):
     for owner, place in ((model, 'norm'), (model.layers[0], 'attention_norm'), (model.layers[1], 'ffn_norm')):
         getattr(owner, place).__class__ = Named
     assert model._fused_decode_supported(torch.zeros(1, 1, 64))
+
+
+class Wrapped(nn.Module):
+    """A block inside a module that hands its attributes on, as compiled and checkpointed ones are."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def __getattr__(self, name):
+        try:
+            return super().__getattr__(name)
+        except AttributeError:
+            return getattr(super().__getattr__('inner'), name)
+
+
+@pytest.mark.parametrize('place', [None, 'attention_norm', 'ffn_norm', 'norm'])
+def test_fused_step_of_wrapped_blocks(fused_step, place):
+    model = model_of('rms')
+    model.layers[0], model.layers[1] = Wrapped(model.layers[0]), Wrapped(model.layers[1])
+    if place:
+        derive(model.norm if place == 'norm' else getattr(model.layers[1], place))
+    assert model._fused_decode_supported(torch.zeros(1, 1, 64)) is (place is None)
