@@ -69,3 +69,30 @@ def test_gradient_of_long_rows(pattern, dtype):
     loss = token_loss(logits, token.expand(rows))
     value, tolerance = expected_scores(logits.detach()[:1], token)['log_probs']
     close(loss, -value[0], tolerance[0] + 2.0 ** -23 * value[0].abs())
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP32])
+@pytest.mark.parametrize('vocab', [65537, 131075, 200001])
+def test_long_rows_of_every_kind(vocab, dtype):
+    """Rows whose sums are joined several times: what is not finite or lowest stands at the start, in the middle, at the
+    end; rows at every alignment."""
+    from bdm_amd import token_log_probs
+    rows, lowest = 272, torch.finfo(dtype).min
+    gen = torch.Generator(device='cuda').manual_seed(vocab)
+    logits = (torch.randn(rows, vocab, generator=gen, device='cuda') * 2.5).to(dtype)
+    tokens = torch.randint(vocab - 1, (rows,), generator=gen, device='cuda')
+    for kind, (value, place) in enumerate((v, p) for v in (torch.nan, torch.inf, torch.finfo(dtype).max)
+                                          for p in (0, vocab // 2, vocab - 1)):
+        logits[kind::17, place] = value
+    logits[9::17] = -torch.inf
+    logits[10::17] = lowest
+    logits[11::17, :vocab // 2] = lowest
+    logits[12::17, vocab // 2:] = -torch.inf
+    logits[13::17, 5:] = lowest
+    logits[14::17, :-5] = -torch.inf
+    logits[15::17] *= 1000
+    for view in (logits, logits[:, 1:]):
+        out = token_log_probs(view, tokens)
+        want = expected_scores(view, tokens)
+        for name in ('log_probs', 'entropy'):
+            close(getattr(out, name), *want[name], name)
